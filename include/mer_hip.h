@@ -389,6 +389,102 @@ int mer_hip_route_linear_gate(const float *d_gate, size_t n_experts, size_t d_mo
                               size_t n_tokens, size_t top_k, const mer_gate_options *options, int32_t *d_ids,
                               float *d_weights, float *d_logits, void *stream);
 
+/* ---- attention side of a layer ---------------------------------------
+ * The operators between a layer's projections and its router, around one
+ * paged key/value cache, so a hidden state can stay on the device from
+ * layer to layer: what the engine computes on the host beside its paged
+ * KV (transformer.rs, block_pool.rs) and offers as the backend's attention
+ * and KV operations (backend/mod.rs).  Pointers to elements are 16-byte
+ * aligned, head_dim is a multiple of 8 up to MER_MAX_HEAD_DIM, and a row's
+ * heads lie side by side; rows are a stride (in elements) apart, so slices
+ * of a packed q|k|v projection are taken as they are.  Strides are
+ * multiples of 16 bytes. */
+
+/* Element types, by their UTH dtype ids (tensor_header.rs:78-90). */
+enum mer_float_type {
+  MER_FLOAT_F32 = 0,
+  MER_FLOAT_F16 = 1,
+  MER_FLOAT_BF16 = 6,
+};
+#define MER_MAX_HEAD_DIM 256
+
+/* A paged cache: k and v are [n_pages][n_kv_heads][page_size][head_dim],
+ * page_size a power of two from 8 to 4096, type f16 or bf16.  The memory is
+ * the caller's; the library keeps nothing of it. */
+typedef struct mer_kv_cache {
+  void *k, *v;
+  int32_t type;          /* MER_FLOAT_F16 or MER_FLOAT_BF16 */
+  uint32_t page_size, n_kv_heads, head_dim;
+  uint64_t n_pages;      /* < 2^31 */
+} mer_kv_cache;
+
+/* Position rotation: element pairs (i, i + rot_dim / 2), or (2i, 2i + 1)
+ * interleaved, of the first rot_dim elements of a head turn by
+ * position * inv_freq[i]; the others stay.  rot_dim is a multiple of 8. */
+typedef struct mer_rope {
+  const float *inv_freq; /* device [rot_dim / 2] */
+  uint32_t rot_dim;
+  int32_t interleaved;
+} mer_rope;
+
+/* Norms of queries and keys for each head, with the rotation in the same
+ * pass: x / sqrt(mean(x^2) + eps) * norm, then the rotation, in f32; rounded
+ * once to out_type.
+ *   d_q [n_tokens][n_heads][head_dim], d_k [n_tokens][n_kv_heads][head_dim]
+ *   (rows q_stride / k_stride elements apart); either may have no heads;
+ *   d_positions[n_tokens] (any sign); rope NULL = no rotation;
+ *   d_q_norm, d_k_norm [head_dim], NULL = no norm;
+ *   outputs likewise, and they may be their inputs themselves where type and
+ *   stride are the same (other overlaps are not allowed). */
+int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
+                         size_t head_dim, const void *d_q, size_t q_stride, const void *d_k, size_t k_stride,
+                         const int32_t *d_positions, const mer_rope *rope, const float *d_q_norm,
+                         const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
+                         size_t k_out_stride, void *stream);
+
+/* Appends keys and values to a paged cache: row t goes to slot d_slots[t] =
+ * page * page_size + place in the page, the keys normed and rotated on the
+ * way (each optional as above), both rounded once to the cache's type.  A
+ * negative slot skips the row (padding); one past the cache skips it too and
+ * records MER_ERR_RESIDENCY_MISS in the device status word.  The slots of a
+ * call are distinct (two rows of one slot leave elements of either). */
+int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
+                      const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
+                      const mer_rope *rope, const float *d_k_norm, float eps, void *stream);
+
+typedef struct mer_attention_options {
+  float scale;           /* of q . k; 0 = 1 / sqrt(head_dim)               */
+  uint32_t window;       /* keys a row sees, itself included; 0 = all      */
+  const float *sinks;    /* device [n_heads]: a logit that takes part in   */
+                         /* the softmax and adds no value; NULL = none     */
+} mer_attention_options;
+
+/* Attention of each sequence's new tokens over its pages, from one token
+ * (decode) to whole prompts, any mix in a call.  Sequence s has rows
+ * d_q_start[s] .. d_q_start[s + 1] of d_q / d_out (n of them; n_tokens rows
+ * in all, rows of no sequence are left as they are) and d_kv_len[s] keys in
+ * the pages d_block_table[s * table_stride + ..], the new tokens' own among
+ * them (mer_hip_kv_append first).  Row i stands at position
+ * p = kv_len - n + i and sees the keys j <= p, with a window j > p - window.
+ * A row that sees no key gives zeros.
+ * d_q and d_out are of the cache's type, n_heads is a multiple of the cache's
+ * n_kv_heads (head h reads kv head h / (n_heads / n_kv_heads)); sums and
+ * softmax are f32, the weights are rounded to the cache's type for the
+ * product with the values.
+ * Pages and places at or beyond kv_len, and pages wholly before every row's
+ * window, are never read; a page id outside the cache reads as zeros and
+ * records MER_ERR_RESIDENCY_MISS in the device status word.  kv_len is cut to
+ * table_stride * page_size (at most 2^30) and rows to n_tokens.
+ * A key or value that is not finite reaches rows of its own sequence only,
+ * but there it may reach rows of the same call that do not see it.
+ * max_q_len and max_kv_len say what the call should be laid out for, as a
+ * captured graph needs it (0 = unknown); results do not depend on their being
+ * right.  options NULL = all defaults. */
+int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
+                            const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
+                            const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
+                            const mer_attention_options *options, void *d_out, size_t out_stride, void *stream);
+
 /* Synthetic bench / test data: fill n_blocks GGUF blocks of expert
  * `expert_index` starting at block `block_begin` with this library's
  * counter-based generator (nibbles / int8 uniform, d = f16(U(lo,hi))). */

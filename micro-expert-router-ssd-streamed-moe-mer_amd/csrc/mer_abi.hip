@@ -1,6 +1,7 @@
 // mer_abi.hip -- extern "C" boundary of the routed-expert SwiGLU FFN
 // (declared in include/mer_hip.h).  Host-side validation mirrors the
 // reference's typed errors; device work is enqueued on the caller's stream.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -15,6 +16,7 @@
 #include <vector>
 
 #include "../../include/mer_hip.h"
+#include "mer_attention.hpp"
 #include "mer_internal.hpp"
 
 using namespace mer;
@@ -84,6 +86,8 @@ struct Workspace {
   size_t stage_floats = 0;
   float *router_buf = nullptr;   // router logits when the caller asks for none
   size_t router_floats = 0;
+  float *attn_buf = nullptr;     // attention: sums of a row's key chunks
+  size_t attn_floats = 0;
   uint32_t *counters = nullptr;  // decode counters (zero between launches) + control lines
   size_t counter_words = 0;
   uint64_t *release = nullptr;   // decode release flags (epoch-valued, zero at allocation)
@@ -215,13 +219,14 @@ void free_workspace(Workspace &w) {
   if (w.scratch) (void)hipFree(w.scratch);
   if (w.stage) (void)hipFree(w.stage);
   if (w.router_buf) (void)hipFree(w.router_buf);
+  if (w.attn_buf) (void)hipFree(w.attn_buf);
   if (w.counters) (void)hipFree(w.counters);
   if (w.release) (void)hipFree(w.release);
-  w.scratch = w.stage = w.router_buf = nullptr;
+  w.scratch = w.stage = w.router_buf = w.attn_buf = nullptr;
   w.counters = nullptr;
   w.release = nullptr;
   w.scratch_refused = SIZE_MAX;
-  w.scratch_floats = w.stage_floats = w.router_floats = w.counter_words = w.release_words = 0;
+  w.scratch_floats = w.stage_floats = w.router_floats = w.attn_floats = w.counter_words = w.release_words = 0;
 }
 
 bool capturing(hipStream_t st) {
@@ -886,6 +891,87 @@ int run_grouped(Workspace &w, int dtype, size_t dm, size_t dff, uint32_t n_token
   return timing_end(tl, st);
 }
 
+// ---- attention side ---------------------------------------------------
+
+// The library's device is also the calling thread's.
+int require_current_device() {
+  const int rc = require_init();
+  if (rc) return rc;
+  int d = -1;
+  if (hipGetDevice(&d) != hipSuccess || d != g_device.load())
+    return fail(MER_ERR_WRONG_DEVICE, "the current device is %d; mer_hip_init selected %d", d, g_device.load());
+  return MER_OK;
+}
+
+int check_float_type(int type, bool f32) {
+  if (type == MER_FLOAT_F16 || type == MER_FLOAT_BF16 || (f32 && type == MER_FLOAT_F32)) return MER_OK;
+  return fail(MER_ERR_UNSUPPORTED_DTYPE, "unsupported element type %d", type);
+}
+
+int check_head_dim(size_t d) {
+  if (d > MER_MAX_HEAD_DIM) return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "head_dim %zu exceeds %d", d, MER_MAX_HEAD_DIM);
+  if (d == 0 || d % 8 != 0) return fail(MER_ERR_INVALID_LAYOUT, "head_dim %zu is no multiple of 8", d);
+  return MER_OK;
+}
+
+int check_rope(const mer_rope *r, size_t head_dim) {
+  if (!r) return MER_OK;
+  if (!r->inv_freq) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs its inverse frequencies");
+  if ((uintptr_t)r->inv_freq & 15u) return fail(MER_ERR_MISALIGNED, "inverse frequencies must be 16-byte aligned");
+  if (r->rot_dim == 0 || r->rot_dim % 8 != 0 || r->rot_dim > head_dim)
+    return fail(MER_ERR_INVALID_LAYOUT, "rot_dim %u must be a multiple of 8 up to head_dim %zu", r->rot_dim, head_dim);
+  return MER_OK;
+}
+
+// Row counts that the launch grids hold.
+int check_rows(size_t n_tokens, size_t heads) {
+  if (heads > 4096) return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "at most 4096 heads, got %zu", heads);
+  if (n_tokens > (1u << 24) || n_tokens * heads > (1u << 26))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "%zu tokens of %zu heads exceed one call (2^24 tokens, 2^26 head rows)",
+                n_tokens, heads);
+  return MER_OK;
+}
+
+int check_cache(const mer_kv_cache *c) {
+  if (!c) return fail(MER_ERR_INVALID_LAYOUT, "null cache");
+  int rc = check_float_type(c->type, false);
+  if (rc) return rc;
+  if ((rc = check_head_dim(c->head_dim))) return rc;
+  if (c->page_size < 8 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
+    return fail(MER_ERR_INVALID_LAYOUT, "page_size %u must be a power of two from 8 to 4096", c->page_size);
+  if (c->n_kv_heads == 0 || c->n_kv_heads > 2048)
+    return fail(MER_ERR_INVALID_LAYOUT, "n_kv_heads %u must be in 1..=2048", c->n_kv_heads);
+  if (c->n_pages == 0 || c->n_pages > 0x7fffffffull)
+    return fail(MER_ERR_INVALID_LAYOUT, "n_pages must be in 1..2^31");
+  if (!c->k || !c->v) return fail(MER_ERR_INVALID_LAYOUT, "null cache memory");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return fail(MER_ERR_MISALIGNED, "cache memory must be 16-byte aligned");
+  return MER_OK;
+}
+
+// Rows of `row` elements, `stride` apart.
+int check_tensor(const char *name, const void *p, int type, size_t stride, size_t row, size_t n_rows) {
+  if (!p) return fail(MER_ERR_INVALID_LAYOUT, "%s is null", name);
+  const size_t size = type == MER_FLOAT_F32 ? 4 : 2;
+  if ((uintptr_t)p & 15u || (n_rows > 1 && stride % (16 / size) != 0))
+    return fail(MER_ERR_MISALIGNED, "rows of %s must be 16-byte aligned (stride %zu elements)", name, stride);
+  if (n_rows > 1 && (stride < row || stride > (size_t(1) << 40)))
+    return fail(MER_ERR_INVALID_LAYOUT, "stride %zu of %s does not fit rows of %zu elements", stride, name, row);
+  return MER_OK;
+}
+
+void set_rope(NormRopeParams *p, const mer_rope *rope, const int32_t *positions, float eps, size_t n_tokens,
+              size_t head_dim) {
+  if (rope) {
+    p->positions = positions;
+    p->inv_freq = rope->inv_freq;
+    p->rot = rope->rot_dim;
+    p->interleaved = rope->interleaved != 0;
+  }
+  p->eps = eps;
+  p->n_tokens = (uint32_t)n_tokens;
+  p->head_dim = (uint32_t)head_dim;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1442,6 +1528,139 @@ int mer_hip_route_linear_gate(const float *d_gate, size_t n_experts, size_t d_mo
   }
   hipError_t e = launch_router(p, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "router launch");
+  return MER_OK;
+}
+
+int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
+                         size_t head_dim, const void *d_q, size_t q_stride, const void *d_k, size_t k_stride,
+                         const int32_t *d_positions, const mer_rope *rope, const float *d_q_norm,
+                         const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
+                         size_t k_out_stride, void *stream) {
+  int rc;
+  if ((rc = check_float_type(in_type, true)) || (rc = check_float_type(out_type, true))) return rc;
+  if ((rc = check_head_dim(head_dim)) || (rc = check_rope(rope, head_dim))) return rc;
+  if ((rc = check_rows(n_tokens, n_heads + n_kv_heads))) return rc;
+  if (n_heads == 0 && n_kv_heads == 0) return fail(MER_ERR_INVALID_LAYOUT, "neither queries nor keys to norm");
+  if (n_tokens == 0) return MER_OK;
+  if (n_heads && ((rc = check_tensor("q", d_q, in_type, q_stride, n_heads * head_dim, n_tokens)) ||
+                  (rc = check_tensor("q output", d_q_out, out_type, q_out_stride, n_heads * head_dim, n_tokens))))
+    return rc;
+  if (n_kv_heads && ((rc = check_tensor("k", d_k, in_type, k_stride, n_kv_heads * head_dim, n_tokens)) ||
+                     (rc = check_tensor("k output", d_k_out, out_type, k_out_stride, n_kv_heads * head_dim, n_tokens))))
+    return rc;
+  if (rope && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
+  if ((rc = require_current_device())) return rc;
+  NormRopeParams p{};
+  p.t[0] = RopeTensor{d_q, d_q_out, d_q_norm, q_stride, q_out_stride, (uint32_t)n_heads};
+  p.t[1] = RopeTensor{d_k, d_k_out, d_k_norm, k_stride, k_out_stride, (uint32_t)n_kv_heads};
+  set_rope(&p, rope, d_positions, eps, n_tokens, head_dim);
+  const hipError_t e = launch_norm_rope(in_type, out_type, p, g_dev[g_device].cus, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "norm and rotation launch");
+  return MER_OK;
+}
+
+int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
+                      const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
+                      const mer_rope *rope, const float *d_k_norm, float eps, void *stream) {
+  int rc;
+  if ((rc = check_cache(cache)) || (rc = check_float_type(in_type, true)) || (rc = check_rope(rope, cache->head_dim)))
+    return rc;
+  if ((rc = check_rows(n_tokens, 2 * (size_t)cache->n_kv_heads))) return rc;
+  if (n_tokens == 0) return MER_OK;
+  const size_t row = (size_t)cache->n_kv_heads * cache->head_dim;
+  if ((rc = check_tensor("k", d_k, in_type, k_stride, row, n_tokens)) ||
+      (rc = check_tensor("v", d_v, in_type, v_stride, row, n_tokens)))
+    return rc;
+  if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
+  if (rope && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if ((uintptr_t)d_k_norm & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
+  if ((rc = require_current_device())) return rc;
+  NormRopeParams p{};
+  p.t[0] = RopeTensor{d_k, cache->k, d_k_norm, k_stride, 0, cache->n_kv_heads};
+  p.t[1] = RopeTensor{d_v, cache->v, nullptr, v_stride, 0, cache->n_kv_heads};
+  set_rope(&p, rope, d_positions, eps, n_tokens, cache->head_dim);
+  p.slots = d_slots;
+  p.n_slots = cache->n_pages * cache->page_size;
+  p.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
+  p.status = g_dev[g_device].status;
+  const hipError_t e = launch_kv_append(in_type, cache->type, p, g_dev[g_device].cus, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "cache append launch");
+  return MER_OK;
+}
+
+int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
+                            const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
+                            const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
+                            const mer_attention_options *options, void *d_out, size_t out_stride, void *stream) {
+  int rc;
+  if ((rc = check_cache(cache)) || (rc = check_rows(n_tokens, n_heads))) return rc;
+  if (n_heads == 0 || n_heads % cache->n_kv_heads != 0)
+    return fail(MER_ERR_INVALID_LAYOUT, "%zu heads are no multiple of %u kv heads", n_heads, cache->n_kv_heads);
+  if (n_seqs > (1u << 20)) return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "attention takes at most 1048576 sequences");
+  if (table_stride > (1u << 30) / cache->page_size)
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a block table row of %zu pages of %u keys exceeds 2^30 keys",
+                table_stride, cache->page_size);
+  if (n_seqs == 0 || n_tokens == 0) return MER_OK;
+  const size_t row = n_heads * cache->head_dim;
+  if ((rc = check_tensor("q", d_q, cache->type, q_stride, row, n_tokens)) ||
+      (rc = check_tensor("output", d_out, cache->type, out_stride, row, n_tokens)))
+    return rc;
+  if (!d_q_start || !d_kv_len || (!d_block_table && table_stride))
+    return fail(MER_ERR_INVALID_LAYOUT, "null sequence description");
+  float scale = options ? options->scale : 0.0f;
+  if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
+  if (!(fabsf(scale) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale is not finite");
+  if ((rc = require_current_device())) return rc;
+  AttnParams p{};
+  p.k = cache->k;
+  p.v = cache->v;
+  p.q = d_q;
+  p.out = d_out;
+  p.table = d_block_table;
+  p.q_start = d_q_start;
+  p.kv_len = d_kv_len;
+  p.q_stride = q_stride;
+  p.out_stride = out_stride;
+  p.table_stride = (uint32_t)table_stride;
+  p.n_seqs = (uint32_t)n_seqs;
+  p.n_tokens = (uint32_t)n_tokens;
+  p.n_pages = (uint32_t)cache->n_pages;
+  p.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
+  p.n_kv_heads = cache->n_kv_heads;
+  p.head_dim = cache->head_dim;
+  p.group = (uint32_t)(n_heads / cache->n_kv_heads);
+  if (options) {
+    p.window = options->window > (1u << 30) ? 0u : options->window;
+    p.sinks = options->sinks;
+  }
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  const size_t cap = table_stride * cache->page_size;
+  if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
+  if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
+  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, p.window,
+                                  g_dev[g_device].cus);
+  if ((uint64_t)plan.n_units * p.n_kv_heads * plan.n_chunks >= (1u << 24))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
+  p.n_units = plan.n_units;
+  p.by_seq = plan.by_seq;
+  p.chunk = plan.chunk;
+  p.n_chunks = plan.n_chunks;
+  p.status = g_dev[g_device].status;
+  const hipStream_t st = (hipStream_t)stream;
+  std::shared_ptr<Workspace> w = workspace_for(st);
+  if (!w) return require_init();
+  std::lock_guard<std::mutex> wl(w->mu);
+  if (w->released) return released_error();
+  if (plan.n_chunks > 1) {
+    rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, plan.part_o_floats + plan.part_ml_floats, size_t(1) << 20, false,
+                    "attention workspace");
+    if (rc) return rc;
+    p.part_o = w->attn_buf;
+    p.part_ml = w->attn_buf + plan.part_o_floats;
+  }
+  const hipError_t e = launch_attention(cache->type, plan, p, st);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "attention launch");
   return MER_OK;
 }
 

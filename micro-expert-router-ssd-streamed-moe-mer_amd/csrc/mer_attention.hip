@@ -1,0 +1,476 @@
+// mer_attention.hip -- attention of a chunk of new tokens over a paged cache.
+//
+// Row i of a sequence's n new tokens sits at position p = kv_len - n + i and
+// sees the keys j <= p (and j > p - window):
+//   o = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) [+ exp(sink - m)]),
+//   s_j = scale * q . k_j, m the running maximum.
+// One pass over the keys: each tile's scores raise m, the sums so far are
+// scaled by exp(m_old - m_new).
+//
+// The heads of a group share their kv head's keys, so a tile's rows are
+// (token, head in group) pairs: row r = token r / group, head r % group.
+//
+// Products run on MFMA with the keys as the rows of the first one: S^T = K Q^T
+// puts a q row into one lane column, so the softmax statistics are one value
+// per lane, and the lane's own scores are, in an order of keys that V^T's
+// operand repeats, what O^T = V^T P^T reads as its second operand: P never
+// leaves the registers.  P is rounded to the cache's type for that product
+// (half a step of a weight <= 1; its sum is kept from the f32 values).
+#include "mer_attention.hpp"
+
+namespace mer {
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+struct F16 {
+  typedef _Float16 T;
+  typedef h8 V8;
+  static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+struct BF16 {
+  typedef __bf16 T;
+  typedef b8 V8;
+  static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// What a lane reads for a key outside the tile's range: rows of zeros.
+__device__ u4 g_zero_row[kMaxHeadDim * 2 / 16];
+
+__device__ __forceinline__ uint32_t lane_id() { return __lane_id(); }
+__device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// A word of an argument array that the whole wave reads, by the scalar path.
+__device__ __forceinline__ int32_t sload(const int32_t *p, uint64_t i) {
+  return ((const __attribute__((address_space(4))) int32_t *)p)[i];
+}
+
+// Asynchronous copy of 16 bytes per lane to LDS at `lds` + 16 * lane.  The
+// compiler does not see it: wait_vm before the data is read.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void async_row16(const uint8_t *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// This wave's LDS reads are done: what they read may be overwritten.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Maximum / sum over the four lanes that hold a 16-row tile's row.
+__device__ __forceinline__ float max_quad(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_quad(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Sequence and row tile of unit u.  Sequence s owns the units from
+// q_start[s] * group / rows + s on: at least as many as it has row tiles,
+// whatever the lengths, so no prefix sum over the sequences is needed.
+// 64 candidates a step.
+template <int ROWS>
+__device__ __forceinline__ void find_unit(const AttnParams &p, uint32_t u, uint32_t *seq, uint32_t *tile) {
+  uint32_t lo = 0, hi = p.n_seqs;
+  auto base = [&](uint32_t s) {
+    const int32_t q = p.q_start[s];
+    return (uint64_t)(q < 0 ? 0 : q) * p.group / ROWS + s;
+  };
+  while (hi - lo > 1) {
+    const uint32_t step = (hi - lo + 63) / 64, s = lo + lane_id() * step;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(s < hi && base(s) <= u);
+    const uint32_t n = m ? (uint32_t)__popcll(m) : 1u;
+    lo += (n - 1) * step;
+    if (lo >= hi) lo = hi - 1;
+    hi = hi < lo + step ? hi : lo + step;
+  }
+  *seq = uni(lo);
+  const uint64_t b = base(lo);
+  *tile = uni(u >= b ? (uint32_t)(u - b) : 0xffffffffu);
+}
+
+// What one row tile of one sequence covers.
+struct Tile {
+  uint32_t row0;     // first (token, head) row of the tile in its sequence
+  uint32_t n_rows;   // rows of the sequence
+  uint32_t tok0;     // first token of the sequence in q / out
+  int32_t pos0;      // position of the sequence's first new token
+  int32_t lo, hi;    // keys that some row of the tile sees
+  int32_t start;     // lo rounded down to whole key tiles
+  uint32_t chunk, n_chunks;
+};
+
+// Key ranges stay clear of what the table cannot hold.
+template <int ROWS>
+__device__ __forceinline__ bool make_tile(const AttnParams &p, uint32_t seq, uint32_t tile, Tile *t) {
+  const int64_t b = sload(p.q_start, seq), e = sload(p.q_start, seq + 1);
+  const int64_t tok0 = b < 0 ? 0 : (b > p.n_tokens ? p.n_tokens : b);
+  const int64_t tok1 = e < tok0 ? tok0 : (e > p.n_tokens ? p.n_tokens : e);
+  const int64_t n = tok1 - tok0;
+  const int64_t rows = n * p.group, row0 = (int64_t)tile * ROWS;
+  if (row0 >= rows) return false;
+  const int64_t cap = (int64_t)p.table_stride << p.page_shift;
+  int64_t len = sload(p.kv_len, seq);
+  len = len < 0 ? 0 : (len > cap ? cap : len);
+  const int64_t last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
+  const int64_t pos0 = len - n;
+  int64_t hi = pos0 + last / p.group + 1;
+  hi = hi < 0 ? 0 : hi;
+  int64_t lo = p.window ? pos0 + row0 / p.group - (int64_t)p.window + 1 : 0;
+  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
+  t->row0 = (uint32_t)row0;
+  t->n_rows = (uint32_t)rows;
+  t->tok0 = (uint32_t)tok0;
+  t->pos0 = (int32_t)pos0;
+  t->lo = (int32_t)lo;
+  t->hi = (int32_t)hi;
+  t->start = (int32_t)lo & ~63;
+  const uint32_t keys = (uint32_t)(t->hi - t->start);
+  // A by_seq unit has partial sums for its first tile only: the tiles of a
+  // sequence longer than the plan says are done in one piece.
+  const uint32_t parts = p.by_seq && tile ? 1 : p.n_chunks;
+  uint32_t c = (keys + parts - 1) / parts;
+  c = (c + 63) & ~63u;
+  t->chunk = c < p.chunk ? p.chunk : c;
+  t->n_chunks = keys ? (keys + t->chunk - 1) / t->chunk : 1;
+  return true;
+}
+
+// Geometry of a head row in LDS: DP elements (head_dim rounded up), in 16-byte
+// pieces whose places are permuted by the row so that neither the row-wise
+// reads of K nor the transposed reads of V pile up on a bank.
+template <int DP>
+struct RowLayout {
+  static constexpr int kPieces = DP * 2 / 16;       // of a row
+  static constexpr int kRowsPerLoad = 64 / kPieces; // rows of one asynchronous copy
+  // K: 16 or 32 lanes read one piece of as many rows.
+  static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
+    return DP == 64 ? (row >> 1) & 7 : row & 15;
+  }
+  // V: a transposed read takes 32 bytes of each of four rows (x 4 groups).
+  static __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
+    return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+  }
+};
+
+// Copies `KEYS` keys from `key0` on (a multiple of 8) to LDS.  Lanes outside
+// [lo, hi), beyond the head dimension or on a page that the cache does not
+// have read zeros.
+template <int DP, int KEYS, bool V>
+__device__ __forceinline__ void load_keys(const AttnParams &p, const int32_t *table, uint32_t head, int32_t key0,
+                                          int32_t lo, int32_t hi, uint32_t lds) {
+  typedef RowLayout<DP> L;
+  const uint32_t lane = lane_id(), sub = lane / L::kPieces, piece = lane % L::kPieces;
+  const uint32_t row_bytes = p.head_dim * 2, mask = (1u << p.page_shift) - 1;
+  const uint8_t *base = (const uint8_t *)(V ? p.v : p.k);
+  const int32_t last_page = (hi - 1) >> p.page_shift, first_page = lo >> p.page_shift;
+#pragma unroll
+  for (int j = 0; j < KEYS / L::kRowsPerLoad; ++j) {
+    const int32_t k0 = key0 + j * L::kRowsPerLoad;
+    int32_t pg = k0 >> p.page_shift;
+    pg = pg > last_page ? last_page : (pg < first_page ? first_page : pg);
+    const int32_t id = sload(table, (uint32_t)pg);
+    const bool known = (uint32_t)id < p.n_pages;
+    const uint64_t at = (((uint64_t)(uint32_t)id * p.n_kv_heads + head) << p.page_shift) + ((uint32_t)k0 & mask);
+    const uint32_t row = (uint32_t)j * L::kRowsPerLoad + sub;
+    const uint32_t logical = piece ^ (V ? L::v_swizzle(row) : L::k_swizzle(row));
+    const int32_t key = k0 + (int32_t)sub;
+    const uint8_t *src = base + at * row_bytes + sub * row_bytes + logical * 16;
+    const bool in = known && key >= lo && key < hi && logical * 8 < p.head_dim;
+    async_row16(in ? src : (const uint8_t *)g_zero_row, lds + (uint32_t)j * 1024u);
+    if (!known && lane == 0 && k0 < hi && k0 + L::kRowsPerLoad > lo) atomicCAS(p.status, 0u, 16u /* residency miss */);
+  }
+}
+
+// Sixteen rows: decode and short chunks.  The waves of a workgroup take the
+// chunk's tiles of 32 keys in turn, each with a ring of LDS of its own (no
+// barriers while the keys stream), and join their sums at the end.
+constexpr int waves16(int dp) { return dp == 256 ? 2 : 4; }
+template <int DP>
+struct Rows16 {
+  static constexpr int kWaves = waves16(DP);
+  static constexpr int kKeys = 32;
+  static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
+  static constexpr int kStages = 2;
+  static constexpr int kLoads = kKeys / RowLayout<DP>::kRowsPerLoad;
+  static constexpr int kLds = kWaves * kStages * 2 * kTileBytes;
+};
+
+template <class E, int DP>
+__global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParams p) {
+  typedef Rows16<DP> C;
+  typedef RowLayout<DP> L;
+  typedef typename E::V8 V8;
+  typedef typename E::T T;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
+  const uint32_t head = blockIdx.x % p.n_kv_heads;
+  const uint32_t rest = blockIdx.x / p.n_kv_heads;
+  const uint32_t c = rest % p.n_chunks, unit = rest / p.n_chunks;
+  uint32_t seq = unit, tile = 0;
+  if (!p.by_seq) find_unit<16>(p, unit, &seq, &tile);
+  for (;; ++tile) {
+  Tile t;
+  if (!make_tile<16>(p, seq, tile, &t)) return;
+  const uint32_t col = lane % 16, quad = lane / 16;
+  if (c < t.n_chunks) {
+    // Q^T: lane column = row of the tile, 8 consecutive dims per 32-dim slab
+    const uint32_t row = t.row0 + col;
+    const bool row_ok = row < t.n_rows;
+    const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
+    const int32_t pos = t.pos0 + (int32_t)tok;
+    V8 q[DP / 32];
+    const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+      const uint32_t d = s * 32 + quad * 8;
+      q[s] = V8{};
+      if (row_ok && d < p.head_dim) q[s] = *(const V8 *)(qp + d);
+    }
+    const uint32_t last = t.row0 + 15 < t.n_rows ? t.row0 + 15 : t.n_rows - 1;
+    const int32_t pos_first = t.pos0 + (int32_t)(t.row0 / p.group), pos_last = t.pos0 + (int32_t)(last / p.group);
+
+    const int32_t begin = t.start + (int32_t)(c * t.chunk);
+    int32_t end = begin + (int32_t)t.chunk;
+    end = end < t.hi ? end : t.hi;
+    const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
+    const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
+    const int32_t *table = p.table + (uint64_t)seq * p.table_stride;
+    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem +
+                          wave * (C::kStages * 2 * C::kTileBytes);
+    auto key_of = [&](int32_t i) { return begin + (i * C::kWaves + (int32_t)wave) * C::kKeys; };
+    auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
+    __syncthreads();  // the last tile's join is done with the LDS
+    for (int32_t i = 0; i < C::kStages && i < mine; ++i) {
+      load_keys<DP, C::kKeys, false>(p, table, head, key_of(i), t.lo, t.hi, slot_of(i));
+      load_keys<DP, C::kKeys, true>(p, table, head, key_of(i), t.lo, t.hi, slot_of(i) + C::kTileBytes);
+    }
+
+    float m = -__builtin_inff(), l = 0.0f;
+    f4 o[DP / 16];
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[d] = f4{0, 0, 0, 0};
+    for (int32_t i = 0; i < mine; ++i) {
+      const int32_t left = mine - i;
+      const int32_t key0 = key_of(i);
+      const uint32_t kb = slot_of(i), vb = kb + C::kTileBytes;
+      if (left == 1) wait_vm<C::kLoads>();
+      else wait_vm<3 * C::kLoads>();
+      f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const uint32_t r = b * 16 + col, piece = (d * 4 + quad) ^ L::k_swizzle(r);
+          const V8 k = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
+          s[b] = E::mfma16(k, q[d], s[b]);
+        }
+      wait_lds();
+      if (left > C::kStages) load_keys<DP, C::kKeys, false>(p, table, head, key_of(i + 2), t.lo, t.hi, kb);
+      // scores in base 2; keys of lane: b * 16 + quad * 4 + e
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s[e / 4][e % 4] * p.scale_log2;
+      const int32_t key_end = key0 + C::kKeys;
+      if (key_end > pos_first + 1 || key_end > t.hi || (p.window && key0 <= pos_last - (int32_t)p.window)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int32_t key = key0 + (e / 4) * 16 + (int32_t)quad * 4 + e % 4;
+          if (key > pos || (p.window && key <= pos - (int64_t)p.window)) x[e] = -__builtin_inff();
+        }
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      mx = fmaxf(max_quad(mx), m);
+      const float mu = mx == -__builtin_inff() ? 0.0f : mx;
+      const float a = __builtin_amdgcn_exp2f(m - mu);
+      f8 e8;
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        e8[e] = __builtin_amdgcn_exp2f(x[e] - mu);
+        sum += e8[e];
+      }
+      l = l * a + sum;
+      if (__builtin_amdgcn_ballot_w64(mx != m)) {
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) o[d] *= a;
+      }
+      m = mx;
+      const V8 pr = __builtin_convertvector(e8, V8);
+      if (left == 1) wait_vm<0>();
+      else if (left == 2) wait_vm<2 * C::kLoads>();
+      else wait_vm<3 * C::kLoads>();
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        s4 v[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t r = b * 16 + quad * 4 + col / 4;
+          const uint32_t piece = (d * 2 + (col % 4) / 2) ^ L::v_swizzle(r);
+          v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + (col % 2) * 8));
+        }
+        const s8 vv = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = E::mfma16(__builtin_bit_cast(V8, vv), pr, o[d]);
+      }
+      wait_lds();
+      if (left > C::kStages) load_keys<DP, C::kKeys, true>(p, table, head, key_of(i + 2), t.lo, t.hi, vb);
+    }
+    l = sum_quad(l);
+    // join the waves: m, l and O of each in LDS
+    __syncthreads();
+    float *jo = (float *)smem;                         // [wave][16][DP]
+    float *jm = jo + C::kWaves * 16 * DP;              // [wave][16][2]
+    if (quad == 0) {
+      jm[(wave * 16 + col) * 2] = m;
+      jm[(wave * 16 + col) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[(wave * 16 + col) * DP + d * 16 + quad * 4] = o[d];
+    __syncthreads();
+    for (uint32_t w = tid; w < 16 * (DP / 8); w += 64 * C::kWaves) {
+      const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, gr = t.row0 + r;
+      if (gr >= t.n_rows || d >= p.head_dim) continue;
+      float mm = -__builtin_inff();
+#pragma unroll
+      for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * 16 + r) * 2]);
+      float ls = 0.0f;
+      f8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int v = 0; v < C::kWaves; ++v) {
+        const float mv = jm[(v * 16 + r) * 2];
+        const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
+        ls += a * jm[(v * 16 + r) * 2 + 1];
+        acc += a * *(const f8 *)&jo[(v * 16 + r) * DP + d];
+      }
+      const uint32_t tk = gr / p.group, hq = head * p.group + gr % p.group;
+      if (t.n_chunks == 1) {
+        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - (mm == -__builtin_inff() ? 0.0f : mm));
+        const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
+        const V8 r8 = __builtin_convertvector(acc * inv, V8);
+        *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
+      } else {
+        const uint64_t at = ((uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c) * 16 + r;
+        *(f8 *)(p.part_o + at * p.head_dim + d) = acc;
+        if (d == 0) *(f2 *)(p.part_ml + at * 2) = f2{mm, ls};
+      }
+    }
+  }
+  if (!p.by_seq) return;
+  }
+}
+
+// Joins the chunks of a row: one workgroup of 256 threads per row, 32 lanes x
+// head_dim / 32 dims by 8 groups of chunks.
+template <class E, int ROWS>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+  typedef typename E::T T;
+  const uint32_t r = blockIdx.x % ROWS, uh = blockIdx.x / ROWS;
+  const uint32_t head = uh % p.n_kv_heads, unit = uh / p.n_kv_heads;
+  uint32_t seq = unit, tile = 0;
+  if (!p.by_seq) find_unit<ROWS>(p, unit, &seq, &tile);
+  Tile t;
+  if (!make_tile<ROWS>(p, seq, tile, &t) || t.n_chunks == 1 || t.row0 + r >= t.n_rows) return;
+  const uint64_t at = ((uint64_t)uh * p.n_chunks) * ROWS + r;
+  __shared__ float so[8][kMaxHeadDim];
+  __shared__ float sl[8];
+  const uint32_t tid = threadIdx.x, g = tid / 32, ln = tid % 32;
+  float mm = -__builtin_inff();
+  for (uint32_t c = ln; c < t.n_chunks; c += 32) mm = fmaxf(mm, p.part_ml[(at + (uint64_t)c * ROWS) * 2]);
+  for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+  const float mu = mm == -__builtin_inff() ? 0.0f : mm;
+  float ls = 0.0f, acc[kMaxHeadDim / 32] = {};
+  for (uint32_t c = g; c < t.n_chunks; c += 8) {
+    const uint64_t i = at + (uint64_t)c * ROWS;
+    const float a = __builtin_amdgcn_exp2f(p.part_ml[i * 2] - mu);
+    ls += a * p.part_ml[i * 2 + 1];
+    for (uint32_t k = 0; k < kMaxHeadDim / 32; ++k)
+      if (k * 32 + ln < p.head_dim) acc[k] += a * p.part_o[i * p.head_dim + k * 32 + ln];
+  }
+  for (uint32_t k = 0; k < kMaxHeadDim / 32; ++k) so[g][k * 32 + ln] = acc[k];
+  if (ln == 0) sl[g] = ls;
+  __syncthreads();
+  if (tid < p.head_dim) {
+    const uint32_t gr = t.row0 + r, tk = gr / p.group, hq = head * p.group + gr % p.group;
+    float o = 0.0f;
+    ls = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      o += so[i][tid];
+      ls += sl[i];
+    }
+    if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - mu);
+    o = ls > 0.0f || ls != ls ? o / ls : 0.0f;
+    ((T *)p.out)[(uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + tid] = (T)o;
+  }
+}
+
+template <class E, int DP>
+hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  typedef Rows16<DP> C;
+  const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
+  hipError_t e = hipFuncSetAttribute((const void *)attn_rows16_kernel<E, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  if (e != hipSuccess) return e;
+  attn_rows16_kernel<E, DP><<<grid, 64 * C::kWaves, C::kLds, st>>>(p);
+  if (plan.n_chunks > 1) attn_join_kernel<E, 16><<<plan.n_units * p.n_kv_heads * 16, 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+template <class E>
+hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  if (p.head_dim <= 64) return launch16<E, 64>(plan, p, st);
+  if (p.head_dim <= 128) return launch16<E, 128>(plan, p, st);
+  return launch16<E, 256>(plan, p, st);
+}
+
+}  // namespace
+
+AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                   size_t max_q_len, size_t max_kv_len, uint32_t window, int cus) {
+  AttnPlan a{};
+  a.rows = 16;
+  a.by_seq = max_q_len * group <= a.rows;
+  // keys of a row tile, from a whole key tile's start on
+  size_t max_keys = max_kv_len;
+  const size_t reach = (size_t)window + (a.rows + group - 1) / group + 64;
+  if (window && reach < max_keys) max_keys = reach;
+  a.n_units = (uint32_t)(a.by_seq ? n_seqs : (n_tokens * group + a.rows - 1) / a.rows + n_seqs);
+  // Workgroups enough to fill the chip twice, chunks of 256 keys or more.
+  const size_t base = (size_t)a.n_units * n_kv_heads, want = 2 * (size_t)cus;
+  size_t chunks = base >= want ? 1 : (want + base - 1) / base;
+  const size_t most = (max_keys + 255) / 256;
+  chunks = chunks > most ? most : chunks;
+  chunks = chunks ? chunks : 1;
+  a.chunk = (uint32_t)(((max_keys + chunks - 1) / chunks + 63) / 64 * 64);
+  a.chunk = a.chunk ? a.chunk : 64;
+  a.n_chunks = (uint32_t)chunks;
+  if (a.n_chunks > 1) {
+    const size_t rows = (size_t)a.n_units * n_kv_heads * a.n_chunks * a.rows;
+    a.part_o_floats = rows * head_dim;
+    a.part_ml_floats = rows * 2;
+  }
+  return a;
+}
+
+hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  return type == kF16 ? launch_typed<F16>(plan, p, st) : launch_typed<BF16>(plan, p, st);
+}
+
+}  // namespace mer

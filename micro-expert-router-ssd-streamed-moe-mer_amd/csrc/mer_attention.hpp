@@ -1,0 +1,74 @@
+// mer_attention.hpp -- arguments of the attention-side kernels (q/k norm and
+// rotation, paged append, paged attention) and their launchers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace mer {
+
+// Element types, by their UTH dtype ids.
+enum FloatType : int { kF32 = 0, kF16 = 1, kBF16 = 6 };
+
+constexpr uint32_t kMaxHeadDim = 256;
+
+// One of q / k / v on its way through norm and rotation.
+struct RopeTensor {
+  const void *in;    // [n_tokens] rows of `heads` heads, in_stride elements apart
+  void *out;         // the same, out_stride elements apart (norm_rope)
+  const float *norm; // [head_dim] weights, or null
+  uint64_t in_stride, out_stride;
+  uint32_t heads;
+};
+
+struct NormRopeParams {
+  RopeTensor t[2];           // q and k
+  const int32_t *positions;  // [n_tokens], or null without rotation
+  const float *inv_freq;     // [rot / 2]
+  uint32_t n_tokens, head_dim, rot, interleaved;
+  float eps;
+  // append: where the rows go
+  const int64_t *slots;      // [n_tokens]; negative = no row
+  uint64_t n_slots;          // n_pages * page_size
+  uint32_t page_shift;
+  uint32_t heads_per_wave;   // consecutive heads that one wave walks
+  uint32_t *status;
+};
+
+hipError_t launch_norm_rope(int in_type, int out_type, const NormRopeParams &p, int cus, hipStream_t st);
+hipError_t launch_kv_append(int in_type, int cache_type, const NormRopeParams &p, int cus, hipStream_t st);
+
+struct AttnParams {
+  const void *k, *v;         // [n_pages][n_kv_heads][page_size][head_dim]
+  const void *q;
+  void *out;
+  const int32_t *table;      // [n_seqs][table_stride]
+  const int32_t *q_start;    // [n_seqs + 1]
+  const int32_t *kv_len;     // [n_seqs]
+  const float *sinks;        // [n_heads], or null
+  uint64_t q_stride, out_stride;
+  uint32_t table_stride, n_seqs, n_tokens;
+  uint32_t n_pages, page_shift, n_kv_heads, head_dim, group;
+  uint32_t window;           // 0 = none
+  float scale_log2;          // scale * log2(e)
+  // decomposition (attn_plan)
+  uint32_t n_units;          // row tiles of a kv head (an upper bound)
+  uint32_t by_seq;           // unit = sequence: every sequence has at most one row tile
+  uint32_t chunk, n_chunks;  // keys of one workgroup, workgroups of one row tile
+  float *part_o;             // [n_units][n_kv_heads][n_chunks][rows][head_dim]
+  float *part_ml;            // [n_units][n_kv_heads][n_chunks][rows][2]
+  uint32_t *status;
+};
+
+struct AttnPlan {
+  uint32_t rows;             // rows of a tile
+  uint32_t n_units, by_seq, chunk, n_chunks;
+  size_t part_o_floats, part_ml_floats;
+};
+
+AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                   size_t max_q_len, size_t max_kv_len, uint32_t window, int cus);
+hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
+
+}  // namespace mer

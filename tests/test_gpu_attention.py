@@ -1,0 +1,389 @@
+"""Norm and rotation of q and k, append to a paged cache, attention over it:
+each against its formula in 64 bits on the CPU.
+
+Tolerances count roundings (half a step of a type t relative to a value is
+finfo(t).eps / 2 = h):
+  - norm and rotation compute in f32 and round once to the output type.  A
+    norm's factor and two products are within 16 f32 half steps of the exact
+    ones (a sum of head_dim / 8 + 3 terms deep <= 35 additions of positive
+    terms enters through a square root: 18 half steps; division, root and
+    three products: 6 more), a turned element adds an angle error of 2^-24 of
+    a turn (2 pi 2^-24 rad) and the sine's own few half steps, relative to the
+    pair's length.  48 f32 half steps of the pair's length cover both:
+    |got - want| <= h_out |want| + 48 h_f32 |pair|.
+  - attention rounds P to the cache's type (h each), so the output is off by
+    at most h sum_j p_j |v_j| / sum_j p_j, and the scores' f32 error
+    (head_dim products of exact 16-bit factors: <= (head_dim / 16 + 8) half
+    steps of sum |q_d k_d| scale, entering the exponent) moves each weight
+    by that much, relatively; twice that with the sum below the fraction; then
+    one rounding of the output.
+"""
+from __future__ import annotations
+
+import itertools
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+# ---- formulas in 64 bits -------------------------------------------------
+
+def norm_rope64(x, w, positions, inv_freq, eps, interleaved):
+    """(result, length of each element's pair) of x [t, h, d]."""
+    y = x.to(torch.float64)
+    if w is not None:
+        y = y / (y.pow(2).mean(2, keepdim=True) + eps).sqrt() * w.to(torch.float64)
+    size = y.abs()
+    if inv_freq is None:
+        return y, size
+    out, half = y.clone(), inv_freq.numel()
+    a = positions.to(torch.float64)[:, None] * inv_freq.to(torch.float64)
+    c, s = a.cos()[:, None], a.sin()[:, None]
+    i = torch.arange(half)
+    u, v = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+    out[..., u] = y[..., u] * c - y[..., v] * s
+    out[..., v] = y[..., v] * c + y[..., u] * s
+    size[..., u] = size[..., v] = (y[..., u] ** 2 + y[..., v] ** 2).sqrt()
+    return out, size
+
+
+def close_rope(got, want, size):
+    bound = HALF[got.dtype] * want.abs() + 48 * HALF[F32] * size + 1e-30
+    if got.dtype == F16:
+        bound = bound + 2.0 ** -25  # half a step of its subnormals
+    err = (got.cpu().to(torch.float64) - want).abs()
+    worst = (err / bound).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f"{worst} of the bound"
+
+
+def attention64(q, k, v, first, window, sinks, scale, h):
+    """One sequence: q [n, H, d], k and v [L, G, d] in float64; row i stands at
+    first + i.  Returns (out, bound) with the rounding bound above."""
+    n, heads, d = q.shape
+    keys, groups, _ = k.shape
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    j, p = torch.arange(keys), first + torch.arange(n)[:, None]
+    seen = j <= p
+    if window:
+        seen &= j > p - window
+    for hd in range(heads):
+        g = hd // (heads // groups)
+        kk, vv, qq = k[:, g], v[:, g], q[:, hd]
+        s = torch.where(seen, qq @ kk.T * scale, -math.inf)
+        size = torch.where(seen, qq.abs() @ kk.abs().T * abs(scale), 0.0)
+        m = s.amax(1, keepdim=True) if keys else torch.full((n, 1), -math.inf, dtype=torch.float64)
+        if sinks is not None:
+            m = m.clamp(min=float(sinks[hd]))
+        m = torch.where(m == -math.inf, 0.0, m)
+        e = torch.exp(s - m)
+        z = e.sum(1, keepdim=True)
+        if sinks is not None:
+            z = z + torch.exp(float(sinks[hd]) - m)
+        ok = z > 0
+        z = torch.where(ok, z, 1.0)
+        out[:, hd] = e @ vv / z
+        weight = h + 2 * (d / 16 + 8) * HALF[F32] * size + 64 * HALF[F32]
+        bound[:, hd] = (e * weight) @ vv.abs() / z
+    return out, bound + h * out.abs()
+
+
+# ---- q / k norm and rotation ---------------------------------------------
+
+def inv_freq(rot, base=1e6):
+    return (base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)).to(F32)
+
+
+@pytest.mark.parametrize("src,dst", list(itertools.product([F32, F16, BF16], [F32, F16, BF16])))
+@pytest.mark.parametrize("tokens,heads,kv,d,rot,interleaved,normed", [
+    (1, 32, 4, 128, 128, False, True),
+    (5, 7, 3, 64, 64, True, True),
+    (37, 3, 1, 80, 40, False, False),
+    (130, 12, 2, 96, 8, True, False),
+    (67, 5, 5, 256, 256, False, True),
+    (33, 1, 1, 8, 8, False, True),
+    (9, 4, 2, 72, 72, False, True),
+    (300, 16, 2, 192, 64, True, True),
+])
+def test_norm_rope(mer, gpu, src, dst, tokens, heads, kv, d, rot, interleaved, normed):
+    g = torch.Generator().manual_seed(tokens * d + heads)
+    row = torch.randn(tokens, (heads + 2 * kv) * d, generator=g).to(src)
+    q, k = row[:, :heads * d].view(tokens, heads, d), row[:, heads * d:(heads + kv) * d].view(tokens, kv, d)
+    pos = torch.randint(0, 1 << 20, (tokens,), generator=g, dtype=torch.int32)
+    pos[0] = 0
+    f = inv_freq(rot)
+    qn = 1 + 0.1 * torch.randn(d, generator=g) if normed else None
+    kn = 1 + 0.1 * torch.randn(d, generator=g) if normed else None
+    dev = row.to(gpu)
+    up = lambda t: None if t is None else t.to(gpu)
+    qo, ko = mer.qk_norm_rope(dev[:, :heads * d].view(tokens, heads, d),
+                              dev[:, heads * d:(heads + kv) * d].view(tokens, kv, d), up(pos), up(f), q_norm=up(qn),
+                              k_norm=up(kn), eps=1e-5, interleaved=interleaved, out_dtype=dst)
+    for got, x, w in ((qo, q, qn), (ko, k, kn)):
+        assert got.dtype == dst and got.shape == x.shape
+        close_rope(got, *norm_rope64(x, w, pos, f, 1e-5, interleaved))
+
+
+def test_norm_rope_parts(mer, gpu):
+    """Only queries; only one norm; no rotation; negative and far positions; no tokens."""
+    g = torch.Generator().manual_seed(1)
+    q, k = torch.randn(11, 4, 64, generator=g), torch.randn(11, 2, 64, generator=g)
+    w = 1 + 0.1 * torch.randn(64, generator=g)
+    f = inv_freq(64)
+    pos = torch.tensor([0, 1, -1, -77, 2 ** 31 - 1, -2 ** 31, 5, 6, 7, 8, 123456789], dtype=torch.int32)
+    d = lambda t: t.to(gpu)
+    qo, none = mer.qk_norm_rope(d(q), None, d(pos), d(f), q_norm=d(w))
+    assert none is None
+    close_rope(qo, *norm_rope64(q, w, pos, f, 1e-6, False))
+    qo, ko = mer.qk_norm_rope(d(q), d(k), d(pos), d(f), k_norm=d(w), interleaved=True)
+    close_rope(qo, *norm_rope64(q, None, pos, f, 1e-6, True))
+    close_rope(ko, *norm_rope64(k, w, pos, f, 1e-6, True))
+    qo, ko = mer.qk_norm_rope(d(q), d(k), None, None, q_norm=d(w), k_norm=d(w))
+    close_rope(qo, *norm_rope64(q, w, None, None, 1e-6, False))
+    close_rope(ko, *norm_rope64(k, w, None, None, 1e-6, False))
+    qo, ko = mer.qk_norm_rope(d(q)[:0], d(k)[:0], d(pos)[:0], d(f))
+    assert qo.shape == (0, 4, 64) and ko.shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_norm_rope_in_place(mer, gpu, dt):
+    """q and k turned where they lie in a packed q|k|v row; v and the gap after it stay."""
+    g = torch.Generator().manual_seed(2)
+    t, h, kv, d = 50, 6, 2, 128
+    row = torch.randn(t, (h + 2 * kv) * d + 16, generator=g).to(dt)
+    dev = row.to(gpu)
+    q, k = dev[:, :h * d].unflatten(1, (h, d)), dev[:, h * d:(h + kv) * d].unflatten(1, (kv, d))
+    pos, f = torch.arange(1000, 1000 + t, dtype=torch.int32), inv_freq(d)
+    w = 1 + 0.1 * torch.randn(d, generator=g)
+    mer.qk_norm_rope(q, k, pos.to(gpu), f.to(gpu), q_norm=w.to(gpu), k_norm=w.to(gpu), q_out=q, k_out=k)
+    got = dev.cpu()
+    assert torch.equal(got[:, (h + kv) * d:], row[:, (h + kv) * d:])
+    close_rope(got[:, :h * d].unflatten(1, (h, d)), *norm_rope64(row[:, :h * d].unflatten(1, (h, d)), w, pos, f, 1e-6, False))
+    close_rope(got[:, h * d:(h + kv) * d].unflatten(1, (kv, d)),
+               *norm_rope64(row[:, h * d:(h + kv) * d].unflatten(1, (kv, d)), w, pos, f, 1e-6, False))
+
+
+# ---- append --------------------------------------------------------------
+
+@pytest.mark.parametrize("src,dst", list(itertools.product([F32, F16, BF16], [F16, BF16])))
+@pytest.mark.parametrize("tokens,kv,d,page,rot,normed", [
+    (1, 8, 128, 16, 128, False), (45, 3, 64, 8, 64, True), (129, 2, 112, 32, 0, False), (70, 1, 256, 256, 128, True),
+])
+def test_append(mer, gpu, src, dst, tokens, kv, d, page, rot, normed):
+    g = torch.Generator().manual_seed(tokens + d)
+    k = torch.randn(tokens, kv, d, generator=g).to(src)
+    v = torch.randn(tokens, kv, d, generator=g).to(src)
+    pages = -(-tokens // page) + 2
+    slots = torch.randperm(pages * page, generator=g)[:tokens]
+    if tokens > 1:
+        slots[::7] = -1
+    ck = torch.full((pages, kv, page, d), 3.5, dtype=dst)
+    cv = torch.full((pages, kv, page, d), -2.5, dtype=dst)
+    pos = torch.randint(0, 100000, (tokens,), generator=g, dtype=torch.int32)
+    f = inv_freq(rot) if rot else None
+    w = 1 + 0.1 * torch.randn(d, generator=g) if normed else None
+    up = lambda t: None if t is None else t.to(gpu)
+    cache = mer.PagedKvCache.wrap(ck.to(gpu), cv.to(gpu))
+    mer.kv_append(cache, up(k), up(v), up(slots), positions=up(pos) if rot else None, inv_freq=up(f), k_norm=up(w))
+    want, size = norm_rope64(k, w, pos, f, 1e-6, False)
+    gk, gv = cache.k.cpu(), cache.v.cpu()
+    written = torch.zeros(pages, page, dtype=torch.bool)
+    for t in range(tokens):
+        if slots[t] < 0:
+            continue
+        pg, at = int(slots[t]) // page, int(slots[t]) % page
+        written[pg, at] = True
+        close_rope(gk[pg, :, at], want[t], size[t])
+        assert torch.equal(gv[pg, :, at], v[t].to(dst))
+    assert (gk.transpose(1, 2)[~written] == 3.5).all() and (gv.transpose(1, 2)[~written] == -2.5).all()
+
+
+def test_append_past_the_cache(mer, gpu):
+    mer.take_device_status()
+    cache = mer.PagedKvCache.wrap(torch.zeros(2, 1, 8, 16, dtype=F16, device=gpu),
+                                  torch.zeros(2, 1, 8, 16, dtype=F16, device=gpu))
+    k = torch.ones(3, 1, 16, dtype=F16, device=gpu)
+    mer.kv_append(cache, k, k, torch.tensor([3, 16, 1 << 40], device=gpu))
+    with pytest.raises(mer.GpuExpertDispatchError):
+        mer.take_device_status()
+    assert cache.k.sum().item() == 16 and cache.v.sum().item() == 16
+
+
+# ---- attention -----------------------------------------------------------
+
+class Batch:
+    """Sequences of (new tokens, keys) with pages in random order, NaN in every
+    place that no sequence has written, page ids of -1 behind each row's pages."""
+
+    def __init__(self, seqs, heads, kv, d, page, dt, seed, spare=3, gap=0, kscale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.seqs, self.page, self.dt = seqs, page, dt
+        need = [-(-max(l, 0) // page) for _, l in seqs]
+        width = max(need + [1]) + 1
+        total = sum(need) + spare
+        order = torch.randperm(total, generator=g).to(torch.int32)
+        self.table = torch.full((len(seqs), width), -1, dtype=torch.int32)
+        self.k = torch.full((total, kv, page, d), math.nan, dtype=dt)
+        self.v = torch.full((total, kv, page, d), math.nan, dtype=dt)
+        self.kk, self.vv, self.start = [], [], [0]
+        at = 0
+        for i, (n, l) in enumerate(seqs):
+            ids = order[at:at + need[i]]
+            at += need[i]
+            self.table[i, :need[i]] = ids
+            kk = (kscale * torch.randn(max(l, 0), kv, d, generator=g)).to(dt)
+            vv = torch.randn(max(l, 0), kv, d, generator=g).to(dt)
+            for j in range(need[i]):
+                part = slice(j * page, min((j + 1) * page, l))
+                m = part.stop - part.start
+                self.k[ids[j], :, :m] = kk[part].transpose(0, 1)
+                self.v[ids[j], :, :m] = vv[part].transpose(0, 1)
+            self.kk.append(kk)
+            self.vv.append(vv)
+            self.start.append(self.start[-1] + n)
+        self.n = self.start[-1] + gap
+        self.q = torch.randn(self.n, heads, d, generator=g).to(dt)
+
+    def run(self, mer, gpu, hints=True, **kw):
+        cache = mer.PagedKvCache.wrap(self.k.to(gpu), self.v.to(gpu))
+        out = torch.full_like(self.q, 7.0, device=gpu)
+        more = dict(max_q_len=max(n for n, _ in self.seqs), max_kv_len=max(l for _, l in self.seqs)) if hints else {}
+        more.update(kw)
+        if more.get("sinks") is not None:
+            more["sinks"] = more["sinks"].to(gpu)
+        return mer.paged_attention(cache, self.q.to(gpu), self.table.to(gpu),
+                                   torch.tensor(self.start, dtype=torch.int32, device=gpu),
+                                   torch.tensor([l for _, l in self.seqs], dtype=torch.int32, device=gpu), out=out,
+                                   **more).cpu()
+
+    def check(self, got, window=0, sinks=None, scale=None):
+        scale = self.q.shape[2] ** -0.5 if scale is None else scale
+        worst = 0.0
+        for i, (n, l) in enumerate(self.seqs):
+            rows = slice(self.start[i], self.start[i + 1])
+            if n == 0:
+                continue
+            want, bound = attention64(self.q[rows].double(), self.kk[i].double(), self.vv[i].double(), l - n, window,
+                                      sinks, scale, HALF[self.dt])
+            bound = bound + (2.0 ** -24 if self.dt == F16 else 1e-30)
+            err = (got[rows].double() - want).abs()
+            assert not err.isnan().any(), f"sequence {i}"
+            worst = max(worst, (err / bound).max().item())
+        assert worst <= 1.0, f"{worst} of the bound"
+        assert (got[self.start[-1]:] == 7.0).all()  # rows of no sequence
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 256, 8, 80, 96, 112, 192])
+@pytest.mark.parametrize("seqs,heads,kv,page", [
+    ([(1, 1)], 4, 4, 16),
+    ([(1, 700)], 32, 4, 16),
+    ([(1, 31), (1, 32), (1, 33), (1, 257), (1, 1)], 8, 2, 32),
+    ([(5, 5), (33, 70), (1, 129), (16, 16)], 6, 2, 8),
+    ([(130, 301)], 7, 1, 64),
+])
+def test_attention(mer, gpu, dt, d, seqs, heads, kv, page):
+    b = Batch(seqs, heads, kv, d, page, dt, seed=d + heads, gap=2)
+    b.check(b.run(mer, gpu))
+
+
+@pytest.mark.parametrize("seqs,heads,kv,d,page", [
+    ([(1, 9000), (1, 100), (1, 4097)], 8, 1, 64, 16),
+    ([(1, 40000)], 16, 1, 128, 128),
+    ([(300, 5000)], 4, 2, 128, 64),
+    ([(700, 700)], 5, 1, 64, 16),
+    ([(64, 3000), (257, 900), (1, 2500), (1, 3), (40, 40)], 16, 2, 128, 32),
+    ([(20, 2600)], 12, 1, 256, 256),
+])
+@pytest.mark.parametrize("window,sink", [(0, False), (100, False), (1, True), (1000, True)])
+def test_attention_long(mer, gpu, seqs, heads, kv, d, page, window, sink):
+    b = Batch(seqs, heads, kv, d, page, BF16, seed=len(seqs) + window)
+    sinks = torch.linspace(-4, 6, heads) if sink else None
+    b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("hints", [dict(max_q_len=1, max_kv_len=1), dict(max_q_len=10 ** 6, max_kv_len=10 ** 6),
+                                   dict(max_q_len=3, max_kv_len=300), {}])
+def test_attention_hints_do_not_matter(mer, gpu, hints):
+    b = Batch([(1, 1500), (37, 400), (3, 2000), (200, 1100)], 8, 2, 64, 16, F16, seed=5)
+    b.check(b.run(mer, gpu, hints=False, **hints))
+
+
+def test_attention_rows_that_see_nothing(mer, gpu):
+    """Sequences without keys, with fewer keys than new tokens, without rows."""
+    b = Batch([(3, 0), (20, 7), (0, 50), (0, 0), (1, 0), (2, 2)], 4, 2, 64, 8, F16, seed=6, gap=3)
+    for sinks in (None, torch.tensor([0.0, -50.0, 50.0, 1.0])):
+        got = b.run(mer, gpu, sinks=sinks)
+        b.check(got, sinks=sinks)
+        assert (got[:3] == 0).all() and (got[3:3 + 13] == 0).all()
+
+
+def test_attention_scores_far_apart(mer, gpu):
+    """Scores of hundreds either way: the running maximum jumps from tile to tile."""
+    for scale in (3.0, -3.0):
+        b = Batch([(1, 3000), (40, 999)], 4, 1, 64, 16, F16, seed=7, kscale=4.0)
+        b.check(b.run(mer, gpu, scale=scale), scale=scale)
+
+
+def test_attention_pages_before_the_window_are_not_read(mer, gpu):
+    b = Batch([(1, 1000), (30, 800)], 8, 2, 128, 16, BF16, seed=8)
+    for i, (n, l) in enumerate(b.seqs):
+        b.table[i, :(l - n - 99) // 16] = -1 if i else 10 ** 6
+    mer.take_device_status()
+    b.check(b.run(mer, gpu, window=100), window=100)
+    mer.take_device_status()
+
+
+def test_attention_page_outside_the_cache(mer, gpu):
+    """Reads as zeros, is recorded, and leaves other sequences alone."""
+    b = Batch([(1, 100), (1, 90)], 2, 1, 64, 16, F16, seed=9)
+    b.table[0, 2] = b.k.shape[0]
+    b.kk[0][32:48] = 0
+    b.vv[0][32:48] = 0
+    mer.take_device_status()
+    got = b.run(mer, gpu)
+    with pytest.raises(mer.GpuExpertDispatchError):
+        mer.take_device_status()
+    b.check(got)
+
+
+def test_attention_strided_and_other_stream(mer, gpu):
+    b = Batch([(9, 200), (1, 64)], 4, 2, 64, 16, BF16, seed=10)
+    wide = torch.zeros(b.n, 8, 64, dtype=BF16, device=gpu)
+    wide[:, 2:6] = b.q.to(gpu)
+    out = torch.full((b.n, 6, 64), 7.0, dtype=BF16, device=gpu)
+    args = [b.table.to(gpu), torch.tensor(b.start, dtype=torch.int32, device=gpu),
+            torch.tensor([l for _, l in b.seqs], dtype=torch.int32, device=gpu)]
+    cache = mer.PagedKvCache.wrap(b.k.to(gpu), b.v.to(gpu))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mer.paged_attention(cache, wide[:, 2:6], *args, out=out[:, 1:5])
+    side.synchronize()
+    assert (out[:, 0] == 7).all() and (out[:, 5] == 7).all()
+    b.check(out[:, 1:5].cpu())
+
+
+def test_attention_of_a_cache_past_4_gib(mer, gpu):
+    """The last pages of a cache whose offsets do not fit 32 bits."""
+    pages, kv, page, d = 20000, 8, 128, 128  # 5 GiB each of k and v
+    cache = mer.PagedKvCache.wrap(torch.zeros(pages, kv, page, d, dtype=F16, device=gpu),
+                                  torch.zeros(pages, kv, page, d, dtype=F16, device=gpu))
+    g = torch.Generator().manual_seed(11)
+    n = 300
+    k, v = torch.randn(n, kv, d, generator=g).to(F16), torch.randn(n, kv, d, generator=g).to(F16)
+    ids = torch.tensor([pages - 1, pages // 2 + 7, pages - 3], dtype=torch.int32)
+    slots = (ids.to(torch.int64)[:, None] * page + torch.arange(page)).view(-1)[:n]
+    mer.kv_append(cache, k.to(gpu), v.to(gpu), slots.to(gpu))
+    q = torch.randn(2, 16, d, generator=g).to(F16)
+    got = mer.paged_attention(cache, q.to(gpu), ids[None].to(gpu), torch.tensor([0, 2], dtype=torch.int32, device=gpu),
+                              torch.tensor([n], dtype=torch.int32, device=gpu))
+    want, bound = attention64(q.double(), k.double(), v.double(), n - 2, 0, None, d ** -0.5, HALF[F16])
+    assert ((got.cpu().double() - want).abs() <= bound + 2.0 ** -24).all()
+    del cache
+    torch.cuda.empty_cache()
