@@ -28,6 +28,7 @@ typedef short s8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct F16 {
@@ -36,12 +37,18 @@ struct F16 {
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
 };
 struct BF16 {
   typedef __bf16 T;
   typedef b8 V8;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -63,10 +70,19 @@ __device__ __forceinline__ int32_t sload(const int32_t *p, uint64_t i) {
 __device__ __forceinline__ void async_row16(const uint8_t *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
+// The same from a base that the whole wave shares, with a byte offset per lane.
+__device__ __forceinline__ void async_row16(const uint8_t *base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// The same and this wave's LDS reads, then the workgroup's barrier.
+template <int N>
+__device__ __forceinline__ void wait_vm_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 // This wave's LDS reads are done: what they read may be overwritten.
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -159,6 +175,8 @@ template <int DP>
 struct RowLayout {
   static constexpr int kPieces = DP * 2 / 16;       // of a row
   static constexpr int kRowsPerLoad = 64 / kPieces; // rows of one asynchronous copy
+  // copies after which the permutations repeat
+  static constexpr int kKOffs = 16 / kRowsPerLoad, kVOffs = kRowsPerLoad < 4 ? 4 / kRowsPerLoad : 1;
   // K: 16 or 32 lanes read one piece of as many rows.
   static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
     return DP == 64 ? (row >> 1) & 7 : row & 15;
@@ -378,6 +396,266 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
   }
 }
 
+// 32 rows a wave: prompts and larger chunks.  The waves of a workgroup share
+// tiles of 64 keys, two stages of K and V in LDS; each wave copies its share
+// of the next tile while the present one is used.
+template <int DP, int WAVES>
+struct Rows32 {
+  static constexpr int kRows = 32 * WAVES;
+  static constexpr int kKeys = 64;
+  static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
+  static constexpr int kLoads = kKeys / RowLayout<DP>::kRowsPerLoad / WAVES;  // K or V copies of a wave
+  static constexpr int kLds = 2 * 2 * kTileBytes;
+};
+
+// A wave's share of a tile: 64 / WAVES keys of K or V from key0 + share on.
+// `ids`: the pages of its 8-key groups.
+template <int DP, int WAVES, bool V>
+__device__ __forceinline__ void load_share(const AttnParams &p, const int32_t *ids, uint32_t head, int32_t key0,
+                                           int32_t lo, int32_t hi, const uint32_t *offs, uint32_t lds, uint32_t wave,
+                                           bool whole) {
+  typedef RowLayout<DP> L;
+  constexpr int kShare = 64 / WAVES, kLoads = Rows32<DP, WAVES>::kLoads;
+  constexpr int kOffs = V ? L::kVOffs : L::kKOffs;
+  const uint32_t row_bytes = p.head_dim * 2, mask = (1u << p.page_shift) - 1, sub = lane_id() / L::kPieces;
+  const uint8_t *base = (const uint8_t *)(V ? p.v : p.k);
+  const int32_t k1 = key0 + (int32_t)wave * kShare;
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int32_t k0 = k1 + j * L::kRowsPerLoad;
+    const uint32_t id = (uint32_t)ids[j * L::kRowsPerLoad / 8];
+    const uint64_t at = (((uint64_t)id * p.n_kv_heads + head) << p.page_shift) + ((uint32_t)k0 & mask);
+    const uint8_t *src = base + at * row_bytes;
+    const uint32_t to = lds + (wave * kLoads + j) * 1024u;
+    if (whole) {
+      async_row16(src, offs[j % kOffs], to);
+    } else {
+      const int32_t key = k0 + (int32_t)sub;
+      const bool in = id < p.n_pages && key >= lo && key < hi;
+      async_row16(in ? src + offs[j % kOffs] : (const uint8_t *)g_zero_row, to);
+    }
+  }
+}
+
+template <class E, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_kernel(AttnParams p) {
+  typedef Rows32<DP, WAVES> C;
+  typedef RowLayout<DP> L;
+  typedef typename E::V8 V8;
+  typedef typename E::T T;
+  constexpr int kGroups = 64 / WAVES / 8;  // 8-key groups of a wave's share
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
+  const uint32_t head = blockIdx.x % p.n_kv_heads;
+  const uint32_t rest = blockIdx.x / p.n_kv_heads;
+  const uint32_t c = rest % p.n_chunks, unit = p.n_units - 1 - rest / p.n_chunks;  // late rows, with more keys, first
+  uint32_t seq, tile;
+  find_unit<C::kRows>(p, unit, &seq, &tile);
+  Tile t;
+  if (!make_tile<C::kRows>(p, seq, tile, &t) || c >= t.n_chunks) return;
+  const uint32_t col = lane % 32, half = lane / 32;
+  const uint32_t row = t.row0 + wave * 32 + col;
+  const bool row_ok = row < t.n_rows;
+  const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
+  const int32_t pos = t.pos0 + (int32_t)tok;
+  // the wave's positions; a wave without rows has none (first > last)
+  const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
+  const bool any = wrow < t.n_rows;
+  const int32_t pos_first = t.pos0 + (int32_t)(wrow / p.group), pos_last = t.pos0 + (int32_t)(wlast / p.group);
+  const float scale = fabsf(p.scale_log2);
+
+  V8 q[DP / 16];
+  const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const uint32_t d = s * 16 + half * 8;
+    q[s] = V8{};
+    if (row_ok && d < p.head_dim) q[s] = *(const V8 *)(qp + d);
+    if (p.scale_log2 < 0) q[s] = -q[s];
+  }
+
+  const int32_t begin = t.start + (int32_t)(c * t.chunk);
+  int32_t end = begin + (int32_t)t.chunk;
+  end = end < t.hi ? end : t.hi;
+  const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
+  const int32_t *table = p.table + (uint64_t)seq * p.table_stride;
+  const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+  const int32_t first_page = t.lo >> p.page_shift, last_page = (t.hi - 1) >> p.page_shift;
+
+  // Byte offset of a lane's piece within the rows of one copy; a piece beyond
+  // the head dimension repeats the first one (q is zero there).
+  uint32_t koff[L::kKOffs], voff[L::kVOffs];
+  {
+    const uint32_t sub = lane / L::kPieces, piece = lane % L::kPieces, row_bytes = p.head_dim * 2;
+#pragma unroll
+    for (uint32_t j = 0; j < L::kKOffs; ++j) {
+      const uint32_t lg = piece ^ L::k_swizzle(j * L::kRowsPerLoad + sub);
+      koff[j] = sub * row_bytes + (lg * 8 < p.head_dim ? lg * 16 : 0);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < L::kVOffs; ++j) {
+      const uint32_t lg = piece ^ L::v_swizzle(j * L::kRowsPerLoad + sub);
+      voff[j] = sub * row_bytes + (lg * 8 < p.head_dim ? lg * 16 : 0);
+    }
+  }
+  int32_t ids[kGroups];
+  auto fetch_ids = [&](int32_t i) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      int32_t pg = (begin + i * C::kKeys + (int32_t)wave * (64 / WAVES) + g * 8) >> p.page_shift;
+      pg = pg > last_page ? last_page : (pg < first_page ? first_page : pg);
+      ids[g] = sload(table, (uint32_t)pg);
+    }
+  };
+  auto whole = [&](int32_t i) {  // every key of the share is there and its page known
+    const int32_t k0 = begin + i * C::kKeys + (int32_t)wave * (64 / WAVES);
+    bool w = k0 >= t.lo && k0 + 64 / WAVES <= t.hi;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) w = w && (uint32_t)ids[g] < p.n_pages;
+    return w;
+  };
+  auto note_unknown = [&](int32_t i) {
+    const int32_t k0 = begin + i * C::kKeys + (int32_t)wave * (64 / WAVES);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if ((uint32_t)ids[g] >= p.n_pages && k0 + g * 8 < t.hi && k0 + g * 8 + 8 > t.lo && lane == 0)
+        atomicCAS(p.status, 0u, 16u /* residency miss */);
+  };
+  auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
+
+  float m = -__builtin_inff(), l = 0.0f;
+  f16v o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+
+  if (n_tiles > 0) {
+    fetch_ids(0);
+    const bool w = whole(0);
+    if (!w) note_unknown(0);
+    load_share<DP, WAVES, false>(p, ids, head, begin, t.lo, t.hi, koff, stage(0), wave, w);
+    load_share<DP, WAVES, true>(p, ids, head, begin, t.lo, t.hi, voff, stage(0) + C::kTileBytes, wave, w);
+    if (n_tiles > 1) fetch_ids(1);
+  }
+  for (int32_t i = 0; i < n_tiles; ++i) {
+    const int32_t key0 = begin + i * C::kKeys;
+    const uint32_t kb = stage(i), vb = kb + C::kTileBytes;
+    const bool more = i + 1 < n_tiles;
+    // all waves' copies of K, and everyone is done with the other stage
+    wait_vm_barrier<C::kLoads>();
+    bool w = false;
+    if (more) {
+      w = whole(i + 1);
+      if (!w) note_unknown(i + 1);
+      load_share<DP, WAVES, false>(p, ids, head, key0 + C::kKeys, t.lo, t.hi, koff, stage(i + 1), wave, w);
+    }
+    const bool live = any && key0 <= pos_last && !(p.window && key0 + C::kKeys <= pos_first - (int32_t)p.window + 1);
+    V8 pr[4];
+    if (live) {
+      f16v s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          const uint32_t r = b * 32 + col, piece = (d * 2 + half) ^ L::k_swizzle(r);
+          const V8 k = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
+          s[b] = E::mfma32(k, q[d], s[b]);
+        }
+      }
+      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi ||
+          (p.window && key0 <= pos_last - (int32_t)p.window)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int32_t key = key0 + b * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
+            if (key > pos || (p.window && key <= pos - (int64_t)p.window)) s[b][e] = -__builtin_inff();
+          }
+      }
+      float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
+      // The maximum in use may lag by up to 8 (weights up to 2^8): O and l
+      // are scaled only when it would lag by more.
+      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx);
+        const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[d] *= a;
+      }
+      const float mu = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f8 x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][h * 8 + e], scale, -mu));
+            l += x[e];
+          }
+          pr[b * 2 + h] = __builtin_convertvector(x, V8);
+        }
+    }
+    if (more) wait_vm_barrier<C::kLoads>();
+    else wait_vm_barrier<0>();
+    if (more) {
+      load_share<DP, WAVES, true>(p, ids, head, key0 + C::kKeys, t.lo, t.hi, voff, stage(i + 1) + C::kTileBytes, wave, w);
+      if (i + 2 < n_tiles) fetch_ids(i + 2);
+    }
+    if (live) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          s4 v[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t r = ks * 16 + b * 8 + half * 4 + lane % 16 / 4;
+            const uint32_t piece = (d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r);
+            v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + lane % 2 * 8));
+          }
+          const s8 vv = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          o[d] = E::mfma32(__builtin_bit_cast(V8, vv), pr[ks], o[d]);
+        }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if (!row_ok) return;
+  if (t.n_chunks == 1) {
+    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - (m == -__builtin_inff() ? 0.0f : m));
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t at = d * 32 + g * 8 + half * 4;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const f4 x = {o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+        if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x * inv, T4);
+      }
+  } else {
+    const uint64_t at = ((uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c) * C::kRows + wave * 32 + col;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t dim = d * 32 + g * 8 + half * 4;
+        if (dim < p.head_dim)
+          *(f4 *)(p.part_o + at * p.head_dim + dim) = f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+      }
+    if (half == 0) *(f2 *)(p.part_ml + at * 2) = f2{m, l};
+  }
+}
+
 // Joins the chunks of a row: one workgroup of 256 threads per row, 32 lanes x
 // head_dim / 32 dims by 8 groups of chunks.
 template <class E, int ROWS>
@@ -433,8 +711,24 @@ hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <class E, int DP>
+hipError_t launch32(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  typedef Rows32<DP, 4> C;
+  const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
+  hipError_t e = hipFuncSetAttribute((const void *)attn_rows32_kernel<E, DP, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  if (e != hipSuccess) return e;
+  attn_rows32_kernel<E, DP, 4><<<grid, 256, C::kLds, st>>>(p);
+  if (plan.n_chunks > 1) attn_join_kernel<E, C::kRows><<<plan.n_units * p.n_kv_heads * C::kRows, 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
 template <class E>
 hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  if (plan.rows == 128) {
+    if (p.head_dim <= 64) return launch32<E, 64>(plan, p, st);
+    if (p.head_dim <= 128) return launch32<E, 128>(plan, p, st);
+    return launch32<E, 256>(plan, p, st);
+  }
   if (p.head_dim <= 64) return launch16<E, 64>(plan, p, st);
   if (p.head_dim <= 128) return launch16<E, 128>(plan, p, st);
   return launch16<E, 256>(plan, p, st);
@@ -445,7 +739,7 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                    size_t max_q_len, size_t max_kv_len, uint32_t window, int cus) {
   AttnPlan a{};
-  a.rows = 16;
+  a.rows = max_q_len * group <= 32 ? 16 : 128;
   a.by_seq = max_q_len * group <= a.rows;
   // keys of a row tile, from a whole key tile's start on
   size_t max_keys = max_kv_len;
