@@ -418,28 +418,22 @@ typedef struct mer_kv_cache {
   uint64_t n_pages;      /* < 2^31 */
 } mer_kv_cache;
 
-/* Position rotation: element pairs (i, i + rot_dim / 2), or (2i, 2i + 1)
- * interleaved, of the first rot_dim elements of a head turn by
- * position * inv_freq[i]; the others stay.  rot_dim is a multiple of 8. */
-typedef struct mer_rope {
-  const float *inv_freq; /* device [rot_dim / 2] */
-  uint32_t rot_dim;
-  int32_t interleaved;
-} mer_rope;
-
 /* Norms of queries and keys for each head, with the rotation in the same
  * pass: x / sqrt(mean(x^2) + eps) * norm, then the rotation, in f32; rounded
- * once to out_type.
+ * once to out_type.  The rotation turns the element pairs (i, i + rot_dim / 2),
+ * or (2i, 2i + 1) interleaved, of a head's first rot_dim elements by
+ * position * inv_freq[i]; the others stay.
  *   d_q [n_tokens][n_heads][head_dim], d_k [n_tokens][n_kv_heads][head_dim]
  *   (rows q_stride / k_stride elements apart); either may have no heads;
- *   d_positions[n_tokens] (any sign); rope NULL = no rotation;
+ *   d_positions[n_tokens] (any sign), d_inv_freq[rot_dim / 2], rot_dim a
+ *   multiple of 8 up to head_dim; rot_dim 0 = no rotation, both unused;
  *   d_q_norm, d_k_norm [head_dim], NULL = no norm;
  *   outputs likewise, and they may be their inputs themselves where type and
  *   stride are the same (other overlaps are not allowed). */
 int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
                          size_t head_dim, const void *d_q, size_t q_stride, const void *d_k, size_t k_stride,
-                         const int32_t *d_positions, const mer_rope *rope, const float *d_q_norm,
-                         const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
+                         const int32_t *d_positions, const float *d_inv_freq, size_t rot_dim, int interleaved,
+                         const float *d_q_norm, const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
                          size_t k_out_stride, void *stream);
 
 /* Appends keys and values to a paged cache: row t goes to slot d_slots[t] =
@@ -450,14 +444,8 @@ int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_he
  * call are distinct (two rows of one slot leave elements of either). */
 int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
                       const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
-                      const mer_rope *rope, const float *d_k_norm, float eps, void *stream);
-
-typedef struct mer_attention_options {
-  float scale;           /* of q . k; 0 = 1 / sqrt(head_dim)               */
-  uint32_t window;       /* keys a row sees, itself included; 0 = all      */
-  const float *sinks;    /* device [n_heads]: a logit that takes part in   */
-                         /* the softmax and adds no value; NULL = none     */
-} mer_attention_options;
+                      const float *d_inv_freq, size_t rot_dim, int interleaved, const float *d_k_norm, float eps,
+                      void *stream);
 
 /* Attention of each sequence's new tokens over its pages, from one token
  * (decode) to whole prompts, any mix in a call.  Sequence s has rows
@@ -466,7 +454,9 @@ typedef struct mer_attention_options {
  * the pages d_block_table[s * table_stride + ..], the new tokens' own among
  * them (mer_hip_kv_append first).  Row i stands at position
  * p = kv_len - n + i and sees the keys j <= p, with a window j > p - window.
- * A row that sees no key gives zeros.
+ * A row that sees no key gives zeros.  scale: of q . k, 0 = 1 / sqrt(head_dim);
+ * window 0 = all keys; d_sinks [n_heads]: a logit per head that takes part in
+ * the softmax and adds no value, NULL = none.
  * d_q and d_out are of the cache's type, n_heads is a multiple of the cache's
  * n_kv_heads (head h reads kv head h / (n_heads / n_kv_heads)); sums and
  * softmax are f32, the weights are rounded to the cache's type for the
@@ -479,11 +469,12 @@ typedef struct mer_attention_options {
  * but there it may reach rows of the same call that do not see it.
  * max_q_len and max_kv_len say what the call should be laid out for, as a
  * captured graph needs it (0 = unknown); results do not depend on their being
- * right.  options NULL = all defaults. */
+ * right. */
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
                             const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
                             const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
-                            const mer_attention_options *options, void *d_out, size_t out_stride, void *stream);
+                            float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
+                            void *stream);
 
 /* Synthetic bench / test data: fill n_blocks GGUF blocks of expert
  * `expert_index` starting at block `block_begin` with this library's

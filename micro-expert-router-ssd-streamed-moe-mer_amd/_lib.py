@@ -47,14 +47,6 @@ class MerKvCache(ctypes.Structure):
                 ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("n_pages", c_u64)]
 
 
-class MerRope(ctypes.Structure):
-    _fields_ = [("inv_freq", c_void), ("rot_dim", ctypes.c_uint32), ("interleaved", ctypes.c_int32)]
-
-
-class MerAttentionOptions(ctypes.Structure):
-    _fields_ = [("scale", c_float), ("window", ctypes.c_uint32), ("sinks", c_void)]
-
-
 class MerSlotStats(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in
                 ("hits", "misses", "prefetches", "evictions", "stale_retirements", "bytes_uploaded", "resident")]
@@ -154,14 +146,14 @@ SIGNATURES = {
         c_int, [c_void, c_size, c_size, c_void, c_size, c_size, ctypes.POINTER(MerGateOptions), c_void, c_void, c_void,
                 c_void]),
     "mer_hip_qk_norm_rope": (
-        c_int, [c_int, c_int, c_size, c_size, c_size, c_size, c_void, c_size, c_void, c_size, c_void,
-                ctypes.POINTER(MerRope), c_void, c_void, c_float, c_void, c_size, c_void, c_size, c_void]),
+        c_int, [c_int, c_int, c_size, c_size, c_size, c_size, c_void, c_size, c_void, c_size, c_void, c_void, c_size,
+                c_int, c_void, c_void, c_float, c_void, c_size, c_void, c_size, c_void]),
     "mer_hip_kv_append": (
-        c_int, [ctypes.POINTER(MerKvCache), c_int, c_size, c_void, c_size, c_void, c_size, c_void, c_void,
-                ctypes.POINTER(MerRope), c_void, c_float, c_void]),
+        c_int, [ctypes.POINTER(MerKvCache), c_int, c_size, c_void, c_size, c_void, c_size, c_void, c_void, c_void,
+                c_size, c_int, c_void, c_float, c_void]),
     "mer_hip_paged_attention": (
         c_int, [ctypes.POINTER(MerKvCache), c_size, c_size, c_size, c_void, c_size, c_void, c_size, c_void, c_void,
-                c_size, c_size, ctypes.POINTER(MerAttentionOptions), c_void, c_size, c_void]),
+                c_size, c_size, c_float, ctypes.c_uint32, c_void, c_void, c_size, c_void]),
     "mer_slot_cache_create": (c_int, [c_int, c_size, c_size, c_size, c_size, ctypes.POINTER(c_void)]),
     "mer_slot_cache_destroy": (c_int, [c_void]),
     "mer_slot_cache_table": (c_void, [c_void]),

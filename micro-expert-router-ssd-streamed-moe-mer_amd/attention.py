@@ -22,54 +22,48 @@ from .errors import raise_for_status
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 6}
 
 
-def _enter(t: torch.Tensor) -> int:
-    """The current stream, for work on t, which must be on the current device."""
-    if not t.is_cuda:
+def _enter(t: torch.Tensor) -> tuple[int, int]:
+    """(device, current stream) for work on t, which must be on the current device."""
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("expected a device tensor")
-    dev = t.device.index
     if dev != torch.cuda.current_device():
         raise ValueError(f"tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     _lib.ensure_init(dev)
-    return torch.cuda.current_stream().cuda_stream
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _on(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-
-
-def _flat(t: torch.Tensor | None, dtype: torch.dtype, n: int, like: torch.Tensor, name: str) -> int:
+def _flat(t: torch.Tensor | None, dtype: torch.dtype, n: int, dev: int, name: str) -> int:
     """Address of a contiguous tensor of n elements (None: 0)."""
     if t is None:
         return 0
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.numel() != n:
-        raise ValueError(f"{name} must have {n} elements, got {t.numel()}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    _on(t, like, name)
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must have {n} elements side by side, got {tuple(t.shape)} strides {t.stride()}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str) -> int:
-    """Stride of the token axis of [tokens, heads, head_dim] whose heads lie
-    side by side."""
+def _rows(t: torch.Tensor, n: int, h: int, d: int, dtype: torch.dtype, dev: int, name: str) -> int:
+    """Stride of the token axis of t, [n, h, d] with its heads side by side."""
+    if t.shape != (n, h, d) or t.dtype != dtype:
+        raise ValueError(f"{name} must be {(n, h, d)} {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+    a, b, c = t.stride()
+    if (d > 1 and c != 1) or (h > 1 and b != d):
+        raise ValueError(f"the heads of {name} must lie side by side (strides {t.stride()})")
+    return a if n > 1 else h * d
+
+
+def _shape(t: torch.Tensor, name: str) -> torch.Size:
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
     if t.dtype not in _TYPES:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    n, h, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
-        raise ValueError(f"the heads of {name} must lie side by side (strides {t.stride()})")
-    return t.stride(0) if n > 1 else h * d
-
-
-def _rope(inv_freq: torch.Tensor | None, interleaved: bool, like: torch.Tensor):
-    if inv_freq is None:
-        return None
-    return _lib.MerRope(_flat(inv_freq, torch.float32, inv_freq.numel(), like, "inv_freq"), 2 * inv_freq.numel(),
-                        1 if interleaved else 0)
+    return t.shape
 
 
 class PagedKvCache:
@@ -103,6 +97,7 @@ class PagedKvCache:
         self._desc = _lib.MerKvCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads,
                                      self.head_dim, self.n_pages)
         self._ref = ctypes.byref(self._desc)
+        self.device = k.get_device()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None,
@@ -120,38 +115,34 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     interleaved     pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2)
     q_out, k_out    may be q and k themselves; else made, of out_dtype (default: q's)
     """
-    stream = _enter(q)
-    dt = (q_out.dtype if q_out is not None else q.dtype) if out_dtype is None else out_dtype
+    dev, stream = _enter(q)
+    n, h, d = _shape(q, "q")
+    src = q.dtype
+    dt = out_dtype if out_dtype is not None else src if q_out is None else q_out.dtype
     if dt not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {dt}")
-    n, h, d = q.shape if q.dim() == 3 else (0, 0, 0)
-    q_stride = _rows(q, "q")
+    q_stride = _rows(q, n, h, d, src, dev, "q")
     if q_out is None:
-        q_out = torch.empty((n, h, d), dtype=dt, device=q.device)
+        q_out, qo_stride = torch.empty((n, h, d), dtype=dt, device=q.device), h * d
+    else:
+        qo_stride = _rows(q_out, n, h, d, dt, dev, "q_out")
     kh = k_ptr = k_stride = ko_ptr = ko_stride = 0
     if k is not None:
-        k_stride = _rows(k, "k")
-        if k.shape[0] != n or k.shape[2] != d or k.dtype != q.dtype:
-            raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-        _on(k, q, "k")
-        kh, k_ptr = k.shape[1], k.data_ptr()
+        kh = _shape(k, "k")[1]
+        k_ptr, k_stride = k.data_ptr(), _rows(k, n, kh, d, src, dev, "k")
         if k_out is None:
-            k_out = torch.empty((n, kh, d), dtype=dt, device=q.device)
-        elif k_out.shape != k.shape or k_out.dtype != dt:
-            raise ValueError(f"k_out must be {tuple(k.shape)} {dt}")
-        _on(k_out, q, "k_out")
-        ko_ptr, ko_stride = k_out.data_ptr(), _rows(k_out, "k_out")
+            k_out, ko_stride = torch.empty((n, kh, d), dtype=dt, device=q.device), kh * d
+        else:
+            ko_stride = _rows(k_out, n, kh, d, dt, dev, "k_out")
+        ko_ptr = k_out.data_ptr()
     elif k_out is not None or k_norm is not None:
         raise ValueError("k_out and k_norm need k")
-    if q_out.shape != q.shape or q_out.dtype != dt:
-        raise ValueError(f"q_out must be {tuple(q.shape)} {dt}")
-    _on(q_out, q, "q_out")
-    rope = _rope(inv_freq, interleaved, q)
+    rot = 0 if inv_freq is None else 2 * inv_freq.numel()
     rc = _lib.lib().mer_hip_qk_norm_rope(
-        _TYPES[q.dtype], _TYPES[dt], n, h, kh, d, q.data_ptr(), q_stride, k_ptr, k_stride,
-        _flat(positions, torch.int32, n, q, "positions"), None if rope is None else ctypes.byref(rope),
-        _flat(q_norm, torch.float32, d, q, "q_norm"), _flat(k_norm, torch.float32, d, q, "k_norm"), eps,
-        q_out.data_ptr(), _rows(q_out, "q_out"), ko_ptr, ko_stride, stream)
+        _TYPES[src], _TYPES[dt], n, h, kh, d, q.data_ptr(), q_stride, k_ptr, k_stride,
+        _flat(positions, torch.int32, n, dev, "positions"), _flat(inv_freq, torch.float32, rot // 2, dev, "inv_freq"),
+        rot, interleaved, _flat(q_norm, torch.float32, d, dev, "q_norm"),
+        _flat(k_norm, torch.float32, d, dev, "k_norm"), eps, q_out.data_ptr(), qo_stride, ko_ptr, ko_stride, stream)
     if rc:
         raise_for_status(rc)
     return q_out, k_out
@@ -167,19 +158,17 @@ def kv_append(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     slots   int64 [tokens], distinct; negative = padding, the row is skipped; a
             slot past the cache is skipped and recorded (take_device_status)
     """
-    stream = _enter(k)
-    ks, vs = _rows(k, "k"), _rows(v, "v")
-    n = k.shape[0]
-    if k.shape != v.shape or k.dtype != v.dtype or tuple(k.shape[1:]) != (cache.n_kv_heads, cache.head_dim):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be "
-                         f"[tokens, {cache.n_kv_heads}, {cache.head_dim}] of one type")
-    _on(v, k, "v")
-    _on(cache.k, k, "cache")
-    rope = _rope(inv_freq, interleaved, k)
+    dev, stream = _enter(k)
+    n, src = _shape(k, "k")[0], k.dtype
+    kh, d = cache.n_kv_heads, cache.head_dim
+    ks, vs = _rows(k, n, kh, d, src, dev, "k"), _rows(v, n, kh, d, src, dev, "v")
+    if cache.device != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device}, expected cuda:{dev}")
+    rot = 0 if inv_freq is None else 2 * inv_freq.numel()
     rc = _lib.lib().mer_hip_kv_append(
-        cache._ref, _TYPES[k.dtype], n, k.data_ptr(), ks, v.data_ptr(), vs, _flat(slots, torch.int64, n, k, "slots"),
-        _flat(positions, torch.int32, n, k, "positions"), None if rope is None else ctypes.byref(rope),
-        _flat(k_norm, torch.float32, cache.head_dim, k, "k_norm"), eps, stream)
+        cache._ref, _TYPES[src], n, k.data_ptr(), ks, v.data_ptr(), vs, _flat(slots, torch.int64, n, dev, "slots"),
+        _flat(positions, torch.int32, n, dev, "positions"), _flat(inv_freq, torch.float32, rot // 2, dev, "inv_freq"),
+        rot, interleaved, _flat(k_norm, torch.float32, d, dev, "k_norm"), eps, stream)
     if rc:
         raise_for_status(rc)
 
@@ -203,29 +192,28 @@ def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Ten
     sinks        float32 [n_heads]: a logit per head that adds no value
     out          like q; made with zeros in rows of no sequence when None
     """
-    stream = _enter(q)
-    qs = _rows(q, "q")
-    n, h, d = q.shape
-    if d != cache.head_dim or q.dtype != cache.k.dtype:
-        raise ValueError(f"q {tuple(q.shape)} {q.dtype} does not go with a cache of head_dim {cache.head_dim}, "
-                         f"{cache.k.dtype}")
-    _on(cache.k, q, "cache")
+    dev, stream = _enter(q)
+    n, h, d = _shape(q, "q")
+    if d != cache.head_dim or q.dtype != cache.k.dtype or cache.device != dev:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} on cuda:{dev} does not go with a cache of head_dim "
+                         f"{cache.head_dim}, {cache.k.dtype} on cuda:{cache.device}")
     if block_table.dim() != 2:
         raise ValueError("block_table must be [n_seqs, pages]")
     seqs, width = block_table.shape
     if out is None:
-        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
-    _on(out, q, "out")
+        out, out_stride = torch.zeros((n, h, d), dtype=q.dtype, device=q.device), h * d
+    else:
+        out_stride = _rows(out, n, h, d, q.dtype, dev, "out")
     if window < 0 or max_q_len < 0 or max_kv_len < 0:
         raise ValueError("window, max_q_len and max_kv_len must not be negative")
-    opts = _lib.MerAttentionOptions(0.0 if scale is None else scale, min(window, 0xffffffff),
-                                    _flat(sinks, torch.float32, h, q, "sinks"))
+    if scale == 0:
+        raise ValueError("the scale must not be zero")
     rc = _lib.lib().mer_hip_paged_attention(
-        cache._ref, seqs, n, h, q.data_ptr(), qs, _flat(block_table, torch.int32, seqs * width, q, "block_table"), width,
-        _flat(q_start, torch.int32, seqs + 1, q, "q_start"), _flat(kv_len, torch.int32, seqs, q, "kv_len"),
-        max_q_len, max_kv_len, ctypes.byref(opts), out.data_ptr(), _rows(out, "out"), stream)
+        cache._ref, seqs, n, h, q.data_ptr(), _rows(q, n, h, d, q.dtype, dev, "q"),
+        _flat(block_table, torch.int32, seqs * width, dev, "block_table"), width,
+        _flat(q_start, torch.int32, seqs + 1, dev, "q_start"), _flat(kv_len, torch.int32, seqs, dev, "kv_len"),
+        max_q_len, max_kv_len, 0.0 if scale is None else scale, min(window, 0xffffffff),
+        _flat(sinks, torch.float32, h, dev, "sinks"), out.data_ptr(), out_stride, stream)
     if rc:
         raise_for_status(rc)
     return out

@@ -914,12 +914,12 @@ int check_head_dim(size_t d) {
   return MER_OK;
 }
 
-int check_rope(const mer_rope *r, size_t head_dim) {
-  if (!r) return MER_OK;
-  if (!r->inv_freq) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs its inverse frequencies");
-  if ((uintptr_t)r->inv_freq & 15u) return fail(MER_ERR_MISALIGNED, "inverse frequencies must be 16-byte aligned");
-  if (r->rot_dim == 0 || r->rot_dim % 8 != 0 || r->rot_dim > head_dim)
-    return fail(MER_ERR_INVALID_LAYOUT, "rot_dim %u must be a multiple of 8 up to head_dim %zu", r->rot_dim, head_dim);
+int check_rope(const float *inv_freq, size_t rot_dim, size_t head_dim) {
+  if (rot_dim == 0) return MER_OK;
+  if (!inv_freq) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs its inverse frequencies");
+  if ((uintptr_t)inv_freq & 15u) return fail(MER_ERR_MISALIGNED, "inverse frequencies must be 16-byte aligned");
+  if (rot_dim % 8 != 0 || rot_dim > head_dim)
+    return fail(MER_ERR_INVALID_LAYOUT, "rot_dim %zu must be a multiple of 8 up to head_dim %zu", rot_dim, head_dim);
   return MER_OK;
 }
 
@@ -959,14 +959,12 @@ int check_tensor(const char *name, const void *p, int type, size_t stride, size_
   return MER_OK;
 }
 
-void set_rope(NormRopeParams *p, const mer_rope *rope, const int32_t *positions, float eps, size_t n_tokens,
-              size_t head_dim) {
-  if (rope) {
-    p->positions = positions;
-    p->inv_freq = rope->inv_freq;
-    p->rot = rope->rot_dim;
-    p->interleaved = rope->interleaved != 0;
-  }
+void set_rope(NormRopeParams *p, const float *inv_freq, size_t rot_dim, int interleaved, const int32_t *positions,
+              float eps, size_t n_tokens, size_t head_dim) {
+  p->positions = positions;
+  p->inv_freq = inv_freq;
+  p->rot = (uint32_t)rot_dim;
+  p->interleaved = interleaved != 0;
   p->eps = eps;
   p->n_tokens = (uint32_t)n_tokens;
   p->head_dim = (uint32_t)head_dim;
@@ -1533,12 +1531,12 @@ int mer_hip_route_linear_gate(const float *d_gate, size_t n_experts, size_t d_mo
 
 int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
                          size_t head_dim, const void *d_q, size_t q_stride, const void *d_k, size_t k_stride,
-                         const int32_t *d_positions, const mer_rope *rope, const float *d_q_norm,
-                         const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
+                         const int32_t *d_positions, const float *d_inv_freq, size_t rot_dim, int interleaved,
+                         const float *d_q_norm, const float *d_k_norm, float eps, void *d_q_out, size_t q_out_stride, void *d_k_out,
                          size_t k_out_stride, void *stream) {
   int rc;
   if ((rc = check_float_type(in_type, true)) || (rc = check_float_type(out_type, true))) return rc;
-  if ((rc = check_head_dim(head_dim)) || (rc = check_rope(rope, head_dim))) return rc;
+  if ((rc = check_head_dim(head_dim)) || (rc = check_rope(d_inv_freq, rot_dim, head_dim))) return rc;
   if ((rc = check_rows(n_tokens, n_heads + n_kv_heads))) return rc;
   if (n_heads == 0 && n_kv_heads == 0) return fail(MER_ERR_INVALID_LAYOUT, "neither queries nor keys to norm");
   if (n_tokens == 0) return MER_OK;
@@ -1548,13 +1546,13 @@ int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_he
   if (n_kv_heads && ((rc = check_tensor("k", d_k, in_type, k_stride, n_kv_heads * head_dim, n_tokens)) ||
                      (rc = check_tensor("k output", d_k_out, out_type, k_out_stride, n_kv_heads * head_dim, n_tokens))))
     return rc;
-  if (rope && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
   if (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
   if ((rc = require_current_device())) return rc;
   NormRopeParams p{};
   p.t[0] = RopeTensor{d_q, d_q_out, d_q_norm, q_stride, q_out_stride, (uint32_t)n_heads};
   p.t[1] = RopeTensor{d_k, d_k_out, d_k_norm, k_stride, k_out_stride, (uint32_t)n_kv_heads};
-  set_rope(&p, rope, d_positions, eps, n_tokens, head_dim);
+  set_rope(&p, d_inv_freq, rot_dim, interleaved, d_positions, eps, n_tokens, head_dim);
   const hipError_t e = launch_norm_rope(in_type, out_type, p, g_dev[g_device].cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "norm and rotation launch");
   return MER_OK;
@@ -1562,9 +1560,10 @@ int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_he
 
 int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
                       const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
-                      const mer_rope *rope, const float *d_k_norm, float eps, void *stream) {
+                      const float *d_inv_freq, size_t rot_dim, int interleaved, const float *d_k_norm, float eps,
+                      void *stream) {
   int rc;
-  if ((rc = check_cache(cache)) || (rc = check_float_type(in_type, true)) || (rc = check_rope(rope, cache->head_dim)))
+  if ((rc = check_cache(cache)) || (rc = check_float_type(in_type, true)) || (rc = check_rope(d_inv_freq, rot_dim, cache->head_dim)))
     return rc;
   if ((rc = check_rows(n_tokens, 2 * (size_t)cache->n_kv_heads))) return rc;
   if (n_tokens == 0) return MER_OK;
@@ -1573,13 +1572,13 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
       (rc = check_tensor("v", d_v, in_type, v_stride, row, n_tokens)))
     return rc;
   if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
-  if (rope && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
   if ((uintptr_t)d_k_norm & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
   if ((rc = require_current_device())) return rc;
   NormRopeParams p{};
   p.t[0] = RopeTensor{d_k, cache->k, d_k_norm, k_stride, 0, cache->n_kv_heads};
   p.t[1] = RopeTensor{d_v, cache->v, nullptr, v_stride, 0, cache->n_kv_heads};
-  set_rope(&p, rope, d_positions, eps, n_tokens, cache->head_dim);
+  set_rope(&p, d_inv_freq, rot_dim, interleaved, d_positions, eps, n_tokens, cache->head_dim);
   p.slots = d_slots;
   p.n_slots = cache->n_pages * cache->page_size;
   p.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
@@ -1592,7 +1591,8 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
                             const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
                             const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
-                            const mer_attention_options *options, void *d_out, size_t out_stride, void *stream) {
+                            float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
+                            void *stream) {
   int rc;
   if ((rc = check_cache(cache)) || (rc = check_rows(n_tokens, n_heads))) return rc;
   if (n_heads == 0 || n_heads % cache->n_kv_heads != 0)
@@ -1608,7 +1608,6 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
     return rc;
   if (!d_q_start || !d_kv_len || (!d_block_table && table_stride))
     return fail(MER_ERR_INVALID_LAYOUT, "null sequence description");
-  float scale = options ? options->scale : 0.0f;
   if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
   if (!(fabsf(scale) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale is not finite");
   if ((rc = require_current_device())) return rc;
@@ -1630,10 +1629,8 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   p.n_kv_heads = cache->n_kv_heads;
   p.head_dim = cache->head_dim;
   p.group = (uint32_t)(n_heads / cache->n_kv_heads);
-  if (options) {
-    p.window = options->window > (1u << 30) ? 0u : options->window;
-    p.sinks = options->sinks;
-  }
+  p.window = window > (1u << 30) ? 0u : window;
+  p.sinks = d_sinks;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   const size_t cap = table_stride * cache->page_size;
   if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;

@@ -18,6 +18,8 @@
 // (half a step of a weight <= 1; its sum is kept from the f32 values).
 #include "mer_attention.hpp"
 
+#include <atomic>
+
 namespace mer {
 namespace {
 
@@ -700,11 +702,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   }
 }
 
+// More than 64 KiB of LDS has to be asked for, once per kernel and device.
+hipError_t allow_lds(const void *fn, int bytes, std::atomic<uint64_t> *devices) {
+  int d = 0;
+  hipError_t e = hipGetDevice(&d);
+  if (e != hipSuccess || (devices->load(std::memory_order_relaxed) >> d & 1)) return e;
+  e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) devices->fetch_or(1ull << d, std::memory_order_relaxed);
+  return e;
+}
+
 template <class E, int DP>
 hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   typedef Rows16<DP> C;
   const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
-  hipError_t e = hipFuncSetAttribute((const void *)attn_rows16_kernel<E, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  static std::atomic<uint64_t> devices{0};
+  const hipError_t e = allow_lds((const void *)attn_rows16_kernel<E, DP>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows16_kernel<E, DP><<<grid, 64 * C::kWaves, C::kLds, st>>>(p);
   if (plan.n_chunks > 1) attn_join_kernel<E, 16><<<plan.n_units * p.n_kv_heads * 16, 256, 0, st>>>(p);
@@ -715,7 +728,8 @@ template <class E, int DP>
 hipError_t launch32(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   typedef Rows32<DP, 4> C;
   const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
-  hipError_t e = hipFuncSetAttribute((const void *)attn_rows32_kernel<E, DP, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  static std::atomic<uint64_t> devices{0};
+  const hipError_t e = allow_lds((const void *)attn_rows32_kernel<E, DP, 4>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows32_kernel<E, DP, 4><<<grid, 256, C::kLds, st>>>(p);
   if (plan.n_chunks > 1) attn_join_kernel<E, C::kRows><<<plan.n_units * p.n_kv_heads * C::kRows, 256, 0, st>>>(p);

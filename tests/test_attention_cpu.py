@@ -23,25 +23,23 @@ def cache(abi, **kw):
 
 
 def norm_rope(abi, **kw):
-    rope = kw.pop("rope", abi.MerRope(P, 64, 0))
     f = dict(in_type=1, out_type=1, n=4, h=4, kv=2, d=64, q=P, qs=256, k=P, ks=128, pos=P,
-             rope=None if rope is None else ctypes.byref(rope), qn=P, kn=P, eps=1e-6, qo=P, qos=256, ko=P, kos=128,
+             freq=P, rot=64, interleaved=0, qn=P, kn=P, eps=1e-6, qo=P, qos=256, ko=P, kos=128,
              stream=None)
     f.update(kw)
     return abi.lib().mer_hip_qk_norm_rope(*f.values())
 
 
 def append(abi, c=None, **kw):
-    rope = kw.pop("rope", abi.MerRope(P, 64, 0))
     f = dict(cache=c if c is not None else cache(abi), in_type=1, n=4, k=P, ks=128, v=P, vs=128, slots=P, pos=P,
-             rope=None if rope is None else ctypes.byref(rope), kn=P, eps=1e-6, stream=None)
+             freq=P, rot=64, interleaved=0, kn=P, eps=1e-6, stream=None)
     f.update(kw)
     return abi.lib().mer_hip_kv_append(*f.values())
 
 
 def attention(abi, c=None, **kw):
     f = dict(cache=c if c is not None else cache(abi), seqs=2, n=4, h=4, q=P, qs=256, table=P, width=4, start=P,
-             lens=P, mq=0, mk=0, options=None, out=P, os=256, stream=None)
+             lens=P, mq=0, mk=0, scale=0.0, window=0, sinks=None, out=P, os=256, stream=None)
     f.update(kw)
     return abi.lib().mer_hip_paged_attention(*f.values())
 
@@ -70,12 +68,12 @@ def test_norm_rope_refuses(abi, change, status):
     assert abi.last_error()[0] == abi.Status[status] and abi.last_error()[1]
 
 
-@pytest.mark.parametrize("rot,freq,status", [(0, P, "INVALID_LAYOUT"), (12, P, "INVALID_LAYOUT"),
+@pytest.mark.parametrize("rot,freq,status", [(4, P, "INVALID_LAYOUT"), (12, P, "INVALID_LAYOUT"),
                                              (72, P, "INVALID_LAYOUT"), (64, 0, "INVALID_LAYOUT"),
                                              (64, P + 8, "MISALIGNED")])
 def test_rotation_refused(abi, rot, freq, status):
-    assert norm_rope(abi, rope=abi.MerRope(freq, rot, 0)) == abi.Status[status]
-    assert append(abi, rope=abi.MerRope(freq, rot, 0)) == abi.Status[status]
+    assert norm_rope(abi, freq=freq, rot=rot) == abi.Status[status]
+    assert append(abi, freq=freq, rot=rot) == abi.Status[status]
 
 
 @pytest.mark.parametrize("change,status", [
@@ -116,8 +114,7 @@ def test_attention_refuses(abi, change, status):
 
 @pytest.mark.parametrize("scale", [float("inf"), float("nan")])
 def test_attention_refuses_a_scale(abi, scale):
-    o = abi.MerAttentionOptions(scale, 0, None)
-    assert attention(abi, options=ctypes.byref(o)) == abi.Status.INVALID_LAYOUT
+    assert attention(abi, scale=scale) == abi.Status.INVALID_LAYOUT
 
 
 def test_python_refusals(mer):
