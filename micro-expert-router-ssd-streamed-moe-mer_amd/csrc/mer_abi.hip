@@ -88,6 +88,8 @@ struct Workspace {
   size_t router_floats = 0;
   float *attn_buf = nullptr;     // attention: sums of a row's key chunks
   size_t attn_floats = 0;
+  uint32_t *attn_counters = nullptr;  // chunks of a row tile that are done (zero between launches)
+  size_t attn_counter_words = 0;
   uint32_t *counters = nullptr;  // decode counters (zero between launches) + control lines
   size_t counter_words = 0;
   uint64_t *release = nullptr;   // decode release flags (epoch-valued, zero at allocation)
@@ -220,13 +222,14 @@ void free_workspace(Workspace &w) {
   if (w.stage) (void)hipFree(w.stage);
   if (w.router_buf) (void)hipFree(w.router_buf);
   if (w.attn_buf) (void)hipFree(w.attn_buf);
+  if (w.attn_counters) (void)hipFree(w.attn_counters);
   if (w.counters) (void)hipFree(w.counters);
   if (w.release) (void)hipFree(w.release);
   w.scratch = w.stage = w.router_buf = w.attn_buf = nullptr;
-  w.counters = nullptr;
+  w.counters = w.attn_counters = nullptr;
   w.release = nullptr;
   w.scratch_refused = SIZE_MAX;
-  w.scratch_floats = w.stage_floats = w.router_floats = w.attn_floats = w.counter_words = w.release_words = 0;
+  w.scratch_floats = w.stage_floats = w.router_floats = w.attn_floats = w.attn_counter_words = w.counter_words = w.release_words = 0;
 }
 
 bool capturing(hipStream_t st) {
@@ -943,6 +946,8 @@ int check_cache(const mer_kv_cache *c) {
     return fail(MER_ERR_INVALID_LAYOUT, "n_kv_heads %u must be in 1..=2048", c->n_kv_heads);
   if (c->n_pages == 0 || c->n_pages > 0x7fffffffull)
     return fail(MER_ERR_INVALID_LAYOUT, "n_pages must be in 1..2^31");
+  if ((uint64_t)c->n_kv_heads * c->page_size * c->head_dim * 2 >= (1ull << 32))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a page of %u keys of %u heads reaches 4 GiB", c->page_size, c->n_kv_heads);
   if (!c->k || !c->v) return fail(MER_ERR_INVALID_LAYOUT, "null cache memory");
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return fail(MER_ERR_MISALIGNED, "cache memory must be 16-byte aligned");
   return MER_OK;
@@ -1653,6 +1658,10 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
     rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, plan.part_o_floats + plan.part_ml_floats, size_t(1) << 20, false,
                     "attention workspace");
     if (rc) return rc;
+    rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, plan.counters, size_t(1) << 14, true,
+                    "attention counters");
+    if (rc) return rc;
+    p.counters = w->attn_counters;
     p.part_o = w->attn_buf;
     p.part_ml = w->attn_buf + plan.part_o_floats;
   }

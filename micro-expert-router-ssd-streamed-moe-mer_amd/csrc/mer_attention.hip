@@ -31,6 +31,7 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct F16 {
@@ -77,6 +78,9 @@ __device__ __forceinline__ void async_row16(const uint8_t *base, uint32_t off, u
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
+// vmcnt(0) alone, in the form that the compiler's own wait counting sees.
+constexpr int kWaitVm0 = 0x0F70;
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -134,39 +138,41 @@ struct Tile {
   uint32_t chunk, n_chunks;
 };
 
-// Key ranges stay clear of what the table cannot hold.
+// Key ranges stay clear of what the table cannot hold.  (Rows are below 2^26
+// and keys up to 2^30; every field is the same in the whole wave.)
 template <int ROWS>
 __device__ __forceinline__ bool make_tile(const AttnParams &p, uint32_t seq, uint32_t tile, Tile *t) {
-  const int64_t b = sload(p.q_start, seq), e = sload(p.q_start, seq + 1);
-  const int64_t tok0 = b < 0 ? 0 : (b > p.n_tokens ? p.n_tokens : b);
-  const int64_t tok1 = e < tok0 ? tok0 : (e > p.n_tokens ? p.n_tokens : e);
-  const int64_t n = tok1 - tok0;
-  const int64_t rows = n * p.group, row0 = (int64_t)tile * ROWS;
-  if (row0 >= rows) return false;
-  const int64_t cap = (int64_t)p.table_stride << p.page_shift;
-  int64_t len = sload(p.kv_len, seq);
+  const int32_t n_tokens = (int32_t)p.n_tokens, group = (int32_t)p.group;
+  const int32_t b = sload(p.q_start, seq), e = sload(p.q_start, seq + 1);
+  const int32_t cap = (int32_t)(p.table_stride << p.page_shift);
+  int32_t len = sload(p.kv_len, seq);
+  const int32_t tok0 = b < 0 ? 0 : (b > n_tokens ? n_tokens : b);
+  const int32_t tok1 = e < tok0 ? tok0 : (e > n_tokens ? n_tokens : e);
+  const int32_t n = tok1 - tok0, rows = n * group;
+  if (tile >= (uint32_t)(rows + ROWS - 1) / ROWS) return false;
+  const int32_t row0 = (int32_t)tile * ROWS;
   len = len < 0 ? 0 : (len > cap ? cap : len);
-  const int64_t last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
-  const int64_t pos0 = len - n;
-  int64_t hi = pos0 + last / p.group + 1;
+  const int32_t last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
+  const int32_t pos0 = len - n;
+  int32_t hi = pos0 + (int32_t)((uint32_t)last / p.group) + 1;
   hi = hi < 0 ? 0 : hi;
-  int64_t lo = p.window ? pos0 + row0 / p.group - (int64_t)p.window + 1 : 0;
+  int32_t lo = p.window ? pos0 + (int32_t)((uint32_t)row0 / p.group) - (int32_t)p.window + 1 : 0;
   lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
-  t->row0 = (uint32_t)row0;
-  t->n_rows = (uint32_t)rows;
-  t->tok0 = (uint32_t)tok0;
-  t->pos0 = (int32_t)pos0;
-  t->lo = (int32_t)lo;
-  t->hi = (int32_t)hi;
-  t->start = (int32_t)lo & ~63;
+  t->row0 = uni((uint32_t)row0);
+  t->n_rows = uni((uint32_t)rows);
+  t->tok0 = uni((uint32_t)tok0);
+  t->pos0 = (int32_t)uni((uint32_t)pos0);
+  t->lo = (int32_t)uni((uint32_t)lo);
+  t->hi = (int32_t)uni((uint32_t)hi);
+  t->start = t->lo & ~63;
   const uint32_t keys = (uint32_t)(t->hi - t->start);
   // A by_seq unit has partial sums for its first tile only: the tiles of a
   // sequence longer than the plan says are done in one piece.
   const uint32_t parts = p.by_seq && tile ? 1 : p.n_chunks;
   uint32_t c = (keys + parts - 1) / parts;
   c = (c + 63) & ~63u;
-  t->chunk = c < p.chunk ? p.chunk : c;
-  t->n_chunks = keys ? (keys + t->chunk - 1) / t->chunk : 1;
+  t->chunk = uni(c < p.chunk ? p.chunk : c);
+  t->n_chunks = uni(keys ? (keys + t->chunk - 1) / t->chunk : 1);
   return true;
 }
 
@@ -177,8 +183,7 @@ template <int DP>
 struct RowLayout {
   static constexpr int kPieces = DP * 2 / 16;       // of a row
   static constexpr int kRowsPerLoad = 64 / kPieces; // rows of one asynchronous copy
-  // copies after which the permutations repeat
-  static constexpr int kKOffs = 16 / kRowsPerLoad, kVOffs = kRowsPerLoad < 4 ? 4 / kRowsPerLoad : 1;
+  static constexpr int kKOffs = 16 / kRowsPerLoad;  // copies after which K's permutation repeats (V's: 8 rows)
   // K: 16 or 32 lanes read one piece of as many rows.
   static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
     return DP == 64 ? (row >> 1) & 7 : row & 15;
@@ -189,32 +194,234 @@ struct RowLayout {
   }
 };
 
-// Copies `KEYS` keys from `key0` on (a multiple of 8) to LDS.  Lanes outside
-// [lo, hi), beyond the head dimension or on a page that the cache does not
-// have read zeros.
-template <int DP, int KEYS, bool V>
-__device__ __forceinline__ void load_keys(const AttnParams &p, const int32_t *table, uint32_t head, int32_t key0,
-                                          int32_t lo, int32_t hi, uint32_t lds) {
+// Asynchronous copies of a wave's share of a tile, SHARE keys from a multiple
+// of 8 on: the pages of its 8-key groups are looked up a tile ahead, so that
+// the lookups are off the copies' path.
+template <int DP, int SHARE>
+struct Share {
   typedef RowLayout<DP> L;
-  const uint32_t lane = lane_id(), sub = lane / L::kPieces, piece = lane % L::kPieces;
-  const uint32_t row_bytes = p.head_dim * 2, mask = (1u << p.page_shift) - 1;
-  const uint8_t *base = (const uint8_t *)(V ? p.v : p.k);
-  const int32_t last_page = (hi - 1) >> p.page_shift, first_page = lo >> p.page_shift;
+  static constexpr int kGroups = SHARE / 8;
+  static constexpr int kLoads = SHARE / L::kRowsPerLoad;  // copies of K, and of V
+  static constexpr int kPerGroup = 8 / L::kRowsPerLoad;   // copies of an 8-key group
+  static constexpr int kOffs = L::kKOffs > kPerGroup ? L::kKOffs : kPerGroup;
+
+  const uint8_t *k, *v;  // of this head in page 0
+  uint32_t page_bytes, row_bytes, page_shift, n_pages;
+  const int32_t *table;
+  int32_t lo, hi;        // keys to copy; others, and those of unknown pages, read zeros
+  int32_t key0, next_key;
+  uint64_t off[kGroups]; // of a group's first row
+  int32_t next_id[kGroups];
+  uint32_t known;        // groups of pages that the cache has, a bit each
+  bool whole;
+  uint32_t koff[kOffs], voff[kPerGroup];  // a lane's piece, from its group's first row
+
+  __device__ __forceinline__ void init(const AttnParams &p, const int32_t *seq_table, uint32_t head, const Tile &t) {
+    row_bytes = p.head_dim * 2;
+    page_shift = p.page_shift;
+    page_bytes = (p.n_kv_heads << page_shift) * row_bytes;
+    n_pages = p.n_pages;
+    k = (const uint8_t *)p.k + (uint64_t)(head << page_shift) * row_bytes;
+    v = (const uint8_t *)p.v + (uint64_t)(head << page_shift) * row_bytes;
+    table = seq_table;
+    lo = t.lo;
+    hi = t.hi;
+    const uint32_t lane = lane_id(), sub = lane / L::kPieces, piece = lane % L::kPieces;
+    // a piece beyond the head dimension repeats the first one (q is zero there)
+    auto at = [&](uint32_t row, uint32_t lg) { return row % 8 * row_bytes + (lg * 8 < p.head_dim ? lg * 16 : 0); };
 #pragma unroll
-  for (int j = 0; j < KEYS / L::kRowsPerLoad; ++j) {
-    const int32_t k0 = key0 + j * L::kRowsPerLoad;
-    int32_t pg = k0 >> p.page_shift;
-    pg = pg > last_page ? last_page : (pg < first_page ? first_page : pg);
-    const int32_t id = sload(table, (uint32_t)pg);
-    const bool known = (uint32_t)id < p.n_pages;
-    const uint64_t at = (((uint64_t)(uint32_t)id * p.n_kv_heads + head) << p.page_shift) + ((uint32_t)k0 & mask);
-    const uint32_t row = (uint32_t)j * L::kRowsPerLoad + sub;
-    const uint32_t logical = piece ^ (V ? L::v_swizzle(row) : L::k_swizzle(row));
-    const int32_t key = k0 + (int32_t)sub;
-    const uint8_t *src = base + at * row_bytes + sub * row_bytes + logical * 16;
-    const bool in = known && key >= lo && key < hi && logical * 8 < p.head_dim;
-    async_row16(in ? src : (const uint8_t *)g_zero_row, lds + (uint32_t)j * 1024u);
-    if (!known && lane == 0 && k0 < hi && k0 + L::kRowsPerLoad > lo) atomicCAS(p.status, 0u, 16u /* residency miss */);
+    for (uint32_t j = 0; j < kOffs; ++j) {
+      const uint32_t row = j * L::kRowsPerLoad + sub;
+      koff[j] = at(row, piece ^ L::k_swizzle(row));
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kPerGroup; ++j) {
+      const uint32_t row = j * L::kRowsPerLoad + sub;
+      voff[j] = at(row, piece ^ L::v_swizzle(row));
+    }
+  }
+
+  // Any key will do: page places are cut to those of [lo, hi), which is not empty.
+  __device__ __forceinline__ void lookup(int32_t key) {
+    next_key = key;
+    const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      int32_t pg = (key + g * 8) >> page_shift;
+      pg = pg > last ? last : (pg < first ? first : pg);
+      next_id[g] = sload(table, (uint32_t)pg);
+    }
+  }
+
+  // On to the share last looked up, before its copies.
+  __device__ __forceinline__ void advance(uint32_t *status) {
+    key0 = next_key;
+    const uint32_t mask = (1u << page_shift) - 1;
+    known = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      off[g] = (uint64_t)(uint32_t)next_id[g] * page_bytes + ((uint32_t)(key0 + g * 8) & mask) * row_bytes;
+      known |= (uint32_t)next_id[g] < n_pages ? 1u << g : 0u;
+    }
+    whole = key0 >= lo && key0 + SHARE <= hi && known == (1u << kGroups) - 1;
+    if (known != (1u << kGroups) - 1 && lane_id() < kGroups) {
+      const int32_t k0 = key0 + (int32_t)lane_id() * 8;
+      if (!(known >> lane_id() & 1) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
+    }
+  }
+
+  template <bool V>
+  __device__ __forceinline__ void copy(uint32_t lds) const {
+    const uint8_t *base = V ? v : k;
+    if (whole) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < kPerGroup; ++i) {
+          const int j = g * kPerGroup + i;
+          async_row16(base + off[g], V ? voff[i] : koff[j % kOffs], lds + j * 1024u);
+        }
+    } else {
+      const uint32_t sub = lane_id() / L::kPieces;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < kPerGroup; ++i) {
+          const int j = g * kPerGroup + i;
+          const int32_t key = key0 + j * L::kRowsPerLoad + (int32_t)sub;
+          const bool in = (known >> g & 1) && key >= lo && key < hi;
+          async_row16(in ? base + off[g] + (V ? voff[i] : koff[j % kOffs]) : (const uint8_t *)g_zero_row, lds + j * 1024u);
+        }
+    }
+  }
+};
+
+// ---- joining the chunks of a row tile ----
+// A workgroup that has done one of several chunks leaves its sums in memory
+// (device-scope stores) and counts itself in; the one that comes last adds
+// the chunks up, in their order, and leaves the count at zero for the next
+// launch.
+constexpr int kDeviceScope = 16;  // sc1: past the caches that other XCDs do not see
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float *p) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t r, uint32_t index, f4 x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), r, index * 4, 0, kDeviceScope);
+}
+__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, uint32_t index, f2 x) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, x), r, index * 4, 0, kDeviceScope);
+}
+
+// True in every thread of the workgroup that comes last.  `flag`: a word of LDS.
+__device__ __forceinline__ bool last_chunk(uint32_t *counter, uint32_t n_chunks, uint32_t *flag) {
+  wait_vm<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (n == n_chunks - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = n == n_chunks - 1;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// Adds up a tile's chunks.  32 lanes hold a row's dims; the groups of 32 take
+// U rows each at a time, or share a row's chunks where there are fewer rows
+// than groups.  `lds`: [threads / 32][DP + 1] floats.
+template <class E, int DP, int ROWS, int THREADS, int U>
+__device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, uint32_t head, float *part_o,
+                                            float *part_ml, float *lds) {
+  typedef typename E::T T;
+  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = 4;
+  typedef float fd __attribute__((ext_vector_type(kDims)));
+  typedef T td __attribute__((ext_vector_type(kDims)));
+  const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
+  const uint32_t g = threadIdx.x / 32, ln = threadIdx.x % 32, dim = ln * kDims;
+  const uint32_t rows = t.n_rows - t.row0 < ROWS ? t.n_rows - t.row0 : ROWS;
+  const uint32_t share = rows < kGroups ? kGroups / rows : 1;  // groups of a row
+  const uint32_t step = kGroups / share;                       // rows at a time
+  auto ml_of = [&](uint32_t c, uint32_t r, bool ok) {
+    return __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(rm, ok ? (c * ROWS + r) * 8 : 0xfffffff0u, 0, kDeviceScope));
+  };
+  for (uint32_t r0 = 0; r0 < rows; r0 += step * U) {
+    uint32_t r[U];
+    bool ok[U];
+    float m[U], l[U];
+    fd acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = r0 + u * step + g / share;
+      ok[u] = g / share < step && r[u] < rows;
+      f2 ml = ml_of(ln, r[u], ok[u] && ln < t.n_chunks);
+      m[u] = ln < t.n_chunks ? ml[0] : -__builtin_inff();
+      l[u] = ln < t.n_chunks ? ml[1] : 0.0f;
+      for (uint32_t c = ln + 32; c < t.n_chunks; c += 32) {
+        ml = ml_of(c, r[u], ok[u]);
+        const float mn = fmaxf(m[u], ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
+        l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+        m[u] = mn;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float mm = m[u];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+      const float mu = mm == -__builtin_inff() ? 0.0f : mm;
+      l[u] *= __builtin_amdgcn_exp2f(m[u] - mu);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) l[u] += __shfl_xor(l[u], d);
+      m[u] = mu;
+      acc[u] = fd{};
+    }
+    for (uint32_t c0 = g % share; c0 < t.n_chunks; c0 += share * kBatch) {
+      fd x[U][kBatch];
+      float w[U][kBatch];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t c = c0 + b * share;
+          const bool in = ok[u] && c < t.n_chunks;
+          w[u][b] = ml_of(c, r[u], in)[0];
+          const uint32_t at = in && dim < p.head_dim ? ((c * ROWS + r[u]) * p.head_dim + dim) * 4 : 0xfffffff0u;
+          if constexpr (kDims == 2) {
+            x[u][b] = __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
+          } else if constexpr (kDims == 4) {
+            x[u][b] = __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
+          } else {
+            const f4 lo = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
+            const f4 hi = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 16, kDeviceScope));
+            x[u][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t c = c0 + b * share;
+          if (c < t.n_chunks) acc[u] += x[u][b] * __builtin_amdgcn_exp2f(w[u][b] - m[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (share > 1) {  // once: rows <= step, U rows of which only the first is one
+        if (ok[u] && g % share) *(fd *)&lds[g * DP + dim] = acc[u];
+        __syncthreads();
+        if (ok[u] && g % share == 0)
+          for (uint32_t k = 1; k < share; ++k) acc[u] += *(fd *)&lds[(g + k) * DP + dim];
+        __syncthreads();
+      }
+      if (ok[u] && g % share == 0 && dim < p.head_dim) {
+        const uint32_t gr = t.row0 + r[u], hq = head * p.group + gr % p.group;
+        float ls = l[u];
+        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - m[u]);
+        const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
+        T *op = (T *)p.out + (uint64_t)(t.tok0 + gr / p.group) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
+        *(td *)op = __builtin_convertvector(acc[u] * inv, td);
+      }
+    }
   }
 }
 
@@ -228,12 +435,12 @@ struct Rows16 {
   static constexpr int kKeys = 32;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kStages = 2;
-  static constexpr int kLoads = kKeys / RowLayout<DP>::kRowsPerLoad;
+  static constexpr int kLoads = Share<DP, kKeys>::kLoads;
   static constexpr int kLds = kWaves * kStages * 2 * kTileBytes;
 };
 
 template <class E, int DP>
-__global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParams p) {
+__global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_eu(1, 2))) void attn_rows16_kernel(AttnParams p) {
   typedef Rows16<DP> C;
   typedef RowLayout<DP> L;
   typedef typename E::V8 V8;
@@ -271,15 +478,22 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
     end = end < t.hi ? end : t.hi;
     const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
     const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
-    const int32_t *table = p.table + (uint64_t)seq * p.table_stride;
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem +
                           wave * (C::kStages * 2 * C::kTileBytes);
     auto key_of = [&](int32_t i) { return begin + (i * C::kWaves + (int32_t)wave) * C::kKeys; };
     auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
     __syncthreads();  // the last tile's join is done with the LDS
+    Share<DP, C::kKeys> sh;
+    sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t);
+    if (mine > 0) sh.lookup(key_of(0));
+    // q has to be there before the first copy goes out: a later wait for it,
+    // which the compiler would put into the loop, would drain the copies.
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
     for (int32_t i = 0; i < C::kStages && i < mine; ++i) {
-      load_keys<DP, C::kKeys, false>(p, table, head, key_of(i), t.lo, t.hi, slot_of(i));
-      load_keys<DP, C::kKeys, true>(p, table, head, key_of(i), t.lo, t.hi, slot_of(i) + C::kTileBytes);
+      sh.advance(p.status);
+      sh.lookup(key_of(i + 1));
+      sh.template copy<false>(slot_of(i));
+      sh.template copy<true>(slot_of(i) + C::kTileBytes);
     }
 
     float m = -__builtin_inff(), l = 0.0f;
@@ -293,16 +507,25 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
       if (left == 1) wait_vm<C::kLoads>();
       else wait_vm<3 * C::kLoads>();
       f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+      V8 k[2][DP / 32];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
+        for (int b = 0; b < 2; ++b) {
           const uint32_t r = b * 16 + col, piece = (d * 4 + quad) ^ L::k_swizzle(r);
-          const V8 k = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
-          s[b] = E::mfma16(k, q[d], s[b]);
+          k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
         }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = E::mfma16(k[b][d], q[d], s[b]);
       wait_lds();
-      if (left > C::kStages) load_keys<DP, C::kKeys, false>(p, table, head, key_of(i + 2), t.lo, t.hi, kb);
+      if (left > C::kStages) {
+        sh.advance(p.status);
+        sh.lookup(key_of(i + C::kStages + 1));
+        sh.template copy<false>(kb);
+      }
       // scores in base 2; keys of lane: b * 16 + quad * 4 + e
       float x[8];
 #pragma unroll
@@ -352,7 +575,7 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
         o[d] = E::mfma16(__builtin_bit_cast(V8, vv), pr, o[d]);
       }
       wait_lds();
-      if (left > C::kStages) load_keys<DP, C::kKeys, true>(p, table, head, key_of(i + 2), t.lo, t.hi, vb);
+      if (left > C::kStages) sh.template copy<true>(vb);
     }
     l = sum_quad(l);
     // join the waves: m, l and O of each in LDS
@@ -366,6 +589,9 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[(wave * 16 + col) * DP + d * 16 + quad * 4] = o[d];
     __syncthreads();
+    const uint64_t part = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks * 16;
+    float *part_o = p.part_o + part * p.head_dim, *part_ml = p.part_ml + part * 2;
+    const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
     for (uint32_t w = tid; w < 16 * (DP / 8); w += 64 * C::kWaves) {
       const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, gr = t.row0 + r;
       if (gr >= t.n_rows || d >= p.head_dim) continue;
@@ -388,11 +614,14 @@ __global__ __launch_bounds__(64 * waves16(DP)) void attn_rows16_kernel(AttnParam
         const V8 r8 = __builtin_convertvector(acc * inv, V8);
         *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
       } else {
-        const uint64_t at = ((uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c) * 16 + r;
-        *(f8 *)(p.part_o + at * p.head_dim + d) = acc;
-        if (d == 0) *(f2 *)(p.part_ml + at * 2) = f2{mm, ls};
+        const uint32_t at = c * 16 + r;
+        put4(ro, at * p.head_dim + d, f4{acc[0], acc[1], acc[2], acc[3]});
+        put4(ro, at * p.head_dim + d + 4, f4{acc[4], acc[5], acc[6], acc[7]});
+        if (d == 0) put2(rm, at * 2, f2{mm, ls});
       }
     }
+    if (t.n_chunks > 1 && last_chunk(p.counters + unit * p.n_kv_heads + head, t.n_chunks, (uint32_t *)(jm + C::kWaves * 32)))
+      join_chunks<E, DP, 16, 64 * C::kWaves, 1>(p, t, head, part_o, part_ml, jo);
   }
   if (!p.by_seq) return;
   }
@@ -406,38 +635,10 @@ struct Rows32 {
   static constexpr int kRows = 32 * WAVES;
   static constexpr int kKeys = 64;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
-  static constexpr int kLoads = kKeys / RowLayout<DP>::kRowsPerLoad / WAVES;  // K or V copies of a wave
+  static constexpr int kShare = kKeys / WAVES;       // keys that a wave copies
+  static constexpr int kLoads = Share<DP, kShare>::kLoads;
   static constexpr int kLds = 2 * 2 * kTileBytes;
 };
-
-// A wave's share of a tile: 64 / WAVES keys of K or V from key0 + share on.
-// `ids`: the pages of its 8-key groups.
-template <int DP, int WAVES, bool V>
-__device__ __forceinline__ void load_share(const AttnParams &p, const int32_t *ids, uint32_t head, int32_t key0,
-                                           int32_t lo, int32_t hi, const uint32_t *offs, uint32_t lds, uint32_t wave,
-                                           bool whole) {
-  typedef RowLayout<DP> L;
-  constexpr int kShare = 64 / WAVES, kLoads = Rows32<DP, WAVES>::kLoads;
-  constexpr int kOffs = V ? L::kVOffs : L::kKOffs;
-  const uint32_t row_bytes = p.head_dim * 2, mask = (1u << p.page_shift) - 1, sub = lane_id() / L::kPieces;
-  const uint8_t *base = (const uint8_t *)(V ? p.v : p.k);
-  const int32_t k1 = key0 + (int32_t)wave * kShare;
-#pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int32_t k0 = k1 + j * L::kRowsPerLoad;
-    const uint32_t id = (uint32_t)ids[j * L::kRowsPerLoad / 8];
-    const uint64_t at = (((uint64_t)id * p.n_kv_heads + head) << p.page_shift) + ((uint32_t)k0 & mask);
-    const uint8_t *src = base + at * row_bytes;
-    const uint32_t to = lds + (wave * kLoads + j) * 1024u;
-    if (whole) {
-      async_row16(src, offs[j % kOffs], to);
-    } else {
-      const int32_t key = k0 + (int32_t)sub;
-      const bool in = id < p.n_pages && key >= lo && key < hi;
-      async_row16(in ? src + offs[j % kOffs] : (const uint8_t *)g_zero_row, to);
-    }
-  }
-}
 
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_kernel(AttnParams p) {
@@ -445,7 +646,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   typedef RowLayout<DP> L;
   typedef typename E::V8 V8;
   typedef typename E::T T;
-  constexpr int kGroups = 64 / WAVES / 8;  // 8-key groups of a wave's share
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
   const uint32_t head = blockIdx.x % p.n_kv_heads;
@@ -480,49 +680,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   int32_t end = begin + (int32_t)t.chunk;
   end = end < t.hi ? end : t.hi;
   const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
-  const int32_t *table = p.table + (uint64_t)seq * p.table_stride;
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
-  const int32_t first_page = t.lo >> p.page_shift, last_page = (t.hi - 1) >> p.page_shift;
-
-  // Byte offset of a lane's piece within the rows of one copy; a piece beyond
-  // the head dimension repeats the first one (q is zero there).
-  uint32_t koff[L::kKOffs], voff[L::kVOffs];
-  {
-    const uint32_t sub = lane / L::kPieces, piece = lane % L::kPieces, row_bytes = p.head_dim * 2;
-#pragma unroll
-    for (uint32_t j = 0; j < L::kKOffs; ++j) {
-      const uint32_t lg = piece ^ L::k_swizzle(j * L::kRowsPerLoad + sub);
-      koff[j] = sub * row_bytes + (lg * 8 < p.head_dim ? lg * 16 : 0);
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < L::kVOffs; ++j) {
-      const uint32_t lg = piece ^ L::v_swizzle(j * L::kRowsPerLoad + sub);
-      voff[j] = sub * row_bytes + (lg * 8 < p.head_dim ? lg * 16 : 0);
-    }
-  }
-  int32_t ids[kGroups];
-  auto fetch_ids = [&](int32_t i) {
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      int32_t pg = (begin + i * C::kKeys + (int32_t)wave * (64 / WAVES) + g * 8) >> p.page_shift;
-      pg = pg > last_page ? last_page : (pg < first_page ? first_page : pg);
-      ids[g] = sload(table, (uint32_t)pg);
-    }
-  };
-  auto whole = [&](int32_t i) {  // every key of the share is there and its page known
-    const int32_t k0 = begin + i * C::kKeys + (int32_t)wave * (64 / WAVES);
-    bool w = k0 >= t.lo && k0 + 64 / WAVES <= t.hi;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) w = w && (uint32_t)ids[g] < p.n_pages;
-    return w;
-  };
-  auto note_unknown = [&](int32_t i) {
-    const int32_t k0 = begin + i * C::kKeys + (int32_t)wave * (64 / WAVES);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if ((uint32_t)ids[g] >= p.n_pages && k0 + g * 8 < t.hi && k0 + g * 8 + 8 > t.lo && lane == 0)
-        atomicCAS(p.status, 0u, 16u /* residency miss */);
-  };
+  Share<DP, C::kShare> sh;
+  sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t);
+  const int32_t my_key = begin + (int32_t)wave * C::kShare;
+  const uint32_t my_lds = wave * (C::kLoads * 1024u);
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
 
   float m = -__builtin_inff(), l = 0.0f;
@@ -533,12 +695,12 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
   if (n_tiles > 0) {
-    fetch_ids(0);
-    const bool w = whole(0);
-    if (!w) note_unknown(0);
-    load_share<DP, WAVES, false>(p, ids, head, begin, t.lo, t.hi, koff, stage(0), wave, w);
-    load_share<DP, WAVES, true>(p, ids, head, begin, t.lo, t.hi, voff, stage(0) + C::kTileBytes, wave, w);
-    if (n_tiles > 1) fetch_ids(1);
+    sh.lookup(my_key);
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);  // q is there before the first copy goes out (as above)
+    sh.advance(p.status);
+    sh.lookup(my_key + C::kKeys);
+    sh.template copy<false>(stage(0) + my_lds);
+    sh.template copy<true>(stage(0) + C::kTileBytes + my_lds);
   }
   for (int32_t i = 0; i < n_tiles; ++i) {
     const int32_t key0 = begin + i * C::kKeys;
@@ -546,11 +708,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     const bool more = i + 1 < n_tiles;
     // all waves' copies of K, and everyone is done with the other stage
     wait_vm_barrier<C::kLoads>();
-    bool w = false;
     if (more) {
-      w = whole(i + 1);
-      if (!w) note_unknown(i + 1);
-      load_share<DP, WAVES, false>(p, ids, head, key0 + C::kKeys, t.lo, t.hi, koff, stage(i + 1), wave, w);
+      sh.advance(p.status);
+      sh.lookup(my_key + (i + 2) * C::kKeys);
+      sh.template copy<false>(stage(i + 1) + my_lds);
     }
     const bool live = any && key0 <= pos_last && !(p.window && key0 + C::kKeys <= pos_first - (int32_t)p.window + 1);
     V8 pr[4];
@@ -607,10 +768,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     }
     if (more) wait_vm_barrier<C::kLoads>();
     else wait_vm_barrier<0>();
-    if (more) {
-      load_share<DP, WAVES, true>(p, ids, head, key0 + C::kKeys, t.lo, t.hi, voff, stage(i + 1) + C::kTileBytes, wave, w);
-      if (i + 2 < n_tiles) fetch_ids(i + 2);
-    }
+    if (more) sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
     if (live) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
@@ -630,8 +788,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     }
   }
   l += __shfl_xor(l, 32);
-  if (!row_ok) return;
   if (t.n_chunks == 1) {
+    if (!row_ok) return;
     if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - (m == -__builtin_inff() ? 0.0f : m));
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
@@ -645,60 +803,23 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x * inv, T4);
       }
   } else {
-    const uint64_t at = ((uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c) * C::kRows + wave * 32 + col;
+    const uint64_t part = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks * C::kRows;
+    float *part_o = p.part_o + part * p.head_dim, *part_ml = p.part_ml + part * 2;
+    const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
+    const uint32_t at = c * C::kRows + wave * 32 + col;
+    if (row_ok) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t dim = d * 32 + g * 8 + half * 4;
-        if (dim < p.head_dim)
-          *(f4 *)(p.part_o + at * p.head_dim + dim) = f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
-      }
-    if (half == 0) *(f2 *)(p.part_ml + at * 2) = f2{m, l};
-  }
-}
-
-// Joins the chunks of a row: one workgroup of 256 threads per row, 32 lanes x
-// head_dim / 32 dims by 8 groups of chunks.
-template <class E, int ROWS>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
-  typedef typename E::T T;
-  const uint32_t r = blockIdx.x % ROWS, uh = blockIdx.x / ROWS;
-  const uint32_t head = uh % p.n_kv_heads, unit = uh / p.n_kv_heads;
-  uint32_t seq = unit, tile = 0;
-  if (!p.by_seq) find_unit<ROWS>(p, unit, &seq, &tile);
-  Tile t;
-  if (!make_tile<ROWS>(p, seq, tile, &t) || t.n_chunks == 1 || t.row0 + r >= t.n_rows) return;
-  const uint64_t at = ((uint64_t)uh * p.n_chunks) * ROWS + r;
-  __shared__ float so[8][kMaxHeadDim];
-  __shared__ float sl[8];
-  const uint32_t tid = threadIdx.x, g = tid / 32, ln = tid % 32;
-  float mm = -__builtin_inff();
-  for (uint32_t c = ln; c < t.n_chunks; c += 32) mm = fmaxf(mm, p.part_ml[(at + (uint64_t)c * ROWS) * 2]);
-  for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-  const float mu = mm == -__builtin_inff() ? 0.0f : mm;
-  float ls = 0.0f, acc[kMaxHeadDim / 32] = {};
-  for (uint32_t c = g; c < t.n_chunks; c += 8) {
-    const uint64_t i = at + (uint64_t)c * ROWS;
-    const float a = __builtin_amdgcn_exp2f(p.part_ml[i * 2] - mu);
-    ls += a * p.part_ml[i * 2 + 1];
-    for (uint32_t k = 0; k < kMaxHeadDim / 32; ++k)
-      if (k * 32 + ln < p.head_dim) acc[k] += a * p.part_o[i * p.head_dim + k * 32 + ln];
-  }
-  for (uint32_t k = 0; k < kMaxHeadDim / 32; ++k) so[g][k * 32 + ln] = acc[k];
-  if (ln == 0) sl[g] = ls;
-  __syncthreads();
-  if (tid < p.head_dim) {
-    const uint32_t gr = t.row0 + r, tk = gr / p.group, hq = head * p.group + gr % p.group;
-    float o = 0.0f;
-    ls = 0.0f;
-    for (int i = 0; i < 8; ++i) {
-      o += so[i][tid];
-      ls += sl[i];
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t dim = d * 32 + g * 8 + half * 4;
+          if (dim < p.head_dim)
+            put4(ro, at * p.head_dim + dim, f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]});
+        }
+      if (half == 0) put2(rm, at * 2, f2{m, l});
     }
-    if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - mu);
-    o = ls > 0.0f || ls != ls ? o / ls : 0.0f;
-    ((T *)p.out)[(uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + tid] = (T)o;
+    if (last_chunk(p.counters + unit * p.n_kv_heads + head, t.n_chunks, (uint32_t *)smem))
+      join_chunks<E, DP, C::kRows, 64 * WAVES, 2>(p, t, head, part_o, part_ml, (float *)smem + 64);
   }
 }
 
@@ -720,7 +841,6 @@ hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   const hipError_t e = allow_lds((const void *)attn_rows16_kernel<E, DP>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows16_kernel<E, DP><<<grid, 64 * C::kWaves, C::kLds, st>>>(p);
-  if (plan.n_chunks > 1) attn_join_kernel<E, 16><<<plan.n_units * p.n_kv_heads * 16, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
@@ -732,7 +852,6 @@ hipError_t launch32(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   const hipError_t e = allow_lds((const void *)attn_rows32_kernel<E, DP, 4>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows32_kernel<E, DP, 4><<<grid, 256, C::kLds, st>>>(p);
-  if (plan.n_chunks > 1) attn_join_kernel<E, C::kRows><<<plan.n_units * p.n_kv_heads * C::kRows, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
@@ -760,10 +879,11 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
   const size_t reach = (size_t)window + (a.rows + group - 1) / group + 64;
   if (window && reach < max_keys) max_keys = reach;
   a.n_units = (uint32_t)(a.by_seq ? n_seqs : (n_tokens * group + a.rows - 1) / a.rows + n_seqs);
-  // Workgroups enough to fill the chip twice, chunks of 256 keys or more.
-  const size_t base = (size_t)a.n_units * n_kv_heads, want = 2 * (size_t)cus;
+  // Workgroups enough to fill the chip several times over, chunks of 256 keys
+  // or more.
+  const size_t base = (size_t)a.n_units * n_kv_heads, want = (a.rows == 16 ? 8 : 4) * (size_t)cus;
   size_t chunks = base >= want ? 1 : (want + base - 1) / base;
-  const size_t most = (max_keys + 255) / 256;
+  const size_t most = (max_keys + (a.rows == 16 ? 255 : 1023)) / (a.rows == 16 ? 256 : 1024);
   chunks = chunks > most ? most : chunks;
   chunks = chunks ? chunks : 1;
   a.chunk = (uint32_t)(((max_keys + chunks - 1) / chunks + 63) / 64 * 64);
@@ -773,6 +893,7 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
     const size_t rows = (size_t)a.n_units * n_kv_heads * a.n_chunks * a.rows;
     a.part_o_floats = rows * head_dim;
     a.part_ml_floats = rows * 2;
+    a.counters = (size_t)a.n_units * n_kv_heads;
   }
   return a;
 }

@@ -58,13 +58,14 @@ struct AttnParams {
   uint32_t chunk, n_chunks;  // keys of one workgroup, workgroups of one row tile
   float *part_o;             // [n_units][n_kv_heads][n_chunks][rows][head_dim]
   float *part_ml;            // [n_units][n_kv_heads][n_chunks][rows][2]
+  uint32_t *counters;        // [n_units][n_kv_heads], zero between launches
   uint32_t *status;
 };
 
 struct AttnPlan {
   uint32_t rows;             // rows of a tile
   uint32_t n_units, by_seq, chunk, n_chunks;
-  size_t part_o_floats, part_ml_floats;
+  size_t part_o_floats, part_ml_floats, counters;  // 0 unless n_chunks > 1
 };
 
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
