@@ -1642,10 +1642,10 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
   const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, p.window,
                                   g_dev[g_device].cus);
-  if ((uint64_t)plan.n_units * p.n_kv_heads * plan.n_chunks >= (1u << 24))
+  if (plan.n_wgs >= (1u << 24))
     return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
+  p.min_granules = plan.min_granules;
   p.n_units = plan.n_units;
-  p.by_seq = plan.by_seq;
   p.chunk = plan.chunk;
   p.n_chunks = plan.n_chunks;
   p.status = g_dev[g_device].status;
@@ -1654,7 +1654,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (!w) return require_init();
   std::lock_guard<std::mutex> wl(w->mu);
   if (w->released) return released_error();
-  if (plan.n_chunks > 1) {
+  if (plan.counters) {
     rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, plan.part_o_floats + plan.part_ml_floats, size_t(1) << 20, false,
                     "attention workspace");
     if (rc) return rc;

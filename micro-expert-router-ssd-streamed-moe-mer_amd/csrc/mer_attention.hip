@@ -19,6 +19,7 @@
 #include "mer_attention.hpp"
 
 #include <atomic>
+#include <stdlib.h>
 
 namespace mer {
 namespace {
@@ -93,14 +94,42 @@ __device__ __forceinline__ void wait_vm_barrier() {
 // This wave's LDS reads are done: what they read may be overwritten.
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The value of lane ^ 32 (^ 16).
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(lane_id() < 32 ? r[1] : r[0]);
+}
+__device__ __forceinline__ float other_row(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(lane_id() & 16 ? r[0] : r[1]);
+}
 // Maximum / sum over the four lanes that hold a 16-row tile's row.
 __device__ __forceinline__ float max_quad(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  x = fmaxf(x, other_row(x));
+  return fmaxf(x, other_half(x));
 }
 __device__ __forceinline__ float sum_quad(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  x += other_row(x);
+  return x + other_half(x);
+}
+// The same over 32 lanes.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max_32(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));   // lane ^ 1
+  x = fmaxf(x, dpp<0x4E>(x));   // lane ^ 2
+  x = fmaxf(x, dpp<0x141>(x));  // the other four of eight
+  x = fmaxf(x, dpp<0x140>(x));  // the other eight of sixteen
+  return fmaxf(x, other_row(x));
+}
+__device__ __forceinline__ float sum_32(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  x += dpp<0x140>(x);
+  return x + other_row(x);
 }
 
 // Sequence and row tile of unit u.  Sequence s owns the units from
@@ -127,52 +156,52 @@ __device__ __forceinline__ void find_unit(const AttnParams &p, uint32_t u, uint3
   *tile = uni(u >= b ? (uint32_t)(u - b) : 0xffffffffu);
 }
 
-// What one row tile of one sequence covers.
+// A sequence's rows and keys, clear of what q and the table cannot hold.
+// (Rows are below 2^26 and keys up to 2^30.)
+struct Span {
+  int32_t tok0, n;   // first token in q / out, new tokens
+  int32_t len;       // keys
+};
+__device__ __forceinline__ Span make_span(const AttnParams &p, int32_t b, int32_t e, int32_t len) {
+  const int32_t n_tokens = (int32_t)p.n_tokens, cap = (int32_t)(p.table_stride << p.page_shift);
+  Span s;
+  s.tok0 = b < 0 ? 0 : (b > n_tokens ? n_tokens : b);
+  const int32_t tok1 = e < s.tok0 ? s.tok0 : (e > n_tokens ? n_tokens : e);
+  s.n = tok1 - s.tok0;
+  s.len = len < 0 ? 0 : (len > cap ? cap : len);
+  return s;
+}
+// Keys [lo, hi) that some of the rows [row0, row1) of a span see.
+__device__ __forceinline__ void see(const AttnParams &p, const Span &s, int32_t row0, int32_t row1, int32_t *lo, int32_t *hi) {
+  const int32_t pos0 = s.len - s.n;
+  const int32_t h = pos0 + (int32_t)((uint32_t)(row1 - 1) / p.group) + 1;
+  const int32_t l = p.window ? pos0 + (int32_t)((uint32_t)row0 / p.group) - (int32_t)p.window + 1 : 0;
+  *hi = h < 0 ? 0 : h;
+  *lo = l < 0 ? 0 : (l > *hi ? *hi : l);
+}
+
+// What one row tile of one sequence covers; every field is the same in the
+// whole wave.
 struct Tile {
   uint32_t row0;     // first (token, head) row of the tile in its sequence
   uint32_t n_rows;   // rows of the sequence
   uint32_t tok0;     // first token of the sequence in q / out
   int32_t pos0;      // position of the sequence's first new token
   int32_t lo, hi;    // keys that some row of the tile sees
-  int32_t start;     // lo rounded down to whole key tiles
-  uint32_t chunk, n_chunks;
 };
-
-// Key ranges stay clear of what the table cannot hold.  (Rows are below 2^26
-// and keys up to 2^30; every field is the same in the whole wave.)
 template <int ROWS>
-__device__ __forceinline__ bool make_tile(const AttnParams &p, uint32_t seq, uint32_t tile, Tile *t) {
-  const int32_t n_tokens = (int32_t)p.n_tokens, group = (int32_t)p.group;
-  const int32_t b = sload(p.q_start, seq), e = sload(p.q_start, seq + 1);
-  const int32_t cap = (int32_t)(p.table_stride << p.page_shift);
-  int32_t len = sload(p.kv_len, seq);
-  const int32_t tok0 = b < 0 ? 0 : (b > n_tokens ? n_tokens : b);
-  const int32_t tok1 = e < tok0 ? tok0 : (e > n_tokens ? n_tokens : e);
-  const int32_t n = tok1 - tok0, rows = n * group;
+__device__ __forceinline__ bool make_tile(const AttnParams &p, const Span &s, uint32_t tile, Tile *t) {
+  const int32_t rows = s.n * (int32_t)p.group;
   if (tile >= (uint32_t)(rows + ROWS - 1) / ROWS) return false;
   const int32_t row0 = (int32_t)tile * ROWS;
-  len = len < 0 ? 0 : (len > cap ? cap : len);
-  const int32_t last = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
-  const int32_t pos0 = len - n;
-  int32_t hi = pos0 + (int32_t)((uint32_t)last / p.group) + 1;
-  hi = hi < 0 ? 0 : hi;
-  int32_t lo = p.window ? pos0 + (int32_t)((uint32_t)row0 / p.group) - (int32_t)p.window + 1 : 0;
-  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
+  int32_t lo, hi;
+  see(p, s, row0, row0 + ROWS < rows ? row0 + ROWS : rows, &lo, &hi);
   t->row0 = uni((uint32_t)row0);
   t->n_rows = uni((uint32_t)rows);
-  t->tok0 = uni((uint32_t)tok0);
-  t->pos0 = (int32_t)uni((uint32_t)pos0);
+  t->tok0 = uni((uint32_t)s.tok0);
+  t->pos0 = (int32_t)uni((uint32_t)(s.len - s.n));
   t->lo = (int32_t)uni((uint32_t)lo);
   t->hi = (int32_t)uni((uint32_t)hi);
-  t->start = t->lo & ~63;
-  const uint32_t keys = (uint32_t)(t->hi - t->start);
-  // A by_seq unit has partial sums for its first tile only: the tiles of a
-  // sequence longer than the plan says are done in one piece.
-  const uint32_t parts = p.by_seq && tile ? 1 : p.n_chunks;
-  uint32_t c = (keys + parts - 1) / parts;
-  c = (c + 63) & ~63u;
-  t->chunk = uni(c < p.chunk ? p.chunk : c);
-  t->n_chunks = uni(keys ? (keys + t->chunk - 1) / t->chunk : 1);
   return true;
 }
 
@@ -328,12 +357,12 @@ __device__ __forceinline__ bool last_chunk(uint32_t *counter, uint32_t n_chunks,
 
 // Adds up a tile's chunks.  32 lanes hold a row's dims; the groups of 32 take
 // U rows each at a time, or share a row's chunks where there are fewer rows
-// than groups.  `lds`: [threads / 32][DP + 1] floats.
-template <class E, int DP, int ROWS, int THREADS, int U>
-__device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, uint32_t head, float *part_o,
-                                            float *part_ml, float *lds) {
+// than groups.  Chunk c is at slot(c) of the partial sums.  `lds`: [threads / 32][DP + 1] floats.
+template <class E, int DP, int ROWS, int THREADS, int U, class Slot>
+__device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, uint32_t head, uint32_t n_chunks,
+                                            Slot slot, float *part_o, float *part_ml, float *lds) {
   typedef typename E::T T;
-  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = 4;
+  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = 8 / U * 4 / (kDims < 4 ? 4 : kDims);
   typedef float fd __attribute__((ext_vector_type(kDims)));
   typedef T td __attribute__((ext_vector_type(kDims)));
   const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
@@ -342,67 +371,80 @@ __device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, 
   const uint32_t share = rows < kGroups ? kGroups / rows : 1;  // groups of a row
   const uint32_t step = kGroups / share;                       // rows at a time
   auto ml_of = [&](uint32_t c, uint32_t r, bool ok) {
-    return __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(rm, ok ? (c * ROWS + r) * 8 : 0xfffffff0u, 0, kDeviceScope));
+    const f2 none = {-__builtin_inff(), 0.0f};
+    const f2 ml = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(rm, ok ? (slot(c) * ROWS + r) * 8 : 0u, 0, kDeviceScope));
+    return ok ? ml : none;
+  };
+  auto o_of = [&](uint32_t c, uint32_t r, bool ok) {
+    const uint32_t at = ok && dim < p.head_dim ? ((slot(c) * ROWS + r) * p.head_dim + dim) * 4 : 0xfffffff0u;  // zeros
+    if constexpr (kDims == 2) {
+      return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
+    } else if constexpr (kDims == 4) {
+      return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
+    } else {
+      const f4 lo = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
+      const f4 hi = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 16, kDeviceScope));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   };
   for (uint32_t r0 = 0; r0 < rows; r0 += step * U) {
     uint32_t r[U];
     bool ok[U];
     float m[U], l[U];
-    fd acc[U];
+    f2 first[U];  // of the chunks 0 .. 31, a lane each
+    fd acc[U], x[U][kBatch];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       r[u] = r0 + u * step + g / share;
       ok[u] = g / share < step && r[u] < rows;
-      f2 ml = ml_of(ln, r[u], ok[u] && ln < t.n_chunks);
-      m[u] = ln < t.n_chunks ? ml[0] : -__builtin_inff();
-      l[u] = ln < t.n_chunks ? ml[1] : 0.0f;
-      for (uint32_t c = ln + 32; c < t.n_chunks; c += 32) {
-        ml = ml_of(c, r[u], ok[u]);
+      first[u] = ml_of(ln, r[u], ok[u] && ln < n_chunks);
+      acc[u] = fd{};
+    }
+    // The first batch of sums is under way with the weights.
+    auto load = [&](uint32_t c0, uint32_t k0, uint32_t end) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t k = k0 + b * share + g % share;
+          x[u][b] = o_of(c0 + k, r[u], ok[u] && k < end);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load(0, 0, n_chunks < 32 ? n_chunks : 32);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = first[u][0];
+      l[u] = first[u][1];
+      for (uint32_t c0 = 32; c0 < n_chunks; c0 += 32) {
+        const f2 ml = ml_of(c0 + ln, r[u], ok[u] && c0 + ln < n_chunks);
         const float mn = fmaxf(m[u], ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
         l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
         m[u] = mn;
       }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float mm = m[u];
-#pragma unroll
-      for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-      const float mu = mm == -__builtin_inff() ? 0.0f : mm;
-      l[u] *= __builtin_amdgcn_exp2f(m[u] - mu);
-#pragma unroll
-      for (int d = 16; d; d >>= 1) l[u] += __shfl_xor(l[u], d);
+      const float mm = max_32(m[u]), mu = mm == -__builtin_inff() ? 0.0f : mm;
+      l[u] = sum_32(l[u] * __builtin_amdgcn_exp2f(m[u] - mu));
       m[u] = mu;
-      acc[u] = fd{};
     }
-    for (uint32_t c0 = g % share; c0 < t.n_chunks; c0 += share * kBatch) {
-      fd x[U][kBatch];
-      float w[U][kBatch];
+    for (uint32_t c0 = 0; c0 < n_chunks; c0 += 32) {
+      float w[U];  // weight of chunk c0 + lane
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        const f2 ml = c0 ? ml_of(c0 + ln, r[u], ok[u] && c0 + ln < n_chunks) : first[u];
+        w[u] = __builtin_amdgcn_exp2f(ml[0] - m[u]);
+      }
+      const uint32_t end = n_chunks - c0 < 32 ? n_chunks - c0 : 32;
+      for (uint32_t k0 = 0; k0 < end; k0 += share * kBatch) {
+        if (c0 + k0) load(c0, k0, end);
 #pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          const uint32_t c = c0 + b * share;
-          const bool in = ok[u] && c < t.n_chunks;
-          w[u][b] = ml_of(c, r[u], in)[0];
-          const uint32_t at = in && dim < p.head_dim ? ((c * ROWS + r[u]) * p.head_dim + dim) * 4 : 0xfffffff0u;
-          if constexpr (kDims == 2) {
-            x[u][b] = __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
-          } else if constexpr (kDims == 4) {
-            x[u][b] = __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
-          } else {
-            const f4 lo = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
-            const f4 hi = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 16, kDeviceScope));
-            x[u][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t k = k0 + b * share + g % share;
+            const float wk = __shfl(w[u], (int)((threadIdx.x & 32) + (k & 31)));
+            acc[u] += x[u][b] * (k < end ? wk : 0.0f);
           }
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          const uint32_t c = c0 + b * share;
-          if (c < t.n_chunks) acc[u] += x[u][b] * __builtin_amdgcn_exp2f(w[u][b] - m[u]);
-        }
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -425,18 +467,105 @@ __device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, 
   }
 }
 
-// Sixteen rows: decode and short chunks.  The waves of a workgroup take the
-// chunk's tiles of 32 keys in turn, each with a ring of LDS of its own (no
-// barriers while the keys stream), and join their sums at the end.
-constexpr int waves16(int dp) { return dp == 256 ? 2 : 4; }
+// Sixteen rows: decode and short chunks.
+//
+// The work is cut into pieces of equal length whatever the sequences are: a
+// granule is kGranule keys of one (row tile, kv head), the granules of all
+// sequences stand in a row (sequence by sequence, unit by unit), and each
+// workgroup takes an equal stretch of them.  A unit that a stretch's end cuts
+// is joined from its pieces.  Nothing of this depends on the host's knowing
+// the lengths.
+//
+// The waves of a workgroup take a piece's tiles of 32 keys in turn, each with
+// a ring of LDS of its own (no barriers while the keys stream), and join
+// their sums at the piece's end.
+constexpr int waves16(int dp) { return dp == 64 ? 4 : 2; }
 template <int DP>
 struct Rows16 {
   static constexpr int kWaves = waves16(DP);
   static constexpr int kKeys = 32;
+  static constexpr int kGranule = 128;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kStages = 2;
   static constexpr int kLoads = Share<DP, kKeys>::kLoads;
   static constexpr int kLds = kWaves * kStages * 2 * kTileBytes;
+};
+
+// Walks the sequences' granules; a wave looks at 256 sequences at a time, four
+// to a lane.  (The host keeps the total below 2^31.)
+struct Granules {
+  uint32_t base, total;  // granules before the sequences in view, of those in view
+  uint32_t upto;         // of the lanes up to this one, within the view
+  uint32_t w[4];
+  int32_t q[5], len[4];  // their q_start and kv_len
+  uint32_t seq0;
+
+  template <int GRANULE>
+  __device__ __forceinline__ void view(const AttnParams &p, uint32_t first) {
+    seq0 = first;
+    const uint32_t s0 = first + lane_id() * 4;
+#pragma unroll
+    for (uint32_t i = 0; i < 5; ++i) {
+      q[i] = p.q_start[s0 + i < p.n_seqs ? s0 + i : p.n_seqs];
+      if (i < 4) len[i] = p.kv_len[s0 + i < p.n_seqs ? s0 + i : 0];
+    }
+    upto = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const Span s = make_span(p, q[i], q[i + 1], len[i]);  // past the last sequence: no rows
+      const uint32_t rows = (uint32_t)s.n * p.group;
+      w[i] = (rows + 15) / 16 * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
+      upto += w[i];
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t x = __shfl_up(upto, d);
+      upto += lane_id() >= (uint32_t)d ? x : 0;
+    }
+    total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+
+  // The sequence at granule x of the view or a later one: its number, the
+  // granules before it and its span.  False if there is none (lengths that
+  // change under the kernel).
+  template <int GRANULE>
+  __device__ __forceinline__ bool find(const AttnParams &p, uint32_t x, uint32_t *seq, uint32_t *before, Span *span) {
+    while (x >= base + total && seq0 + 256 < p.n_seqs) {
+      base += total;
+      view<GRANULE>(p, seq0 + 256);
+    }
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(base + upto > x);
+    if (!beyond) return false;
+    const int at = __builtin_ctzll(beyond);
+    auto get = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+    const uint32_t w0 = get(w[0]), w1 = get(w[1]), w2 = get(w[2]), w3 = get(w[3]);
+    const uint32_t b0 = base + get(upto) - w0 - w1 - w2 - w3, b1 = b0 + w0, b2 = b1 + w1, b3 = b2 + w2;
+    const int i = (x >= b1) + (x >= b2) + (x >= b3);
+    *seq = seq0 + (uint32_t)(at * 4 + i);
+    *before = i == 0 ? b0 : (i == 1 ? b1 : (i == 2 ? b2 : b3));
+    int32_t v[5], n[4];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      v[k] = (int32_t)get((uint32_t)q[k]);
+      if (k < 4) n[k] = (int32_t)get((uint32_t)len[k]);
+    }
+    const int32_t vb = i == 0 ? v[0] : (i == 1 ? v[1] : (i == 2 ? v[2] : v[3]));
+    const int32_t ve = i == 0 ? v[1] : (i == 1 ? v[2] : (i == 2 ? v[3] : v[4]));
+    *span = make_span(p, vb, ve, i == 0 ? n[0] : (i == 1 ? n[1] : (i == 2 ? n[2] : n[3])));
+    return true;
+  }
+
+  // Granules of each of a sequence's units, over the keys that its rows see.
+  template <int GRANULE>
+  static __device__ __forceinline__ uint32_t granules(const AttnParams &p, const Span &s, int32_t *start) {
+    if (s.n == 0) return 0;
+    int32_t lo, hi;
+    see(p, s, 0, s.n * (int32_t)p.group, &lo, &hi);
+    lo &= ~31;
+    if (start) *start = lo;
+    const uint32_t g = (uint32_t)(hi - lo + GRANULE - 1) / GRANULE;
+    return g ? g : 1;  // rows without keys are done, too
+  }
 };
 
 template <class E, int DP>
@@ -447,21 +576,52 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
   typedef typename E::T T;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
-  const uint32_t head = blockIdx.x % p.n_kv_heads;
-  const uint32_t rest = blockIdx.x / p.n_kv_heads;
-  const uint32_t c = rest % p.n_chunks, unit = rest / p.n_chunks;
-  uint32_t seq = unit, tile = 0;
-  if (!p.by_seq) find_unit<16>(p, unit, &seq, &tile);
-  for (;; ++tile) {
-  Tile t;
-  if (!make_tile<16>(p, seq, tile, &t)) return;
   const uint32_t col = lane % 16, quad = lane / 16;
-  if (c < t.n_chunks) {
+
+  Granules gr;
+  gr.base = 0;
+  gr.view<C::kGranule>(p, 0);
+  uint32_t all = gr.total;
+  if (p.n_seqs > 256) {
+    for (uint32_t s = 256; s < p.n_seqs; s += 256) {
+      gr.view<C::kGranule>(p, s);
+      all += gr.total;
+    }
+    gr.view<C::kGranule>(p, 0);
+  }
+  uint32_t per = uni((all + gridDim.x - 1) / gridDim.x);
+  per = per < p.min_granules ? p.min_granules : per;
+  uint32_t x = blockIdx.x * per;
+  const uint32_t x1 = all - (all < x ? all : x) < per ? all : x + per;
+  bool first_piece = true;
+  while (x < x1) {
+    uint32_t seq, before;
+    Span span;
+    if (!gr.find<C::kGranule>(p, x, &seq, &before, &span)) return;
+    int32_t start = 0;
+    const uint32_t n_gran = uni(Granules::granules<C::kGranule>(p, span, &start));
+    const uint32_t unit = uni((x - before) / n_gran), tile = uni(unit / p.n_kv_heads), head = unit - tile * p.n_kv_heads;
+    const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
+    const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
+    // the unit's pieces: workgroups first_wg .. first_wg + n_pieces - 1
+    const uint32_t first_wg = g0 == 0 ? blockIdx.x : uni(unit0 / per);
+    const uint32_t n_pieces = uni((unit0 + n_gran - 1) / per) - first_wg + 1;
+    const uint32_t first_slot = 2 * first_wg + (first_wg * per == unit0 ? 0 : 1);
+    const uint32_t my_slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+    first_piece = false;
+    x += count;
+    Tile t;
+    make_tile<16>(p, span, tile, &t);  // the tile is one of the sequence's
+    start = (int32_t)uni((uint32_t)start);
+    int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
+    if (p.window && begin < (t.lo & ~31)) begin = t.lo & ~31;
+    end = end < t.hi ? end : t.hi;
+
     // Q^T: lane column = row of the tile, 8 consecutive dims per 32-dim slab
     const uint32_t row = t.row0 + col;
     const bool row_ok = row < t.n_rows;
     const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
-    const int32_t pos = t.pos0 + (int32_t)tok;
+    const int32_t pos = t.pos0 + (int32_t)tok, window = p.window ? (int32_t)p.window : 0x40000000;
     V8 q[DP / 32];
     const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
@@ -473,16 +633,13 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
     const uint32_t last = t.row0 + 15 < t.n_rows ? t.row0 + 15 : t.n_rows - 1;
     const int32_t pos_first = t.pos0 + (int32_t)(t.row0 / p.group), pos_last = t.pos0 + (int32_t)(last / p.group);
 
-    const int32_t begin = t.start + (int32_t)(c * t.chunk);
-    int32_t end = begin + (int32_t)t.chunk;
-    end = end < t.hi ? end : t.hi;
-    const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
+    const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
     const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem +
                           wave * (C::kStages * 2 * C::kTileBytes);
     auto key_of = [&](int32_t i) { return begin + (i * C::kWaves + (int32_t)wave) * C::kKeys; };
     auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
-    __syncthreads();  // the last tile's join is done with the LDS
+    __syncthreads();  // the last piece is done with the LDS
     Share<DP, C::kKeys> sh;
     sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t);
     if (mine > 0) sh.lookup(key_of(0));
@@ -531,11 +688,12 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = s[e / 4][e % 4] * p.scale_log2;
       const int32_t key_end = key0 + C::kKeys;
-      if (key_end > pos_first + 1 || key_end > t.hi || (p.window && key0 <= pos_last - (int32_t)p.window)) {
+      if (key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window) {
+        const int32_t last = pos - key0 - (int32_t)quad * 4, before = last - window;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int32_t key = key0 + (e / 4) * 16 + (int32_t)quad * 4 + e % 4;
-          if (key > pos || (p.window && key <= pos - (int64_t)p.window)) x[e] = -__builtin_inff();
+          const int32_t at = (e / 4) * 16 + e % 4;
+          x[e] = at > last || at <= before ? -__builtin_inff() : x[e];
         }
       }
       float mx = x[0];
@@ -589,12 +747,10 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[(wave * 16 + col) * DP + d * 16 + quad * 4] = o[d];
     __syncthreads();
-    const uint64_t part = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks * 16;
-    float *part_o = p.part_o + part * p.head_dim, *part_ml = p.part_ml + part * 2;
-    const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
+    const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);
     for (uint32_t w = tid; w < 16 * (DP / 8); w += 64 * C::kWaves) {
-      const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, gr = t.row0 + r;
-      if (gr >= t.n_rows || d >= p.head_dim) continue;
+      const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, rr = t.row0 + r;
+      if (rr >= t.n_rows || d >= p.head_dim) continue;
       float mm = -__builtin_inff();
 #pragma unroll
       for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * 16 + r) * 2]);
@@ -607,23 +763,22 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
         ls += a * jm[(v * 16 + r) * 2 + 1];
         acc += a * *(const f8 *)&jo[(v * 16 + r) * DP + d];
       }
-      const uint32_t tk = gr / p.group, hq = head * p.group + gr % p.group;
-      if (t.n_chunks == 1) {
+      const uint32_t tk = rr / p.group, hq = head * p.group + rr % p.group;
+      if (n_pieces == 1) {
         if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - (mm == -__builtin_inff() ? 0.0f : mm));
         const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
         const V8 r8 = __builtin_convertvector(acc * inv, V8);
         *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
       } else {
-        const uint32_t at = c * 16 + r;
-        put4(ro, at * p.head_dim + d, f4{acc[0], acc[1], acc[2], acc[3]});
-        put4(ro, at * p.head_dim + d + 4, f4{acc[4], acc[5], acc[6], acc[7]});
-        if (d == 0) put2(rm, at * 2, f2{mm, ls});
+        const uint32_t to = my_slot * 16 + r;
+        put4(ro, to * p.head_dim + d, f4{acc[0], acc[1], acc[2], acc[3]});
+        put4(ro, to * p.head_dim + d + 4, f4{acc[4], acc[5], acc[6], acc[7]});
+        if (d == 0) put2(rm, to * 2, f2{mm, ls});
       }
     }
-    if (t.n_chunks > 1 && last_chunk(p.counters + unit * p.n_kv_heads + head, t.n_chunks, (uint32_t *)(jm + C::kWaves * 32)))
-      join_chunks<E, DP, 16, 64 * C::kWaves, 1>(p, t, head, part_o, part_ml, jo);
-  }
-  if (!p.by_seq) return;
+    if (n_pieces > 1 && last_chunk(p.counters + first_wg, n_pieces, (uint32_t *)(jm + C::kWaves * 32)))
+      join_chunks<E, DP, 16, 64 * C::kWaves, 1>(
+          p, t, head, n_pieces, [&](uint32_t c) { return c ? 2 * (first_wg + c) : first_slot; }, p.part_o, p.part_ml, jo);
   }
 }
 
@@ -654,12 +809,20 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   uint32_t seq, tile;
   find_unit<C::kRows>(p, unit, &seq, &tile);
   Tile t;
-  if (!make_tile<C::kRows>(p, seq, tile, &t) || c >= t.n_chunks) return;
+  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
+  if (!make_tile<C::kRows>(p, span, tile, &t)) return;
+  // chunks: the plan's, longer ones where the keys are more than it was told
+  const int32_t start = t.lo & ~(C::kKeys - 1);
+  const uint32_t keys = (uint32_t)(t.hi - start);
+  uint32_t chunk = ((keys + p.n_chunks - 1) / p.n_chunks + C::kKeys - 1) & ~(C::kKeys - 1);
+  chunk = uni(chunk < p.chunk ? p.chunk : chunk);
+  const uint32_t n_chunks = uni(keys ? (keys + chunk - 1) / chunk : 1);
+  if (c >= n_chunks) return;
   const uint32_t col = lane % 32, half = lane / 32;
   const uint32_t row = t.row0 + wave * 32 + col;
   const bool row_ok = row < t.n_rows;
   const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
-  const int32_t pos = t.pos0 + (int32_t)tok;
+  const int32_t pos = t.pos0 + (int32_t)tok, window = p.window ? (int32_t)p.window : 0x40000000;
   // the wave's positions; a wave without rows has none (first > last)
   const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
   const bool any = wrow < t.n_rows;
@@ -676,8 +839,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     if (p.scale_log2 < 0) q[s] = -q[s];
   }
 
-  const int32_t begin = t.start + (int32_t)(c * t.chunk);
-  int32_t end = begin + (int32_t)t.chunk;
+  const int32_t begin = start + (int32_t)(c * chunk);
+  int32_t end = begin + (int32_t)chunk;
   end = end < t.hi ? end : t.hi;
   const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
@@ -713,7 +876,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
       sh.lookup(my_key + (i + 2) * C::kKeys);
       sh.template copy<false>(stage(i + 1) + my_lds);
     }
-    const bool live = any && key0 <= pos_last && !(p.window && key0 + C::kKeys <= pos_first - (int32_t)p.window + 1);
+    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
     V8 pr[4];
     if (live) {
       f16v s[2];
@@ -729,19 +892,20 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         }
       }
       if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi ||
-          (p.window && key0 <= pos_last - (int32_t)p.window)) {
+          key0 <= pos_last - window) {
+        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int32_t key = key0 + b * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
-            if (key > pos || (p.window && key <= pos - (int64_t)p.window)) s[b][e] = -__builtin_inff();
+            const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
+            s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
           }
       }
       float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
+      mx = fmaxf(mx, other_half(mx)) * scale;
       // The maximum in use may lag by up to 8 (weights up to 2^8): O and l
       // are scaled only when it would lag by more.
       if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
@@ -787,8 +951,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         }
     }
   }
-  l += __shfl_xor(l, 32);
-  if (t.n_chunks == 1) {
+  l += other_half(l);
+  if (n_chunks == 1) {
     if (!row_ok) return;
     if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - (m == -__builtin_inff() ? 0.0f : m));
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -818,8 +982,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         }
       if (half == 0) put2(rm, at * 2, f2{m, l});
     }
-    if (last_chunk(p.counters + unit * p.n_kv_heads + head, t.n_chunks, (uint32_t *)smem))
-      join_chunks<E, DP, C::kRows, 64 * WAVES, 2>(p, t, head, part_o, part_ml, (float *)smem + 64);
+    if (last_chunk(p.counters + unit * p.n_kv_heads + head, n_chunks, (uint32_t *)smem))
+      join_chunks<E, DP, C::kRows, 64 * WAVES, 2>(
+          p, t, head, n_chunks, [](uint32_t k) { return k; }, part_o, part_ml, (float *)smem + 64);
   }
 }
 
@@ -836,22 +1001,20 @@ hipError_t allow_lds(const void *fn, int bytes, std::atomic<uint64_t> *devices) 
 template <class E, int DP>
 hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   typedef Rows16<DP> C;
-  const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
   static std::atomic<uint64_t> devices{0};
   const hipError_t e = allow_lds((const void *)attn_rows16_kernel<E, DP>, C::kLds, &devices);
   if (e != hipSuccess) return e;
-  attn_rows16_kernel<E, DP><<<grid, 64 * C::kWaves, C::kLds, st>>>(p);
+  attn_rows16_kernel<E, DP><<<plan.n_wgs, 64 * C::kWaves, C::kLds, st>>>(p);
   return hipGetLastError();
 }
 
 template <class E, int DP>
 hipError_t launch32(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   typedef Rows32<DP, 4> C;
-  const uint32_t grid = plan.n_units * plan.n_chunks * p.n_kv_heads;
   static std::atomic<uint64_t> devices{0};
   const hipError_t e = allow_lds((const void *)attn_rows32_kernel<E, DP, 4>, C::kLds, &devices);
   if (e != hipSuccess) return e;
-  attn_rows32_kernel<E, DP, 4><<<grid, 256, C::kLds, st>>>(p);
+  attn_rows32_kernel<E, DP, 4><<<plan.n_wgs, 256, C::kLds, st>>>(p);
   return hipGetLastError();
 }
 
@@ -869,31 +1032,40 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 
 }  // namespace
 
+static size_t envi(const char *n, size_t d) { const char *v = getenv(n); return v ? (size_t)atoi(v) : d; }
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                    size_t max_q_len, size_t max_kv_len, uint32_t window, int cus) {
   AttnPlan a{};
   a.rows = max_q_len * group <= 32 ? 16 : 128;
-  a.by_seq = max_q_len * group <= a.rows;
+  if (a.rows == 16) {
+    a.n_wgs = (uint32_t)cus * envi("W16", 2);
+    a.min_granules = envi("M16", 2);
+    a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
+    a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
+    a.counters = a.n_wgs;
+    return a;
+  }
+  a.n_units = (uint32_t)((n_tokens * group + a.rows - 1) / a.rows + n_seqs);
   // keys of a row tile, from a whole key tile's start on
   size_t max_keys = max_kv_len;
   const size_t reach = (size_t)window + (a.rows + group - 1) / group + 64;
   if (window && reach < max_keys) max_keys = reach;
-  a.n_units = (uint32_t)(a.by_seq ? n_seqs : (n_tokens * group + a.rows - 1) / a.rows + n_seqs);
-  // Workgroups enough to fill the chip several times over, chunks of 256 keys
+  // Workgroups enough to fill the chip several times over, chunks of 1024 keys
   // or more.
-  const size_t base = (size_t)a.n_units * n_kv_heads, want = (a.rows == 16 ? 8 : 4) * (size_t)cus;
+  const size_t base = (size_t)a.n_units * n_kv_heads, want = envi("W32", 4) * (size_t)cus;
   size_t chunks = base >= want ? 1 : (want + base - 1) / base;
-  const size_t most = (max_keys + (a.rows == 16 ? 255 : 1023)) / (a.rows == 16 ? 256 : 1024);
+  const size_t most = (max_keys + 1023) / 1024;
   chunks = chunks > most ? most : chunks;
   chunks = chunks ? chunks : 1;
   a.chunk = (uint32_t)(((max_keys + chunks - 1) / chunks + 63) / 64 * 64);
   a.chunk = a.chunk ? a.chunk : 64;
   a.n_chunks = (uint32_t)chunks;
+  a.n_wgs = (uint32_t)(base * chunks < UINT32_MAX ? base * chunks : UINT32_MAX);
   if (a.n_chunks > 1) {
-    const size_t rows = (size_t)a.n_units * n_kv_heads * a.n_chunks * a.rows;
+    const size_t rows = (size_t)a.n_wgs * a.rows;
     a.part_o_floats = rows * head_dim;
     a.part_ml_floats = rows * 2;
-    a.counters = (size_t)a.n_units * n_kv_heads;
+    a.counters = base;
   }
   return a;
 }

@@ -53,19 +53,20 @@ struct AttnParams {
   uint32_t window;           // 0 = none
   float scale_log2;          // scale * log2(e)
   // decomposition (attn_plan)
-  uint32_t n_units;          // row tiles of a kv head (an upper bound)
-  uint32_t by_seq;           // unit = sequence: every sequence has at most one row tile
-  uint32_t chunk, n_chunks;  // keys of one workgroup, workgroups of one row tile
-  float *part_o;             // [n_units][n_kv_heads][n_chunks][rows][head_dim]
-  float *part_ml;            // [n_units][n_kv_heads][n_chunks][rows][2]
-  uint32_t *counters;        // [n_units][n_kv_heads], zero between launches
+  uint32_t min_granules;     // 16-row tiles: least granules of a workgroup
+  uint32_t n_units;          // 128-row tiles of a kv head (an upper bound)
+  uint32_t chunk, n_chunks;  // 128-row tiles: keys of one workgroup, workgroups of one row tile
+  float *part_o;             // partial sums [slot][rows][head_dim]
+  float *part_ml;            // their maxima and weights [slot][rows][2]
+  uint32_t *counters;        // finished pieces of a row tile, zero between launches
   uint32_t *status;
 };
 
 struct AttnPlan {
   uint32_t rows;             // rows of a tile
-  uint32_t n_units, by_seq, chunk, n_chunks;
-  size_t part_o_floats, part_ml_floats, counters;  // 0 unless n_chunks > 1
+  uint32_t n_wgs;
+  uint32_t min_granules, n_units, chunk, n_chunks;
+  size_t part_o_floats, part_ml_floats, counters;  // workspace
 };
 
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
