@@ -869,28 +869,60 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     const int32_t key0 = begin + i * C::kKeys;
     const uint32_t kb = stage(i), vb = kb + C::kTileBytes;
     const bool more = i + 1 < n_tiles;
-    // all waves' copies of K, and everyone is done with the other stage
-    wait_vm_barrier<C::kLoads>();
+    // all waves' copies of this tile are there, and everyone is done with the
+    // other stage, which the next tile's copies fill meanwhile
+    wait_vm_barrier<0>();
     if (more) {
       sh.advance(p.status);
       sh.lookup(my_key + (i + 2) * C::kKeys);
       sh.template copy<false>(stage(i + 1) + my_lds);
+      sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
     }
     const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
-    V8 pr[4];
     if (live) {
+      // V's operand for 16 keys and 32 dims: 4 + 4 keys in the order in which
+      // the scores lie in their lanes
+      auto v_of = [&](int ks, int d) {
+        s4 x[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t r = ks * 16 + b * 8 + half * 4 + lane % 16 / 4;
+          const uint32_t piece = (d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r);
+          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + lane % 2 * 8));
+        }
+        return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
       f16v s[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+      // operands are read a batch ahead of the products, so that the reads'
+      // latency is paid once a batch and not once a product
+      constexpr int kBatch = DP / 16 < 8 ? DP / 16 : 8;
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          const uint32_t r = b * 32 + col, piece = (d * 2 + half) ^ L::k_swizzle(r);
-          const V8 k = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
-          s[b] = E::mfma32(k, q[d], s[b]);
-        }
+      for (int d0 = 0; d0 < DP / 16; d0 += kBatch) {
+        V8 k[2][kBatch];
+#pragma unroll
+        for (int d = 0; d < kBatch; ++d)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t r = b * 32 + col, piece = ((d0 + d) * 2 + half) ^ L::k_swizzle(r);
+            k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < kBatch; ++d)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[b] = E::mfma32(k[b][d], q[d0 + d], s[b]);
       }
+      V8 v[2][DP / 32];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, d);
+      __builtin_amdgcn_sched_barrier(0);
       if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi ||
           key0 <= pos_last - window) {
         const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
@@ -917,38 +949,28 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         for (int d = 0; d < DP / 32; ++d) o[d] *= a;
       }
       const float mu = m == -__builtin_inff() ? 0.0f : m;
+      V8 pr[4];
+      float sums[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int ks = 0; ks < 4; ++ks) {
+        f8 x;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f8 x;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][h * 8 + e], scale, -mu));
-            l += x[e];
-          }
-          pr[b * 2 + h] = __builtin_convertvector(x, V8);
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
+          sums[e % 2] += x[e];
         }
-    }
-    if (more) wait_vm_barrier<C::kLoads>();
-    else wait_vm_barrier<0>();
-    if (more) sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
-    if (live) {
+        pr[ks] = __builtin_convertvector(x, V8);
+      }
+      l += sums[0] + sums[1];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
+      for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          s4 v[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t r = ks * 16 + b * 8 + half * 4 + lane % 16 / 4;
-            const uint32_t piece = (d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r);
-            v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + lane % 2 * 8));
-          }
-          const s8 vv = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-          o[d] = E::mfma32(__builtin_bit_cast(V8, vv), pr[ks], o[d]);
+          o[d] = E::mfma32(v[ks % 2][d], pr[ks], o[d]);
+          if (ks < 2) v[ks % 2][d] = v_of(ks + 2, d);
         }
+      }
     }
   }
   l += other_half(l);
