@@ -1654,7 +1654,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (!w) return require_init();
   std::lock_guard<std::mutex> wl(w->mu);
   if (w->released) return released_error();
-  if (plan.counters) {
+  if (plan.part_o_floats) {
     rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, plan.part_o_floats + plan.part_ml_floats, size_t(1) << 20, false,
                     "attention workspace");
     if (rc) return rc;

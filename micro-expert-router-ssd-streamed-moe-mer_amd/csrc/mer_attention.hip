@@ -19,6 +19,7 @@
 #include "mer_attention.hpp"
 
 #include <atomic>
+#include <math.h>
 #include <stdlib.h>
 
 namespace mer {
@@ -795,6 +796,16 @@ struct Rows32 {
   static constexpr int kLds = 2 * 2 * kTileBytes;
 };
 
+// Keys of a chunk and chunks of a tile: the plan's, longer ones where the keys
+// are more than it was told.
+template <int KEYS>
+__device__ __forceinline__ void chunks_of(const AttnParams &p, const Tile &t, uint32_t *chunk, uint32_t *n_chunks) {
+  const uint32_t keys = (uint32_t)(t.hi - (t.lo & ~(KEYS - 1)));
+  const uint32_t c = ((keys + p.n_chunks - 1) / p.n_chunks + KEYS - 1) & ~(KEYS - 1);
+  *chunk = uni(c < p.chunk ? p.chunk : c);
+  *n_chunks = uni(keys ? (keys + *chunk - 1) / *chunk : 1);
+}
+
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_kernel(AttnParams p) {
   typedef Rows32<DP, WAVES> C;
@@ -805,18 +816,17 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
   const uint32_t head = blockIdx.x % p.n_kv_heads;
   const uint32_t rest = blockIdx.x / p.n_kv_heads;
-  const uint32_t c = rest % p.n_chunks, unit = p.n_units - 1 - rest / p.n_chunks;  // late rows, with more keys, first
+  // Chunk by chunk, so that neighbours are alike (workgroups go round the
+  // shader engines in a fixed order); late rows, with more keys, first.
+  const uint32_t c = rest / p.n_units, unit = p.n_units - 1 - rest % p.n_units;
   uint32_t seq, tile;
   find_unit<C::kRows>(p, unit, &seq, &tile);
   Tile t;
   const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
   if (!make_tile<C::kRows>(p, span, tile, &t)) return;
-  // chunks: the plan's, longer ones where the keys are more than it was told
+  uint32_t chunk, n_chunks;
+  chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
   const int32_t start = t.lo & ~(C::kKeys - 1);
-  const uint32_t keys = (uint32_t)(t.hi - start);
-  uint32_t chunk = ((keys + p.n_chunks - 1) / p.n_chunks + C::kKeys - 1) & ~(C::kKeys - 1);
-  chunk = uni(chunk < p.chunk ? p.chunk : chunk);
-  const uint32_t n_chunks = uni(keys ? (keys + chunk - 1) / chunk : 1);
   if (c >= n_chunks) return;
   const uint32_t col = lane % 32, half = lane / 32;
   const uint32_t row = t.row0 + wave * 32 + col;
@@ -989,24 +999,61 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x * inv, T4);
       }
   } else {
-    const uint64_t part = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks * C::kRows;
-    float *part_o = p.part_o + part * p.head_dim, *part_ml = p.part_ml + part * 2;
-    const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
-    const uint32_t at = c * C::kRows + wave * 32 + col;
-    if (row_ok) {
+    // A partial sum lies as the accumulators do, so every store is a whole
+    // kilobyte.
+    const uint64_t slot = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c;
+    float *po = p.part_o + (slot * WAVES + wave) * (32 * DP) + lane * 4;
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t dim = d * 32 + g * 8 + half * 4;
-          if (dim < p.head_dim)
-            put4(ro, at * p.head_dim + dim, f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]});
-        }
-      if (half == 0) put2(rm, at * 2, f2{m, l});
-    }
-    if (last_chunk(p.counters + unit * p.n_kv_heads + head, n_chunks, (uint32_t *)smem))
-      join_chunks<E, DP, C::kRows, 64 * WAVES, 2>(
-          p, t, head, n_chunks, [](uint32_t k) { return k; }, part_o, part_ml, (float *)smem + 64);
+      for (int g = 0; g < 4; ++g)
+        *(f4 *)(po + (d * 4 + g) * 256) = f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+    if (half == 0) *(f2 *)(p.part_ml + ((slot * WAVES + wave) * 32 + col) * 2) = f2{m, l};
+  }
+}
+
+// Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
+// its accumulators spread over four waves.
+template <class E, int DP, int WAVES>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+  typedef Rows32<DP, WAVES> C;
+  typedef typename E::T T;
+  constexpr int kVecs = DP / 32;  // 1 KiB vectors of accumulators of each of the four waves
+  const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64), col = lane % 32, half = lane / 32;
+  const uint32_t w = blockIdx.x % WAVES, uh = blockIdx.x / WAVES, head = uh % p.n_kv_heads, unit = uh / p.n_kv_heads;
+  uint32_t seq, tile, chunk, n_chunks;
+  find_unit<C::kRows>(p, unit, &seq, &tile);
+  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
+  Tile t;
+  if (!make_tile<C::kRows>(p, span, tile, &t)) return;
+  chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
+  const uint32_t row = t.row0 + w * 32 + col;
+  if (n_chunks == 1 || row - col >= t.n_rows) return;
+  const uint64_t slot0 = (uint64_t)uh * p.n_chunks;
+  const float *ml = p.part_ml + ((slot0 * WAVES + w) * 32 + col) * 2;
+  const float *po = p.part_o + (slot0 * WAVES + w) * (32 * DP) + wave * 256 + lane * 4;
+  float m = -__builtin_inff(), l = 0.0f;
+  for (uint32_t c = 0; c < n_chunks; ++c) m = fmaxf(m, ml[c * (WAVES * 64)]);
+  const float mu = m == -__builtin_inff() ? 0.0f : m;
+  f4 acc[kVecs] = {};
+#pragma unroll 4
+  for (uint32_t c = 0; c < n_chunks; ++c) {
+    const f2 x = *(const f2 *)(ml + c * (WAVES * 64));
+    const float a = __builtin_amdgcn_exp2f(x[0] - mu);
+    l += a * x[1];
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) acc[v] += a * *(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024);
+  }
+  if (row >= t.n_rows) return;
+  const uint32_t hd = head * p.group + row % p.group;
+  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - mu);
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  T *op = (T *)p.out + (uint64_t)(t.tok0 + row / p.group) * p.out_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const uint32_t at = v * 32 + wave * 8 + half * 4;  // vector v * 4 + wave
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(acc[v] * inv, T4);
   }
 }
 
@@ -1037,6 +1084,7 @@ hipError_t launch32(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   const hipError_t e = allow_lds((const void *)attn_rows32_kernel<E, DP, 4>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows32_kernel<E, DP, 4><<<plan.n_wgs, 256, C::kLds, st>>>(p);
+  if (plan.n_chunks > 1) attn_join_kernel<E, DP, 4><<<plan.n_units * p.n_kv_heads * 4, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
@@ -1072,22 +1120,44 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
   size_t max_keys = max_kv_len;
   const size_t reach = (size_t)window + (a.rows + group - 1) / group + 64;
   if (window && reach < max_keys) max_keys = reach;
-  // Workgroups enough to fill the chip several times over, chunks of 1024 keys
-  // or more.
-  const size_t base = (size_t)a.n_units * n_kv_heads, want = envi("W32", 4) * (size_t)cus;
-  size_t chunks = base >= want ? 1 : (want + base - 1) / base;
-  const size_t most = (max_keys + 1023) / 1024;
-  chunks = chunks > most ? most : chunks;
-  chunks = chunks ? chunks : 1;
-  a.chunk = (uint32_t)(((max_keys + chunks - 1) / chunks + 63) / 64 * 64);
+  // How many chunks a row tile's keys are cut into, by the time of the busiest
+  // CU in units of a 64-key tile at full rate.  A CU holds `resident`
+  // workgroups; alone, one runs at 0.72 of the rate that they reach together
+  // (two of 128-element heads; 1.02 against 0.74 PFLOP/s).  Rows of a prompt
+  // see half its keys on average, longest first, which fills the rounds by
+  // itself (`uneven`), and so do sequences of different lengths.  kStart,
+  // kSplit, kJoin: a workgroup's start, its partial sums, the join's launch.
+  // Measured, 520 rows x 8 over 28000 keys: 1 chunk 805 us, 2 586 us, 4 582 us,
+  // 8 593 us, 16 616 us; a 4096-token prompt: 1 chunk 168 us, 2 190 us.
+  const double resident = head_dim <= 64 ? 3 : (head_dim <= 128 ? 2 : 1), alone = resident > 1 ? 0.72 : 1.0;
+  const double kStart = 1.0, kSplit = 1.5, kJoin = 6.0;
+  const double units = ((double)(n_tokens * group) / a.rows + 0.5 * (double)(n_seqs - 1)) * n_kv_heads;
+  const double longest = (double)(max_keys + 63) / 64, spread = (double)(max_q_len < max_keys ? max_q_len : max_keys) / 64;
+  const double mean = window ? longest : longest - spread / 2, even = mean * units / cus;
+  double uneven = longest > 0 ? 2 * (longest - mean) / longest : 0;
+  uneven = n_seqs > 1 && uneven < 0.5 ? 0.5 : uneven;
+  const size_t base = (size_t)a.n_units * n_kv_heads;
+  double best = 0;
+  a.n_chunks = 1;
+  for (size_t n = 1; n <= 64 && (n == 1 || (longest / n >= 4 && base * n <= 16 * resident * cus)); ++n) {
+    const double per_cu = ceil(units) * n / cus, k = ceil(per_cu), len = mean / n;
+    const double last = k - floor(k / resident) * resident;  // workgroups of the last round
+    const double whole = (k - last + (last == 1 ? 1 / alone : last)) * len;
+    const double smooth = fmax(longest / n / (per_cu > 1 ? 1.0 : alone), even);
+    const double est = smooth + fmax(whole - smooth, 0.0) * (1 - uneven) + per_cu * kStart + (n > 1 ? per_cu * kSplit + kJoin : 0);
+    if (n == 1 || est < best) {
+      best = est;
+      a.n_chunks = (uint32_t)n;
+    }
+  }
+  if (getenv("NC")) a.n_chunks = atoi(getenv("NC"));
+  a.chunk = (uint32_t)(((max_keys + a.n_chunks - 1) / a.n_chunks + 63) / 64 * 64);
   a.chunk = a.chunk ? a.chunk : 64;
-  a.n_chunks = (uint32_t)chunks;
-  a.n_wgs = (uint32_t)(base * chunks < UINT32_MAX ? base * chunks : UINT32_MAX);
+  a.n_wgs = (uint32_t)(base * a.n_chunks < UINT32_MAX ? base * a.n_chunks : UINT32_MAX);
   if (a.n_chunks > 1) {
     const size_t rows = (size_t)a.n_wgs * a.rows;
-    a.part_o_floats = rows * head_dim;
+    a.part_o_floats = rows * (head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256));
     a.part_ml_floats = rows * 2;
-    a.counters = base;
   }
   return a;
 }

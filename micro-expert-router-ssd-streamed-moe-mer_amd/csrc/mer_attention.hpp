@@ -27,7 +27,7 @@ struct NormRopeParams {
   const int32_t *positions;  // [n_tokens], or null without rotation
   const float *inv_freq;     // [rot / 2]
   uint32_t n_tokens, head_dim, rot, interleaved;
-  float eps;
+  float eps, inv_dim;
   // append: where the rows go
   const int64_t *slots;      // [n_tokens]; negative = no row
   uint64_t n_slots;          // n_pages * page_size

@@ -31,6 +31,14 @@ template <> struct Elem<kF32> { typedef float T; typedef f4 V; };
 template <> struct Elem<kF16> { typedef _Float16 T; typedef h4 V; };
 template <> struct Elem<kBF16> { typedef __bf16 T; typedef b4 V; };
 
+// 1 / sqrt(x) to two units in the last place; subnormal x, which the
+// instruction takes for zero, are scaled up first.
+__device__ __forceinline__ float inv_sqrt(float x) {
+  const bool small = x < 0x1p-96f;
+  const float r = __builtin_amdgcn_rsqf(small ? x * 0x1p96f : x);
+  return small ? r * 0x1p48f : r;
+}
+
 // Passes of a wave: loads of all of them are in flight before the first is used.
 constexpr uint32_t kPasses = 4;
 
@@ -78,16 +86,29 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   }
   const bool turned = in_row && j * 8 < p.rot;
   f4 cs = {1, 1, 1, 1}, sn = {0, 0, 0, 0};
-  if (turned) {
+  if (p.rot) {
+    // The wave's lanes make one angle each (two where there are more than 64)
+    // and hand the cosine and sine to the lanes that turn by it.
+    constexpr int kAngles = LANES > 16 ? 2 : 1;
     const double pos = (double)p.positions[token];
-    const f4 f = *(const f4 *)(p.inv_freq + 4 * j);
+    float c[kAngles], s[kAngles];
+#pragma unroll
+    for (int a = 0; a < kAngles; ++a) {
+      const uint32_t f = a * 64 + lane;
+      const double t = pos * (double)p.inv_freq[f < p.rot / 2 ? f : 0] * 0.15915494309189535;  // 1 / (2 pi): turns
+      sincospif((float)(2.0 * (t - rint(t))), &s[a], &c[a]);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double t = pos * (double)f[i] * 0.15915494309189535;  // 1 / (2 pi): turns
-      float s, c;
-      sincospif((float)(2.0 * (t - rint(t))), &s, &c);
-      cs[i] = c;
-      sn[i] = s;
+      const uint32_t f = 4 * j + i;
+      const float c0 = __shfl(c[0], (int)(f % 64)), s0 = __shfl(s[0], (int)(f % 64));
+      cs[i] = c0;
+      sn[i] = s0;
+      if (kAngles > 1) {
+        const float c1 = __shfl(c[kAngles - 1], (int)(f % 64)), s1 = __shfl(s[kAngles - 1], (int)(f % 64));
+        cs[i] = f < 64 ? c0 : c1;
+        sn[i] = f < 64 ? s0 : s1;
+      }
     }
   }
 #pragma unroll
@@ -104,7 +125,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
 #pragma unroll
       for (int d = LANES / 2; d; d >>= 1) ss += __shfl_xor(ss, d);
       if (w && in_row) {
-        const float r = 1.0f / sqrtf(ss / (float)p.head_dim + p.eps);
+        const float r = inv_sqrt(ss * p.inv_dim + p.eps);
         a = a * r * *(const f4 *)(w + o0);
         b = b * r * *(const f4 *)(w + o1);
       }
@@ -149,7 +170,11 @@ hipError_t launch_lanes(NormRopeParams p, int cus, hipStream_t st) {
   uint32_t passes = (heads + per_pass - 1) / per_pass;
   passes = passes > kPasses ? kPasses : passes;
   while (passes > 1 && (uint64_t)p.n_tokens * ((heads + passes * per_pass - 1) / (passes * per_pass)) < 8ull * cus) passes /= 2;
+  // the same passes for every wave of a token
+  const uint32_t all = (heads + per_pass - 1) / per_pass, per_token = (all + passes - 1) / passes;
+  passes = (all + per_token - 1) / per_token;
   p.heads_per_wave = passes * per_pass;
+  p.inv_dim = 1.0f / (float)p.head_dim;
   const uint64_t waves = (uint64_t)p.n_tokens * ((heads + p.heads_per_wave - 1) / p.heads_per_wave);
   const uint32_t grid = (uint32_t)((waves + 3) / 4);
   if (lanes == 8) norm_rope_kernel<IN, OUT, 8, APPEND><<<grid, 256, 0, st>>>(p);
