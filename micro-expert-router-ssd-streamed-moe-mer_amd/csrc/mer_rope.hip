@@ -39,6 +39,24 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return small ? r * 0x1p48f : r;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// Sum over groups of LANES lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ float sum_lanes(float x) {
+  x += dpp<0xB1>(x);   // lane ^ 1
+  x += dpp<0x4E>(x);   // lane ^ 2
+  x += dpp<0x141>(x);  // the other four of eight
+  if (LANES > 8) x += dpp<0x140>(x);  // the other eight of sixteen
+  if (LANES > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return x;
+}
+
 // Passes of a wave: loads of all of them are in flight before the first is used.
 constexpr uint32_t kPasses = 4;
 
@@ -50,10 +68,10 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   constexpr uint32_t kHeads = 64 / LANES;  // of a pass
   const uint32_t heads = p.t[0].heads + p.t[1].heads;
   const uint32_t per_token = (heads + p.heads_per_wave - 1) / p.heads_per_wave;
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const uint32_t token = (uint32_t)(wave / per_token);
+  const uint32_t wave = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t token = (uint32_t)__builtin_amdgcn_readfirstlane(wave / per_token);
   if (token >= p.n_tokens) return;
-  const uint32_t head0 = (uint32_t)(wave % per_token) * p.heads_per_wave;
+  const uint32_t head0 = (wave - token * per_token) * p.heads_per_wave;
   const uint32_t head1 = head0 + p.heads_per_wave < heads ? head0 + p.heads_per_wave : heads;
   const uint32_t lane = __lane_id(), j = lane % LANES, sub = lane / LANES;
   const bool in_row = j * 8 < p.head_dim;
@@ -68,6 +86,25 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
       if (lane == 0) atomicCAS(p.status, 0u, (uint32_t)MER_ERR_RESIDENCY_MISS);
       return;
     }
+  }
+
+  // What the angles and norms need is on its way before the rows.
+  constexpr int kAngles = LANES > 16 ? 2 : 1;
+  int32_t position = 0;
+  float freq[kAngles];
+  if (p.rot) {
+    position = p.positions[token];
+#pragma unroll
+    for (int a = 0; a < kAngles; ++a) {
+      const uint32_t f = a * 64 + lane;
+      freq[a] = p.inv_freq[f < p.rot / 2 ? f : 0];
+    }
+  }
+  const uint32_t tensor0 = head0 >= p.t[0].heads, tensor1 = head1 > p.t[0].heads;
+  f4 w0[2], w1[2];
+  if (in_row) {
+    if (!tensor0 && p.t[0].norm) w0[0] = *(const f4 *)(p.t[0].norm + o0), w1[0] = *(const f4 *)(p.t[0].norm + o1);
+    if (tensor1 && p.t[1].norm) w0[1] = *(const f4 *)(p.t[1].norm + o0), w1[1] = *(const f4 *)(p.t[1].norm + o1);
   }
 
   VI x0[kPasses], x1[kPasses];
@@ -89,13 +126,11 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   if (p.rot) {
     // The wave's lanes make one angle each (two where there are more than 64)
     // and hand the cosine and sine to the lanes that turn by it.
-    constexpr int kAngles = LANES > 16 ? 2 : 1;
-    const double pos = (double)p.positions[token];
+    const double pos = (double)position;
     float c[kAngles], s[kAngles];
 #pragma unroll
     for (int a = 0; a < kAngles; ++a) {
-      const uint32_t f = a * 64 + lane;
-      const double t = pos * (double)p.inv_freq[f < p.rot / 2 ? f : 0] * 0.15915494309189535;  // 1 / (2 pi): turns
+      const double t = pos * (double)freq[a] * 0.15915494309189535;  // 1 / (2 pi): turns
       sincospif((float)(2.0 * (t - rint(t))), &s[a], &c[a]);
     }
 #pragma unroll
@@ -117,17 +152,16 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
     if (head0 + k * kHeads >= head1) break;  // the whole wave
     const bool second = h >= p.t[0].heads;
     f4 a = __builtin_convertvector(x0[k], f4), b = __builtin_convertvector(x1[k], f4);
-    const float *w = second ? p.t[1].norm : p.t[0].norm;
+    const bool normed = (second ? p.t[1].norm : p.t[0].norm) != nullptr;
     if (p.t[0].norm || p.t[1].norm) {
       float ss = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-      for (int d = LANES / 2; d; d >>= 1) ss += __shfl_xor(ss, d);
-      if (w && in_row) {
+      ss = sum_lanes<LANES>(ss);
+      if (normed && in_row) {
         const float r = inv_sqrt(ss * p.inv_dim + p.eps);
-        a = a * r * *(const f4 *)(w + o0);
-        b = b * r * *(const f4 *)(w + o1);
+        a = a * r * (second ? w0[1] : w0[0]);
+        b = b * r * (second ? w1[1] : w1[0]);
       }
     }
     if (turned && !(APPEND && second)) {
