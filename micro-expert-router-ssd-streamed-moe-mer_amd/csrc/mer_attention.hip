@@ -860,6 +860,18 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   const uint32_t my_lds = wave * (C::kLoads * 1024u);
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
 
+  // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
+  // dims a product.  V: 16 keys x 32 dims, 4 + 4 keys of a lane in the order
+  // in which the scores lie in their lanes.
+  uint32_t k_lane[DP / 16], v_lane[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) k_lane[d] = col * (DP * 2) + ((d * 2 + half) ^ L::k_swizzle(col)) * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) {
+    const uint32_t r = half * 4 + lane % 16 / 4;
+    v_lane[d] = r * (DP * 2) + ((d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r)) * 16 + lane % 2 * 8;
+  }
+
   float m = -__builtin_inff(), l = 0.0f;
   f16v o[DP / 32];
 #pragma unroll
@@ -890,17 +902,12 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     }
     const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
     if (live) {
-      // V's operand for 16 keys and 32 dims: 4 + 4 keys in the order in which
-      // the scores lie in their lanes
       auto v_of = [&](int ks, int d) {
         s4 x[2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t r = ks * 16 + b * 8 + half * 4 + lane % 16 / 4;
-          const uint32_t piece = (d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r);
+        for (int b = 0; b < 2; ++b)
           x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + lane % 2 * 8));
-        }
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + v_lane[d] + (ks * 16 + b * 8) * (DP * 2)));
         return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
       };
       f16v s[2];
@@ -910,29 +917,32 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
         for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
       // operands are read a batch ahead of the products, so that the reads'
       // latency is paid once a batch and not once a product
-      constexpr int kBatch = DP / 16 < 8 ? DP / 16 : 8;
+      constexpr int kBatch = DP == 128 ? 8 : 4;
 #pragma unroll
       for (int d0 = 0; d0 < DP / 16; d0 += kBatch) {
         V8 k[2][kBatch];
 #pragma unroll
         for (int d = 0; d < kBatch; ++d)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t r = b * 32 + col, piece = ((d0 + d) * 2 + half) ^ L::k_swizzle(r);
-            k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
-          }
+          for (int b = 0; b < 2; ++b)
+            k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d0 + d] + b * 32 * (DP * 2));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = 0; d < kBatch; ++d)
 #pragma unroll
           for (int b = 0; b < 2; ++b) s[b] = E::mfma32(k[b][d], q[d0 + d], s[b]);
       }
-      V8 v[2][DP / 32];
+      constexpr int kAhead = DP == 256 ? 1 : 2;
+      V8 v[kAhead][DP / 32];
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+      for (int ks = 0; ks < kAhead; ++ks)
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, d);
       __builtin_amdgcn_sched_barrier(0);
+      // The vector work goes first, so that the products of the other
+      // workgroup's wave run beside it (4096-token prompt 185 -> 166 us; heads
+      // of 64, which are all vector work, lose by it).
+      if (DP > 64) __builtin_amdgcn_s_setprio(2);
       if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi ||
           key0 <= pos_last - window) {
         const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
@@ -973,12 +983,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
       }
       l += sums[0] + sums[1];
       __builtin_amdgcn_sched_barrier(0);
+      if (DP > 64) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          o[d] = E::mfma32(v[ks % 2][d], pr[ks], o[d]);
-          if (ks < 2) v[ks % 2][d] = v_of(ks + 2, d);
+          o[d] = E::mfma32(v[ks % kAhead][d], pr[ks], o[d]);
+          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, d);
         }
       }
     }
