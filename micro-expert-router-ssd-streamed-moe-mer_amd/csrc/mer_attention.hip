@@ -20,7 +20,6 @@
 
 #include <atomic>
 #include <math.h>
-#include <stdlib.h>
 
 namespace mer {
 namespace {
@@ -56,6 +55,8 @@ struct BF16 {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+constexpr float kLog2E = 1.44269504088896341f;
 
 // What a lane reads for a key outside the tile's range: rows of zeros.
 __device__ u4 g_zero_row[kMaxHeadDim * 2 / 16];
@@ -326,10 +327,10 @@ struct Share {
   }
 };
 
-// ---- joining the chunks of a row tile ----
-// A workgroup that has done one of several chunks leaves its sums in memory
+// ---- joining the pieces of a unit ----
+// A workgroup that has done one of several pieces leaves its sums in memory
 // (device-scope stores) and counts itself in; the one that comes last adds
-// the chunks up, in their order, and leaves the count at zero for the next
+// the pieces up, in their order, and leaves the count at zero for the next
 // launch.
 constexpr int kDeviceScope = 16;  // sc1: past the caches that other XCDs do not see
 
@@ -344,40 +345,46 @@ __device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, uint32_t index, f
 }
 
 // True in every thread of the workgroup that comes last.  `flag`: a word of LDS.
-__device__ __forceinline__ bool last_chunk(uint32_t *counter, uint32_t n_chunks, uint32_t *flag) {
+__device__ __forceinline__ bool last_piece(uint32_t *counter, uint32_t n_pieces, uint32_t *flag) {
   wait_vm<0>();
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (n == n_chunks - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = n == n_chunks - 1;
+    if (n == n_pieces - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = n == n_pieces - 1;
   }
   __syncthreads();
   return *flag != 0;
 }
 
-// Adds up a tile's chunks.  32 lanes hold a row's dims; the groups of 32 take
-// U rows each at a time, or share a row's chunks where there are fewer rows
-// than groups.  Chunk c is at slot(c) of the partial sums.  `lds`: [threads / 32][DP + 1] floats.
-template <class E, int DP, int ROWS, int THREADS, int U, class Slot>
-__device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, uint32_t head, uint32_t n_chunks,
-                                            Slot slot, float *part_o, float *part_ml, float *lds) {
+// Adds up a unit's pieces: piece 0 is at first_slot of the partial sums, piece
+// c at 2 * (first_wg + c).  32 lanes hold a row's dims; the groups of 32 take
+// a row each, or share a row's pieces where there are fewer rows than groups.
+// A batch of pieces is in flight at once; what a lane reads beyond the pieces,
+// rows or dims that there are is left out.
+// `lds`: [THREADS / 32][DP] floats.
+template <class E, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, uint32_t head, uint32_t first_wg,
+                                            uint32_t first_slot, uint32_t n_pieces, float *lds) {
   typedef typename E::T T;
-  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = 8 / U * 4 / (kDims < 4 ? 4 : kDims);
+  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = DP == 256 ? 8 : 16;
   typedef float fd __attribute__((ext_vector_type(kDims)));
   typedef T td __attribute__((ext_vector_type(kDims)));
-  const __amdgpu_buffer_rsrc_t ro = part_rsrc(part_o), rm = part_rsrc(part_ml);
+  const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);
   const uint32_t g = threadIdx.x / 32, ln = threadIdx.x % 32, dim = ln * kDims;
   const uint32_t rows = t.n_rows - t.row0 < ROWS ? t.n_rows - t.row0 : ROWS;
   const uint32_t share = rows < kGroups ? kGroups / rows : 1;  // groups of a row
-  const uint32_t step = kGroups / share;                       // rows at a time
-  auto ml_of = [&](uint32_t c, uint32_t r, bool ok) {
+  const uint32_t step = kGroups / share, part = g % share;     // rows at a time
+  auto row_of = [&](uint32_t c, uint32_t r) { return (c ? 2 * (first_wg + c) : first_slot) * ROWS + r; };
+  auto ml_of = [&](uint32_t c, uint32_t r) {  // nothing beyond the pieces
     const f2 none = {-__builtin_inff(), 0.0f};
-    const f2 ml = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(rm, ok ? (slot(c) * ROWS + r) * 8 : 0u, 0, kDeviceScope));
-    return ok ? ml : none;
+    const f2 ml = __builtin_bit_cast(
+        f2, __builtin_amdgcn_raw_buffer_load_b64(rm, row_of(c < n_pieces ? c : 0, r) * 8, 0, kDeviceScope));
+    return c < n_pieces ? ml : none;
   };
-  auto o_of = [&](uint32_t c, uint32_t r, bool ok) {
-    const uint32_t at = ok && dim < p.head_dim ? ((slot(c) * ROWS + r) * p.head_dim + dim) * 4 : 0xfffffff0u;  // zeros
+  const uint32_t my_dim = dim < p.head_dim ? dim : 0;
+  auto o_of = [&](uint32_t c, uint32_t r) {
+    const uint32_t at = (row_of(c, r) * p.head_dim + my_dim) * 4;
     if constexpr (kDims == 2) {
       return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
     } else if constexpr (kDims == 4) {
@@ -388,82 +395,55 @@ __device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, 
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   };
-  for (uint32_t r0 = 0; r0 < rows; r0 += step * U) {
-    uint32_t r[U];
-    bool ok[U];
-    float m[U], l[U];
-    f2 first[U];  // of the chunks 0 .. 31, a lane each
-    fd acc[U], x[U][kBatch];
+  for (uint32_t r0 = 0; r0 < rows; r0 += step) {
+    const uint32_t mine = r0 + g / share, r = mine < rows ? mine : rows - 1;
+    // The first batch of sums is under way with the weights; `first`: of the
+    // pieces 0 .. 31, a lane each.
+    const f2 first = ml_of(ln, r);
+    fd acc = {}, x[kBatch];
+    auto load = [&](uint32_t c0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = r0 + u * step + g / share;
-      ok[u] = g / share < step && r[u] < rows;
-      first[u] = ml_of(ln, r[u], ok[u] && ln < n_chunks);
-      acc[u] = fd{};
-    }
-    // The first batch of sums is under way with the weights.
-    auto load = [&](uint32_t c0, uint32_t k0, uint32_t end) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          const uint32_t k = k0 + b * share + g % share;
-          x[u][b] = o_of(c0 + k, r[u], ok[u] && k < end);
-        }
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        const uint32_t c = c0 + b * share + part;
+        x[b] = o_of(c < n_pieces ? c : n_pieces - 1, r);
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
-    load(0, 0, n_chunks < 32 ? n_chunks : 32);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      m[u] = first[u][0];
-      l[u] = first[u][1];
-      for (uint32_t c0 = 32; c0 < n_chunks; c0 += 32) {
-        const f2 ml = ml_of(c0 + ln, r[u], ok[u] && c0 + ln < n_chunks);
-        const float mn = fmaxf(m[u], ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
-        l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
-        m[u] = mn;
-      }
-      const float mm = max_32(m[u]), mu = mm == -__builtin_inff() ? 0.0f : mm;
-      l[u] = sum_32(l[u] * __builtin_amdgcn_exp2f(m[u] - mu));
-      m[u] = mu;
+    load(0);
+    float m = first[0], l = first[1];
+    for (uint32_t c0 = 32; c0 < n_pieces; c0 += 32) {
+      const f2 ml = ml_of(c0 + ln, r);
+      const float mn = fmaxf(m, ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
+      l = l * __builtin_amdgcn_exp2f(m - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+      m = mn;
     }
-    for (uint32_t c0 = 0; c0 < n_chunks; c0 += 32) {
-      float w[U];  // weight of chunk c0 + lane
+    const float mm = max_32(m), mu = mm == -__builtin_inff() ? 0.0f : mm;
+    l = sum_32(l * __builtin_amdgcn_exp2f(m - mu));
+    for (uint32_t c0 = 0; c0 < n_pieces; c0 += 32) {
+      const f2 ml = c0 ? ml_of(c0 + ln, r) : first;
+      const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece c0 + lane
+      for (uint32_t k0 = 0; k0 < 32 && c0 + k0 < n_pieces; k0 += share * kBatch) {
+        if (c0 + k0) load(c0 + k0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const f2 ml = c0 ? ml_of(c0 + ln, r[u], ok[u] && c0 + ln < n_chunks) : first[u];
-        w[u] = __builtin_amdgcn_exp2f(ml[0] - m[u]);
-      }
-      const uint32_t end = n_chunks - c0 < 32 ? n_chunks - c0 : 32;
-      for (uint32_t k0 = 0; k0 < end; k0 += share * kBatch) {
-        if (c0 + k0) load(c0, k0, end);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (uint32_t b = 0; b < kBatch; ++b) {
-            const uint32_t k = k0 + b * share + g % share;
-            const float wk = __shfl(w[u], (int)((threadIdx.x & 32) + (k & 31)));
-            acc[u] += x[u][b] * (k < end ? wk : 0.0f);
-          }
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t k = k0 + b * share + part;
+          const float wk = __shfl(w, (int)((threadIdx.x & 32) + (k & 31)));
+          if (k < 32 && c0 + k < n_pieces) acc += x[b] * wk;
+        }
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (share > 1) {  // once: rows <= step, U rows of which only the first is one
-        if (ok[u] && g % share) *(fd *)&lds[g * DP + dim] = acc[u];
-        __syncthreads();
-        if (ok[u] && g % share == 0)
-          for (uint32_t k = 1; k < share; ++k) acc[u] += *(fd *)&lds[(g + k) * DP + dim];
-        __syncthreads();
-      }
-      if (ok[u] && g % share == 0 && dim < p.head_dim) {
-        const uint32_t gr = t.row0 + r[u], hq = head * p.group + gr % p.group;
-        float ls = l[u];
-        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - m[u]);
-        const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
-        T *op = (T *)p.out + (uint64_t)(t.tok0 + gr / p.group) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
-        *(td *)op = __builtin_convertvector(acc[u] * inv, td);
-      }
+    if (share > 1) {  // in the one pass that there is then
+      if (part) *(fd *)&lds[g * DP + dim] = acc;
+      __syncthreads();
+      if (part == 0)
+        for (uint32_t k = 1; k < share; ++k) acc += *(fd *)&lds[(g + k) * DP + dim];
+    }
+    if (mine < rows && part == 0 && dim < p.head_dim) {
+      const uint32_t gr = t.row0 + r, hq = head * p.group + gr % p.group;
+      if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu);
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      T *op = (T *)p.out + (uint64_t)(t.tok0 + gr / p.group) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
+      *(td *)op = __builtin_convertvector(acc * inv, td);
     }
   }
 }
@@ -480,10 +460,10 @@ __device__ __forceinline__ void join_chunks(const AttnParams &p, const Tile &t, 
 // The waves of a workgroup take a piece's tiles of 32 keys in turn, each with
 // a ring of LDS of its own (no barriers while the keys stream), and join
 // their sums at the piece's end.
-constexpr int waves16(int dp) { return dp == 64 ? 4 : 2; }
-template <int DP>
+template <int DP, int WAVES, int NR>
 struct Rows16 {
-  static constexpr int kWaves = waves16(DP);
+  static constexpr int kWaves = WAVES;
+  static constexpr int kRows = 16 * NR;
   static constexpr int kKeys = 32;
   static constexpr int kGranule = 128;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
@@ -501,7 +481,7 @@ struct Granules {
   int32_t q[5], len[4];  // their q_start and kv_len
   uint32_t seq0;
 
-  template <int GRANULE>
+  template <int GRANULE, int ROWS>
   __device__ __forceinline__ void view(const AttnParams &p, uint32_t first) {
     seq0 = first;
     const uint32_t s0 = first + lane_id() * 4;
@@ -515,7 +495,7 @@ struct Granules {
     for (uint32_t i = 0; i < 4; ++i) {
       const Span s = make_span(p, q[i], q[i + 1], len[i]);  // past the last sequence: no rows
       const uint32_t rows = (uint32_t)s.n * p.group;
-      w[i] = (rows + 15) / 16 * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
+      w[i] = (rows + ROWS - 1) / ROWS * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
       upto += w[i];
     }
 #pragma unroll
@@ -529,11 +509,11 @@ struct Granules {
   // The sequence at granule x of the view or a later one: its number, the
   // granules before it and its span.  False if there is none (lengths that
   // change under the kernel).
-  template <int GRANULE>
+  template <int GRANULE, int ROWS>
   __device__ __forceinline__ bool find(const AttnParams &p, uint32_t x, uint32_t *seq, uint32_t *before, Span *span) {
     while (x >= base + total && seq0 + 256 < p.n_seqs) {
       base += total;
-      view<GRANULE>(p, seq0 + 256);
+      view<GRANULE, ROWS>(p, seq0 + 256);
     }
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(base + upto > x);
     if (!beyond) return false;
@@ -569,9 +549,9 @@ struct Granules {
   }
 };
 
-template <class E, int DP>
-__global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_eu(1, 2))) void attn_rows16_kernel(AttnParams p) {
-  typedef Rows16<DP> C;
+template <class E, int DP, int WAVES, int NR>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, DP == 64 ? 2 : 1))) void attn_rows16_kernel(AttnParams p) {
+  typedef Rows16<DP, WAVES, NR> C;
   typedef RowLayout<DP> L;
   typedef typename E::V8 V8;
   typedef typename E::T T;
@@ -579,16 +559,26 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
   const uint32_t col = lane % 16, quad = lane / 16;
 
+  // where a lane reads its operands, from a tile's start
+  uint32_t k_lane[DP / 32], v_lane[DP / 16];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) k_lane[d] = col * (DP * 2) + ((d * 4 + quad) ^ L::k_swizzle(col)) * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) {
+    const uint32_t r = quad * 4 + col / 4;
+    v_lane[d] = r * (DP * 2) + ((d * 2 + col % 4 / 2) ^ L::v_swizzle(r)) * 16 + col % 2 * 8;
+  }
+
   Granules gr;
   gr.base = 0;
-  gr.view<C::kGranule>(p, 0);
+  gr.view<C::kGranule, C::kRows>(p, 0);
   uint32_t all = gr.total;
   if (p.n_seqs > 256) {
     for (uint32_t s = 256; s < p.n_seqs; s += 256) {
-      gr.view<C::kGranule>(p, s);
+      gr.view<C::kGranule, C::kRows>(p, s);
       all += gr.total;
     }
-    gr.view<C::kGranule>(p, 0);
+    gr.view<C::kGranule, C::kRows>(p, 0);
   }
   uint32_t per = uni((all + gridDim.x - 1) / gridDim.x);
   per = per < p.min_granules ? p.min_granules : per;
@@ -598,7 +588,7 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
   while (x < x1) {
     uint32_t seq, before;
     Span span;
-    if (!gr.find<C::kGranule>(p, x, &seq, &before, &span)) return;
+    if (!gr.find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
     int32_t start = 0;
     const uint32_t n_gran = uni(Granules::granules<C::kGranule>(p, span, &start));
     const uint32_t unit = uni((x - before) / n_gran), tile = uni(unit / p.n_kv_heads), head = unit - tile * p.n_kv_heads;
@@ -612,26 +602,29 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
     first_piece = false;
     x += count;
     Tile t;
-    make_tile<16>(p, span, tile, &t);  // the tile is one of the sequence's
+    make_tile<C::kRows>(p, span, tile, &t);  // the tile is one of the sequence's
     start = (int32_t)uni((uint32_t)start);
     int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
     if (p.window && begin < (t.lo & ~31)) begin = t.lo & ~31;
     end = end < t.hi ? end : t.hi;
 
-    // Q^T: lane column = row of the tile, 8 consecutive dims per 32-dim slab
-    const uint32_t row = t.row0 + col;
-    const bool row_ok = row < t.n_rows;
-    const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
-    const int32_t pos = t.pos0 + (int32_t)tok, window = p.window ? (int32_t)p.window : 0x40000000;
-    V8 q[DP / 32];
-    const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
+    // Q^T: lane column = a row of each group of 16, 8 consecutive dims per 32-dim slab
+    const int32_t window = p.window ? (int32_t)p.window : 0x40000000;
+    V8 q[NR][DP / 32];
+    int32_t pos[NR];
 #pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-      const uint32_t d = s * 32 + quad * 8;
-      q[s] = V8{};
-      if (row_ok && d < p.head_dim) q[s] = *(const V8 *)(qp + d);
+    for (int n = 0; n < NR; ++n) {
+      const uint32_t row = t.row0 + n * 16 + col, tok = row / p.group, hd = head * p.group + row % p.group;
+      pos[n] = t.pos0 + (int32_t)tok;
+      const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+      for (int s = 0; s < DP / 32; ++s) {
+        const uint32_t d = s * 32 + quad * 8;
+        q[n][s] = V8{};
+        if (row < t.n_rows && d < p.head_dim) q[n][s] = *(const V8 *)(qp + d);
+      }
     }
-    const uint32_t last = t.row0 + 15 < t.n_rows ? t.row0 + 15 : t.n_rows - 1;
+    const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
     const int32_t pos_first = t.pos0 + (int32_t)(t.row0 / p.group), pos_last = t.pos0 + (int32_t)(last / p.group);
 
     const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
@@ -654,69 +647,81 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
       sh.template copy<true>(slot_of(i) + C::kTileBytes);
     }
 
-    float m = -__builtin_inff(), l = 0.0f;
-    f4 o[DP / 16];
+    float m[NR], l[NR];
+    f4 o[NR][DP / 16];
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) o[d] = f4{0, 0, 0, 0};
+    for (int n = 0; n < NR; ++n) {
+      m[n] = -__builtin_inff();
+      l[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[n][d] = f4{0, 0, 0, 0};
+    }
     for (int32_t i = 0; i < mine; ++i) {
       const int32_t left = mine - i;
       const int32_t key0 = key_of(i);
       const uint32_t kb = slot_of(i), vb = kb + C::kTileBytes;
       if (left == 1) wait_vm<C::kLoads>();
       else wait_vm<3 * C::kLoads>();
-      f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+      f4 s[NR][2];
       V8 k[2][DP / 32];
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t r = b * 16 + col, piece = (d * 4 + quad) ^ L::k_swizzle(r);
-          k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + r * (DP * 2) + piece * 16);
-        }
+        for (int b = 0; b < 2; ++b)
+          k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d] + b * 16 * (DP * 2));
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int n = 0; n < NR; ++n) {
+        s[n][0] = s[n][1] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = E::mfma16(k[b][d], q[d], s[b]);
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[n][b] = E::mfma16(k[b][d], q[n][d], s[n][b]);
+      }
       wait_lds();
       if (left > C::kStages) {
         sh.advance(p.status);
         sh.lookup(key_of(i + C::kStages + 1));
         sh.template copy<false>(kb);
       }
-      // scores in base 2; keys of lane: b * 16 + quad * 4 + e
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[e / 4][e % 4] * p.scale_log2;
       const int32_t key_end = key0 + C::kKeys;
-      if (key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window) {
-        const int32_t last = pos - key0 - (int32_t)quad * 4, before = last - window;
+      const bool partial = key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window;
+      V8 pr[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        // scores in base 2; keys of lane: b * 16 + quad * 4 + e
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[n][e / 4][e % 4] * p.scale_log2;
+        if (partial) {
+          const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4, before = last_key - window;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int32_t at = (e / 4) * 16 + e % 4;
+            x[e] = at > last_key || at <= before ? -__builtin_inff() : x[e];
+          }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+        mx = fmaxf(max_quad(mx), m[n]);
+        const float mu = mx == -__builtin_inff() ? 0.0f : mx;
+        const float a = __builtin_amdgcn_exp2f(m[n] - mu);
+        f8 e8;
+        float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int32_t at = (e / 4) * 16 + e % 4;
-          x[e] = at > last || at <= before ? -__builtin_inff() : x[e];
+          e8[e] = __builtin_amdgcn_exp2f(x[e] - mu);
+          sum += e8[e];
         }
-      }
-      float mx = x[0];
+        l[n] = l[n] * a + sum;
+        if (__builtin_amdgcn_ballot_w64(mx != m[n])) {
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-      mx = fmaxf(max_quad(mx), m);
-      const float mu = mx == -__builtin_inff() ? 0.0f : mx;
-      const float a = __builtin_amdgcn_exp2f(m - mu);
-      f8 e8;
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        e8[e] = __builtin_amdgcn_exp2f(x[e] - mu);
-        sum += e8[e];
+          for (int d = 0; d < DP / 16; ++d) o[n][d] *= a;
+        }
+        m[n] = mx;
+        pr[n] = __builtin_convertvector(e8, V8);
       }
-      l = l * a + sum;
-      if (__builtin_amdgcn_ballot_w64(mx != m)) {
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) o[d] *= a;
-      }
-      m = mx;
-      const V8 pr = __builtin_convertvector(e8, V8);
       if (left == 1) wait_vm<0>();
       else if (left == 2) wait_vm<2 * C::kLoads>();
       else wait_vm<3 * C::kLoads>();
@@ -724,62 +729,60 @@ __global__ __launch_bounds__(64 * waves16(DP)) __attribute__((amdgpu_waves_per_e
       for (int d = 0; d < DP / 16; ++d) {
         s4 v[2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t r = b * 16 + quad * 4 + col / 4;
-          const uint32_t piece = (d * 2 + (col % 4) / 2) ^ L::v_swizzle(r);
+        for (int b = 0; b < 2; ++b)
           v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + r * (DP * 2) + piece * 16 + (col % 2) * 8));
-        }
-        const s8 vv = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        o[d] = E::mfma16(__builtin_bit_cast(V8, vv), pr, o[d]);
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + v_lane[d] + b * 16 * (DP * 2)));
+        const V8 vv = __builtin_bit_cast(V8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[n][d] = E::mfma16(vv, pr[n], o[n][d]);
       }
       wait_lds();
       if (left > C::kStages) sh.template copy<true>(vb);
     }
-    l = sum_quad(l);
     // join the waves: m, l and O of each in LDS
     __syncthreads();
-    float *jo = (float *)smem;                         // [wave][16][DP]
-    float *jm = jo + C::kWaves * 16 * DP;              // [wave][16][2]
-    if (quad == 0) {
-      jm[(wave * 16 + col) * 2] = m;
-      jm[(wave * 16 + col) * 2 + 1] = l;
-    }
+    float *jo = (float *)smem;                      // [wave][row][DP]
+    float *jm = jo + C::kWaves * C::kRows * DP;     // [wave][row][2]
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[(wave * 16 + col) * DP + d * 16 + quad * 4] = o[d];
+    for (int n = 0; n < NR; ++n) {
+      const uint32_t at = wave * C::kRows + n * 16 + col;
+      l[n] = sum_quad(l[n]);
+      if (quad == 0) *(f2 *)&jm[at * 2] = f2{m[n], l[n]};
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[at * DP + d * 16 + quad * 4] = o[n][d];
+    }
     __syncthreads();
     const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);
-    for (uint32_t w = tid; w < 16 * (DP / 8); w += 64 * C::kWaves) {
+    for (uint32_t w = tid; w < C::kRows * (DP / 8); w += 64 * C::kWaves) {
       const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, rr = t.row0 + r;
       if (rr >= t.n_rows || d >= p.head_dim) continue;
       float mm = -__builtin_inff();
 #pragma unroll
-      for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * 16 + r) * 2]);
+      for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * C::kRows + r) * 2]);
       float ls = 0.0f;
       f8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int v = 0; v < C::kWaves; ++v) {
-        const float mv = jm[(v * 16 + r) * 2];
+        const float mv = jm[(v * C::kRows + r) * 2];
         const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
-        ls += a * jm[(v * 16 + r) * 2 + 1];
-        acc += a * *(const f8 *)&jo[(v * 16 + r) * DP + d];
+        ls += a * jm[(v * C::kRows + r) * 2 + 1];
+        acc += a * *(const f8 *)&jo[(v * C::kRows + r) * DP + d];
       }
       const uint32_t tk = rr / p.group, hq = head * p.group + rr % p.group;
       if (n_pieces == 1) {
-        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * 1.44269504088896341f - (mm == -__builtin_inff() ? 0.0f : mm));
+        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm));
         const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
         const V8 r8 = __builtin_convertvector(acc * inv, V8);
         *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
       } else {
-        const uint32_t to = my_slot * 16 + r;
+        const uint32_t to = my_slot * C::kRows + r;
         put4(ro, to * p.head_dim + d, f4{acc[0], acc[1], acc[2], acc[3]});
         put4(ro, to * p.head_dim + d + 4, f4{acc[4], acc[5], acc[6], acc[7]});
         if (d == 0) put2(rm, to * 2, f2{mm, ls});
       }
     }
-    if (n_pieces > 1 && last_chunk(p.counters + first_wg, n_pieces, (uint32_t *)(jm + C::kWaves * 32)))
-      join_chunks<E, DP, 16, 64 * C::kWaves, 1>(
-          p, t, head, n_pieces, [&](uint32_t c) { return c ? 2 * (first_wg + c) : first_slot; }, p.part_o, p.part_ml, jo);
+    if (n_pieces > 1 && last_piece(p.counters + first_wg, n_pieces, (uint32_t *)(jm + C::kWaves * C::kRows * 2)))
+      join_pieces<E, DP, C::kRows, 64 * C::kWaves>(p, t, head, first_wg, first_slot, n_pieces, jo);
   }
 }
 
@@ -997,7 +1000,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   l += other_half(l);
   if (n_chunks == 1) {
     if (!row_ok) return;
-    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - (m == -__builtin_inff() ? 0.0f : m));
+    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m));
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
@@ -1057,7 +1060,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   }
   if (row >= t.n_rows) return;
   const uint32_t hd = head * p.group + row % p.group;
-  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * 1.44269504088896341f - mu);
+  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu);
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   T *op = (T *)p.out + (uint64_t)(t.tok0 + row / p.group) * p.out_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
@@ -1078,14 +1081,26 @@ hipError_t allow_lds(const void *fn, int bytes, std::atomic<uint64_t> *devices) 
   return e;
 }
 
+template <class E, int DP, int WAVES, int NR>
+hipError_t launch16w(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
+  typedef Rows16<DP, WAVES, NR> C;
+  static std::atomic<uint64_t> devices{0};
+  const hipError_t e = allow_lds((const void *)attn_rows16_kernel<E, DP, WAVES, NR>, C::kLds, &devices);
+  if (e != hipSuccess) return e;
+  attn_rows16_kernel<E, DP, WAVES, NR><<<plan.n_wgs, 64 * WAVES, C::kLds, st>>>(p);
+  return hipGetLastError();
+}
 template <class E, int DP>
 hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
-  typedef Rows16<DP> C;
-  static std::atomic<uint64_t> devices{0};
-  const hipError_t e = allow_lds((const void *)attn_rows16_kernel<E, DP>, C::kLds, &devices);
-  if (e != hipSuccess) return e;
-  attn_rows16_kernel<E, DP><<<plan.n_wgs, 64 * C::kWaves, C::kLds, st>>>(p);
-  return hipGetLastError();
+  constexpr int kWide = DP == 256 ? 2 : 4;
+  const bool wide = plan.waves == kWide, narrow = plan.waves == 1 && DP < 256;
+  if (plan.rows == 16 && wide) return launch16w<E, DP, kWide, 1>(plan, p, st);
+  if (plan.rows == 32 && wide) return launch16w<E, DP, kWide, 2>(plan, p, st);
+  if constexpr (DP < 256) {
+    if (plan.rows == 16 && narrow) return launch16w<E, DP, 1, 1>(plan, p, st);
+    if (plan.rows == 32 && narrow) return launch16w<E, DP, 1, 2>(plan, p, st);
+  }
+  return hipErrorInvalidValue;
 }
 
 template <class E, int DP>
@@ -1113,14 +1128,20 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 
 }  // namespace
 
-static size_t envi(const char *n, size_t d) { const char *v = getenv(n); return v ? (size_t)atoi(v) : d; }
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                    size_t max_q_len, size_t max_kv_len, uint32_t window, int cus) {
   AttnPlan a{};
-  a.rows = max_q_len * group <= 32 ? 16 : 128;
-  if (a.rows == 16) {
-    a.n_wgs = (uint32_t)cus * envi("W16", 2);
-    a.min_granules = envi("M16", 2);
+  a.rows = max_q_len * group <= 16 ? 16 : (max_q_len * group <= 32 ? 32 : 128);
+  if (a.rows <= 32) {
+    // Long stretches of few units: the widest workgroups, as many as the CUs
+    // hold at once.  Many short units: as many waves, each a workgroup of its
+    // own, so that one's piece ends while the others' keys stream (512
+    // sequences of 60 - 300 keys: 135 us wide, 95 us narrow; 8 of 1000: 11 us
+    // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
+    const bool narrow = head_dim <= 128 && (uint64_t)n_seqs * n_kv_heads >= 4ull * cus;
+    a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);
+    a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 64 ? 2 : 1);
+    a.min_granules = 1;
     a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
     a.counters = a.n_wgs;
@@ -1161,7 +1182,6 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
       a.n_chunks = (uint32_t)n;
     }
   }
-  if (getenv("NC")) a.n_chunks = atoi(getenv("NC"));
   a.chunk = (uint32_t)(((max_keys + a.n_chunks - 1) / a.n_chunks + 63) / 64 * 64);
   a.chunk = a.chunk ? a.chunk : 64;
   a.n_wgs = (uint32_t)(base * a.n_chunks < UINT32_MAX ? base * a.n_chunks : UINT32_MAX);

@@ -64,7 +64,7 @@ struct AttnParams {
 
 struct AttnPlan {
   uint32_t rows;             // rows of a tile
-  uint32_t n_wgs;
+  uint32_t n_wgs, waves;     // workgroups, waves of each (tiles of 16 and 32 rows)
   uint32_t min_granules, n_units, chunk, n_chunks;
   size_t part_o_floats, part_ml_floats, counters;  // workspace
 };

@@ -307,6 +307,16 @@ def test_attention_long(mer, gpu, seqs, heads, kv, d, page, window, sink):
     b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
 
 
+@pytest.mark.parametrize("n,heads,kv,d", [(600, 4, 2, 64), (300, 20, 4, 128), (257, 2, 1, 256), (2100, 2, 1, 64)])
+@pytest.mark.parametrize("more", [0, 1])
+def test_attention_many_sequences(mer, gpu, n, heads, kv, d, more):
+    """More sequences than a wave views at once, some without rows or keys, and
+    enough of them for the workgroups of one wave."""
+    seqs = [((i % 7 != 3) * (1 + more * (i % 2)), (37 * i) % 211) for i in range(n)]
+    b = Batch(seqs, heads, kv, d, 8, F16, seed=n)
+    b.check(b.run(mer, gpu))
+
+
 @pytest.mark.parametrize("hints", [dict(max_q_len=1, max_kv_len=1), dict(max_q_len=10 ** 6, max_kv_len=10 ** 6),
                                    dict(max_q_len=3, max_kv_len=300), {}])
 def test_attention_hints_do_not_matter(mer, gpu, hints):
