@@ -1634,6 +1634,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   p.n_kv_heads = cache->n_kv_heads;
   p.head_dim = cache->head_dim;
   p.group = (uint32_t)(n_heads / cache->n_kv_heads);
+  set_reciprocals(&p);
   p.window = window > (1u << 30) ? 0u : window;
   p.sinks = d_sinks;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);

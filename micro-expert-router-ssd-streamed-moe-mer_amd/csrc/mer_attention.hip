@@ -64,6 +64,16 @@ __device__ u4 g_zero_row[kMaxHeadDim * 2 / 16];
 __device__ __forceinline__ uint32_t lane_id() { return __lane_id(); }
 __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
+// x / group and x / n_kv_heads for x below 2^26, by the reciprocals that the
+// host prepared: exact, since m = ceil(2^s / d) with s = 26 + ceil(log2 d)
+// makes x m / 2^s exceed x / d by less than 1 / d.
+__device__ __forceinline__ uint32_t by_group(const AttnParams &p, uint32_t x) {
+  return (uint32_t)(((uint64_t)x * p.group_mul) >> p.group_shift);
+}
+__device__ __forceinline__ uint32_t by_heads(const AttnParams &p, uint32_t x) {
+  return (uint32_t)(((uint64_t)x * p.heads_mul) >> p.heads_shift);
+}
+
 // A word of an argument array that the whole wave reads, by the scalar path.
 __device__ __forceinline__ int32_t sload(const int32_t *p, uint64_t i) {
   return ((const __attribute__((address_space(4))) int32_t *)p)[i];
@@ -176,8 +186,8 @@ __device__ __forceinline__ Span make_span(const AttnParams &p, int32_t b, int32_
 // Keys [lo, hi) that some of the rows [row0, row1) of a span see.
 __device__ __forceinline__ void see(const AttnParams &p, const Span &s, int32_t row0, int32_t row1, int32_t *lo, int32_t *hi) {
   const int32_t pos0 = s.len - s.n;
-  const int32_t h = pos0 + (int32_t)((uint32_t)(row1 - 1) / p.group) + 1;
-  const int32_t l = p.window ? pos0 + (int32_t)((uint32_t)row0 / p.group) - (int32_t)p.window + 1 : 0;
+  const int32_t h = pos0 + (int32_t)by_group(p, (uint32_t)(row1 - 1)) + 1;
+  const int32_t l = p.window ? pos0 + (int32_t)by_group(p, (uint32_t)row0) - (int32_t)p.window + 1 : 0;
   *hi = h < 0 ? 0 : h;
   *lo = l < 0 ? 0 : (l > *hi ? *hi : l);
 }
@@ -439,10 +449,10 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
         for (uint32_t k = 1; k < share; ++k) acc += *(fd *)&lds[(g + k) * DP + dim];
     }
     if (mine < rows && part == 0 && dim < p.head_dim) {
-      const uint32_t gr = t.row0 + r, hq = head * p.group + gr % p.group;
+      const uint32_t gr = t.row0 + r, tk = by_group(p, gr), hq = head * p.group + gr - tk * p.group;
       if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      T *op = (T *)p.out + (uint64_t)(t.tok0 + gr / p.group) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
+      T *op = (T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
       *(td *)op = __builtin_convertvector(acc * inv, td);
     }
   }
@@ -472,6 +482,11 @@ struct Rows16 {
   static constexpr int kLds = kWaves * kStages * 2 * kTileBytes;
 };
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+
 // Walks the sequences' granules; a wave looks at 256 sequences at a time, four
 // to a lane.  (The host keeps the total below 2^31.)
 struct Granules {
@@ -498,11 +513,12 @@ struct Granules {
       w[i] = (rows + ROWS - 1) / ROWS * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
       upto += w[i];
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t x = __shfl_up(upto, d);
-      upto += lane_id() >= (uint32_t)d ? x : 0;
-    }
+    upto += scan_step<0x111, 0xf>(upto);  // from 1, 2, 4 and 8 lanes before, in rows of 16
+    upto += scan_step<0x112, 0xf>(upto);
+    upto += scan_step<0x114, 0xf>(upto);
+    upto += scan_step<0x118, 0xf>(upto);
+    upto += scan_step<0x142, 0xa>(upto);  // the row before's last to rows 1 and 3
+    upto += scan_step<0x143, 0xc>(upto);  // lane 31's to rows 2 and 3
     total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   }
 
@@ -591,12 +607,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     if (!gr.find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
     int32_t start = 0;
     const uint32_t n_gran = uni(Granules::granules<C::kGranule>(p, span, &start));
-    const uint32_t unit = uni((x - before) / n_gran), tile = uni(unit / p.n_kv_heads), head = unit - tile * p.n_kv_heads;
+    const uint32_t unit = uni((x - before) / n_gran), tile = uni(by_heads(p, unit)), head = unit - tile * p.n_kv_heads;
     const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
     const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
     // the unit's pieces: workgroups first_wg .. first_wg + n_pieces - 1
-    const uint32_t first_wg = g0 == 0 ? blockIdx.x : uni(unit0 / per);
-    const uint32_t n_pieces = uni((unit0 + n_gran - 1) / per) - first_wg + 1;
+    const uint32_t first_wg = g0 == 0 ? blockIdx.x : (per == 1 ? unit0 : uni(unit0 / per));
+    const uint32_t last_wg = g0 + count == n_gran ? blockIdx.x : (per == 1 ? unit0 + n_gran - 1 : uni((unit0 + n_gran - 1) / per));
+    const uint32_t n_pieces = last_wg - first_wg + 1;
     const uint32_t first_slot = 2 * first_wg + (first_wg * per == unit0 ? 0 : 1);
     const uint32_t my_slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
     first_piece = false;
@@ -614,7 +631,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     int32_t pos[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const uint32_t row = t.row0 + n * 16 + col, tok = row / p.group, hd = head * p.group + row % p.group;
+      const uint32_t row = t.row0 + n * 16 + col, tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
       pos[n] = t.pos0 + (int32_t)tok;
       const T *qp = (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
@@ -625,7 +642,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       }
     }
     const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
-    const int32_t pos_first = t.pos0 + (int32_t)(t.row0 / p.group), pos_last = t.pos0 + (int32_t)(last / p.group);
+    const int32_t pos_first = t.pos0 + (int32_t)by_group(p, t.row0), pos_last = t.pos0 + (int32_t)by_group(p, last);
 
     const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
     const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
@@ -768,7 +785,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
         ls += a * jm[(v * C::kRows + r) * 2 + 1];
         acc += a * *(const f8 *)&jo[(v * C::kRows + r) * DP + d];
       }
-      const uint32_t tk = rr / p.group, hq = head * p.group + rr % p.group;
+      const uint32_t tk = by_group(p, rr), hq = head * p.group + rr - tk * p.group;
       if (n_pieces == 1) {
         if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm));
         const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
@@ -834,12 +851,12 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   const uint32_t col = lane % 32, half = lane / 32;
   const uint32_t row = t.row0 + wave * 32 + col;
   const bool row_ok = row < t.n_rows;
-  const uint32_t tok = row / p.group, hd = head * p.group + row % p.group;
+  const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
   const int32_t pos = t.pos0 + (int32_t)tok, window = p.window ? (int32_t)p.window : 0x40000000;
   // the wave's positions; a wave without rows has none (first > last)
   const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
   const bool any = wrow < t.n_rows;
-  const int32_t pos_first = t.pos0 + (int32_t)(wrow / p.group), pos_last = t.pos0 + (int32_t)(wlast / p.group);
+  const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
   const float scale = fabsf(p.scale_log2);
 
   V8 q[DP / 16];
@@ -1059,10 +1076,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     for (int v = 0; v < kVecs; ++v) acc[v] += a * *(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024);
   }
   if (row >= t.n_rows) return;
-  const uint32_t hd = head * p.group + row % p.group;
+  const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
   if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu);
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  T *op = (T *)p.out + (uint64_t)(t.tok0 + row / p.group) * p.out_stride + (uint64_t)hd * p.head_dim;
+  T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     const uint32_t at = v * 32 + wave * 8 + half * 4;  // vector v * 4 + wave
@@ -1191,6 +1208,17 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
     a.part_ml_floats = rows * 2;
   }
   return a;
+}
+
+void set_reciprocals(AttnParams *p) {
+  auto set = [](uint32_t d, uint32_t *mul, uint32_t *shift) {
+    uint32_t log2 = 0;
+    while ((1u << log2) < d) ++log2;
+    *shift = 26 + log2;
+    *mul = (uint32_t)(((1ull << *shift) + d - 1) / d);
+  };
+  set(p->group, &p->group_mul, &p->group_shift);
+  set(p->n_kv_heads, &p->heads_mul, &p->heads_shift);
 }
 
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st) {

@@ -50,6 +50,7 @@ struct AttnParams {
   uint64_t q_stride, out_stride;
   uint32_t table_stride, n_seqs, n_tokens;
   uint32_t n_pages, page_shift, n_kv_heads, head_dim, group;
+  uint32_t group_mul, group_shift, heads_mul, heads_shift;  // reciprocals (set_reciprocals)
   uint32_t window;           // 0 = none
   float scale_log2;          // scale * log2(e)
   // decomposition (attn_plan)
@@ -71,6 +72,7 @@ struct AttnPlan {
 
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                    size_t max_q_len, size_t max_kv_len, uint32_t window, int cus);
+void set_reciprocals(AttnParams *p);
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
 
 }  // namespace mer
