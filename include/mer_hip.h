@@ -465,8 +465,7 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * window, are never read; a page id outside the cache reads as zeros and
  * records MER_ERR_RESIDENCY_MISS in the device status word.  kv_len is cut to
  * table_stride * page_size (at most 2^30) and rows to n_tokens.
- * A key or value that is not finite reaches rows of its own sequence only,
- * but there it may reach rows of the same call that do not see it.
+ * A key or value that is not finite reaches the rows that see it and no others.
  * max_q_len and max_kv_len say what the call should be laid out for, as a
  * captured graph needs it (0 = unknown); results do not depend on their being
  * right. */

@@ -1641,8 +1641,8 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   const size_t cap = table_stride * cache->page_size;
   if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
-  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, p.window,
-                                  g_dev[g_device].cus);
+  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
+                                  p.window, g_dev[g_device].cus);
   if (plan.n_wgs >= (1u << 24))
     return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
   p.min_granules = plan.min_granules;

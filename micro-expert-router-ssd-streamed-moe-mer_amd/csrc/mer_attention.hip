@@ -38,6 +38,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 struct F16 {
   typedef _Float16 T;
   typedef h8 V8;
+  static constexpr uint32_t kExponent = 0x7c00u, kOne = 0x3c00u;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -48,6 +49,7 @@ struct F16 {
 struct BF16 {
   typedef __bf16 T;
   typedef b8 V8;
+  static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -337,6 +339,65 @@ struct Share {
   }
 };
 
+// ---- values that are not finite ----
+// Where a tile holds keys that some rows do not see, their weight of zero must
+// not meet an infinity or a NaN.  Such a tile's values are looked over.  If one
+// is not finite, three products find the rows in which a NaN, +inf or -inf has
+// a weight, which a mark notes for the end, and it is cleared from the tile.
+// Marks are two bits an element: +inf, -inf, both for a NaN.
+
+// Whether one of the values of [at, at + 64 * BYTES) of LDS is not finite.
+template <class E, int BYTES>
+__device__ __forceinline__ bool not_finite(uint32_t at) {
+  constexpr uint32_t kMask = E::kExponent * 0x10001u, kCarry = (0x8000u - E::kExponent) * 0x10001u;
+  uint32_t found = 0;
+#pragma unroll 1
+  for (int i = 0; i < BYTES / 16; ++i) {
+    const u4 x = *(const __attribute__((address_space(3))) u4 *)(uintptr_t)(at + (i * 64 + lane_id()) * 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) found |= (x[k] & kMask) + kCarry;  // an exponent of ones carries into the sign's place
+  }
+  return __builtin_amdgcn_ballot_w64(found & 0x80008000u) != 0;
+}
+template <class E, int BYTES>
+__device__ __forceinline__ void clear_not_finite(uint32_t at) {
+#pragma unroll 1
+  for (int i = 0; i < BYTES / 2; ++i) {
+    __attribute__((address_space(3))) uint16_t *x =
+        (__attribute__((address_space(3))) uint16_t *)(uintptr_t)(at + (i * 64 + lane_id()) * 2);
+    if ((*x & E::kExponent) == E::kExponent) *x = 0;
+  }
+}
+// Ones where there is a NaN, +inf or -inf (kind 0, 1, 2), else zeros.
+template <class E>
+__device__ __forceinline__ typename E::V8 where(typename E::V8 v, uint32_t kind) {
+  u4 x = __builtin_bit_cast(u4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t b = x[i] >> h & 0xffffu, a = b & 0x7fffu;
+      const bool is = kind == 0 ? a > E::kExponent : b == (E::kExponent | (kind - 1) << 15);
+      word |= (is ? E::kOne : 0u) << h;
+    }
+    x[i] = word;
+  }
+  return __builtin_bit_cast(typename E::V8, x);
+}
+// The marks of N elements in which that kind has the weights x.
+template <int N, class V>
+__device__ __forceinline__ uint32_t mark(V x, uint32_t kind) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) bits |= x[e] > 0.0f ? 1u << 2 * e : 0u;
+  return bits * (kind == 0 ? 3 : kind);
+}
+__device__ __forceinline__ float add_mark(float o, uint32_t bits) {
+  o += bits & 1 ? __builtin_inff() : 0.0f;
+  return o + (bits & 2 ? -__builtin_inff() : 0.0f);
+}
+
 // ---- joining the pieces of a unit ----
 // A workgroup that has done one of several pieces leaves its sums in memory
 // (device-scope stores) and counts itself in; the one that comes last adds
@@ -488,7 +549,7 @@ __device__ __forceinline__ uint32_t scan_step(uint32_t x) {
 }
 
 // Walks the sequences' granules; a wave looks at 256 sequences at a time, four
-// to a lane.  (The host keeps the total below 2^31.)
+// to a lane.  (attn_plan keeps the total below 2^31.)
 struct Granules {
   uint32_t base, total;  // granules before the sequences in view, of those in view
   uint32_t upto;         // of the lanes up to this one, within the view
@@ -579,11 +640,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
   uint32_t k_lane[DP / 32], v_lane[DP / 16];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) k_lane[d] = col * (DP * 2) + ((d * 4 + quad) ^ L::k_swizzle(col)) * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 16; ++d) {
+  auto v_at = [&](uint32_t d) {
     const uint32_t r = quad * 4 + col / 4;
-    v_lane[d] = r * (DP * 2) + ((d * 2 + col % 4 / 2) ^ L::v_swizzle(r)) * 16 + col % 2 * 8;
-  }
+    return r * (DP * 2) + ((d * 2 + col % 4 / 2) ^ L::v_swizzle(r)) * 16 + col % 2 * 8;
+  };
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) v_lane[d] = v_at(d);
 
   Granules gr;
   gr.base = 0;
@@ -619,7 +681,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     first_piece = false;
     x += count;
     Tile t;
-    make_tile<C::kRows>(p, span, tile, &t);  // the tile is one of the sequence's
+    if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads) return;  // (spans that overlap, past 2^32)
     start = (int32_t)uni((uint32_t)start);
     int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
     if (p.window && begin < (t.lo & ~31)) begin = t.lo & ~31;
@@ -666,6 +728,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 
     float m[NR], l[NR];
     f4 o[NR][DP / 16];
+    uint32_t marks[NR][DP / 64] = {};
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       m[n] = -__builtin_inff();
@@ -742,20 +805,48 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       if (left == 1) wait_vm<0>();
       else if (left == 2) wait_vm<2 * C::kLoads>();
       else wait_vm<3 * C::kLoads>();
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        s4 v[2];
+      auto v_of = [&](uint32_t at) {
+        s4 x[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + v_lane[d] + b * 16 * (DP * 2)));
-        const V8 vv = __builtin_bit_cast(V8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + b * 16 * (DP * 2)));
+        return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      if (partial && pos_first != pos_last && not_finite<E, C::kTileBytes / 64>(vb)) {
+        // rolled up: few registers
+#pragma unroll 1
+        for (uint32_t i = 0; i < 3 * (DP / 16); ++i) {
+          const uint32_t d = i / 3, kind = i % 3;
+          const V8 v = where<E>(v_of(v_at(d)), kind);
 #pragma unroll
-        for (int n = 0; n < NR; ++n) o[n][d] = E::mfma16(vv, pr[n], o[n][d]);
+          for (int n = 0; n < NR; ++n) {
+            const uint32_t bits = mark<4>(E::mfma16(v, pr[n], f4{0, 0, 0, 0}), kind) << d % 4 * 8;
+#pragma unroll
+            for (uint32_t k = 0; k < DP / 64; ++k) marks[n][k] |= k == d / 4 ? bits : 0;
+          }
+        }
+        wait_lds();
+        clear_not_finite<E, C::kTileBytes / 64>(vb);
+        wait_lds();
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const V8 v = v_of(v_lane[d]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[n][d] = E::mfma16(v, pr[n], o[n][d]);
       }
       wait_lds();
       if (left > C::kStages) sh.template copy<true>(vb);
     }
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        if (__builtin_amdgcn_ballot_w64(marks[n][d / 4])) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][d][e] = add_mark(o[n][d][e], marks[n][d / 4] >> (d % 4 * 8 + e * 2));
+        }
     // join the waves: m, l and O of each in LDS
     __syncthreads();
     float *jo = (float *)smem;                      // [wave][row][DP]
@@ -813,7 +904,7 @@ struct Rows32 {
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kShare = kKeys / WAVES;       // keys that a wave copies
   static constexpr int kLoads = Share<DP, kShare>::kLoads;
-  static constexpr int kLds = 2 * 2 * kTileBytes;
+  static constexpr int kLds = 2 * 2 * kTileBytes + 16;  // and a flag
 };
 
 // Keys of a chunk and chunks of a tile: the plan's, longer ones where the keys
@@ -827,7 +918,7 @@ __device__ __forceinline__ void chunks_of(const AttnParams &p, const Tile &t, ui
 }
 
 template <class E, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_kernel(AttnParams p) {
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) void attn_rows32_kernel(AttnParams p) {
   typedef Rows32<DP, WAVES> C;
   typedef RowLayout<DP> L;
   typedef typename E::V8 V8;
@@ -857,6 +948,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
   const bool any = wrow < t.n_rows;
   const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
+  // the workgroup's
+  const uint32_t tlast = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
+  const int32_t wg_first = t.pos0 + (int32_t)by_group(p, t.row0), wg_last = t.pos0 + (int32_t)by_group(p, tlast);
   const float scale = fabsf(p.scale_log2);
 
   V8 q[DP / 16];
@@ -880,19 +974,26 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
   const uint32_t my_lds = wave * (C::kLoads * 1024u);
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
 
+  // set where a tile that not all rows see all of has a value that is not finite
+  volatile uint32_t *flag = (volatile uint32_t *)(smem + 4 * C::kTileBytes);
+  if (threadIdx.x == 0) *flag = 0;
+  __syncthreads();
+
   // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
   // dims a product.  V: 16 keys x 32 dims, 4 + 4 keys of a lane in the order
   // in which the scores lie in their lanes.
   uint32_t k_lane[DP / 16], v_lane[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 16; ++d) k_lane[d] = col * (DP * 2) + ((d * 2 + half) ^ L::k_swizzle(col)) * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d) {
+  auto v_at = [&](uint32_t d) {
     const uint32_t r = half * 4 + lane % 16 / 4;
-    v_lane[d] = r * (DP * 2) + ((d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r)) * 16 + lane % 2 * 8;
-  }
+    return r * (DP * 2) + ((d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ L::v_swizzle(r)) * 16 + lane % 2 * 8;
+  };
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) v_lane[d] = v_at(d);
 
   float m = -__builtin_inff(), l = 0.0f;
+  uint32_t marks[DP / 32] = {};
   f16v o[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -911,9 +1012,15 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
     const int32_t key0 = begin + i * C::kKeys;
     const uint32_t kb = stage(i), vb = kb + C::kTileBytes;
     const bool more = i + 1 < n_tiles;
+    const bool part_seen = wg_first != wg_last && (key0 + C::kKeys > wg_first + 1 || key0 <= wg_last - window);
+    if (part_seen) {
+      wait_vm<0>();
+      if (not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds)) *flag = 1;
+    }
     // all waves' copies of this tile are there, and everyone is done with the
     // other stage, which the next tile's copies fill meanwhile
     wait_vm_barrier<0>();
+    const bool flagged = part_seen && uni(*flag);
     if (more) {
       sh.advance(p.status);
       sh.lookup(my_key + (i + 2) * C::kKeys);
@@ -921,13 +1028,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
       sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
     }
     const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
-    if (live) {
-      auto v_of = [&](int ks, int d) {
+    if (live || flagged) {
+      auto v_of = [&](int ks, uint32_t at) {
         s4 x[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
           x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + v_lane[d] + (ks * 16 + b * 8) * (DP * 2)));
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
         return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
       };
       f16v s[2];
@@ -957,14 +1064,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
 #pragma unroll
       for (int ks = 0; ks < kAhead; ++ks)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, d);
+        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
       __builtin_amdgcn_sched_barrier(0);
       // The vector work goes first, so that the products of the other
       // workgroup's wave run beside it (4096-token prompt 185 -> 166 us; heads
       // of 64, which are all vector work, lose by it).
       if (DP > 64) __builtin_amdgcn_s_setprio(2);
-      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi ||
-          key0 <= pos_last - window) {
+      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
         const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -1004,17 +1110,49 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_rows32_ker
       l += sums[0] + sums[1];
       __builtin_amdgcn_sched_barrier(0);
       if (DP > 64) __builtin_amdgcn_s_setprio(0);
+      if (flagged) {
+        // rolled up: few registers
+#pragma unroll 1
+        for (uint32_t i = 0; i < 3 * (DP / 32); ++i) {
+          const uint32_t d = i / 3, kind = i % 3;
+          f16v x;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            x = E::mfma32(where<E>(v_of(ks, v_at(d)), kind), pr[ks], x);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          const uint32_t bits = mark<16>(x, kind);
+#pragma unroll
+          for (uint32_t k = 0; k < DP / 32; ++k) marks[k] |= k == d ? bits : 0;
+        }
+        __syncthreads();
+        clear_not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
+        if (threadIdx.x == 0) *flag = 0;
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < kAhead; ++ks)
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
+      }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           o[d] = E::mfma32(v[ks % kAhead][d], pr[ks], o[d]);
-          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, d);
+          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
         }
       }
     }
   }
   l += other_half(l);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+    if (__builtin_amdgcn_ballot_w64(marks[d])) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = add_mark(o[d][e], marks[d] >> 2 * e);
+    }
   if (n_chunks == 1) {
     if (!row_ok) return;
     if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m));
@@ -1146,9 +1284,12 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 }  // namespace
 
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                   size_t max_q_len, size_t max_kv_len, uint32_t window, int cus) {
+                   size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus) {
   AttnPlan a{};
   a.rows = max_q_len * group <= 16 ? 16 : (max_q_len * group <= 32 ? 32 : 128);
+  // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
+  const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
+  if (small_tiles * (table_keys / 128 + 2) >= (1ull << 31)) a.rows = 128;
   if (a.rows <= 32) {
     // Long stretches of few units: the widest workgroups, as many as the CUs
     // hold at once.  Many short units: as many waves, each a workgroup of its

@@ -71,7 +71,7 @@ struct AttnPlan {
 };
 
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                   size_t max_q_len, size_t max_kv_len, uint32_t window, int cus);
+                   size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus);
 void set_reciprocals(AttnParams *p);
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
 

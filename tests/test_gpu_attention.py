@@ -349,6 +349,57 @@ def test_attention_pages_before_the_window_are_not_read(mer, gpu):
     mer.take_device_status()
 
 
+@pytest.mark.parametrize("heads,kv,d,seqs,window,split", [
+    (16, 2, 128, [(2, 75), (1, 40)], 0, False),     # 16-row tiles
+    (16, 2, 64, [(4, 300), (3, 3)], 20, False),     # 32-row tiles
+    (4, 1, 256, [(8, 70)], 0, False),
+    (4, 2, 64, [(90, 90), (200, 333)], 0, False),   # 128-row tiles
+    (8, 1, 128, [(150, 400)], 70, False),
+    (2, 1, 256, [(130, 200)], 33, False),
+    (8, 1, 128, [(40, 9000)], 0, True),             # their keys in chunks
+])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attention_values_that_are_not_finite(mer, gpu, dt, heads, kv, d, seqs, window, split):
+    """An infinity or NaN in a value reaches the rows that see its key and no
+    other ones, and only its own dimension of them.  (Keys near zero, so that
+    every weight is an ordinary number.)"""
+    b = Batch(seqs, heads, kv, d, 16, dt, seed=12, kscale=0.1)
+    marks = []  # (sequence, key, kv head, dimension, value)
+    for i, (n, l) in enumerate(seqs):
+        for j, x in enumerate((math.nan, math.inf, -math.inf, math.inf, -math.inf, math.nan)):
+            marks.append((i, max(l - 1 - j * max(n // 4, 1), 0), j % kv, (5 * j + 3) % d if j < 4 else 8, x))
+        marks.append((i, 0, 0, 11, math.inf))
+    clean = [v.clone() for v in b.vv]
+    for i, key, g, at, x in marks:
+        b.vv[i][key, g, at] = x
+        clean[i][key, g, at] = 0
+        b.v[b.table[i, key // 16], g, key % 16, at] = x
+    got = b.run(mer, gpu, window=window).double()
+    group = heads // kv
+    for i, (n, l) in enumerate(seqs):
+        want, bound = attention64(b.q[b.start[i]:b.start[i + 1]].double(), b.kk[i].double(), clean[i].double(), l - n,
+                                  window, None, d ** -0.5, HALF[dt])
+        for g in range(kv):
+            vv, rows = b.vv[i][:, g].double(), got[b.start[i]:b.start[i + 1], g * group:(g + 1) * group]
+            for r in range(n):
+                lo, hi = max(l - n + r + 1 - window, 0) if window else 0, l - n + r + 1
+                odd = torch.where(vv[lo:hi].isfinite(), 0.0, vv[lo:hi]).sum(0)  # [d]
+                for hd in range(group):
+                    x, w, h = rows[r, hd], want[r, g * group + hd], bound[r, g * group + hd]
+                    ok = torch.where(odd.isnan(), x.isnan(), torch.where(odd != 0, x == odd, (x - w).abs() <= h + 2.0 ** -24))
+                    assert ok.all(), (i, g, r, hd, x[~ok], w[~ok], odd[~ok])
+
+
+def test_attention_of_a_wide_table(mer, gpu):
+    """A table of 2^30 keys a row and heads enough that 32 bits would not count
+    their pieces."""
+    b = Batch([(1, 300), (2, 77), (1, 0), (1, 1)], 64, 64, 8, 4096, F16, seed=13)
+    table = torch.full((4, 1 << 18), -1, dtype=torch.int32)
+    table[:, :b.table.shape[1]] = b.table
+    b.table = table
+    b.check(b.run(mer, gpu))
+
+
 def test_attention_page_outside_the_cache(mer, gpu):
     """Reads as zeros, is recorded, and leaves other sequences alone."""
     b = Batch([(1, 100), (1, 90)], 2, 1, 64, 16, F16, seed=9)
