@@ -342,8 +342,8 @@ struct Share {
 // ---- values that are not finite ----
 // Where a tile holds keys that some rows do not see, their weight of zero must
 // not meet an infinity or a NaN.  Such a tile's values are looked over.  If one
-// is not finite, three products find the rows in which a NaN, +inf or -inf has
-// a weight, which a mark notes for the end, and it is cleared from the tile.
+// is not finite, three products find the rows that see a NaN, +inf or -inf,
+// which a mark notes for the end, and it is cleared from the tile.
 // Marks are two bits an element: +inf, -inf, both for a NaN.
 
 // Whether one of the values of [at, at + 64 * BYTES) of LDS is not finite.
@@ -385,7 +385,19 @@ __device__ __forceinline__ typename E::V8 where(typename E::V8 v, uint32_t kind)
   }
   return __builtin_bit_cast(typename E::V8, x);
 }
-// The marks of N elements in which that kind has the weights x.
+// A lane's part of the weights, with one for each key that its row sees:
+// element e's key is `first` + e / 4 * STEP + e % 4.
+template <class E, int STEP>
+__device__ __forceinline__ typename E::V8 ones(int32_t first, int32_t last, int32_t before) {
+  u4 x;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const int32_t a = first + e / 4 * STEP + e % 4, b = a + 1;
+    x[e / 2] = (a <= last && a > before ? E::kOne : 0u) | (b <= last && b > before ? E::kOne << 16 : 0u);
+  }
+  return __builtin_bit_cast(typename E::V8, x);
+}
+// The marks of N elements that x keys of that kind reach.
 template <int N, class V>
 __device__ __forceinline__ uint32_t mark(V x, uint32_t kind) {
   uint32_t bits = 0;
@@ -821,7 +833,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
           const V8 v = where<E>(v_of(v_at(d)), kind);
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
-            const uint32_t bits = mark<4>(E::mfma16(v, pr[n], f4{0, 0, 0, 0}), kind) << d % 4 * 8;
+            const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4;
+            const V8 seen = ones<E, 16>(0, last_key, last_key - window);
+            const uint32_t bits = mark<4>(E::mfma16(v, seen, f4{0, 0, 0, 0}), kind) << d % 4 * 8;
 #pragma unroll
             for (uint32_t k = 0; k < DP / 64; ++k) marks[n][k] |= k == d / 4 ? bits : 0;
           }
@@ -904,7 +918,7 @@ struct Rows32 {
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kShare = kKeys / WAVES;       // keys that a wave copies
   static constexpr int kLoads = Share<DP, kShare>::kLoads;
-  static constexpr int kLds = 2 * 2 * kTileBytes + 16;  // and a flag
+  static constexpr int kLds = 2 * 2 * kTileBytes + 2 * WAVES * 4;  // and flags
 };
 
 // Keys of a chunk and chunks of a tile: the plan's, longer ones where the keys
@@ -974,10 +988,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
   const uint32_t my_lds = wave * (C::kLoads * 1024u);
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
 
-  // set where a tile that not all rows see all of has a value that is not finite
-  volatile uint32_t *flag = (volatile uint32_t *)(smem + 4 * C::kTileBytes);
-  if (threadIdx.x == 0) *flag = 0;
-  __syncthreads();
+  // a word for each stage and wave: its share of a tile that not all rows see
+  // all of has a value that is not finite
+  volatile uint32_t *flags = (volatile uint32_t *)(smem + 4 * C::kTileBytes);
 
   // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
   // dims a product.  V: 16 keys x 32 dims, 4 + 4 keys of a lane in the order
@@ -1015,28 +1028,54 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
     const bool part_seen = wg_first != wg_last && (key0 + C::kKeys > wg_first + 1 || key0 <= wg_last - window);
     if (part_seen) {
       wait_vm<0>();
-      if (not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds)) *flag = 1;
+      flags[(i & 1) * WAVES + wave] = not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
     }
     // all waves' copies of this tile are there, and everyone is done with the
     // other stage, which the next tile's copies fill meanwhile
     wait_vm_barrier<0>();
-    const bool flagged = part_seen && uni(*flag);
+    uint32_t flagged = 0;
+    if (part_seen) {
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) flagged |= flags[(i & 1) * WAVES + w];
+      flagged = uni(flagged);
+    }
     if (more) {
       sh.advance(p.status);
       sh.lookup(my_key + (i + 2) * C::kKeys);
       sh.template copy<false>(stage(i + 1) + my_lds);
       sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
     }
-    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
-    if (live || flagged) {
-      auto v_of = [&](int ks, uint32_t at) {
-        s4 x[2];
+    auto v_of = [&](int ks, uint32_t at) {
+      s4 x[2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
-        return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-      };
+      for (int b = 0; b < 2; ++b)
+        x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
+      return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    if (flagged) {
+#pragma unroll 1
+      for (uint32_t i = 0; i < 3 * (DP / 32); ++i) {  // rolled up: few registers
+        const uint32_t d = i / 3, kind = i % 3;
+        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
+        f16v x;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll 1
+        for (int ks = 0; ks < 4; ++ks) {
+          const V8 seen = ones<E, 8>(ks * 16, last, before);
+          x = E::mfma32(where<E>(v_of(ks, v_at(d)), kind), seen, x);
+        }
+        const uint32_t bits = mark<16>(x, kind);
+#pragma unroll
+        for (uint32_t k = 0; k < DP / 32; ++k) marks[k] |= k == d ? bits : 0;
+      }
+      __syncthreads();
+      clear_not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
+      __syncthreads();
+    }
+    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
+    if (live) {
       f16v s[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -1110,32 +1149,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
       l += sums[0] + sums[1];
       __builtin_amdgcn_sched_barrier(0);
       if (DP > 64) __builtin_amdgcn_s_setprio(0);
-      if (flagged) {
-        // rolled up: few registers
-#pragma unroll 1
-        for (uint32_t i = 0; i < 3 * (DP / 32); ++i) {
-          const uint32_t d = i / 3, kind = i % 3;
-          f16v x;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            x = E::mfma32(where<E>(v_of(ks, v_at(d)), kind), pr[ks], x);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          const uint32_t bits = mark<16>(x, kind);
-#pragma unroll
-          for (uint32_t k = 0; k < DP / 32; ++k) marks[k] |= k == d ? bits : 0;
-        }
-        __syncthreads();
-        clear_not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
-        if (threadIdx.x == 0) *flag = 0;
-        __syncthreads();
-#pragma unroll
-        for (int ks = 0; ks < kAhead; ++ks)
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
-      }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
