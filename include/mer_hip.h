@@ -427,7 +427,7 @@ typedef struct mer_kv_cache {
  *   (rows q_stride / k_stride elements apart); either may have no heads;
  *   d_positions[n_tokens] (any sign), d_inv_freq[rot_dim / 2], rot_dim a
  *   multiple of 8 up to head_dim; rot_dim 0 = no rotation, both unused;
- *   d_q_norm, d_k_norm [head_dim], NULL = no norm;
+ *   d_q_norm, d_k_norm [head_dim], NULL = no norm; eps finite, >= 0;
  *   outputs likewise, and they may be their inputs themselves where type and
  *   stride are the same (other overlaps are not allowed). */
 int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
@@ -466,6 +466,7 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * records MER_ERR_RESIDENCY_MISS in the device status word.  kv_len is cut to
  * table_stride * page_size (at most 2^30) and rows to n_tokens.
  * A key or value that is not finite reaches the rows that see it and no others.
+ * d_out may be d_q itself with the same stride (other overlaps are not allowed).
  * max_q_len and max_kv_len say what the call should be laid out for, as a
  * captured graph needs it (0 = unknown); results do not depend on their being
  * right. */

@@ -190,7 +190,7 @@ def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Ten
     scale        of q . k, default 1 / sqrt(head_dim)
     window       keys a row sees, itself included; 0 = all
     sinks        float32 [n_heads]: a logit per head that adds no value
-    out          like q; made with zeros in rows of no sequence when None
+    out          like q, or q itself; made with zeros in rows of no sequence when None
     """
     dev, stream = _enter(q)
     n, h, d = _shape(q, "q")

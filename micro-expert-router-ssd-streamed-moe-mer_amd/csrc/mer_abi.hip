@@ -964,6 +964,18 @@ int check_tensor(const char *name, const void *p, int type, size_t stride, size_
   return MER_OK;
 }
 
+int check_eps(bool norm, float eps) {
+  if (norm && !(eps >= 0.0f && eps < __builtin_inff()))
+    return fail(MER_ERR_INVALID_LAYOUT, "eps must be finite and not negative, got %g", (double)eps);
+  return MER_OK;
+}
+
+// Index arrays lie as their elements do.
+int check_words(const char *name, const void *p, size_t size) {
+  if ((uintptr_t)p & (size - 1)) return fail(MER_ERR_MISALIGNED, "%s must be %zu-byte aligned", name, size);
+  return MER_OK;
+}
+
 void set_rope(NormRopeParams *p, const float *inv_freq, size_t rot_dim, int interleaved, const int32_t *positions,
               float eps, size_t n_tokens, size_t head_dim) {
   p->positions = positions;
@@ -1552,6 +1564,7 @@ int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_he
                      (rc = check_tensor("k output", d_k_out, out_type, k_out_stride, n_kv_heads * head_dim, n_tokens))))
     return rc;
   if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if ((rc = check_eps(d_q_norm || d_k_norm, eps)) || (rc = check_words("positions", d_positions, 4))) return rc;
   if (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
   if ((rc = require_current_device())) return rc;
   NormRopeParams p{};
@@ -1578,6 +1591,9 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
     return rc;
   if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
   if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if ((rc = check_eps(d_k_norm, eps)) || (rc = check_words("positions", d_positions, 4)) ||
+      (rc = check_words("slots", d_slots, 8)))
+    return rc;
   if ((uintptr_t)d_k_norm & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
   if ((rc = require_current_device())) return rc;
   NormRopeParams p{};
@@ -1613,6 +1629,9 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
     return rc;
   if (!d_q_start || !d_kv_len || (!d_block_table && table_stride))
     return fail(MER_ERR_INVALID_LAYOUT, "null sequence description");
+  if ((rc = check_words("the block table", d_block_table, 4)) || (rc = check_words("q_start", d_q_start, 4)) ||
+      (rc = check_words("kv_len", d_kv_len, 4)) || (rc = check_words("sinks", d_sinks, 4)))
+    return rc;
   if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
   if (!(fabsf(scale) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale is not finite");
   if ((rc = require_current_device())) return rc;

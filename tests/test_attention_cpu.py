@@ -62,6 +62,8 @@ def test_good_arguments_get_as_far_as_the_device(abi):
     (dict(q=None), "INVALID_LAYOUT"), (dict(ko=None), "INVALID_LAYOUT"), (dict(pos=None), "INVALID_LAYOUT"),
     (dict(q=P + 2), "MISALIGNED"), (dict(qs=260), "MISALIGNED"), (dict(qs=248), "INVALID_LAYOUT"),
     (dict(kos=0), "INVALID_LAYOUT"), (dict(qn=P + 4), "MISALIGNED"), (dict(ks=1 << 41), "INVALID_LAYOUT"),
+    (dict(pos=P + 2), "MISALIGNED"), (dict(eps=-1e-6), "INVALID_LAYOUT"), (dict(eps=float("nan")), "INVALID_LAYOUT"),
+    (dict(eps=float("inf"), qn=0), "INVALID_LAYOUT"),
 ])
 def test_norm_rope_refuses(abi, change, status):
     assert norm_rope(abi, **change) == abi.Status[status]
@@ -97,6 +99,7 @@ def test_null_cache_refused(abi):
     (dict(in_type=3), "UNSUPPORTED_DTYPE"), (dict(k=None), "INVALID_LAYOUT"), (dict(v=P + 4), "MISALIGNED"),
     (dict(ks=132), "MISALIGNED"), (dict(vs=120), "INVALID_LAYOUT"), (dict(slots=None), "INVALID_LAYOUT"),
     (dict(pos=None), "INVALID_LAYOUT"), (dict(n=1 << 25), "SHAPE_EXCEEDS_WORKSPACE"),
+    (dict(slots=P + 4), "MISALIGNED"), (dict(pos=P + 1), "MISALIGNED"), (dict(eps=-1.0), "INVALID_LAYOUT"),
 ])
 def test_append_refuses(abi, change, status):
     assert append(abi, **change) == abi.Status[status]
@@ -106,6 +109,7 @@ def test_append_refuses(abi, change, status):
     (dict(h=3), "INVALID_LAYOUT"), (dict(h=0), "INVALID_LAYOUT"), (dict(seqs=(1 << 20) + 1), "SHAPE_EXCEEDS_WORKSPACE"),
     (dict(width=(1 << 26) + 1), "SHAPE_EXCEEDS_WORKSPACE"), (dict(q=None), "INVALID_LAYOUT"),
     (dict(qs=250), "MISALIGNED"), (dict(out=P + 6), "MISALIGNED"), (dict(table=None), "INVALID_LAYOUT"),
+    (dict(start=P + 2), "MISALIGNED"), (dict(lens=P + 1), "MISALIGNED"), (dict(table=P + 2), "MISALIGNED"),
     (dict(start=None), "INVALID_LAYOUT"), (dict(lens=None), "INVALID_LAYOUT"), (dict(n=1 << 25), "SHAPE_EXCEEDS_WORKSPACE"),
 ])
 def test_attention_refuses(abi, change, status):

@@ -349,6 +349,20 @@ def test_attention_pages_before_the_window_are_not_read(mer, gpu):
     mer.take_device_status()
 
 
+@pytest.mark.parametrize("seqs,heads,kv,d", [([(1, 5000), (1, 3)], 8, 1, 128), ([(150, 900), (7, 7)], 8, 2, 64),
+                                             ([(40, 6000)], 8, 1, 256)])
+def test_attention_in_place(mer, gpu, seqs, heads, kv, d):
+    b = Batch(seqs, heads, kv, d, 16, BF16, seed=14)
+    q = b.q.to(gpu)
+    cache = mer.PagedKvCache.wrap(b.k.to(gpu), b.v.to(gpu))
+    args = (b.table.to(gpu), torch.tensor(b.start, dtype=torch.int32, device=gpu),
+            torch.tensor([l for _, l in seqs], dtype=torch.int32, device=gpu))
+    want = mer.paged_attention(cache, q, *args)
+    assert mer.paged_attention(cache, q, *args, out=q) is q
+    assert torch.equal(q, want)
+    b.check(q.cpu())
+
+
 @pytest.mark.parametrize("heads,kv,d,seqs,window,split", [
     (16, 2, 128, [(2, 75), (1, 40)], 0, False),     # 16-row tiles
     (16, 2, 64, [(4, 300), (3, 3)], 20, False),     # 32-row tiles
@@ -388,6 +402,22 @@ def test_attention_values_that_are_not_finite(mer, gpu, dt, heads, kv, d, seqs, 
                     x, w, h = rows[r, hd], want[r, g * group + hd], bound[r, g * group + hd]
                     ok = torch.where(odd.isnan(), x.isnan(), torch.where(odd != 0, x == odd, (x - w).abs() <= h + 2.0 ** -24))
                     assert ok.all(), (i, g, r, hd, x[~ok], w[~ok], odd[~ok])
+
+
+@pytest.mark.parametrize("n,l,heads,kv,d", [(3, 75, 8, 2, 128), (6, 300, 8, 2, 64), (150, 400, 4, 2, 64), (40, 9000, 8, 1, 128)])
+@pytest.mark.parametrize("x", [math.nan, math.inf])
+def test_attention_key_that_is_not_finite(mer, gpu, n, l, heads, kv, d, x):
+    """The last token's key: its own rows of that kv head have no answer, all
+    others are as if it were not there."""
+    b = Batch([(n, l)], heads, kv, d, 16, F16, seed=15)
+    b.k[b.table[0, (l - 1) // 16], 0, (l - 1) % 16, 5] = x
+    b.q[-1].abs_()  # its score is +inf, or NaN
+    got = b.run(mer, gpu)
+    group = heads // kv
+    assert got[-1, :group].isnan().all()
+    want, bound = attention64(b.q.double(), b.kk[0].double(), b.vv[0].double(), l - n, 0, None, d ** -0.5, HALF[F16])
+    err, bound = (got.double() - want).abs(), bound + 2.0 ** -24
+    assert (err[:-1] <= bound[:-1]).all() and (err[-1, group:] <= bound[-1, group:]).all()
 
 
 def test_attention_of_a_wide_table(mer, gpu):
