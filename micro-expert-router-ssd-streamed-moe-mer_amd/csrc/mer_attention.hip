@@ -543,6 +543,11 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
 // The waves of a workgroup take a piece's tiles of 32 keys in turn, each with
 // a ring of LDS of its own (no barriers while the keys stream), and join
 // their sums at the piece's end.
+//
+// Bound by the memory: every wave has two tiles of K and V on the way, 128 KiB
+// a CU for heads of 128.  64 sequences of 200 - 8000 keys, 32 / 8 heads, bf16:
+// 203 us (5.1 TB/s); one of 131,000 keys, f16: 96 us (5.6 TB/s; plain reads
+// reach 5.9).  A single short one is bound by latency (700 keys: 11 us).
 template <int DP, int WAVES, int NR>
 struct Rows16 {
   static constexpr int kWaves = WAVES;
@@ -911,6 +916,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 // 32 rows a wave: prompts and larger chunks.  The waves of a workgroup share
 // tiles of 64 keys, two stages of K and V in LDS; each wave copies its share
 // of the next tile while the present one is used.
+//
+// Bound by the matrix units (48% of the cycles) and the vector units (49%),
+// which overlap only between the two workgroups that a CU holds of 128-element
+// heads.  32 rows a wave read each operand from LDS half as often as 16 would;
+// 64-key tiles leave 64 KiB for each of the two workgroups.  A 4096-token
+// prompt, 32 / 8 heads of 128, bf16: 157 us (877 TFLOP/s); 16384 tokens: 0.98
+// PFLOP/s; 4096 tokens of 64 heads of 64, where softmax outweighs the
+// products: 183 - 192 us (735 TFLOP/s); 2048 of 16 heads of 256 (one workgroup
+// a CU): 94 us (366 TFLOP/s).
 template <int DP, int WAVES>
 struct Rows32 {
   static constexpr int kRows = 32 * WAVES;
@@ -1195,7 +1209,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 }
 
 // Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
-// its accumulators spread over four waves.
+// its accumulators spread over four waves.  Bound by the memory: nine chunks
+// of 1040 rows x 32 heads of 128 in 27 us.
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   typedef Rows32<DP, WAVES> C;
@@ -1263,10 +1278,9 @@ hipError_t launch16(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   constexpr int kWide = DP == 256 ? 2 : 4;
   const bool wide = plan.waves == kWide, narrow = plan.waves == 1 && DP < 256;
   if (plan.rows == 16 && wide) return launch16w<E, DP, kWide, 1>(plan, p, st);
-  if (plan.rows == 32 && wide) return launch16w<E, DP, kWide, 2>(plan, p, st);
   if constexpr (DP < 256) {
+    if (plan.rows == 32 && wide) return launch16w<E, DP, kWide, 2>(plan, p, st);
     if (plan.rows == 16 && narrow) return launch16w<E, DP, 1, 1>(plan, p, st);
-    if (plan.rows == 32 && narrow) return launch16w<E, DP, 1, 2>(plan, p, st);
   }
   return hipErrorInvalidValue;
 }
@@ -1299,7 +1313,19 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                    size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus) {
   AttnPlan a{};
-  a.rows = max_q_len * group <= 16 ? 16 : (max_q_len * group <= 32 ? 32 : 128);
+  // Up to 16 rows a sequence: tiles of 16.  17 to 32 (a few tokens, or groups of
+  // more than 16 heads): 128-row tiles where there are units enough to give the
+  // CUs two workgroups (64 sequences of 8 x 4 rows, 500 - 2000 keys, 8 kv heads of
+  // 128: 67 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 61 us); two tiles of
+  // 16 where there is little to read (1 of 4000: 16 us, 32 23 us; 8 of 4000 - 8000:
+  // 66 and 52 us) and for heads of 256, whose 32 rows would not fit the registers
+  // (8 of 4000 - 8000: 75 and 86 us).  Above, tiles of 128 (8 x 48 rows: 46 us, 32
+  // 75 us).
+  const uint64_t pairs = (uint64_t)n_seqs * n_kv_heads;
+  a.rows = 128;
+  if (max_q_len * group <= 16) a.rows = 16;
+  else if (max_q_len * group <= 32 && pairs < (uint64_t)cus)
+    a.rows = head_dim > 128 || pairs * max_kv_len < 1024ull * cus ? 16 : 32;
   // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
   const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
   if (small_tiles * (table_keys / 128 + 2) >= (1ull << 31)) a.rows = 128;
@@ -1309,7 +1335,7 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
     // own, so that one's piece ends while the others' keys stream (512
     // sequences of 60 - 300 keys: 135 us wide, 95 us narrow; 8 of 1000: 11 us
     // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
-    const bool narrow = head_dim <= 128 && (uint64_t)n_seqs * n_kv_heads >= 4ull * cus;
+    const bool narrow = head_dim <= 128 && pairs >= 4ull * cus;
     a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);
     a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 64 ? 2 : 1);
     a.min_granules = 1;

@@ -16,6 +16,11 @@
 // Angles: position * inv_freq / 2 pi in 64 bits, less its nearest whole
 // number of turns, so far positions keep the same absolute error (2^-25 of a
 // turn) as near ones.
+//
+// Bound by the memory: q and k of 4096 tokens, 32 + 4 heads of 128, bf16, 15.0
+// us for 75.5 MB (5.0 TB/s; a large copy reaches 5.5); 4096 tokens of 8 f32
+// heads to a bf16 cache with the key's norm 10.1 us for 50.4 MB.  One token
+// takes 2.6 us, which is the launch and two dependent loads.
 #include "../../include/mer_hip.h"
 #include "mer_attention.hpp"
 

@@ -307,6 +307,19 @@ def test_attention_long(mer, gpu, seqs, heads, kv, d, page, window, sink):
     b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
 
 
+@pytest.mark.parametrize("n_seqs,new,keys,heads,kv,d,window", [
+    (1, 5, 4000, 16, 4, 128, 0), (3, 7, 900, 9, 3, 64, 50), (3, 20, 700, 4, 4, 256, 0),  # tiles of 16
+    (2, 9, 17000, 24, 8, 128, 0), (2, 8, 17500, 32, 8, 64, 900),                         # of 32
+    (130, 8, 150, 8, 2, 64, 0), (70, 6, 333, 16, 4, 128, 100), (260, 17, 40, 1, 1, 256, 0),  # of 128
+])
+def test_attention_few_tokens(mer, gpu, n_seqs, new, keys, heads, kv, d, window):
+    """A few tokens of each sequence: 17 to 32 rows of a kv head."""
+    seqs = [(new - i % 2, keys - 3 * i % 37) for i in range(n_seqs)]
+    b = Batch(seqs, heads, kv, d, 16, BF16, seed=n_seqs + new)
+    sinks = torch.linspace(-3, 3, heads) if window else None
+    b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
+
+
 @pytest.mark.parametrize("n,heads,kv,d", [(600, 4, 2, 64), (300, 20, 4, 128), (257, 2, 1, 256), (2100, 2, 1, 64)])
 @pytest.mark.parametrize("more", [0, 1])
 def test_attention_many_sequences(mer, gpu, n, heads, kv, d, more):
