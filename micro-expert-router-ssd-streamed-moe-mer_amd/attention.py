@@ -27,7 +27,7 @@ def _enter(t: torch.Tensor) -> tuple[int, int]:
     dev = t.get_device()
     if dev < 0:
         raise ValueError("expected a device tensor")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     _lib.ensure_init(dev)
     return dev, torch._C._cuda_getCurrentRawStream(dev)
@@ -64,6 +64,11 @@ def _shape(t: torch.Tensor, name: str) -> torch.Size:
     if t.dtype not in _TYPES:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
     return t.shape
+
+
+def _new(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An output like t (rows of heads side by side, which _rows has checked) without gaps."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format, dtype=dtype)
 
 
 class PagedKvCache:
@@ -123,7 +128,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {dt}")
     q_stride = _rows(q, n, h, d, src, dev, "q")
     if q_out is None:
-        q_out, qo_stride = torch.empty((n, h, d), dtype=dt, device=q.device), h * d
+        q_out, qo_stride = _new(q, dt), h * d
     else:
         qo_stride = _rows(q_out, n, h, d, dt, dev, "q_out")
     kh = k_ptr = k_stride = ko_ptr = ko_stride = 0
@@ -131,7 +136,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         kh = _shape(k, "k")[1]
         k_ptr, k_stride = k.data_ptr(), _rows(k, n, kh, d, src, dev, "k")
         if k_out is None:
-            k_out, ko_stride = torch.empty((n, kh, d), dtype=dt, device=q.device), kh * d
+            k_out, ko_stride = _new(k, dt), kh * d
         else:
             ko_stride = _rows(k_out, n, kh, d, dt, dev, "k_out")
         ko_ptr = k_out.data_ptr()
