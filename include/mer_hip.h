@@ -469,7 +469,10 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * d_out may be d_q itself with the same stride (other overlaps are not allowed).
  * max_q_len and max_kv_len say what the call should be laid out for, as a
  * captured graph needs it (0 = unknown); results do not depend on their being
- * right. */
+ * right.
+ * Sums of a call's parts lie in the stream's workspace: calls on one stream,
+ * and replays of the graphs captured on it, must not overlap each other (on
+ * one stream they do not). */
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
                             const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
                             const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,

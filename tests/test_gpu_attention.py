@@ -433,6 +433,24 @@ def test_attention_key_that_is_not_finite(mer, gpu, n, l, heads, kv, d, x):
     assert (err[:-1] <= bound[:-1]).all() and (err[-1, group:] <= bound[-1, group:]).all()
 
 
+@pytest.mark.parametrize("n", [2, 60])
+def test_attention_lengths_past_the_arrays(mer, gpu, n):
+    """kv_len is cut to what the table holds, rows to those of q; negative
+    lengths and starts are empty."""
+    b = Batch([(n, 96)], 4, 2, 64, 16, F16, seed=16)
+    cache = mer.PagedKvCache.wrap(b.k.to(gpu), b.v.to(gpu))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)
+    table = b.table[:, :6].contiguous().to(gpu)
+    got = mer.paged_attention(cache, b.q.to(gpu), table, i32(0, 2 ** 31 - 1), i32(2 ** 31 - 1))
+    b.check(got.cpu())
+    for start, lens in (((-5, n), (96,)), ((0, n), (96,))):
+        b.check(mer.paged_attention(cache, b.q.to(gpu), table, i32(*start), i32(*lens)).cpu())
+    for start, lens in (((0, n), (-1,)), ((n, 0), (96,)), ((0, -7), (96,)), ((n + 3, n + 9), (96,))):
+        got = mer.paged_attention(cache, b.q.to(gpu), table, i32(*start), i32(*lens))
+        assert (got == 0).all(), (start, lens)
+    mer.take_device_status()
+
+
 def test_attention_of_a_wide_table(mer, gpu):
     """A table of 2^30 keys a row and heads enough that 32 bits would not count
     their pieces."""
