@@ -1119,10 +1119,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
       __builtin_amdgcn_sched_barrier(0);
-      // The vector work goes first, so that the products of the other
-      // workgroup's wave run beside it (4096-token prompt 185 -> 166 us; heads
-      // of 64, which are all vector work, lose by it).
-      if (DP > 64) __builtin_amdgcn_s_setprio(2);
+      // From here to the tile's end a wave goes before one that is at its scores,
+      // whose products run beside it (4096-token prompt, against equal
+      // priorities: 184 -> 158 us), and each quarter of the products beside the
+      // next quarter's weights (173 -> 158 us).
+      __builtin_amdgcn_s_setprio(1);
       if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
         const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
 #pragma unroll
@@ -1150,8 +1151,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
       const float mu = m == -__builtin_inff() ? 0.0f : m;
       V8 pr[4];
       float sums[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
+      auto weights = [&](int ks) {
         f8 x;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -1159,18 +1159,21 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
           sums[e % 2] += x[e];
         }
         pr[ks] = __builtin_convertvector(x, V8);
-      }
-      l += sums[0] + sums[1];
+      };
+      weights(0);
       __builtin_amdgcn_sched_barrier(0);
-      if (DP > 64) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
+        if (ks + 1 < 4) weights(ks + 1);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           o[d] = E::mfma32(v[ks % kAhead][d], pr[ks], o[d]);
           if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
+      l += sums[0] + sums[1];
     }
   }
   l += other_half(l);
