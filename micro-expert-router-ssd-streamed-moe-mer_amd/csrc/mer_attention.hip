@@ -440,15 +440,17 @@ __device__ __forceinline__ bool last_piece(uint32_t *counter, uint32_t n_pieces,
   return *flag != 0;
 }
 
-// Adds up a unit's pieces: piece 0 is at first_slot of the partial sums, piece
-// c at 2 * (first_wg + c).  32 lanes hold a row's dims; the groups of 32 take
+// Adds up pieces c0, c0 + every, .. (n of them) of a unit: piece 0 is at
+// first_slot of the partial sums, piece c at 2 * (first_wg + c).  The result is
+// the unit's (`done`), or takes piece c0's place.  32 lanes hold a row's dims; the groups of 32 take
 // a row each, or share a row's pieces where there are fewer rows than groups.
 // A batch of pieces is in flight at once; what a lane reads beyond the pieces,
 // rows or dims that there are is left out.
 // `lds`: [THREADS / 32][DP] floats.
 template <class E, int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, uint32_t head, uint32_t first_wg,
-                                            uint32_t first_slot, uint32_t n_pieces, float *lds) {
+                                            uint32_t first_slot, uint32_t c0, uint32_t every, uint32_t n, bool done,
+                                            float *lds) {
   typedef typename E::T T;
   constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = DP == 256 ? 8 : 16;
   typedef float fd __attribute__((ext_vector_type(kDims)));
@@ -458,16 +460,19 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
   const uint32_t rows = t.n_rows - t.row0 < ROWS ? t.n_rows - t.row0 : ROWS;
   const uint32_t share = rows < kGroups ? kGroups / rows : 1;  // groups of a row
   const uint32_t step = kGroups / share, part = g % share;     // rows at a time
-  auto row_of = [&](uint32_t c, uint32_t r) { return (c ? 2 * (first_wg + c) : first_slot) * ROWS + r; };
-  auto ml_of = [&](uint32_t c, uint32_t r) {  // nothing beyond the pieces
+  auto row_of = [&](uint32_t i, uint32_t r) {
+    const uint32_t c = c0 + i * every;
+    return (c ? 2 * (first_wg + c) : first_slot) * ROWS + r;
+  };
+  auto ml_of = [&](uint32_t i, uint32_t r) {  // nothing beyond the pieces
     const f2 none = {-__builtin_inff(), 0.0f};
     const f2 ml = __builtin_bit_cast(
-        f2, __builtin_amdgcn_raw_buffer_load_b64(rm, row_of(c < n_pieces ? c : 0, r) * 8, 0, kDeviceScope));
-    return c < n_pieces ? ml : none;
+        f2, __builtin_amdgcn_raw_buffer_load_b64(rm, row_of(i < n ? i : 0, r) * 8, 0, kDeviceScope));
+    return i < n ? ml : none;
   };
   const uint32_t my_dim = dim < p.head_dim ? dim : 0;
-  auto o_of = [&](uint32_t c, uint32_t r) {
-    const uint32_t at = (row_of(c, r) * p.head_dim + my_dim) * 4;
+  auto o_of = [&](uint32_t i, uint32_t r) {
+    const uint32_t at = (row_of(i, r) * p.head_dim + my_dim) * 4;
     if constexpr (kDims == 2) {
       return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
     } else if constexpr (kDims == 4) {
@@ -484,34 +489,34 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
     // pieces 0 .. 31, a lane each.
     const f2 first = ml_of(ln, r);
     fd acc = {}, x[kBatch];
-    auto load = [&](uint32_t c0) {
+    auto load = [&](uint32_t i0) {
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint32_t c = c0 + b * share + part;
-        x[b] = o_of(c < n_pieces ? c : n_pieces - 1, r);
+        const uint32_t i = i0 + b * share + part;
+        x[b] = o_of(i < n ? i : n - 1, r);
       }
       __builtin_amdgcn_sched_barrier(0);
     };
     load(0);
     float m = first[0], l = first[1];
-    for (uint32_t c0 = 32; c0 < n_pieces; c0 += 32) {
-      const f2 ml = ml_of(c0 + ln, r);
+    for (uint32_t i0 = 32; i0 < n; i0 += 32) {
+      const f2 ml = ml_of(i0 + ln, r);
       const float mn = fmaxf(m, ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
       l = l * __builtin_amdgcn_exp2f(m - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
       m = mn;
     }
     const float mm = max_32(m), mu = mm == -__builtin_inff() ? 0.0f : mm;
     l = sum_32(l * __builtin_amdgcn_exp2f(m - mu));
-    for (uint32_t c0 = 0; c0 < n_pieces; c0 += 32) {
-      const f2 ml = c0 ? ml_of(c0 + ln, r) : first;
-      const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece c0 + lane
-      for (uint32_t k0 = 0; k0 < 32 && c0 + k0 < n_pieces; k0 += share * kBatch) {
-        if (c0 + k0) load(c0 + k0);
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+      const f2 ml = i0 ? ml_of(i0 + ln, r) : first;
+      const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece i0 + lane
+      for (uint32_t k0 = 0; k0 < 32 && i0 + k0 < n; k0 += share * kBatch) {
+        if (i0 + k0) load(i0 + k0);
 #pragma unroll
         for (uint32_t b = 0; b < kBatch; ++b) {
           const uint32_t k = k0 + b * share + part;
           const float wk = __shfl(w, (int)((threadIdx.x & 32) + (k & 31)));
-          if (k < 32 && c0 + k < n_pieces) acc += x[b] * wk;
+          if (k < 32 && i0 + k < n) acc += x[b] * wk;
         }
       }
     }
@@ -521,7 +526,20 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
       if (part == 0)
         for (uint32_t k = 1; k < share; ++k) acc += *(fd *)&lds[(g + k) * DP + dim];
     }
-    if (mine < rows && part == 0 && dim < p.head_dim) {
+    if (mine < rows && part == 0 && dim < p.head_dim && !done) {
+      const uint32_t to = row_of(0, r);
+      typedef uint32_t ud __attribute__((ext_vector_type(kDims < 4 ? kDims : 4)));
+#pragma unroll
+      for (uint32_t k = 0; k < kDims; k += 4) {
+        ud u;
+#pragma unroll
+        for (uint32_t e = 0; e < (kDims < 4 ? kDims : 4); ++e) u[e] = __float_as_uint(acc[k + e]);
+        if constexpr (kDims == 2) __builtin_amdgcn_raw_buffer_store_b64(u, ro, (to * p.head_dim + dim) * 4, 0, kDeviceScope);
+        else __builtin_amdgcn_raw_buffer_store_b128(u, ro, (to * p.head_dim + dim + k) * 4, 0, kDeviceScope);
+      }
+      if (ln == 0) put2(rm, to * 2, f2{mm, l});
+    }
+    if (mine < rows && part == 0 && dim < p.head_dim && done) {
       const uint32_t gr = t.row0 + r, tk = by_group(p, gr), hq = head * p.group + gr - tk * p.group;
       if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -908,8 +926,26 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
         if (d == 0) put2(rm, to * 2, f2{mm, ls});
       }
     }
-    if (n_pieces > 1 && last_piece(p.counters + first_wg, n_pieces, (uint32_t *)(jm + C::kWaves * C::kRows * 2)))
-      join_pieces<E, DP, C::kRows, 64 * C::kWaves>(p, t, head, first_wg, first_slot, n_pieces, jo);
+    // Many pieces are joined in two steps, sixteen at a time (a unit's counters
+    // do not meet another one's: in each third of them a workgroup begins, or
+    // goes on with, one unit that is cut).  128 pieces (a token over 131,000 keys
+    // of 2 heads of 256): 81 us in one step, 57 us in two; 32 pieces (8000 keys of
+    // 8 heads of 128): 17 us in one, 21 us in two.
+    if (n_pieces > 1) {
+      uint32_t *flag = (uint32_t *)(jm + C::kWaves * C::kRows * 2);
+      auto join = [&](uint32_t c0, uint32_t every, uint32_t n, bool done) {
+        join_pieces<E, DP, C::kRows, 64 * C::kWaves>(p, t, head, first_wg, first_slot, c0, every, n, done, jo);
+      };
+      constexpr uint32_t kJoin = 16;
+      const uint32_t c0 = (blockIdx.x - first_wg) / kJoin * kJoin, n = n_pieces - c0 < kJoin ? n_pieces - c0 : kJoin;
+      if (n_pieces <= 2 * kJoin) {
+        if (last_piece(p.counters + first_wg, n_pieces, flag)) join(0, 1, n_pieces, true);
+      } else if (n == 1 || last_piece(p.counters + (c0 ? gridDim.x : 0) + first_wg + c0, n, flag)) {
+        if (n > 1) join(c0, 1, n, false);
+        if (last_piece(p.counters + 2 * gridDim.x + first_wg, (n_pieces + kJoin - 1) / kJoin, flag))
+          join(0, kJoin, (n_pieces + kJoin - 1) / kJoin, true);
+      }
+    }
   }
 }
 
@@ -1344,7 +1380,7 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
     a.min_granules = 1;
     a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
-    a.counters = a.n_wgs;
+    a.counters = 3 * (size_t)a.n_wgs;
     return a;
   }
   a.n_units = (uint32_t)((n_tokens * group + a.rows - 1) / a.rows + n_seqs);

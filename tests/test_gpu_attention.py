@@ -307,6 +307,17 @@ def test_attention_long(mer, gpu, seqs, heads, kv, d, page, window, sink):
     b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
 
 
+@pytest.mark.parametrize("keys", [4096, 4219, 4300, 6200, 33000])
+@pytest.mark.parametrize("heads,d", [(3, 128), (16, 64), (9, 256)])
+def test_attention_many_pieces(mer, gpu, keys, heads, d):
+    """One unit over as many workgroups as there are stretches of 128 keys: 32,
+    33, 34, 49 and all of them; three calls, whose workgroups end in other orders."""
+    b = Batch([(1, keys)], heads, 1, d, 64, F16, seed=keys)
+    got = [b.run(mer, gpu) for _ in range(3)]
+    b.check(got[0])
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
 @pytest.mark.parametrize("n_seqs,new,keys,heads,kv,d,window", [
     (1, 5, 4000, 16, 4, 128, 0), (3, 7, 900, 9, 3, 64, 50), (3, 20, 700, 4, 4, 256, 0),  # tiles of 16
     (2, 9, 17000, 24, 8, 128, 0), (2, 8, 17500, 32, 8, 64, 900),                         # of 32
