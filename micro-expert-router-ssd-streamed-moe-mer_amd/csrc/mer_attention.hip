@@ -953,14 +953,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 // tiles of 64 keys, two stages of K and V in LDS; each wave copies its share
 // of the next tile while the present one is used.
 //
-// Bound by the matrix units (48% of the cycles) and the vector units (49%),
-// which overlap only between the two workgroups that a CU holds of 128-element
+// Bound by the matrix units (47% of the cycles) and the vector units (49%),
+// which overlap but in part: a wave's last products run beside its weights, its
+// first ones only beside the other workgroup that a CU holds of 128-element
 // heads.  32 rows a wave read each operand from LDS half as often as 16 would;
 // 64-key tiles leave 64 KiB for each of the two workgroups.  A 4096-token
-// prompt, 32 / 8 heads of 128, bf16: 157 us (877 TFLOP/s); 16384 tokens: 0.98
+// prompt, 32 / 8 heads of 128, bf16: 152 us (902 TFLOP/s); 16384 tokens: 1.0
 // PFLOP/s; 4096 tokens of 64 heads of 64, where softmax outweighs the
-// products: 183 - 192 us (735 TFLOP/s); 2048 of 16 heads of 256 (one workgroup
-// a CU): 94 us (366 TFLOP/s).
+// products: 182 us (755 TFLOP/s); 2048 of 16 heads of 256 (one workgroup a CU):
+// 88 us (390 TFLOP/s).
 template <int DP, int WAVES>
 struct Rows32 {
   static constexpr int kRows = 32 * WAVES;
