@@ -1249,8 +1249,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 }
 
 // Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
-// its accumulators spread over four waves.  Bound by the memory: nine chunks
-// of 1040 rows x 32 heads of 128 in 27 us.
+// its accumulators spread over four waves.  Bound by the memory: four chunks
+// of 1040 tokens x 32 heads of 128 in 15 us, nine in 27 us.
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   typedef Rows32<DP, WAVES> C;
@@ -1394,25 +1394,31 @@ AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv
   // workgroups; alone, one runs at 0.72 of the rate that they reach together
   // (two of 128-element heads; 1.02 against 0.74 PFLOP/s).  Rows of a prompt
   // see half its keys on average, longest first, which fills the rounds by
-  // itself (`uneven`), and so do sequences of different lengths.  kStart,
-  // kSplit, kJoin: a workgroup's start, its partial sums, the join's launch.
-  // Measured, 520 rows x 8 over 28000 keys: 1 chunk 805 us, 2 586 us, 4 582 us,
-  // 8 593 us, 16 616 us; a 4096-token prompt: 1 chunk 168 us, 2 190 us.
+  // itself (`uneven`).  Only the longest sequence is known: of several, the
+  // others are taken to be shorter (`ragged`) and to fill the rounds by half.
+  // kStart, kSplit, kJoin: a workgroup's start, its partial sums, the join.
+  // Measured, two sequences of 520 rows x 8 over 28000 keys: 1 chunk 794 us, 2 532
+  // us, 3 642 us, 4 538 us, 5 599 us, 8 558 us, 16 606 us; 512 tokens over 8000 keys:
+  // 1 193 us, 2 119 us, 4 83 us, 5 110 us, 8 94 us; three prompts of 500 - 900
+  // tokens: 1 32 us, 2 46 us.
   const double resident = head_dim <= 64 ? 3 : (head_dim <= 128 ? 2 : 1), alone = resident > 1 ? 0.72 : 1.0;
-  const double kStart = 1.0, kSplit = 1.5, kJoin = 6.0;
+  const double kStart = 1.0, kSplit = 1.5, kJoin = 9.0;
+  const double ragged = n_seqs > 1 ? 0.9 : 1.0;
   const double units = ((double)(n_tokens * group) / a.rows + 0.5 * (double)(n_seqs - 1)) * n_kv_heads;
   const double longest = (double)(max_keys + 63) / 64, spread = (double)(max_q_len < max_keys ? max_q_len : max_keys) / 64;
-  const double mean = window ? longest : longest - spread / 2, even = mean * units / cus;
+  const double mean = window ? longest : longest - spread / 2, even = mean * units * ragged / cus;
   double uneven = longest > 0 ? 2 * (longest - mean) / longest : 0;
   uneven = n_seqs > 1 && uneven < 0.5 ? 0.5 : uneven;
   const size_t base = (size_t)a.n_units * n_kv_heads;
   double best = 0;
   a.n_chunks = 1;
   for (size_t n = 1; n <= 64 && (n == 1 || (longest / n >= 4 && base * n <= 16 * resident * cus)); ++n) {
-    const double per_cu = ceil(units) * n / cus, k = ceil(per_cu), len = mean / n;
+    const double per_cu = ceil(units) * n / cus, k = ceil(per_cu * ragged), len = mean / n;
     const double last = k - floor(k / resident) * resident;  // workgroups of the last round
     const double whole = (k - last + (last == 1 ? 1 / alone : last)) * len;
-    const double smooth = fmax(longest / n / (per_cu > 1 ? 1.0 : alone), even);
+    // the longest workgroup beside as many as share its CU
+    const double beside = fmin(fmax(per_cu, 1.0), resident), rate = alone + (1 - alone) * fmin(beside - 1, 1.0);
+    const double smooth = fmax(longest / n * beside / rate, even);
     const double est = smooth + fmax(whole - smooth, 0.0) * (1 - uneven) + per_cu * kStart + (n > 1 ? per_cu * kSplit + kJoin : 0);
     if (n == 1 || est < best) {
       best = est;
