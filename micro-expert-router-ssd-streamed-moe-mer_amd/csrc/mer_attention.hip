@@ -39,6 +39,11 @@ struct F16 {
   typedef _Float16 T;
   typedef h8 V8;
   static constexpr uint32_t kExponent = 0x7c00u, kOne = 0x3c00u;
+  // Weights are taken 2^7 times larger, their sum and the sinks with them: up to
+  // 2^15 where the maximum lags by 8, and subnormal only below 2^-21 of the
+  // largest (2^-14 as they are, where a row's one large weight may meet a value
+  // smaller than what 32 others lose).
+  static constexpr float kUp = 7.0f;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -50,6 +55,7 @@ struct BF16 {
   typedef __bf16 T;
   typedef b8 V8;
   static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
+  static constexpr float kUp = 0.0f;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -541,7 +547,7 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
     }
     if (mine < rows && part == 0 && dim < p.head_dim && done) {
       const uint32_t gr = t.row0 + r, tk = by_group(p, gr), hq = head * p.group + gr - tk * p.group;
-      if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu);
+      if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu + E::kUp);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       T *op = (T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
       *(td *)op = __builtin_convertvector(acc * inv, td);
@@ -826,7 +832,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          e8[e] = __builtin_amdgcn_exp2f(x[e] - mu);
+          e8[e] = __builtin_amdgcn_exp2f(x[e] - (mu - E::kUp));
           sum += e8[e];
         }
         l[n] = l[n] * a + sum;
@@ -915,7 +921,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       }
       const uint32_t tk = by_group(p, rr), hq = head * p.group + rr - tk * p.group;
       if (n_pieces == 1) {
-        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm));
+        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm) + E::kUp);
         const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
         const V8 r8 = __builtin_convertvector(acc * inv, V8);
         *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
@@ -1185,7 +1191,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) o[d] *= a;
       }
-      const float mu = m == -__builtin_inff() ? 0.0f : m;
+      const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
       V8 pr[4];
       float sums[2] = {0.0f, 0.0f};
       auto weights = [&](int ks) {
@@ -1222,7 +1228,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
     }
   if (n_chunks == 1) {
     if (!row_ok) return;
-    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m));
+    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m) + E::kUp);
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll
@@ -1283,7 +1289,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   }
   if (row >= t.n_rows) return;
   const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
-  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu);
+  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu + E::kUp);
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
 #pragma unroll

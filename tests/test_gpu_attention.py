@@ -318,6 +318,29 @@ def test_attention_many_pieces(mer, gpu, keys, heads, d):
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+@pytest.mark.parametrize("n,window", [(1, 33), (3, 33), (40, 33), (260, 33), (200, 0)])
+def test_attention_small_weights_count(mer, gpu, n, window):
+    """One key far ahead of 32 others in every window, with values of zero: what
+    the others add, 2^-15 to 2^-18 of it each, is all there is."""
+    seqs, heads, d = [(n, 300)], 4, 64
+    b = Batch(seqs, heads, 1, d, 16, F16, seed=17)
+    big = torch.arange(300) % 33 == 0
+    b.q[:] = 0
+    b.q[..., 0] = 1
+    b.kk[0][:] = 0
+    b.kk[0][:, 0, 0] = torch.where(big, 12.0, torch.linspace(-0.45, 1.6, 300)).to(F16)
+    b.vv[0][:] = b.vv[0].abs() + 0.5
+    b.vv[0][big] = 0
+    for j in range(300):
+        b.k[b.table[0, j // 16], :, j % 16] = b.kk[0][j]
+        b.v[b.table[0, j // 16], :, j % 16] = b.vv[0][j]
+    got = b.run(mer, gpu, scale=1.0, window=window)
+    want, bound = attention64(b.q.double(), b.kk[0].double(), b.vv[0].double(), 300 - n, window, None, 1.0, HALF[F16])
+    # f16 weights and outputs; an output below 2^-14 rounds by 2^-25
+    assert ((got.double() - want).abs() <= bound + 2.0 ** -25).all()
+    assert (want > 2.0 ** -14).all()
+
+
 @pytest.mark.parametrize("n_seqs,new,keys,heads,kv,d,window", [
     (1, 5, 4000, 16, 4, 128, 0), (3, 7, 900, 9, 3, 64, 50), (3, 20, 700, 4, 4, 256, 0),  # tiles of 16
     (2, 9, 17000, 24, 8, 128, 0), (2, 8, 17500, 32, 8, 64, 900),                         # of 32
