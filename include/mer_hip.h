@@ -427,7 +427,8 @@ typedef struct mer_kv_cache {
  *   (rows q_stride / k_stride elements apart); either may have no heads;
  *   d_positions[n_tokens] (any sign), d_inv_freq[rot_dim / 2], rot_dim a
  *   multiple of 8 up to head_dim; rot_dim 0 = no rotation, both unused;
- *   d_q_norm, d_k_norm [head_dim], NULL = no norm; eps finite, >= 0;
+ *   d_q_norm, d_k_norm [head_dim], NULL = no norm; eps finite, >= 0 (squares
+ *   are summed in f32: a head whose sum passes 3.4e38 gives zeros);
  *   outputs likewise, and they may be their inputs themselves where type and
  *   stride are the same (other overlaps are not allowed). */
 int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_heads, size_t n_kv_heads,
