@@ -1660,8 +1660,10 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   const size_t cap = table_stride * cache->page_size;
   if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
+  const int cus = g_dev[g_device].cus;
+  const size_t reserve = attn_reserve(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
   const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
-                                  p.window, g_dev[g_device].cus);
+                                  p.window, cus, reserve);
   if (plan.n_wgs >= (1u << 24))
     return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
   p.min_granules = plan.min_granules;
@@ -1674,12 +1676,14 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (!w) return require_init();
   std::lock_guard<std::mutex> wl(w->mu);
   if (w->released) return released_error();
-  if (plan.part_o_floats) {
-    rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, plan.part_o_floats + plan.part_ml_floats, size_t(1) << 20, false,
-                    "attention workspace");
+  // Every call reserves what its sizes may need, one chunk or not, so that no
+  // smaller one moves the buffer; a captured call only what it uses.
+  size_t floats = plan.part_o_floats + plan.part_ml_floats;
+  if (w->attn_floats < reserve && !capturing(st)) floats = reserve;
+  if (floats) {
+    rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, floats, 0, false, "attention workspace");
     if (rc) return rc;
-    rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, plan.counters, size_t(1) << 14, true,
-                    "attention counters");
+    rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, attn_counters(cus), 0, true, "attention counters");
     if (rc) return rc;
     p.counters = w->attn_counters;
     p.part_o = w->attn_buf;

@@ -1356,92 +1356,6 @@ hipError_t launch_typed(const AttnPlan &plan, const AttnParams &p, hipStream_t s
 
 }  // namespace
 
-AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                   size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus) {
-  AttnPlan a{};
-  // Up to 16 rows a sequence: tiles of 16.  17 to 32 (a few tokens, or groups of
-  // more than 16 heads): 128-row tiles where there are units enough to give the
-  // CUs two workgroups (64 sequences of 8 x 4 rows, 500 - 2000 keys, 8 kv heads of
-  // 128: 67 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 61 us); two tiles of
-  // 16 where there is little to read (1 of 4000: 16 us, 32 23 us; 8 of 4000 - 8000:
-  // 66 and 52 us) and for heads of 256, whose 32 rows would not fit the registers
-  // (8 of 4000 - 8000: 75 and 86 us).  Above, tiles of 128 (8 x 48 rows: 46 us, 32
-  // 75 us).
-  const uint64_t pairs = (uint64_t)n_seqs * n_kv_heads;
-  a.rows = 128;
-  if (max_q_len * group <= 16) a.rows = 16;
-  else if (max_q_len * group <= 32 && pairs < (uint64_t)cus)
-    a.rows = head_dim > 128 || pairs * max_kv_len < 1024ull * cus ? 16 : 32;
-  // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
-  const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
-  if (small_tiles * (table_keys / 128 + 2) >= (1ull << 31)) a.rows = 128;
-  if (a.rows <= 32) {
-    // Long stretches of few units: the widest workgroups, as many as the CUs
-    // hold at once.  Many short units: as many waves, each a workgroup of its
-    // own, so that one's piece ends while the others' keys stream (512
-    // sequences of 60 - 300 keys: 135 us wide, 95 us narrow; 8 of 1000: 11 us
-    // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
-    const bool narrow = head_dim <= 128 && pairs >= 4ull * cus;
-    a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);
-    a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 64 ? 2 : 1);
-    a.min_granules = 1;
-    a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
-    a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
-    a.counters = 3 * (size_t)a.n_wgs;
-    return a;
-  }
-  a.n_units = (uint32_t)((n_tokens * group + a.rows - 1) / a.rows + n_seqs);
-  // keys of a row tile, from a whole key tile's start on
-  size_t max_keys = max_kv_len;
-  const size_t reach = (size_t)window + (a.rows + group - 1) / group + 64;
-  if (window && reach < max_keys) max_keys = reach;
-  // How many chunks a row tile's keys are cut into, by the time of the busiest
-  // CU in units of a 64-key tile at full rate.  A CU holds `resident`
-  // workgroups; alone, one runs at 0.72 of the rate that they reach together
-  // (two of 128-element heads; 1.02 against 0.74 PFLOP/s).  Rows of a prompt
-  // see half its keys on average, longest first, which fills the rounds by
-  // itself (`uneven`).  Only the longest sequence is known: of several, the
-  // others are taken to be shorter (`ragged`) and to fill the rounds by half.
-  // kStart, kSplit, kJoin: a workgroup's start, its partial sums, the join.
-  // Measured, two sequences of 520 rows x 8 over 28000 keys: 1 chunk 794 us, 2 532
-  // us, 3 642 us, 4 538 us, 5 599 us, 8 558 us, 16 606 us; 512 tokens over 8000 keys:
-  // 1 193 us, 2 119 us, 4 83 us, 5 110 us, 8 94 us; three prompts of 500 - 900
-  // tokens: 1 32 us, 2 46 us.
-  const double resident = head_dim <= 64 ? 3 : (head_dim <= 128 ? 2 : 1), alone = resident > 1 ? 0.72 : 1.0;
-  const double kStart = 1.0, kSplit = 1.5, kJoin = 9.0;
-  const double ragged = n_seqs > 1 ? 0.9 : 1.0;
-  const double units = ((double)(n_tokens * group) / a.rows + 0.5 * (double)(n_seqs - 1)) * n_kv_heads;
-  const double longest = (double)(max_keys + 63) / 64, spread = (double)(max_q_len < max_keys ? max_q_len : max_keys) / 64;
-  const double mean = window ? longest : longest - spread / 2, even = mean * units * ragged / cus;
-  double uneven = longest > 0 ? 2 * (longest - mean) / longest : 0;
-  uneven = n_seqs > 1 && uneven < 0.5 ? 0.5 : uneven;
-  const size_t base = (size_t)a.n_units * n_kv_heads;
-  double best = 0;
-  a.n_chunks = 1;
-  for (size_t n = 1; n <= 64 && (n == 1 || (longest / n >= 4 && base * n <= 16 * resident * cus)); ++n) {
-    const double per_cu = ceil(units) * n / cus, k = ceil(per_cu * ragged), len = mean / n;
-    const double last = k - floor(k / resident) * resident;  // workgroups of the last round
-    const double whole = (k - last + (last == 1 ? 1 / alone : last)) * len;
-    // the longest workgroup beside as many as share its CU
-    const double beside = fmin(fmax(per_cu, 1.0), resident), rate = alone + (1 - alone) * fmin(beside - 1, 1.0);
-    const double smooth = fmax(longest / n * beside / rate, even);
-    const double est = smooth + fmax(whole - smooth, 0.0) * (1 - uneven) + per_cu * kStart + (n > 1 ? per_cu * kSplit + kJoin : 0);
-    if (n == 1 || est < best) {
-      best = est;
-      a.n_chunks = (uint32_t)n;
-    }
-  }
-  a.chunk = (uint32_t)(((max_keys + a.n_chunks - 1) / a.n_chunks + 63) / 64 * 64);
-  a.chunk = a.chunk ? a.chunk : 64;
-  a.n_wgs = (uint32_t)(base * a.n_chunks < UINT32_MAX ? base * a.n_chunks : UINT32_MAX);
-  if (a.n_chunks > 1) {
-    const size_t rows = (size_t)a.n_wgs * a.rows;
-    a.part_o_floats = rows * (head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256));
-    a.part_ml_floats = rows * 2;
-  }
-  return a;
-}
-
 void set_reciprocals(AttnParams *p) {
   auto set = [](uint32_t d, uint32_t *mul, uint32_t *shift) {
     uint32_t log2 = 0;

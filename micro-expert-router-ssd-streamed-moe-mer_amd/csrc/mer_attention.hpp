@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "mer_attention_plan.hpp"
+
 namespace mer {
 
 // Element types, by their UTH dtype ids.
@@ -63,15 +65,6 @@ struct AttnParams {
   uint32_t *status;
 };
 
-struct AttnPlan {
-  uint32_t rows;             // rows of a tile
-  uint32_t n_wgs, waves;     // workgroups, waves of each (tiles of 16 and 32 rows)
-  uint32_t min_granules, n_units, chunk, n_chunks;
-  size_t part_o_floats, part_ml_floats, counters;  // workspace
-};
-
-AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                   size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus);
 void set_reciprocals(AttnParams *p);
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
 
