@@ -88,6 +88,7 @@ struct Workspace {
   size_t router_floats = 0;
   float *attn_buf = nullptr;     // attention: sums of a row's key chunks
   size_t attn_floats = 0;
+  size_t attn_refused = SIZE_MAX;  // smallest size that the device refused
   uint32_t *attn_counters = nullptr;  // chunks of a row tile that are done (zero between launches)
   size_t attn_counter_words = 0;
   uint32_t *counters = nullptr;  // decode counters (zero between launches) + control lines
@@ -228,7 +229,7 @@ void free_workspace(Workspace &w) {
   w.scratch = w.stage = w.router_buf = w.attn_buf = nullptr;
   w.counters = w.attn_counters = nullptr;
   w.release = nullptr;
-  w.scratch_refused = SIZE_MAX;
+  w.scratch_refused = w.attn_refused = SIZE_MAX;
   w.scratch_floats = w.stage_floats = w.router_floats = w.attn_floats = w.attn_counter_words = w.counter_words = w.release_words = 0;
 }
 
@@ -274,31 +275,36 @@ int ensure_scratch(Workspace &w, size_t floats, float **out) {
   return rc;
 }
 
-// At least `need` floats, and `want` where the device has them outside
-// capture.  The buffer in use is given up only for a larger one at hand, so a
-// device too full for `want` still serves what `need` covers; a size once
+// Grow a buffer to `want` floats where the device has them outside capture.
+// The one in use is given up only for a larger one at hand; a size once
 // refused is not asked for again.
-int ensure_scratch_upto(Workspace &w, size_t need, size_t want, float **out) {
-  if (w.scratch_floats < want && want < w.scratch_refused && !capturing(w.stream)) {
-    const size_t floats = want < (size_t(1) << 20) ? size_t(1) << 20 : want;
-    float *buf = nullptr;
-    if (hipMalloc(reinterpret_cast<void **>(&buf), floats * sizeof(float)) != hipSuccess) {
-      (void)hipGetLastError();  // the next launch's check must not see it
-      w.scratch_refused = want;
-    } else {
-      if (w.scratch) {
-        const hipError_t e = hipStreamSynchronize(w.stream);
-        if (e != hipSuccess) {
-          (void)hipFree(buf);
-          return hip_fail(e, MER_ERR_DEVICE_LOST, "synchronise before workspace growth");
-        }
-        (void)hipFree(w.scratch);
-      }
-      w.scratch = buf;
-      w.scratch_floats = floats;
-    }
+int grow_if_possible(Workspace &w, float **buf, size_t *cap, size_t *refused, size_t want) {
+  if (*cap >= want || want >= *refused || capturing(w.stream)) return MER_OK;
+  const size_t floats = want < (size_t(1) << 20) ? size_t(1) << 20 : want;
+  float *grown = nullptr;
+  if (hipMalloc(reinterpret_cast<void **>(&grown), floats * sizeof(float)) != hipSuccess) {
+    (void)hipGetLastError();  // the next launch's check must not see it
+    *refused = want;
+    return MER_OK;
   }
-  return ensure_scratch(w, need, out);
+  if (*buf) {
+    const hipError_t e = hipStreamSynchronize(w.stream);
+    if (e != hipSuccess) {
+      (void)hipFree(grown);
+      return hip_fail(e, MER_ERR_DEVICE_LOST, "synchronise before workspace growth");
+    }
+    (void)hipFree(*buf);
+  }
+  *buf = grown;
+  *cap = floats;
+  return MER_OK;
+}
+
+// At least `need` floats, and `want` where the device has them: a device too
+// full for `want` still serves what `need` covers.
+int ensure_scratch_upto(Workspace &w, size_t need, size_t want, float **out) {
+  const int rc = grow_if_possible(w, &w.scratch, &w.scratch_floats, &w.scratch_refused, want);
+  return rc ? rc : ensure_scratch(w, need, out);
 }
 
 // Decode counters: `words` per launch plus the control lines, all zero
@@ -1662,14 +1668,6 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
   const int cus = g_dev[g_device].cus;
   const size_t reserve = attn_reserve(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
-  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
-                                  p.window, cus, reserve);
-  if (plan.n_wgs >= (1u << 24))
-    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
-  p.min_granules = plan.min_granules;
-  p.n_units = plan.n_units;
-  p.chunk = plan.chunk;
-  p.n_chunks = plan.n_chunks;
   p.status = g_dev[g_device].status;
   const hipStream_t st = (hipStream_t)stream;
   std::shared_ptr<Workspace> w = workspace_for(st);
@@ -1677,14 +1675,26 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   std::lock_guard<std::mutex> wl(w->mu);
   if (w->released) return released_error();
   // Every call reserves what its sizes may need, one chunk or not, so that no
-  // smaller one moves the buffer; a captured call only what it uses.
-  size_t floats = plan.part_o_floats + plan.part_ml_floats;
-  if (w->attn_floats < reserve && !capturing(st)) floats = reserve;
-  if (floats) {
-    rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, floats, 0, false, "attention workspace");
-    if (rc) return rc;
+  // smaller one moves the buffer.  Where the device refuses that, the call is
+  // planned within what there is, down to one chunk without partial sums.
+  if ((rc = grow_if_possible(*w, &w->attn_buf, &w->attn_floats, &w->attn_refused, reserve))) return rc;
+  const size_t floats = reserve < w->attn_refused ? reserve : w->attn_floats;
+  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
+                                  p.window, cus, floats);
+  if (plan.n_wgs >= (1u << 24))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
+  p.min_granules = plan.min_granules;
+  p.n_units = plan.n_units;
+  p.chunk = plan.chunk;
+  p.n_chunks = plan.n_chunks;
+  const size_t need = plan.part_o_floats + plan.part_ml_floats;
+  // (there already, but for a captured call that no other went before)
+  if (need && (rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, need, 0, false, "attention workspace"))) return rc;
+  if (need || (!w->attn_counters && !capturing(st))) {
     rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, attn_counters(cus), 0, true, "attention counters");
     if (rc) return rc;
+  }
+  if (need) {
     p.counters = w->attn_counters;
     p.part_o = w->attn_buf;
     p.part_ml = w->attn_buf + plan.part_o_floats;

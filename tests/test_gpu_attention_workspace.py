@@ -84,3 +84,54 @@ def test_smaller_calls_keep_the_workspace(mer, gpu, heads, kv, d):
     mer.take_device_status()
     del graphs
     mer.stream_release(s)
+
+
+def test_a_full_device_runs_fewer_chunks(mer, gpu):
+    """A device that refuses what a chunk reserves still answers it, and the
+    buffer that a captured decode step points to stays where it is."""
+    say("attention workspace refused")
+    heads, kv, d, keys = 16, 4, 128, 8192
+    decode, chunk = (Call(mer, gpu, n, keys, heads, kv, d, 64, 70 + n) for n in (1, 600))
+    want, got = torch.zeros_like(chunk.out), torch.zeros_like(decode.out)
+    s, other = torch.cuda.Stream(device=gpu), torch.cuda.Stream(device=gpu)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        chunk.run(want)  # in chunks
+        decode.run(got)
+    with torch.cuda.stream(s):
+        decode.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        decode.run()
+    held = []
+    for step in (8 << 30, 1 << 30, 128 << 20):  # until less than 256 MiB are left
+        while torch.cuda.mem_get_info(gpu)[0] > step + (100 << 20):
+            held.append(torch.empty(step, dtype=torch.uint8, device=gpu))
+    free = torch.cuda.mem_get_info(gpu)[0]
+    assert free < 250 << 20
+    try:
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                chunk.run()
+        torch.cuda.synchronize()
+        # (the runtime may give back memory of its own when it refuses)
+        assert torch.cuda.mem_get_info(gpu)[0] >= free, "nothing was there to take"
+        decode.out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+    finally:
+        held.clear()
+        torch.cuda.empty_cache()
+    assert torch.equal(decode.out, got)
+    # both sides round the weights and the output once; 512 half steps of f32 cover the scores' sums
+    h = HALF[BF16]
+    flat = chunk.cache.v[chunk.table[0].long()].transpose(1, 2).reshape(-1, kv, d)[:keys]
+    most = flat.float().abs().amax(0).repeat_interleave(heads // kv, 0)
+    assert ((chunk.out.float() - want.float()).abs() <= 2 * (h + 512 * HALF[torch.float32]) * most + 2 * h * want.float().abs()).all()
+    assert chunk.out.float().abs().sum() > 0
+    mer.take_device_status()
+    del graph
+    for st in (s, other):
+        mer.stream_release(st)
