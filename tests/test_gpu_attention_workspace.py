@@ -91,7 +91,7 @@ def test_a_full_device_runs_fewer_chunks(mer, gpu):
     buffer that a captured decode step points to stays where it is."""
     say("attention workspace refused")
     heads, kv, d, keys = 16, 4, 128, 8192
-    decode, chunk = (Call(mer, gpu, n, keys, heads, kv, d, 64, 70 + n) for n in (1, 600))
+    decode, chunk = (Call(mer, gpu, n, keys, heads, kv, d, 64, 70 + n) for n in (1, 1200))  # the chunk reserves 256 MiB
     want, got = torch.zeros_like(chunk.out), torch.zeros_like(decode.out)
     s, other = torch.cuda.Stream(device=gpu), torch.cuda.Stream(device=gpu)
     torch.cuda.synchronize()
