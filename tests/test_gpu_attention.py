@@ -467,6 +467,23 @@ def test_attention_key_that_is_not_finite(mer, gpu, n, l, heads, kv, d, x):
     assert (err[:-1] <= bound[:-1]).all() and (err[-1, group:] <= bound[-1, group:]).all()
 
 
+@pytest.mark.parametrize("n,l,heads,kv", [(1, 200, 8, 2), (5, 260, 12, 2), (140, 333, 4, 2), (40, 9000, 8, 1)])
+@pytest.mark.parametrize("d", [8, 64, 72, 80, 96, 112, 128, 192, 200, 256])
+@pytest.mark.parametrize("x", [math.inf, -math.inf])
+def test_attention_key_that_no_row_minds(mer, gpu, n, l, heads, kv, d, x):
+    """Infinities in keys, against a q of the other sign: scores of -inf, so
+    these keys weigh nothing and every row has the answer of the others."""
+    b = Batch([(n, l)], heads, kv, d, 16, F16, seed=18)
+    dims = (3, d - 1)
+    for at in dims:
+        b.q[..., at] = -math.copysign(1.0, x) * (b.q[..., at].abs() + 0.5)
+    for key in (0, 37, l // 2, l - n - 1, max(l - n // 2 - 1, 1)):
+        at = dims[key % 2]
+        b.k[b.table[0, key // 16], :, key % 16, at] = x
+        b.kk[0][key, :, at] = math.copysign(3e4, x)  # of q's >= 0.5: exp(-900) at most
+    b.check(b.run(mer, gpu))
+
+
 @pytest.mark.parametrize("n", [2, 60])
 def test_attention_lengths_past_the_arrays(mer, gpu, n):
     """kv_len is cut to what the table holds, rows to those of q; negative
