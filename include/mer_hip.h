@@ -468,6 +468,8 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * table_stride * page_size (at most 2^30) and rows to n_tokens.
  * A key or value that is not finite reaches the rows that see it and no others.
  * d_out may be d_q itself with the same stride (other overlaps are not allowed).
+ * The lengths, starts and table must stay as they are while the call runs (its
+ * own result is lost otherwise, later ones are not).
  * max_q_len and max_kv_len say what the call should be laid out for, as a
  * captured graph needs it (0 = unknown); results do not depend on their being
  * right.

@@ -89,7 +89,7 @@ struct Workspace {
   float *attn_buf = nullptr;     // attention: sums of a row's key chunks
   size_t attn_floats = 0;
   size_t attn_refused = SIZE_MAX;  // smallest size that the device refused
-  uint32_t *attn_counters = nullptr;  // chunks of a row tile that are done (zero between launches)
+  uint64_t *attn_counters = nullptr;  // attention: tickets and counters of pieces that are done
   size_t attn_counter_words = 0;
   uint32_t *counters = nullptr;  // decode counters (zero between launches) + control lines
   size_t counter_words = 0;
@@ -227,8 +227,8 @@ void free_workspace(Workspace &w) {
   if (w.counters) (void)hipFree(w.counters);
   if (w.release) (void)hipFree(w.release);
   w.scratch = w.stage = w.router_buf = w.attn_buf = nullptr;
-  w.counters = w.attn_counters = nullptr;
-  w.release = nullptr;
+  w.counters = nullptr;
+  w.release = w.attn_counters = nullptr;
   w.scratch_refused = w.attn_refused = SIZE_MAX;
   w.scratch_floats = w.stage_floats = w.router_floats = w.attn_floats = w.attn_counter_words = w.counter_words = w.release_words = 0;
 }

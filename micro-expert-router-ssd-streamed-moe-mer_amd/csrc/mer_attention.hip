@@ -452,8 +452,7 @@ __device__ __forceinline__ float add_mark(float o, uint32_t bits) {
 // ---- joining the pieces of a unit ----
 // A workgroup that has done one of several pieces leaves its sums in memory
 // (device-scope stores) and counts itself in; the one that comes last adds
-// the pieces up, in their order, and leaves the count at zero for the next
-// launch.
+// the pieces up, in their order.
 constexpr int kDeviceScope = 16;  // sc1: past the caches that other XCDs do not see
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float *p) {
@@ -466,14 +465,15 @@ __device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, uint32_t index, f
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, x), r, index * 4, 0, kDeviceScope);
 }
 
-// True in every thread of the workgroup that comes last.  `flag`: a word of LDS.
-__device__ __forceinline__ bool last_piece(uint32_t *counter, uint32_t n_pieces, uint32_t *flag) {
+// True in every thread of the workgroup that comes last.  `epoch`: the launch's,
+// in thread 0; `flag`: a word of LDS.
+__device__ __forceinline__ bool last_piece(uint64_t *counter, uint64_t epoch, uint32_t n_pieces, uint32_t *flag) {
   wait_vm<0>();
   __syncthreads();
   if (threadIdx.x == 0) {
-    const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (n == n_pieces - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = n == n_pieces - 1;
+    (void)__hip_atomic_fetch_max(counter, epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t n = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = attn_is_last(n, n_pieces);
   }
   __syncthreads();
   return *flag != 0;
@@ -721,6 +721,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 #pragma unroll
   for (int d = 0; d < DP / 16; ++d) v_lane[d] = v_at(d);
 
+  uint64_t epoch = 0;  // in thread 0
+  if (tid == 0)
+    epoch = attn_epoch(__hip_atomic_fetch_add(p.counters + blockIdx.x % kAttnTickets * kAttnTicketWords,
+                                              attn_ticket(blockIdx.x, gridDim.x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+
   Granules gr;
   gr.base = 0;
   gr.view<C::kGranule, C::kRows>(p, 0);
@@ -755,7 +760,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     first_piece = false;
     x += count;
     Tile t;
-    if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads) return;  // (spans that overlap, past 2^32)
+    // (spans that overlap, past 2^32, or lengths that change under the kernel)
+    if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads || last_wg >= gridDim.x) return;
     start = (int32_t)uni((uint32_t)start);
     int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
     if (p.window && begin < (t.lo & ~31)) begin = t.lo & ~31;
@@ -978,11 +984,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       };
       constexpr uint32_t kJoin = 16;
       const uint32_t c0 = (blockIdx.x - first_wg) / kJoin * kJoin, n = n_pieces - c0 < kJoin ? n_pieces - c0 : kJoin;
+      uint64_t *const counters = p.counters + kAttnTickets * kAttnTicketWords + first_wg;
       if (n_pieces <= 2 * kJoin) {
-        if (last_piece(p.counters + first_wg, n_pieces, flag)) join(0, 1, n_pieces, true);
-      } else if (n == 1 || last_piece(p.counters + (c0 ? gridDim.x : 0) + first_wg + c0, n, flag)) {
+        if (last_piece(counters, epoch, n_pieces, flag)) join(0, 1, n_pieces, true);
+      } else if (n == 1 || last_piece(counters + (c0 ? gridDim.x : 0) + c0, epoch, n, flag)) {
         if (n > 1) join(c0, 1, n, false);
-        if (last_piece(p.counters + 2 * gridDim.x + first_wg, (n_pieces + kJoin - 1) / kJoin, flag))
+        if (last_piece(counters + 2 * gridDim.x, epoch, (n_pieces + kJoin - 1) / kJoin, flag))
           join(0, kJoin, (n_pieces + kJoin - 1) / kJoin, true);
       }
     }

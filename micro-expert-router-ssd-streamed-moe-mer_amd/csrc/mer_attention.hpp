@@ -61,7 +61,7 @@ struct AttnParams {
   uint32_t chunk, n_chunks;  // 128-row tiles: keys of one workgroup, workgroups of one row tile
   float *part_o;             // partial sums [slot][rows][head_dim]
   float *part_ml;            // their maxima and weights [slot][rows][2]
-  uint32_t *counters;        // finished pieces of a row tile, zero between launches
+  uint64_t *counters;        // tickets, then finished pieces of a unit (mer_attention_plan.hpp)
   uint32_t *status;
 };
 

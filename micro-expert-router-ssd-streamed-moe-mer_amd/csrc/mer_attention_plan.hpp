@@ -15,8 +15,25 @@ struct AttnPlan {
   size_t part_o_floats, part_ml_floats;  // partial sums
 };
 
-// Counters of the 16- and 32-row tiles: three for each of their workgroups.
-inline size_t attn_counters(int cus) { return 3 * 8 * (size_t)cus; }
+// Counters of the 16- and 32-row tiles, 64 bits each.  Of a launch, workgroups
+// that have done a piece of a unit count themselves in (three counters for each
+// of at most 8 workgroups a CU); the last one joins the pieces.  No launch
+// relies on what an earlier one left there: a counter holds an epoch above its
+// count, and whoever counts first raises it to its own launch's epoch.  Epochs
+// come from tickets, each a sum to which the workgroups of a launch that share it
+// (every kAttnTickets-th) add kAttnEpoch in all, so that all of them find the same
+// multiple of it there, in whatever order they come.  32 tickets, a cache line
+// each: one for all cost 1024 workgroups 10 us.
+constexpr uint32_t kAttnTickets = 32, kAttnTicketWords = 16;
+constexpr uint64_t kAttnEpoch = 1u << 16;
+constexpr size_t attn_counters(int cus) { return kAttnTickets * kAttnTicketWords + 3 * 8 * (size_t)cus; }
+// What workgroup `wg` of `n_wgs` adds to ticket wg % kAttnTickets.
+constexpr uint64_t attn_ticket(uint32_t wg, uint32_t n_wgs) {
+  return wg < kAttnTickets ? kAttnEpoch - (n_wgs - 1 - wg) / kAttnTickets : 1;
+}
+constexpr uint64_t attn_epoch(uint64_t ticket) { return ticket & ~(kAttnEpoch - 1); }
+// Whether a counter that stood at `before` has its last piece now.
+constexpr bool attn_is_last(uint64_t before, uint32_t n_pieces) { return (before & (kAttnEpoch - 1)) == n_pieces - 1; }
 
 // Partial sums are given 256 MiB at most.
 constexpr size_t kAttnRegionFloats = size_t(1) << 26;
@@ -85,7 +102,8 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
     a.min_granules = 1;
     a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
-    if (a.part_o_floats + a.part_ml_floats <= floats) return a;
+    // (a launch takes every ticket and counts up to kAttnEpoch at most)
+    if (a.part_o_floats + a.part_ml_floats <= floats && a.n_wgs >= kAttnTickets && a.n_wgs < kAttnEpoch / 2) return a;
     a = AttnPlan{};
     a.rows = 128;
   }

@@ -1,7 +1,8 @@
 """The attention call's plan (csrc/mer_attention_plan.hpp), compiled and run on
 the CPU: a call that is no larger than another in any size reserves no more, so
 it never moves a workspace that served the larger one, and every plan keeps
-within what it was given."""
+within what it was given.  And the counters of the pieces that are joined, played
+through: a launch counts right whatever an earlier one left in them."""
 from __future__ import annotations
 
 import os
@@ -63,7 +64,7 @@ int main() {
         CHECK(w || (size_t)p.chunk * p.n_chunks >= s.keys);
         CHECK(p.n_chunks == 1 || need == base * p.n_chunks * 128 * (attn_padded_dim(s.dim) + 2));
       } else {
-        CHECK(3 * (size_t)p.n_wgs <= attn_counters(cus) && need == 2 * (size_t)p.n_wgs * p.rows * (s.dim + 2));
+        CHECK(3 * (size_t)p.n_wgs + kAttnTickets * kAttnTicketWords <= attn_counters(cus) && p.n_wgs >= kAttnTickets && need == 2 * (size_t)p.n_wgs * p.rows * (s.dim + 2));
         CHECK(p.rows == 16 || q * s.group > 16);
       }
       if (floats == r && b + 1 < n2 && cus == 256) {  // plans alone would move the buffer for a smaller call
@@ -79,11 +80,77 @@ int main() {
 """
 
 
+COUNTERS = r"""
+#include "mer_attention_plan.hpp"
+#include <algorithm>
+#include <random>
+#include <stdio.h>
+#include <vector>
+using namespace mer;
+// Launches whose workgroups take their tickets, open a counter and count in it,
+// each step in any order between workgroups.  Some launches leave counts behind:
+// workgroups that stop after any of their steps, or count twice.
+int main() {
+  std::mt19937 rng(1);
+  auto below = [&](uint32_t n) { return (uint32_t)(rng() % n); };
+  std::vector<uint64_t> tickets(kAttnTickets, 0), counters(2048, 0);
+  const uint32_t grids[] = {32, 33, 63, 64, 100, 256, 512, 1024, 2048};
+  long units = 0, bad = 0, left = 0;
+  for (int launch = 0; launch < 400; ++launch) {
+    const uint32_t n = grids[below(9)];
+    const bool broken = below(3) == 0;
+    std::vector<uint32_t> first(n), pieces(n), step(n, 0), stop(n, 3), live(n), last_of(n, 0), counted(n, 0);
+    std::vector<uint64_t> epoch(n);
+    for (uint32_t w = 0; w < n;) {  // units of neighbouring workgroups
+      const uint32_t k = std::min(n - w, 1 + below(40));
+      for (uint32_t i = 0; i < k; ++i) first[w + i] = w, pieces[w + i] = k;
+      w += k;
+    }
+    if (broken) for (uint32_t w = 0; w < n; ++w) if (below(4) == 0) stop[w] = 1 + below(2), left += 1;
+    for (uint32_t w = 0; w < n; ++w) live[w] = w;
+    while (!live.empty()) {
+      const uint32_t at = below((uint32_t)live.size()), w = live[at];
+      if (step[w] == 0) {
+        uint64_t &t = tickets[w % kAttnTickets];
+        epoch[w] = attn_epoch(t);
+        t += attn_ticket(w, n);
+      } else if (step[w] == 1) {
+        counters[first[w]] = std::max(counters[first[w]], epoch[w]);
+      } else {
+        const int times = broken && below(8) == 0 ? 2 : 1;
+        for (int i = 0; i < times; ++i) {
+          const uint64_t before = counters[first[w]]++;
+          ++counted[first[w]];
+          if (attn_is_last(before, pieces[w])) {
+            ++last_of[first[w]];
+            if (!broken && counted[first[w]] != pieces[w]) ++bad;
+          }
+        }
+      }
+      if (++step[w] == stop[w]) live[at] = live.back(), live.pop_back();
+    }
+    for (uint32_t w = 0; w < n; ++w) if (epoch[w] != (uint64_t)launch * kAttnEpoch) ++bad;
+    if (!broken) for (uint32_t w = 0; w < n; ++w) if (first[w] == w) ++units, bad += last_of[w] != 1;
+  }
+  printf("%ld units joined, %ld workgroups stopped before, %ld failures\n", units, left, bad);
+  return bad || !units || !left;
+}
+"""
+
+
+def test_counters_of_a_launch_that_others_left_theirs_to(tmp_path):
+    build_and_run(tmp_path, COUNTERS)
+
+
 def test_reserve_grows_and_holds_every_plan(tmp_path):
+    build_and_run(tmp_path, "#include <initializer_list>\n" + MAIN)
+
+
+def build_and_run(tmp_path, main):
     gxx = shutil.which("g++")
     if not gxx:
         pytest.skip("g++ not available")
-    (tmp_path / "plan.cpp").write_text("#include <initializer_list>\n" + MAIN)
+    (tmp_path / "plan.cpp").write_text(main)
     r = subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", CSRC, str(tmp_path / "plan.cpp"),
                         "-o", str(tmp_path / "plan")], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-2000:]
