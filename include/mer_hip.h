@@ -466,7 +466,10 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * window, are never read; a page id outside the cache reads as zeros and
  * records MER_ERR_RESIDENCY_MISS in the device status word.  kv_len is cut to
  * table_stride * page_size (at most 2^30) and rows to n_tokens.
- * A key or value that is not finite reaches the rows that see it and no others.
+ * A key or value that is not finite reaches the rows that see it and no others:
+ * an infinity or NaN in a value makes its element of their answers that (both
+ * infinities a NaN), however small its weight; scores of +inf or NaN leave a
+ * row no answer (NaN), keys at -inf count nothing (zeros if there is no other).
  * d_out may be d_q itself with the same stride (other overlaps are not allowed).
  * The lengths, starts and table must stay as they are while the call runs (its
  * own result is lost otherwise, later ones are not).

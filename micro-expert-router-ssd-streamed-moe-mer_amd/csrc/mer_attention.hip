@@ -379,11 +379,16 @@ struct Share {
 };
 
 // ---- values that are not finite ----
-// Where a tile holds keys that some rows do not see, their weight of zero must
-// not meet an infinity or a NaN.  Such a tile's values are looked over.  If one
-// is not finite, three products find the rows that see a NaN, +inf or -inf,
-// which a mark notes for the end, and it is cleared from the tile.
+// An infinity or a NaN reaches the rows that see its key, whatever their weight
+// of it, and no others; but in the products it meets weights of zero, of keys
+// that a row does not see or that rounded to it, and makes a NaN.  So sums that
+// are not finite are made once more with care: a tile's values are looked over,
+// three products find the rows that see a NaN, +inf or -inf, which a mark notes
+// for the end, and these values are cleared from the tile.  (Looking over the
+// tiles that rows see in part, every time, cost prompts 1 - 2% and a window of
+// 1024 with heads of 64 5%.)
 // Marks are two bits an element: +inf, -inf, both for a NaN.
+template <bool CAREFUL> struct Pass { static constexpr bool careful = CAREFUL; };
 
 // Whether one of the values of [at, at + 64 * BYTES) of LDS is not finite.
 template <class E, int BYTES>
@@ -448,6 +453,27 @@ __device__ __forceinline__ float add_mark(float o, uint32_t bits) {
   o += bits & 1 ? __builtin_inff() : 0.0f;
   return o + (bits & 2 ? -__builtin_inff() : 0.0f);
 }
+
+// x * w; with care an infinity (a mark's) stays one where the weight is zero.
+template <class V, class P>
+__device__ __forceinline__ V weigh(V x, float w, P) {
+  V y = x * w;
+  if constexpr (P::careful) {
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(V) / sizeof(float); ++i) y[i] = w == 0.0f && fabsf(x[i]) == __builtin_inff() ? x[i] : y[i];
+  }
+  return y;
+}
+// Zero, or a NaN if one of x's elements is not finite.
+template <class V>
+__device__ __forceinline__ float probe(V x) {
+  float z = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(V) / sizeof(float); ++i) z = __builtin_fmaf(x[i], 0.0f, z);
+  return z;
+}
+// Whether some lane has a NaN.
+__device__ __forceinline__ bool not_a_number(float x) { return __builtin_amdgcn_ballot_w64(x != x) != 0; }
 
 // ---- joining the pieces of a unit ----
 // A workgroup that has done one of several pieces leaves its sums in memory
@@ -527,7 +553,7 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
     // The first batch of sums is under way with the weights; `first`: of the
     // pieces 0 .. 31, a lane each.
     const f2 first = ml_of(ln, r);
-    fd acc = {}, x[kBatch];
+    fd acc, x[kBatch];
     auto load = [&](uint32_t i0) {
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b) {
@@ -546,19 +572,24 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
     }
     const float mm = max_32(m), mu = mm == -__builtin_inff() ? 0.0f : mm;
     l = sum_32(l * __builtin_amdgcn_exp2f(m - mu));
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-      const f2 ml = i0 ? ml_of(i0 + ln, r) : first;
-      const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece i0 + lane
-      for (uint32_t k0 = 0; k0 < 32 && i0 + k0 < n; k0 += share * kBatch) {
-        if (i0 + k0) load(i0 + k0);
+    auto add_up = [&](auto pass) {
+      acc = fd{};
+      for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        const f2 ml = i0 ? ml_of(i0 + ln, r) : first;
+        const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece i0 + lane
+        for (uint32_t k0 = 0; k0 < 32 && i0 + k0 < n; k0 += share * kBatch) {
+          if (i0 + k0 || decltype(pass)::careful) load(i0 + k0);
 #pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          const uint32_t k = k0 + b * share + part;
-          const float wk = __shfl(w, (int)((threadIdx.x & 32) + (k & 31)));
-          if (k < 32 && i0 + k < n) acc += x[b] * wk;
+          for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t k = k0 + b * share + part;
+            const float wk = __shfl(w, (int)((threadIdx.x & 32) + (k & 31)));
+            if (k < 32 && i0 + k < n) acc += weigh(x[b], wk, pass);
+          }
         }
       }
-    }
+    };
+    add_up(Pass<false>());
+    if (not_a_number(probe(acc))) add_up(Pass<true>());
     if (share > 1) {  // in the one pass that there is then
       if (part) *(fd *)&lds[g * DP + dim] = acc;
       __syncthreads();
@@ -583,7 +614,7 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
       if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu + E::kUp);
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       T *op = (T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
-      *(td *)op = __builtin_convertvector(acc * inv, td);
+      *(td *)op = __builtin_convertvector(weigh(acc, inv, Pass<true>()), td);
     }
   }
 }
@@ -800,127 +831,137 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     // q has to be there before the first copy goes out: a later wait for it,
     // which the compiler would put into the loop, would drain the copies.
     __builtin_amdgcn_s_waitcnt(kWaitVm0);
-    for (int32_t i = 0; i < C::kStages && i < mine; ++i) {
-      sh.advance(p.status);
-      sh.lookup(key_of(i + 1));
-      sh.template copy<false>(slot_of(i));
-      sh.template copy<true>(slot_of(i) + C::kTileBytes);
-    }
-
     float m[NR], l[NR];
     f4 o[NR][DP / 16];
     uint32_t marks[NR][DP / 64] = {};
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      m[n] = -__builtin_inff();
-      l[n] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) o[n][d] = f4{0, 0, 0, 0};
-    }
-    for (int32_t i = 0; i < mine; ++i) {
-      const int32_t left = mine - i;
-      const int32_t key0 = key_of(i);
-      const uint32_t kb = slot_of(i), vb = kb + C::kTileBytes;
-      if (left == 1) wait_vm<C::kLoads>();
-      else wait_vm<3 * C::kLoads>();
-      f4 s[NR][2];
-      V8 k[2][DP / 32];
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d] + b * 16 * (DP * 2));
-      __builtin_amdgcn_sched_barrier(0);
+    for (bool careful = false;; careful = true) {
+      if (careful) sh.lookup(key_of(0));
+      for (int32_t i = 0; i < C::kStages && i < mine; ++i) {
+        sh.advance(p.status);
+        sh.lookup(key_of(i + 1));
+        sh.template copy<false>(slot_of(i));
+        sh.template copy<true>(slot_of(i) + C::kTileBytes);
+      }
+
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        s[n][0] = s[n][1] = f4{0, 0, 0, 0};
+        m[n] = -__builtin_inff();
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) o[n][d] = f4{0, 0, 0, 0};
+      }
+      for (int32_t i = 0; i < mine; ++i) {
+        const int32_t left = mine - i;
+        const int32_t key0 = key_of(i);
+        const uint32_t kb = slot_of(i), vb = kb + C::kTileBytes;
+        if (left == 1) wait_vm<C::kLoads>();
+        else wait_vm<3 * C::kLoads>();
+        f4 s[NR][2];
+        V8 k[2][DP / 32];
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) s[n][b] = E::mfma16(k[b][d], q[n][d], s[n][b]);
-      }
-      wait_lds();
-      if (left > C::kStages) {
-        sh.advance(p.status);
-        sh.lookup(key_of(i + C::kStages + 1));
-        sh.template copy<false>(kb);
-      }
-      const int32_t key_end = key0 + C::kKeys;
-      const bool partial = key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window;
-      V8 pr[NR];
+          for (int b = 0; b < 2; ++b)
+            k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d] + b * 16 * (DP * 2));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        // scores in base 2; keys of lane: b * 16 + quad * 4 + e
-        float x[8];
+        for (int n = 0; n < NR; ++n) {
+          s[n][0] = s[n][1] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[n][e / 4][e % 4] * p.scale_log2;
-        if (partial) {
-          const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4, before = last_key - window;
+          for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) s[n][b] = E::mfma16(k[b][d], q[n][d], s[n][b]);
+        }
+        wait_lds();
+        if (left > C::kStages) {
+          sh.advance(p.status);
+          sh.lookup(key_of(i + C::kStages + 1));
+          sh.template copy<false>(kb);
+        }
+        const int32_t key_end = key0 + C::kKeys;
+        const bool partial = key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window;
+        V8 pr[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          // scores in base 2; keys of lane: b * 16 + quad * 4 + e
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = s[n][e / 4][e % 4] * p.scale_log2;
+          if (partial) {
+            const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4, before = last_key - window;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int32_t at = (e / 4) * 16 + e % 4;
+              x[e] = at > last_key || at <= before ? -__builtin_inff() : x[e];
+            }
+          }
+          float mx = x[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+          mx = fmaxf(max_quad(mx), m[n]);
+          const float mu = mx == -__builtin_inff() ? 0.0f : mx;
+          const float a = __builtin_amdgcn_exp2f(m[n] - mu);
+          f8 e8;
+          float sum = 0.0f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int32_t at = (e / 4) * 16 + e % 4;
-            x[e] = at > last_key || at <= before ? -__builtin_inff() : x[e];
+            e8[e] = __builtin_amdgcn_exp2f(x[e] - (mu - E::kUp));
+            sum += e8[e];
           }
+          l[n] = l[n] * a + sum;
+          if (__builtin_amdgcn_ballot_w64(mx != m[n])) {
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) o[n][d] *= a;
+          }
+          m[n] = mx;
+          pr[n] = __builtin_convertvector(e8, V8);
         }
-        float mx = x[0];
+        if (left == 1) wait_vm<0>();
+        else if (left == 2) wait_vm<2 * C::kLoads>();
+        else wait_vm<3 * C::kLoads>();
+        auto v_of = [&](uint32_t at) {
+          s4 x[2];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-        mx = fmaxf(max_quad(mx), m[n]);
-        const float mu = mx == -__builtin_inff() ? 0.0f : mx;
-        const float a = __builtin_amdgcn_exp2f(m[n] - mu);
-        f8 e8;
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          e8[e] = __builtin_amdgcn_exp2f(x[e] - (mu - E::kUp));
-          sum += e8[e];
-        }
-        l[n] = l[n] * a + sum;
-        if (__builtin_amdgcn_ballot_w64(mx != m[n])) {
-#pragma unroll
-          for (int d = 0; d < DP / 16; ++d) o[n][d] *= a;
-        }
-        m[n] = mx;
-        pr[n] = __builtin_convertvector(e8, V8);
-      }
-      if (left == 1) wait_vm<0>();
-      else if (left == 2) wait_vm<2 * C::kLoads>();
-      else wait_vm<3 * C::kLoads>();
-      auto v_of = [&](uint32_t at) {
-        s4 x[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + b * 16 * (DP * 2)));
-        return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-      };
-      if (partial && pos_first != pos_last && not_finite<E, C::kTileBytes / 64>(vb)) {
-        // rolled up: few registers
+          for (int b = 0; b < 2; ++b)
+            x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + b * 16 * (DP * 2)));
+          return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        if (careful && not_finite<E, C::kTileBytes / 64>(vb)) {
+          // rolled up: few registers
 #pragma unroll 1
-        for (uint32_t i = 0; i < 3 * (DP / 16); ++i) {
-          const uint32_t d = i / 3, kind = i % 3;
-          const V8 v = where<E>(v_of(v_at(d)), kind);
+          for (uint32_t i = 0; i < 3 * (DP / 16); ++i) {
+            const uint32_t d = i / 3, kind = i % 3;
+            const V8 v = where<E>(v_of(v_at(d)), kind);
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4;
-            const V8 seen = ones<E, 16>(0, last_key, last_key - window);
-            const uint32_t bits = mark<4>(E::mfma16(v, seen, f4{0, 0, 0, 0}), kind) << d % 4 * 8;
+            for (int n = 0; n < NR; ++n) {
+              const int32_t last_key = pos[n] - key0 - (int32_t)quad * 4;
+              const V8 seen = ones<E, 16>(0, last_key, last_key - window);
+              const uint32_t bits = mark<4>(E::mfma16(v, seen, f4{0, 0, 0, 0}), kind) << d % 4 * 8;
 #pragma unroll
-            for (uint32_t k = 0; k < DP / 64; ++k) marks[n][k] |= k == d / 4 ? bits : 0;
+              for (uint32_t k = 0; k < DP / 64; ++k) marks[n][k] |= k == d / 4 ? bits : 0;
+            }
           }
+          wait_lds();
+          clear_not_finite<E, C::kTileBytes / 64>(vb);
+          wait_lds();
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          const V8 v = v_of(v_lane[d]);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o[n][d] = E::mfma16(v, pr[n], o[n][d]);
         }
         wait_lds();
-        clear_not_finite<E, C::kTileBytes / 64>(vb);
-        wait_lds();
+        if (left > C::kStages) sh.template copy<true>(vb);
       }
+      if (careful) break;
+      float z = 0.0f;
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        const V8 v = v_of(v_lane[d]);
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < NR; ++n) o[n][d] = E::mfma16(v, pr[n], o[n][d]);
-      }
-      wait_lds();
-      if (left > C::kStages) sh.template copy<true>(vb);
+        for (int d = 0; d < DP / 16; ++d) z += probe(o[n][d]);
+      if (!not_a_number(z)) break;
     }
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -950,20 +991,26 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       float mm = -__builtin_inff();
 #pragma unroll
       for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * C::kRows + r) * 2]);
-      float ls = 0.0f;
-      f8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
+      float ls;
+      f8 acc;
+      auto add_up = [&](auto pass) {
+        ls = 0.0f;
+        acc = f8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-      for (int v = 0; v < C::kWaves; ++v) {
-        const float mv = jm[(v * C::kRows + r) * 2];
-        const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
-        ls += a * jm[(v * C::kRows + r) * 2 + 1];
-        acc += a * *(const f8 *)&jo[(v * C::kRows + r) * DP + d];
-      }
+        for (int v = 0; v < C::kWaves; ++v) {
+          const float mv = jm[(v * C::kRows + r) * 2];
+          const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
+          ls += a * jm[(v * C::kRows + r) * 2 + 1];
+          acc += weigh(*(const f8 *)&jo[(v * C::kRows + r) * DP + d], a, pass);
+        }
+      };
+      add_up(Pass<false>());
+      if (not_a_number(probe(acc))) add_up(Pass<true>());
       const uint32_t tk = by_group(p, rr), hq = head * p.group + rr - tk * p.group;
       if (n_pieces == 1) {
         if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm) + E::kUp);
         const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
-        const V8 r8 = __builtin_convertvector(acc * inv, V8);
+        const V8 r8 = __builtin_convertvector(weigh(acc, inv, Pass<true>()), V8);
         *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
       } else {
         const uint32_t to = my_slot * C::kRows + r;
@@ -1060,9 +1107,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
   const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
   const bool any = wrow < t.n_rows;
   const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
-  // the workgroup's
-  const uint32_t tlast = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
-  const int32_t wg_first = t.pos0 + (int32_t)by_group(p, t.row0), wg_last = t.pos0 + (int32_t)by_group(p, tlast);
   const float scale = fabsf(p.scale_log2);
 
   V8 q[DP / 16];
@@ -1086,8 +1130,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
   const uint32_t my_lds = wave * (C::kLoads * 1024u);
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
 
-  // a word for each stage and wave: its share of a tile that not all rows see
-  // all of has a value that is not finite
+  // a word for each stage and wave: its share of a tile has a value that is not
+  // finite, and at the end one of its sums is not
   volatile uint32_t *flags = (volatile uint32_t *)(smem + 4 * C::kTileBytes);
 
   // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
@@ -1103,164 +1147,179 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) v_lane[d] = v_at(d);
 
-  float m = -__builtin_inff(), l = 0.0f;
+  float m, l;
   uint32_t marks[DP / 32] = {};
   f16v o[DP / 32];
+  auto all_tiles = [&](auto pass) {
+    constexpr bool careful = decltype(pass)::careful;
+    m = -__builtin_inff();
+    l = 0.0f;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
-  if (n_tiles > 0) {
-    sh.lookup(my_key);
-    __builtin_amdgcn_s_waitcnt(kWaitVm0);  // q is there before the first copy goes out (as above)
-    sh.advance(p.status);
-    sh.lookup(my_key + C::kKeys);
-    for (int32_t i = 0; i < 2; ++i) sh.clear_pads(stage(i) + my_lds);
-    sh.template copy<false>(stage(0) + my_lds);
-    sh.template copy<true>(stage(0) + C::kTileBytes + my_lds);
-  }
-  for (int32_t i = 0; i < n_tiles; ++i) {
-    const int32_t key0 = begin + i * C::kKeys;
-    const uint32_t kb = stage(i), vb = kb + C::kTileBytes;
-    const bool more = i + 1 < n_tiles;
-    const bool part_seen = wg_first != wg_last && (key0 + C::kKeys > wg_first + 1 || key0 <= wg_last - window);
-    if (part_seen) {
-      wait_vm<0>();
-      flags[(i & 1) * WAVES + wave] = not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
-    }
-    // all waves' copies of this tile are there, and everyone is done with the
-    // other stage, which the next tile's copies fill meanwhile
-    wait_vm_barrier<0>();
-    uint32_t flagged = 0;
-    if (part_seen) {
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) flagged |= flags[(i & 1) * WAVES + w];
-      flagged = uni(flagged);
-    }
-    if (more) {
+    if (n_tiles > 0) {
+      sh.lookup(my_key);
+      __builtin_amdgcn_s_waitcnt(kWaitVm0);  // q is there before the first copy goes out (as above)
       sh.advance(p.status);
-      sh.lookup(my_key + (i + 2) * C::kKeys);
-      sh.template copy<false>(stage(i + 1) + my_lds);
-      sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
+      sh.lookup(my_key + C::kKeys);
+      for (int32_t i = 0; i < 2; ++i) sh.clear_pads(stage(i) + my_lds);
+      sh.template copy<false>(stage(0) + my_lds);
+      sh.template copy<true>(stage(0) + C::kTileBytes + my_lds);
     }
-    auto v_of = [&](int ks, uint32_t at) {
-      s4 x[2];
+    for (int32_t i = 0; i < n_tiles; ++i) {
+      const int32_t key0 = begin + i * C::kKeys;
+      const uint32_t kb = stage(i), vb = kb + C::kTileBytes;
+      const bool more = i + 1 < n_tiles;
+      if (careful) {
+        wait_vm<0>();
+        flags[(i & 1) * WAVES + wave] = not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
+      }
+      // all waves' copies of this tile are there, and everyone is done with the
+      // other stage, which the next tile's copies fill meanwhile
+      wait_vm_barrier<0>();
+      uint32_t flagged = 0;
+      if (careful) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-        x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
-      return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    if (flagged) {
-#pragma unroll 1
-      for (uint32_t i = 0; i < 3 * (DP / 32); ++i) {  // rolled up: few registers
-        const uint32_t d = i / 3, kind = i % 3;
-        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
-        f16v x;
+        for (int w = 0; w < WAVES; ++w) flagged |= flags[(i & 1) * WAVES + w];
+        flagged = uni(flagged);
+      }
+      if (more) {
+        sh.advance(p.status);
+        sh.lookup(my_key + (i + 2) * C::kKeys);
+        sh.template copy<false>(stage(i + 1) + my_lds);
+        sh.template copy<true>(stage(i + 1) + C::kTileBytes + my_lds);
+      }
+      auto v_of = [&](int ks, uint32_t at) {
+        s4 x[2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+        for (int b = 0; b < 2; ++b)
+          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
+        return __builtin_bit_cast(V8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      if (careful && flagged) {
 #pragma unroll 1
-        for (int ks = 0; ks < 4; ++ks) {
-          const V8 seen = ones<E, 8>(ks * 16, last, before);
-          x = E::mfma32(where<E>(v_of(ks, v_at(d)), kind), seen, x);
+        for (uint32_t i = 0; i < 3 * (DP / 32); ++i) {  // rolled up: few registers
+          const uint32_t d = i / 3, kind = i % 3;
+          const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
+          f16v x;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll 1
+          for (int ks = 0; ks < 4; ++ks) {
+            const V8 seen = ones<E, 8>(ks * 16, last, before);
+            x = E::mfma32(where<E>(v_of(ks, v_at(d)), kind), seen, x);
+          }
+          const uint32_t bits = mark<16>(x, kind);
+#pragma unroll
+          for (uint32_t k = 0; k < DP / 32; ++k) marks[k] |= k == d ? bits : 0;
         }
-        const uint32_t bits = mark<16>(x, kind);
-#pragma unroll
-        for (uint32_t k = 0; k < DP / 32; ++k) marks[k] |= k == d ? bits : 0;
+        __syncthreads();
+        clear_not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
+        __syncthreads();
       }
-      __syncthreads();
-      clear_not_finite<E, C::kTileBytes / WAVES / 64>(vb + my_lds);
-      __syncthreads();
-    }
-    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
-    if (live) {
-      f16v s[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-      // operands are read a batch ahead of the products, so that the reads'
-      // latency is paid once a batch and not once a product
-      constexpr int kBatch = DP == 128 ? 8 : 4;
-#pragma unroll
-      for (int d0 = 0; d0 < DP / 16; d0 += kBatch) {
-        V8 k[2][kBatch];
-#pragma unroll
-        for (int d = 0; d < kBatch; ++d)
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d0 + d] + b * 32 * (DP * 2));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int d = 0; d < kBatch; ++d)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) s[b] = E::mfma32(k[b][d], q[d0 + d], s[b]);
-      }
-      constexpr int kAhead = DP == 256 ? 1 : 2;
-      V8 v[kAhead][DP / 32];
-#pragma unroll
-      for (int ks = 0; ks < kAhead; ++ks)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
-      __builtin_amdgcn_sched_barrier(0);
-      // From here to the tile's end a wave goes before one that is at its scores,
-      // whose products run beside it (4096-token prompt, against equal
-      // priorities: 184 -> 158 us), and each quarter of the products beside the
-      // next quarter's weights (173 -> 158 us).
-      __builtin_amdgcn_s_setprio(1);
-      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
-        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
+      const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
+      if (live) {
+        f16v s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
-            s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
-          }
-      }
-      float mx = fmaxf(s[0][0], s[1][0]);
+          for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+        // operands are read a batch ahead of the products, so that the reads'
+        // latency is paid once a batch and not once a product
+        constexpr int kBatch = DP == 128 ? 8 : 4;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
-      mx = fmaxf(mx, other_half(mx)) * scale;
-      // The maximum in use may lag by up to 8 (weights up to 2^8): O and l
-      // are scaled only when it would lag by more.
-      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
-        const float mn = fmaxf(m, mx);
-        const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= a;
+        for (int d0 = 0; d0 < DP / 16; d0 += kBatch) {
+          V8 k[2][kBatch];
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] *= a;
-      }
-      const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
-      V8 pr[4];
-      float sums[2] = {0.0f, 0.0f};
-      auto weights = [&](int ks) {
-        f8 x;
+          for (int d = 0; d < kBatch; ++d)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
-          sums[e % 2] += x[e];
+            for (int b = 0; b < 2; ++b)
+              k[b][d] = *(const __attribute__((address_space(3))) V8 *)(uintptr_t)(kb + k_lane[d0 + d] + b * 32 * (DP * 2));
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int d = 0; d < kBatch; ++d)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) s[b] = E::mfma32(k[b][d], q[d0 + d], s[b]);
         }
-        pr[ks] = __builtin_convertvector(x, V8);
-      };
-      weights(0);
-      __builtin_amdgcn_sched_barrier(0);
+        constexpr int kAhead = DP == 256 ? 1 : 2;
+        V8 v[kAhead][DP / 32];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks + 1 < 4) weights(ks + 1);
+        for (int ks = 0; ks < kAhead; ++ks)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          o[d] = E::mfma32(v[ks % kAhead][d], pr[ks], o[d]);
-          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
-        }
+          for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
         __builtin_amdgcn_sched_barrier(0);
+        // From here to the tile's end a wave goes before one that is at its scores,
+        // whose products run beside it (4096-token prompt, against equal
+        // priorities: 184 -> 158 us), and each quarter of the products beside the
+        // next quarter's weights (173 -> 158 us).
+        __builtin_amdgcn_s_setprio(1);
+        if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
+          const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
+              s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
+            }
+        }
+        float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+        mx = fmaxf(mx, other_half(mx)) * scale;
+        // The maximum in use may lag by up to 8 (weights up to 2^8): O and l
+        // are scaled only when it would lag by more.
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
+          const float mn = fmaxf(m, mx);
+          const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= a;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) o[d] *= a;
+        }
+        const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
+        V8 pr[4];
+        float sums[2] = {0.0f, 0.0f};
+        auto weights = [&](int ks) {
+          f8 x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
+            sums[e % 2] += x[e];
+          }
+          pr[ks] = __builtin_convertvector(x, V8);
+        };
+        weights(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          if (ks + 1 < 4) weights(ks + 1);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            o[d] = E::mfma32(v[ks % kAhead][d], pr[ks], o[d]);
+            if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        l += sums[0] + sums[1];
       }
-      __builtin_amdgcn_s_setprio(0);
-      l += sums[0] + sums[1];
     }
-  }
+  };
+  all_tiles(Pass<false>());
+  float z = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) z += probe(o[d]);
+  flags[wave] = not_a_number(z);
+  __syncthreads();
+  uint32_t again = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) again |= flags[w];
+  __syncthreads();  // everyone has read them, and is done with the tiles
+  if (uni(again)) all_tiles(Pass<true>());
   l += other_half(l);
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -1280,7 +1339,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
         const uint32_t at = d * 32 + g * 8 + half * 4;
         typedef T T4 __attribute__((ext_vector_type(4)));
         const f4 x = {o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
-        if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x * inv, T4);
+        if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(weigh(x, inv, Pass<true>()), T4);
       }
   } else {
     // A partial sum lies as the accumulators do, so every store is a whole
@@ -1317,18 +1376,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   const uint64_t slot0 = (uint64_t)uh * p.n_chunks;
   const float *ml = p.part_ml + ((slot0 * WAVES + w) * 32 + col) * 2;
   const float *po = p.part_o + (slot0 * WAVES + w) * (32 * DP) + wave * 256 + lane * 4;
-  float m = -__builtin_inff(), l = 0.0f;
+  float m = -__builtin_inff(), l;
   for (uint32_t c = 0; c < n_chunks; ++c) m = fmaxf(m, ml[c * (WAVES * 64)]);
   const float mu = m == -__builtin_inff() ? 0.0f : m;
-  f4 acc[kVecs] = {};
-#pragma unroll 4
-  for (uint32_t c = 0; c < n_chunks; ++c) {
-    const f2 x = *(const f2 *)(ml + c * (WAVES * 64));
-    const float a = __builtin_amdgcn_exp2f(x[0] - mu);
-    l += a * x[1];
+  f4 acc[kVecs];
+  auto add_up = [&](auto pass) {
+    l = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) acc[v] += a * *(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024);
-  }
+    for (int v = 0; v < kVecs; ++v) acc[v] = f4{0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t c = 0; c < n_chunks; ++c) {
+      const f2 x = *(const f2 *)(ml + c * (WAVES * 64));
+      const float a = __builtin_amdgcn_exp2f(x[0] - mu);
+      l += a * x[1];
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) acc[v] += weigh(*(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024), a, pass);
+    }
+  };
+  add_up(Pass<false>());
+  float z = 0.0f;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) z += probe(acc[v]);
+  if (not_a_number(z)) add_up(Pass<true>());
   if (row >= t.n_rows) return;
   const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
   if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu + E::kUp);
@@ -1338,7 +1407,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   for (int v = 0; v < kVecs; ++v) {
     const uint32_t at = v * 32 + wave * 8 + half * 4;  // vector v * 4 + wave
     typedef T T4 __attribute__((ext_vector_type(4)));
-    if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(acc[v] * inv, T4);
+    if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(weigh(acc[v], inv, Pass<true>()), T4);
   }
 }
 

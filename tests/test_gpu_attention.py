@@ -451,6 +451,44 @@ def test_attention_values_that_are_not_finite(mer, gpu, dt, heads, kv, d, seqs, 
                     assert ok.all(), (i, g, r, hd, x[~ok], w[~ok], odd[~ok])
 
 
+@pytest.mark.parametrize("n,l,heads,kv,d", [
+    (1, 700, 8, 2, 128), (1, 6000, 8, 1, 64), (1, 40000, 4, 1, 128), (1, 3000, 3, 1, 256),  # 16-row tiles, pieces
+    (3, 2000, 16, 2, 192), (6, 3000, 20, 4, 64),
+    (60, 300, 4, 2, 64), (300, 900, 4, 1, 128), (40, 9000, 8, 1, 128), (130, 1000, 2, 1, 256), (70, 400, 4, 2, 80),
+])
+@pytest.mark.parametrize("window,sink", [(0, None), (0, 2000.0), (150, None)])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attention_infinite_values_of_no_weight(mer, gpu, dt, n, l, heads, kv, d, window, sink):
+    """Scores that grow with the key, so that weights far back round to zero: an
+    infinity or NaN there reaches every row that sees its key all the same, in
+    whatever tile, piece or chunk it lies and whatever the call is told to expect."""
+    b = Batch([(n, l)], heads, kv, d, 16, dt, seed=19)
+    b.q[:] = 0
+    b.q[..., 0] = 1
+    b.kk[0][:] = 0
+    b.kk[0][..., 0] = (torch.arange(l) * (600.0 / l)).to(dt)[:, None]
+    clean = b.vv[0].clone()
+    for i, key in enumerate((0, 40, l // 3, l // 2, l - n - 70, l - n, l - n // 2 - 1, l - 1)):
+        for j, x in enumerate((math.inf, -math.inf, math.nan)):
+            at = (7 * i + 2 * j) % d
+            b.vv[0][max(key, 0), i % kv, at] = x
+    b.vv[0][41, 0, 7 % d] = -math.inf
+    clean[~b.vv[0].isfinite()] = 0
+    for j in range(l):
+        b.k[b.table[0, j // 16], :, j % 16] = b.kk[0][j]
+        b.v[b.table[0, j // 16], :, j % 16] = b.vv[0][j]
+    sinks = None if sink is None else torch.full((heads,), sink)
+    want, bound = attention64(b.q.double(), b.kk[0].double(), clean.double(), l - n, window, sinks, 1.0, HALF[dt])
+    bound = bound + (2.0 ** -24 if dt == F16 else 1e-30)
+    odd = torch.where(b.vv[0].isfinite(), 0.0, b.vv[0].double())  # [l, kv, d]
+    rows = [odd[max(l - n + r + 1 - window, 0) if window else 0:l - n + r + 1].sum(0) for r in range(n)]
+    odd = torch.stack(rows).repeat_interleave(heads // kv, 1)
+    for hints in (dict(max_q_len=n, max_kv_len=l), {}, dict(max_q_len=1, max_kv_len=1), dict(max_q_len=10 ** 6)):
+        got = b.run(mer, gpu, hints=False, scale=1.0, window=window, sinks=sinks, **hints).double()
+        ok = torch.where(odd.isnan(), got.isnan(), torch.where(odd != 0, got == odd, (got - want).abs() <= bound))
+        assert ok.all(), (hints, (~ok).nonzero()[:4], got[~ok][:4], want[~ok][:4], odd[~ok][:4])
+
+
 @pytest.mark.parametrize("n,l,heads,kv,d", [(3, 75, 8, 2, 128), (6, 300, 8, 2, 64), (150, 400, 4, 2, 64), (40, 9000, 8, 1, 128)])
 @pytest.mark.parametrize("x", [math.nan, math.inf])
 def test_attention_key_that_is_not_finite(mer, gpu, n, l, heads, kv, d, x):
