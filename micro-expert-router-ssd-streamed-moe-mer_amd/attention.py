@@ -75,7 +75,9 @@ class PagedKvCache:
     """Keys and values of one layer in pages: k and v are
     [n_pages, n_kv_heads, page_size, head_dim] tensors, float16 or bfloat16.
     Slot s of the cache is place s % page_size of page s // page_size; which
-    pages belong to which sequence is the caller's business (block tables)."""
+    pages belong to which sequence is the caller's business (block tables).
+    k and v are written in place; a cache over other tensors is another cache
+    (wrap)."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.float16, device=None):
@@ -97,12 +99,16 @@ class PagedKvCache:
             raise ValueError("k and v must be contiguous")
         if k.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"a cache is float16 or bfloat16, got {k.dtype}")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self._desc = _lib.MerKvCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads,
                                      self.head_dim, self.n_pages)
         self._ref = ctypes.byref(self._desc)
         self.device = k.get_device()
+
+    # The calls go by the addresses taken above, so these cannot be replaced.
+    k = property(lambda self: self._k, doc="the keys")
+    v = property(lambda self: self._v, doc="the values")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None,

@@ -130,3 +130,14 @@ def test_python_refusals(mer):
         mer.PagedKvCache.wrap(torch.zeros(1, 1, 8, 64).half(), torch.zeros(2, 1, 8, 64).half())
     with pytest.raises(ValueError):
         mer.PagedKvCache.wrap(torch.zeros(1, 1, 8, 128).half()[..., ::2], torch.zeros(1, 1, 8, 64).half())
+
+
+def test_the_tensors_of_a_cache_cannot_be_replaced(mer):
+    """A call goes by the addresses of the cache's own tensors; one over other
+    tensors is another cache."""
+    k, v = torch.zeros(2, 1, 8, 64).half(), torch.ones(2, 1, 8, 64).half()
+    cache = mer.PagedKvCache.wrap(k, v)
+    for name in ("k", "v"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(2, 1, 8, 64).half())
+    assert cache.k is k and cache.v is v and (cache._desc.k, cache._desc.v) == (k.data_ptr(), v.data_ptr())
