@@ -1639,7 +1639,8 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
       (rc = check_words("kv_len", d_kv_len, 4)) || (rc = check_words("sinks", d_sinks, 4)))
     return rc;
   if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
-  if (!(fabsf(scale) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale is not finite");
+  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+  if (!(fabsf(scale_log2) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale %g is not finite in base 2", (double)scale);
   if ((rc = require_current_device())) return rc;
   AttnParams p{};
   p.k = cache->k;
@@ -1662,7 +1663,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   set_reciprocals(&p);
   p.window = window > (1u << 30) ? 0u : window;
   p.sinks = d_sinks;
-  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   const size_t cap = table_stride * cache->page_size;
   if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;

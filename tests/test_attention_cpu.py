@@ -141,3 +141,13 @@ def test_the_tensors_of_a_cache_cannot_be_replaced(mer):
         with pytest.raises(AttributeError):
             setattr(cache, name, torch.zeros(2, 1, 8, 64).half())
     assert cache.k is k and cache.v is v and (cache._desc.k, cache._desc.v) == (k.data_ptr(), v.data_ptr())
+
+
+def test_attention_refuses_a_scale_that_overflows_in_base_2(abi):
+    """scale * log2(e), which the kernels multiply with, has to be finite too."""
+    good, bad = 2.35e38, 2.36e38  # 3.4028e38 / log2(e) = 2.3587e38
+    expected = abi.Status.NOT_INITIALIZED
+    for sign in (1, -1):
+        assert attention(abi, scale=sign * bad) == abi.Status.INVALID_LAYOUT
+        if not torch.cuda.is_available():
+            assert attention(abi, scale=sign * good) == expected
