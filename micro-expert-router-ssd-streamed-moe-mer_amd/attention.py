@@ -217,8 +217,8 @@ def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Ten
         out_stride = _rows(out, n, h, d, q.dtype, dev, "out")
     if window < 0 or max_q_len < 0 or max_kv_len < 0:
         raise ValueError("window, max_q_len and max_kv_len must not be negative")
-    if scale == 0:
-        raise ValueError("the scale must not be zero")
+    if scale is not None and ctypes.c_float(scale).value == 0:  # which the entry point takes for the default
+        raise ValueError(f"the scale {scale} is zero in float32")
     rc = _lib.lib().mer_hip_paged_attention(
         cache._ref, seqs, n, h, q.data_ptr(), _rows(q, n, h, d, q.dtype, dev, "q"),
         _flat(block_table, torch.int32, seqs * width, dev, "block_table"), width,

@@ -377,3 +377,14 @@ def test_nothing_to_do(mer, gpu):
     q, k = mer.qk_norm_rope(z(0, 4, 64), z(0, 2, 64), i32(0), inv_freq(64).to(gpu))
     assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
     mer.take_device_status()
+
+
+def test_a_scale_that_float32_rounds_to_zero_is_refused(mer, gpu):
+    """Zero means the default scale at the entry point: a scale below float32's
+    least number must not turn into it."""
+    cache = mer.PagedKvCache(4, 16, 2, 64, F16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)
+    q = torch.ones(1, 4, 64, dtype=F16, device=gpu)
+    for scale in (0, 0.0, -0.0, 1e-50, -1e-300):
+        with pytest.raises(ValueError):
+            mer.paged_attention(cache, q, i32(0).view(1, 1), i32(0, 1), i32(1), scale=scale)
