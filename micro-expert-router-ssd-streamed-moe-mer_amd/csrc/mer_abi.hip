@@ -1560,7 +1560,8 @@ int mer_hip_qk_norm_rope(int in_type, int out_type, size_t n_tokens, size_t n_he
   int rc;
   if ((rc = check_float_type(in_type, true)) || (rc = check_float_type(out_type, true))) return rc;
   if ((rc = check_head_dim(head_dim)) || (rc = check_rope(d_inv_freq, rot_dim, head_dim))) return rc;
-  if ((rc = check_rows(n_tokens, n_heads + n_kv_heads))) return rc;
+  // (each by itself too: their sum may wrap)
+  if ((rc = check_rows(0, n_heads)) || (rc = check_rows(0, n_kv_heads)) || (rc = check_rows(n_tokens, n_heads + n_kv_heads))) return rc;
   if (n_heads == 0 && n_kv_heads == 0) return fail(MER_ERR_INVALID_LAYOUT, "neither queries nor keys to norm");
   if (n_tokens == 0) return MER_OK;
   if (n_heads && ((rc = check_tensor("q", d_q, in_type, q_stride, n_heads * head_dim, n_tokens)) ||

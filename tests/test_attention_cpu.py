@@ -151,3 +151,8 @@ def test_attention_refuses_a_scale_that_overflows_in_base_2(abi):
         assert attention(abi, scale=sign * bad) == abi.Status.INVALID_LAYOUT
         if not torch.cuda.is_available():
             assert attention(abi, scale=sign * good) == expected
+
+
+@pytest.mark.parametrize("h,kv", [((1 << 64) - 1, 2), (3, (1 << 64) - 1), (1 << 63, 1 << 63)])
+def test_norm_rope_refuses_heads_whose_sum_wraps(abi, h, kv):
+    assert norm_rope(abi, n=1, h=h, kv=kv) == abi.Status.SHAPE_EXCEEDS_WORKSPACE
