@@ -634,7 +634,7 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
 //
 // Bound by the memory: every wave has two tiles of K and V on the way, 128 KiB
 // a CU for heads of 128.  64 sequences of 200 - 8000 keys, 32 / 8 heads, bf16:
-// 203 us (5.1 TB/s); one of 131,000 keys, f16: 96 us (5.6 TB/s; plain reads
+// 203 us (5.1 TB/s); one of 131,000 keys, f16: 97 us (5.5 TB/s; plain reads
 // reach 5.9).  A single short one is bound by latency (700 keys: 11 us).
 template <int DP, int WAVES, int NR>
 struct Rows16 {
@@ -1022,7 +1022,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     // Many pieces are joined in two steps, sixteen at a time (a unit's counters
     // do not meet another one's: in each third of them a workgroup begins, or
     // goes on with, one unit that is cut).  128 pieces (a token over 131,000 keys
-    // of 2 heads of 256): 81 us in one step, 57 us in two; 32 pieces (8000 keys of
+    // of 2 heads of 256): 81 us in one step, 59 us in two; 32 pieces (8000 keys of
     // 8 heads of 128): 17 us in one, 21 us in two.
     if (n_pieces > 1) {
       uint32_t *flag = (uint32_t *)(jm + C::kWaves * C::kRows * 2);
@@ -1047,15 +1047,17 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 // tiles of 64 keys, two stages of K and V in LDS; each wave copies its share
 // of the next tile while the present one is used.
 //
-// Bound by the matrix units (47% of the cycles) and the vector units (49%),
-// which overlap but in part: a wave's last products run beside its weights, its
-// first ones only beside the other workgroup that a CU holds of 128-element
-// heads.  32 rows a wave read each operand from LDS half as often as 16 would;
+// Bound by the matrix and the vector units, which overlap but in part: a wave's
+// last products run beside its weights, its first ones only beside the other
+// workgroup that a CU holds of 128-element heads.  They are busy 47% and 50% of
+// the cycles over a prompt of 8192 tokens, 41% and 46% of 4096, heads of 64 42%
+// and 74%, of 256 17% and 24%.  32 rows a wave read each operand from LDS half as often as 16 would;
 // 64-key tiles leave 64 KiB for each of the two workgroups.  A 4096-token
-// prompt, 32 / 8 heads of 128, bf16: 152 us (902 TFLOP/s); 16384 tokens: 1.0
+// prompt, 32 / 8 heads of 128, bf16: 150 us (917 TFLOP/s); 16384 tokens: 1.0
 // PFLOP/s; 4096 tokens of 64 heads of 64, where softmax outweighs the
-// products: 182 us (755 TFLOP/s); 2048 of 16 heads of 256 (one workgroup a CU):
-// 88 us (390 TFLOP/s).
+// products: 175 us (784 TFLOP/s); 2048 of 16 heads of 256 (one workgroup a CU):
+// 84 us (408 TFLOP/s).  Padded heads do the products of the size above them:
+// 4096 tokens of 80 140 us, of 96 142, of 112 145.
 template <int DP, int WAVES>
 struct Rows32 {
   static constexpr int kRows = 32 * WAVES;
@@ -1357,7 +1359,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
 
 // Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
 // its accumulators spread over four waves.  Bound by the memory: four chunks
-// of 1040 tokens x 32 heads of 128 in 15 us, nine in 27 us.
+// of 1040 tokens x 32 heads of 128 in 16 us.
 template <class E, int DP, int WAVES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   typedef Rows32<DP, WAVES> C;

@@ -77,8 +77,8 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
   // Up to 16 rows a sequence: tiles of 16.  17 to 32 (a few tokens, or groups of
   // more than 16 heads): 128-row tiles where there are units enough to give the
   // CUs two workgroups (64 sequences of 8 x 4 rows, 500 - 2000 keys, 8 kv heads of
-  // 128: 67 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 61 us); two tiles of
-  // 16 where there is little to read (1 of 4000: 16 us, 32 23 us; 8 of 4000 - 8000:
+  // 128: 68 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 60 us); two tiles of
+  // 16 where there is little to read (1 of 4000: 17 us, 32 23 us; 8 of 4000 - 8000:
   // 66 and 52 us) and for heads of 256, whose 32 rows would not fit the registers
   // (8 of 4000 - 8000: 75 and 86 us).  Above, tiles of 128 (8 x 48 rows: 46 us, 32
   // 75 us).
@@ -94,7 +94,7 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
     // Long stretches of few units: the widest workgroups, as many as the CUs
     // hold at once.  Many short units: as many waves, each a workgroup of its
     // own, so that one's piece ends while the others' keys stream (512
-    // sequences of 60 - 300 keys: 135 us wide, 95 us narrow; 8 of 1000: 11 us
+    // sequences of 60 - 300 keys: 135 us wide, 98 us narrow; 8 of 1000: 11 us
     // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
     const bool narrow = head_dim <= 128 && pairs >= 4ull * cus;
     a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);

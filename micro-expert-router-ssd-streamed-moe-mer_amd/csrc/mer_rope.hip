@@ -14,12 +14,13 @@
 // its token and turns every head with them.
 //
 // Angles: position * inv_freq / 2 pi in 64 bits, less its nearest whole
-// number of turns, so far positions keep the same absolute error (2^-25 of a
-// turn) as near ones.
+// number of turns, so far positions keep nearly the error of near ones (2^-26 of
+// a turn from the last rounding; the product adds less up to positions of 10^8,
+// and up to 2^-23 at the ends of 32 bits).
 //
-// Bound by the memory: q and k of 4096 tokens, 32 + 4 heads of 128, bf16, 15.0
-// us for 75.5 MB (5.0 TB/s; a large copy reaches 5.5); 4096 tokens of 8 f32
-// heads to a bf16 cache with the key's norm 10.1 us for 50.4 MB.  One token
+// Bound by the memory: q and k of 4096 tokens, 32 + 4 heads of 128, bf16, 14.3
+// us for 75.5 MB (5.3 TB/s; a large copy reaches 5.5); 4096 tokens of 8 f32
+// heads to a bf16 cache with the key's norm 10.9 us for 50.4 MB.  One token
 // takes 2.6 us, which is the launch and two dependent loads.
 #include "../../include/mer_hip.h"
 #include "mer_attention.hpp"
