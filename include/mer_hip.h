@@ -483,8 +483,8 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * max_kv_len, unknown ones as n_tokens and the table): 17 MB for up to 16 rows
  * (max_q_len x query heads of a kv head), up to 256 MiB above.  A call that is
  * no larger than an earlier one in any of them leaves it where it is.  What
- * the device refuses is not asked for again: the keys are then cut into as
- * many chunks as the memory at hand allows, down to one. */
+ * the device refuses is not asked for again, nor is the buffer then moved for
+ * less: the keys are cut into as many chunks as it holds sums of, down to one. */
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
                             const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
                             const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,

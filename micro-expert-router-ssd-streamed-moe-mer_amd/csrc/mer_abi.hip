@@ -88,7 +88,7 @@ struct Workspace {
   size_t router_floats = 0;
   float *attn_buf = nullptr;     // attention: sums of a row's key chunks
   size_t attn_floats = 0;
-  size_t attn_refused = SIZE_MAX;  // smallest size that the device refused
+  size_t attn_refused = SIZE_MAX;  // the size that the device refused
   uint64_t *attn_counters = nullptr;  // attention: tickets and counters of pieces that are done
   size_t attn_counter_words = 0;
   uint32_t *counters = nullptr;  // decode counters (zero between launches) + control lines
@@ -276,10 +276,12 @@ int ensure_scratch(Workspace &w, size_t floats, float **out) {
 }
 
 // Grow a buffer to `want` floats where the device has them outside capture.
-// The one in use is given up only for a larger one at hand; a size once
-// refused is not asked for again.
+// The one in use is given up only for a larger one at hand, and no more once a
+// size was refused: the call that wanted it went on with this one, so a smaller
+// call must not move it (a captured graph holds its address), though the device
+// may have the memory for that by now.
 int grow_if_possible(Workspace &w, float **buf, size_t *cap, size_t *refused, size_t want) {
-  if (*cap >= want || want >= *refused || capturing(w.stream)) return MER_OK;
+  if (*cap >= want || want >= *refused || (*buf && *refused != SIZE_MAX) || capturing(w.stream)) return MER_OK;
   const size_t floats = want < (size_t(1) << 20) ? size_t(1) << 20 : want;
   float *grown = nullptr;
   if (hipMalloc(reinterpret_cast<void **>(&grown), floats * sizeof(float)) != hipSuccess) {
@@ -1680,7 +1682,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   // smaller one moves the buffer.  Where the device refuses that, the call is
   // planned within what there is, down to one chunk without partial sums.
   if ((rc = grow_if_possible(*w, &w->attn_buf, &w->attn_floats, &w->attn_refused, reserve))) return rc;
-  const size_t floats = reserve < w->attn_refused ? reserve : w->attn_floats;
+  const size_t floats = w->attn_refused == SIZE_MAX ? reserve : w->attn_floats;
   const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
                                   p.window, cus, floats);
   if (plan.n_wgs >= (1u << 24))

@@ -91,7 +91,7 @@ def test_a_full_device_runs_fewer_chunks(mer, gpu):
     buffer that a captured decode step points to stays where it is."""
     say("attention workspace refused")
     heads, kv, d, keys = 16, 4, 128, 8192
-    decode, chunk = (Call(mer, gpu, n, keys, heads, kv, d, 64, 70 + n) for n in (1, 1200))  # the chunk reserves 256 MiB
+    decode, chunk, less = (Call(mer, gpu, n, keys, heads, kv, d, 64, 70 + n) for n in (1, 1200, 300))  # the chunk reserves 256 MiB
     want, got = torch.zeros_like(chunk.out), torch.zeros_like(decode.out)
     s, other = torch.cuda.Stream(device=gpu), torch.cuda.Stream(device=gpu)
     torch.cuda.synchronize()
@@ -124,6 +124,17 @@ def test_a_full_device_runs_fewer_chunks(mer, gpu):
     finally:
         held.clear()
         torch.cuda.empty_cache()
+    assert torch.equal(decode.out, got)
+    # with the memory back, a smaller call that would have reserved more than there is leaves the buffer, too
+    free = torch.cuda.mem_get_info(gpu)[0]
+    with torch.cuda.stream(s):
+        less.run()
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info(gpu)[0] == free, "a smaller call moved the workspace"
+    decode.out.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
     assert torch.equal(decode.out, got)
     # both sides round the weights and the output once; 512 half steps of f32 cover the scores' sums
     h = HALF[BF16]
