@@ -491,6 +491,59 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
                             float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
                             void *stream);
 
+/* ---- a paged cache held in 4 bits ----
+ * The same cache at 4.5 bits an element instead of 16, for longer contexts and
+ * larger batches: blocks of 32 neighbouring elements of a head as GGUF's Q4_0
+ * has them, codes n from 0 to 15 and a scale d, value d (n - 8).
+ *   codes  [n_pages][n_kv_heads][page_size][head_dim / 2] bytes; a block's 16
+ *          bytes hold its elements 0 .. 15 in their low and 16 .. 31 in their
+ *          high halves
+ *   scales [n_pages][n_kv_heads][head_dim / 32][page_size] f16
+ * head_dim is a multiple of 32 up to MER_MAX_HEAD_DIM, page_size a power of
+ * two from 8 to 4096; the memory is the caller's and 16-byte aligned.
+ * Attention takes what is there: any codes, any finite scale (products of code
+ * and scale are rounded to f16 where a scale has more than eight bits). */
+typedef struct mer_kv_cache_q4 {
+  void *k_codes, *v_codes, *k_scales, *v_scales;
+  uint32_t page_size, n_kv_heads, head_dim;
+  uint64_t n_pages;      /* < 2^31 */
+} mer_kv_cache_q4;
+
+/* mer_hip_kv_append to such a cache; arguments, skipped rows and errors are
+ * the same.  A block's scale is |a| / 8 of its element a of largest magnitude
+ * (the positive one of two equal ones), rounded to five bits (half to even)
+ * and to f16, at most 7936, with the sign opposite to a's; its codes are
+ * round(x / d) + 8 (half to even) cut to 0 .. 15.  With five bits of scale all
+ * values are exact in f16 and bf16.  Keys are normed and rotated in f64 and
+ * rounded to f32 before.  Where a token's key or value of a head is not finite
+ * or exceeds 65504, all scales of both are NaN: it reads as NaN. */
+int mer_hip_kv_append_q4(const mer_kv_cache_q4 *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
+                         const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
+                         const float *d_inv_freq, size_t rot_dim, int interleaved, const float *d_k_norm, float eps,
+                         void *stream);
+
+/* Rows of such a cache back: keys and values of slot d_slots[r] to row r of
+ * d_k and d_v ([n_rows][n_kv_heads][head_dim] of out_type, rows a stride
+ * apart), exact for what kv_append_q4 wrote.  A slot may be named any number
+ * of times; a negative one gives a row of zeros, one past the cache too, and
+ * records MER_ERR_RESIDENCY_MISS in the device status word. */
+int mer_hip_kv_read_q4(const mer_kv_cache_q4 *cache, int out_type, size_t n_rows, const int64_t *d_slots, void *d_k,
+                       size_t k_stride, void *d_v, size_t v_stride, void *stream);
+
+/* mer_hip_paged_attention over such a cache, q and output of `type` (f16 or
+ * bf16); what is said there holds here, with these differences.  Keys and
+ * values take part as they are held and queries as they are (bf16 ones beside
+ * their row's largest down to 2^-39 of it); sums and softmax are f32, the
+ * weights are rounded to f16.  A key whose scales are not finite leaves the
+ * rows that see it no answer (NaN), and rows that do not see it untouched;
+ * scales of values that are not finite count as zero (kv_append_q4 makes the
+ * key's so too, and thereby the row's answer NaN). */
+int mer_hip_paged_attention_q4(const mer_kv_cache_q4 *cache, int type, size_t n_seqs, size_t n_tokens, size_t n_heads,
+                               const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
+                               const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
+                               float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
+                               void *stream);
+
 /* Synthetic bench / test data: fill n_blocks GGUF blocks of expert
  * `expert_index` starting at block `block_begin` with this library's
  * counter-based generator (nibbles / int8 uniform, d = f16(U(lo,hi))). */

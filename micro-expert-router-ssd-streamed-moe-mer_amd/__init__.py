@@ -6,7 +6,7 @@ gfx950 library libmer_hip.so; this package is its host-side mirror of the
 reference's expert-execution interface.
 """
 from . import _lib
-from .attention import PagedKvCache, kv_append, paged_attention, qk_norm_rope
+from .attention import PagedKvCache, PagedKvCacheQ4, kv_append, kv_read, paged_attention, qk_norm_rope
 from .errors import (
     BufferTooSmall,
     Candle,

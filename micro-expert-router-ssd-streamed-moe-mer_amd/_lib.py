@@ -47,6 +47,12 @@ class MerKvCache(ctypes.Structure):
                 ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("n_pages", c_u64)]
 
 
+class MerKvCacheQ4(ctypes.Structure):
+    _fields_ = [("k_codes", c_void), ("v_codes", c_void), ("k_scales", c_void), ("v_scales", c_void),
+                ("page_size", ctypes.c_uint32), ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("n_pages", c_u64)]
+
+
 class MerSlotStats(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in
                 ("hits", "misses", "prefetches", "evictions", "stale_retirements", "bytes_uploaded", "resident")]
@@ -154,6 +160,14 @@ SIGNATURES = {
     "mer_hip_paged_attention": (
         c_int, [ctypes.POINTER(MerKvCache), c_size, c_size, c_size, c_void, c_size, c_void, c_size, c_void, c_void,
                 c_size, c_size, c_float, ctypes.c_uint32, c_void, c_void, c_size, c_void]),
+    "mer_hip_kv_append_q4": (
+        c_int, [ctypes.POINTER(MerKvCacheQ4), c_int, c_size, c_void, c_size, c_void, c_size, c_void, c_void, c_void,
+                c_size, c_int, c_void, c_float, c_void]),
+    "mer_hip_kv_read_q4": (
+        c_int, [ctypes.POINTER(MerKvCacheQ4), c_int, c_size, c_void, c_void, c_size, c_void, c_size, c_void]),
+    "mer_hip_paged_attention_q4": (
+        c_int, [ctypes.POINTER(MerKvCacheQ4), c_int, c_size, c_size, c_size, c_void, c_size, c_void, c_size, c_void,
+                c_void, c_size, c_size, c_float, ctypes.c_uint32, c_void, c_void, c_size, c_void]),
     "mer_slot_cache_create": (c_int, [c_int, c_size, c_size, c_size, c_size, ctypes.POINTER(c_void)]),
     "mer_slot_cache_destroy": (c_int, [c_void]),
     "mer_slot_cache_table": (c_void, [c_void]),

@@ -1,7 +1,8 @@
 """The attention side of a layer, between its projections and its router:
 norms and rotation of queries and keys, the append to a paged key/value
 cache and attention over it, over mer_hip_qk_norm_rope / mer_hip_kv_append /
-mer_hip_paged_attention.
+mer_hip_paged_attention; the cache may be held in 4 bits (PagedKvCacheQ4,
+mer_hip_kv_append_q4 / mer_hip_kv_read_q4 / mer_hip_paged_attention_q4).
 
 They stand in for what the engine does on the host between a layer's dense
 projections and its routed experts (transformer.rs, the paged KV of
@@ -111,6 +112,60 @@ class PagedKvCache:
     v = property(lambda self: self._v, doc="the values")
 
 
+class PagedKvCacheQ4:
+    """Keys and values of one layer in pages, held in 4 bits: blocks of 32
+    elements of a head, as GGUF's Q4_0 has them, with a float16 scale d and
+    codes n that stand for d (n - 8); 4.5 bits an element.
+      k_codes, v_codes    uint8 [n_pages, n_kv_heads, page_size, head_dim // 2]: a
+                          block's 16 bytes hold elements 0 .. 15 in their low and
+                          16 .. 31 in their high halves
+      k_scales, v_scales  float16 [n_pages, n_kv_heads, head_dim // 32, page_size]
+    Slots, pages and block tables are as in PagedKvCache, and so are kv_append
+    and paged_attention; kv_read gives rows back.  The tensors are written in
+    place; a cache over other tensors is another cache (wrap)."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device=None):
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        codes = lambda: torch.empty((n_pages, n_kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=dev)
+        scales = lambda: torch.empty((n_pages, n_kv_heads, head_dim // 32, page_size), dtype=torch.float16, device=dev)
+        if head_dim % 32:
+            raise ValueError(f"head_dim {head_dim} is no multiple of a block's 32 elements")
+        self._set(codes(), scales(), codes(), scales())
+
+    @classmethod
+    def wrap(cls, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+             v_scales: torch.Tensor) -> "PagedKvCacheQ4":
+        """A cache over the caller's own tensors."""
+        self = cls.__new__(cls)
+        self._set(k_codes, k_scales, v_codes, v_scales)
+        return self
+
+    def _set(self, k_codes, k_scales, v_codes, v_scales) -> None:
+        tensors = (k_codes, k_scales, v_codes, v_scales)
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+            raise ValueError("codes must be alike: [n_pages, n_kv_heads, page_size, head_dim // 2]")
+        n, h, page, half = k_codes.shape
+        if half % 16 or k_scales.shape != (n, h, half // 16, page) or v_scales.shape != k_scales.shape:
+            raise ValueError(f"codes {tuple(k_codes.shape)} take scales [n_pages, n_kv_heads, head_dim // 32, page_size], "
+                             f"got {tuple(k_scales.shape)} and {tuple(v_scales.shape)}")
+        if len({t.device for t in tensors}) != 1 or not all(t.is_contiguous() for t in tensors):
+            raise ValueError("codes and scales must be contiguous, on one device")
+        if [t.dtype for t in tensors] != [torch.uint8, torch.float16] * 2:
+            raise TypeError("codes are uint8 and scales float16, got " + ", ".join(str(t.dtype) for t in tensors))
+        self._k_codes, self._k_scales, self._v_codes, self._v_scales = tensors
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, h, page, 2 * half
+        self._desc = _lib.MerKvCacheQ4(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                                       page, h, 2 * half, n)
+        self._ref = ctypes.byref(self._desc)
+        self.device = k_codes.get_device()
+
+    # The calls go by the addresses taken above, so these cannot be replaced.
+    k_codes = property(lambda self: self._k_codes, doc="the keys' codes")
+    k_scales = property(lambda self: self._k_scales, doc="the keys' scales")
+    v_codes = property(lambda self: self._v_codes, doc="the values' codes")
+    v_scales = property(lambda self: self._v_scales, doc="the values' scales")
+
+
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None,
                  inv_freq: torch.Tensor | None, *, q_norm: torch.Tensor | None = None,
                  k_norm: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
@@ -159,7 +214,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     return q_out, k_out
 
 
-def kv_append(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *,
+def kv_append(cache: PagedKvCache | PagedKvCacheQ4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *,
               positions: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
               k_norm: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False) -> None:
     """Rows of k and v to their slots of the cache, the keys normed and
@@ -168,6 +223,11 @@ def kv_append(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     k, v    [tokens, n_kv_heads, head_dim] float32 / float16 / bfloat16
     slots   int64 [tokens], distinct; negative = padding, the row is skipped; a
             slot past the cache is skipped and recorded (take_device_status)
+
+    A PagedKvCacheQ4 takes them in 4 bits, each block of 32 elements with the
+    scale of its largest one; the keys' norm and rotation are then done in 64
+    bits, and a token's head whose key or value is not finite or exceeds 65504
+    reads as NaN.
     """
     dev, stream = _enter(k)
     n, src = _shape(k, "k")[0], k.dtype
@@ -176,7 +236,9 @@ def kv_append(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     if cache.device != dev:
         raise ValueError(f"the cache is on cuda:{cache.device}, expected cuda:{dev}")
     rot = 0 if inv_freq is None else 2 * inv_freq.numel()
-    rc = _lib.lib().mer_hip_kv_append(
+    lib = _lib.lib()
+    append = lib.mer_hip_kv_append_q4 if isinstance(cache, PagedKvCacheQ4) else lib.mer_hip_kv_append
+    rc = append(
         cache._ref, _TYPES[src], n, k.data_ptr(), ks, v.data_ptr(), vs, _flat(slots, torch.int64, n, dev, "slots"),
         _flat(positions, torch.int32, n, dev, "positions"), _flat(inv_freq, torch.float32, rot // 2, dev, "inv_freq"),
         rot, interleaved, _flat(k_norm, torch.float32, d, dev, "k_norm"), eps, stream)
@@ -184,14 +246,50 @@ def kv_append(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
         raise_for_status(rc)
 
 
-def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
+def kv_read(cache: PagedKvCacheQ4, slots: torch.Tensor, *, out_dtype: torch.dtype | None = None,
+            k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
+    """Rows of a cache held in 4 bits, back as (k, v) [len(slots), n_kv_heads,
+    head_dim]; values that kv_append wrote are exact in every type.
+
+    slots         int64, any number of times the same; negative = a row of zeros; a
+                  slot past the cache too, and recorded (take_device_status)
+    k_out, v_out  rows any 16-byte stride apart, of one type; else made, of
+                  out_dtype (default float16)
+    """
+    if not isinstance(cache, PagedKvCacheQ4):
+        raise TypeError(f"kv_read reads a PagedKvCacheQ4, got {type(cache).__name__}")
+    dev, stream = _enter(slots)
+    if cache.device != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device}, expected cuda:{dev}")
+    n, h, d = slots.numel(), cache.n_kv_heads, cache.head_dim
+    given = k_out if k_out is not None else v_out
+    dt = out_dtype if out_dtype is not None else torch.float16 if given is None else given.dtype
+    if dt not in _TYPES:
+        raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {dt}")
+    if k_out is None:
+        k_out, ks = torch.empty((n, h, d), dtype=dt, device=slots.device), h * d
+    else:
+        ks = _rows(k_out, n, h, d, dt, dev, "k_out")
+    if v_out is None:
+        v_out, vs = torch.empty((n, h, d), dtype=dt, device=slots.device), h * d
+    else:
+        vs = _rows(v_out, n, h, d, dt, dev, "v_out")
+    rc = _lib.lib().mer_hip_kv_read_q4(cache._ref, _TYPES[dt], n, _flat(slots, torch.int64, n, dev, "slots"),
+                                       k_out.data_ptr(), ks, v_out.data_ptr(), vs, stream)
+    if rc:
+        raise_for_status(rc)
+    return k_out, v_out
+
+
+def paged_attention(cache: PagedKvCache | PagedKvCacheQ4, q: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
                     kv_len: torch.Tensor, *, max_q_len: int = 0, max_kv_len: int = 0, scale: float | None = None,
                     window: int = 0, sinks: torch.Tensor | None = None,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of each sequence's new tokens over its pages; decode steps,
     prompt chunks and mixes of both in one call.
 
-    q            [tokens, n_heads, head_dim] of the cache's type
+    q            [tokens, n_heads, head_dim] of the cache's type (float16 or
+                 bfloat16 for a PagedKvCacheQ4)
     block_table  int32 [n_seqs, pages]: page ids of each sequence, in order
     q_start      int32 [n_seqs + 1]: sequence s has rows q_start[s] .. q_start[s + 1]
     kv_len       int32 [n_seqs]: its keys in the cache, the new tokens' own among
@@ -205,9 +303,12 @@ def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Ten
     """
     dev, stream = _enter(q)
     n, h, d = _shape(q, "q")
-    if d != cache.head_dim or q.dtype != cache.k.dtype or cache.device != dev:
+    q4 = isinstance(cache, PagedKvCacheQ4)
+    fits = q.dtype != torch.float32 if q4 else q.dtype == cache.k.dtype
+    if d != cache.head_dim or not fits or cache.device != dev:
+        held = "held in 4 bits" if q4 else str(cache.k.dtype)
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} on cuda:{dev} does not go with a cache of head_dim "
-                         f"{cache.head_dim}, {cache.k.dtype} on cuda:{cache.device}")
+                         f"{cache.head_dim}, {held} on cuda:{cache.device}")
     if block_table.dim() != 2:
         raise ValueError("block_table must be [n_seqs, pages]")
     seqs, width = block_table.shape
@@ -219,8 +320,11 @@ def paged_attention(cache: PagedKvCache, q: torch.Tensor, block_table: torch.Ten
         raise ValueError("window, max_q_len and max_kv_len must not be negative")
     if scale is not None and ctypes.c_float(scale).value == 0:  # which the entry point takes for the default
         raise ValueError(f"the scale {scale} is zero in float32")
-    rc = _lib.lib().mer_hip_paged_attention(
-        cache._ref, seqs, n, h, q.data_ptr(), _rows(q, n, h, d, q.dtype, dev, "q"),
+    lib = _lib.lib()
+    attend, what = ((lib.mer_hip_paged_attention_q4, (cache._ref, _TYPES[q.dtype])) if q4 else
+                    (lib.mer_hip_paged_attention, (cache._ref,)))
+    rc = attend(
+        *what, seqs, n, h, q.data_ptr(), _rows(q, n, h, d, q.dtype, dev, "q"),
         _flat(block_table, torch.int32, seqs * width, dev, "block_table"), width,
         _flat(q_start, torch.int32, seqs + 1, dev, "q_start"), _flat(kv_len, torch.int32, seqs, dev, "kv_len"),
         max_q_len, max_kv_len, 0.0 if scale is None else scale, min(window, 0xffffffff),

@@ -13,8 +13,10 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libmer_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["mer_kernels.hip", "mer_decode.hip", "mer_router.hip", "mer_grouped.hip", "mer_rope.hip", "mer_attention.hip", "mer_slots.hip", "mer_format.cpp", "mer_abi.hip"]
-HEADERS = ["mer_device.hpp", "mer_internal.hpp", "mer_grouped_plan.hpp", "mer_attention.hpp", "mer_attention_plan.hpp"]
+SOURCES = ["mer_kernels.hip", "mer_decode.hip", "mer_router.hip", "mer_grouped.hip", "mer_rope.hip", "mer_attention.hip",
+           "mer_cache_q4.hip", "mer_attention_q4.hip", "mer_slots.hip", "mer_format.cpp", "mer_abi.hip"]
+HEADERS = ["mer_device.hpp", "mer_internal.hpp", "mer_grouped_plan.hpp", "mer_attention.hpp", "mer_attention_plan.hpp",
+           "mer_attention_device.hpp"]
 
 HIPCC_FLAGS = [
     "-std=c++17",

@@ -943,22 +943,45 @@ int check_rows(size_t n_tokens, size_t heads) {
   return MER_OK;
 }
 
-int check_cache(const mer_kv_cache *c) {
-  if (!c) return fail(MER_ERR_INVALID_LAYOUT, "null cache");
-  int rc = check_float_type(c->type, false);
+// What a cache of either form is made of.
+template <class Cache>
+int check_pages(const Cache *c) {
+  const int rc = check_head_dim(c->head_dim);
   if (rc) return rc;
-  if ((rc = check_head_dim(c->head_dim))) return rc;
   if (c->page_size < 8 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
     return fail(MER_ERR_INVALID_LAYOUT, "page_size %u must be a power of two from 8 to 4096", c->page_size);
   if (c->n_kv_heads == 0 || c->n_kv_heads > 2048)
     return fail(MER_ERR_INVALID_LAYOUT, "n_kv_heads %u must be in 1..=2048", c->n_kv_heads);
   if (c->n_pages == 0 || c->n_pages > 0x7fffffffull)
     return fail(MER_ERR_INVALID_LAYOUT, "n_pages must be in 1..2^31");
+  return MER_OK;
+}
+int check_cache(const mer_kv_cache *c) {
+  if (!c) return fail(MER_ERR_INVALID_LAYOUT, "null cache");
+  int rc = check_float_type(c->type, false);
+  if (rc || (rc = check_pages(c))) return rc;
   if ((uint64_t)c->n_kv_heads * c->page_size * c->head_dim * 2 >= (1ull << 32))
     return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a page of %u keys of %u heads reaches 4 GiB", c->page_size, c->n_kv_heads);
   if (!c->k || !c->v) return fail(MER_ERR_INVALID_LAYOUT, "null cache memory");
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return fail(MER_ERR_MISALIGNED, "cache memory must be 16-byte aligned");
   return MER_OK;
+}
+int check_cache(const mer_kv_cache_q4 *c) {
+  if (!c) return fail(MER_ERR_INVALID_LAYOUT, "null cache");
+  const int rc = check_pages(c);
+  if (rc) return rc;
+  if (c->head_dim % kQ4Block != 0)
+    return fail(MER_ERR_INVALID_LAYOUT, "head_dim %u is no multiple of the block's %u elements", c->head_dim, kQ4Block);
+  if ((uint64_t)c->n_kv_heads * c->page_size * c->head_dim / 2 >= (1ull << 32))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a page of %u keys of %u heads reaches 4 GiB", c->page_size, c->n_kv_heads);
+  if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return fail(MER_ERR_INVALID_LAYOUT, "null cache memory");
+  if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes | (uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 15u)
+    return fail(MER_ERR_MISALIGNED, "cache memory must be 16-byte aligned");
+  return MER_OK;
+}
+CacheQ4 planes(const mer_kv_cache_q4 &c) {
+  return CacheQ4{{(uint8_t *)c.k_codes, (uint8_t *)c.v_codes}, {(uint16_t *)c.k_scales, (uint16_t *)c.v_scales},
+                 c.n_pages * c.page_size, (uint32_t)__builtin_ctz(c.page_size), c.n_kv_heads, c.head_dim};
 }
 
 // Rows of `row` elements, `stride` apart.
@@ -981,6 +1004,127 @@ int check_eps(bool norm, float eps) {
 // Index arrays lie as their elements do.
 int check_words(const char *name, const void *p, size_t size) {
   if ((uintptr_t)p & (size - 1)) return fail(MER_ERR_MISALIGNED, "%s must be %zu-byte aligned", name, size);
+  return MER_OK;
+}
+
+// The arguments of an append to a cache of either form; then the device.
+template <class Cache>
+int check_append(const Cache *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride, const void *d_v,
+                 size_t v_stride, const int64_t *d_slots, const int32_t *d_positions, const float *d_inv_freq,
+                 size_t rot_dim, const float *d_k_norm, float eps) {
+  int rc;
+  if ((rc = check_cache(cache)) || (rc = check_float_type(in_type, true)) || (rc = check_rope(d_inv_freq, rot_dim, cache->head_dim)))
+    return rc;
+  if ((rc = check_rows(n_tokens, 2 * (size_t)cache->n_kv_heads))) return rc;
+  if (n_tokens == 0) return MER_OK;
+  const size_t row = (size_t)cache->n_kv_heads * cache->head_dim;
+  if ((rc = check_tensor("k", d_k, in_type, k_stride, row, n_tokens)) ||
+      (rc = check_tensor("v", d_v, in_type, v_stride, row, n_tokens)))
+    return rc;
+  if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
+  if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
+  if ((rc = check_eps(d_k_norm, eps)) || (rc = check_words("positions", d_positions, 4)) ||
+      (rc = check_words("slots", d_slots, 8)))
+    return rc;
+  if ((uintptr_t)d_k_norm & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
+  return require_current_device();
+}
+
+// The arguments of attention over a cache of either form, q and output of
+// `type`; then the device.  Leaves what they say in *p, but for the cache's
+// memory (nothing to do: MER_OK and no tokens in it).
+template <class Cache>
+int attention_params(const Cache *cache, int type, size_t n_seqs, size_t n_tokens, size_t n_heads, const void *d_q,
+                     size_t q_stride, const int32_t *d_block_table, size_t table_stride, const int32_t *d_q_start,
+                     const int32_t *d_kv_len, float scale, uint32_t window, const float *d_sinks, void *d_out,
+                     size_t out_stride, AttnParams *p) {
+  int rc;
+  if ((rc = check_cache(cache)) || (rc = check_rows(n_tokens, n_heads))) return rc;
+  if (n_heads == 0 || n_heads % cache->n_kv_heads != 0)
+    return fail(MER_ERR_INVALID_LAYOUT, "%zu heads are no multiple of %u kv heads", n_heads, cache->n_kv_heads);
+  if (n_seqs > (1u << 20)) return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "attention takes at most 1048576 sequences");
+  if (table_stride > (1u << 30) / cache->page_size)
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a block table row of %zu pages of %u keys exceeds 2^30 keys",
+                table_stride, cache->page_size);
+  if (n_seqs == 0 || n_tokens == 0) return MER_OK;
+  const size_t row = n_heads * cache->head_dim;
+  if ((rc = check_tensor("q", d_q, type, q_stride, row, n_tokens)) ||
+      (rc = check_tensor("output", d_out, type, out_stride, row, n_tokens)))
+    return rc;
+  if (!d_q_start || !d_kv_len || (!d_block_table && table_stride))
+    return fail(MER_ERR_INVALID_LAYOUT, "null sequence description");
+  if ((rc = check_words("the block table", d_block_table, 4)) || (rc = check_words("q_start", d_q_start, 4)) ||
+      (rc = check_words("kv_len", d_kv_len, 4)) || (rc = check_words("sinks", d_sinks, 4)))
+    return rc;
+  if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
+  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+  if (!(fabsf(scale_log2) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale %g is not finite in base 2", (double)scale);
+  if ((rc = require_current_device())) return rc;
+  p->q = d_q;
+  p->out = d_out;
+  p->table = d_block_table;
+  p->q_start = d_q_start;
+  p->kv_len = d_kv_len;
+  p->q_stride = q_stride;
+  p->out_stride = out_stride;
+  p->table_stride = (uint32_t)table_stride;
+  p->n_seqs = (uint32_t)n_seqs;
+  p->n_tokens = (uint32_t)n_tokens;
+  p->n_pages = (uint32_t)cache->n_pages;
+  p->page_shift = (uint32_t)__builtin_ctz(cache->page_size);
+  p->n_kv_heads = cache->n_kv_heads;
+  p->head_dim = cache->head_dim;
+  p->group = (uint32_t)(n_heads / cache->n_kv_heads);
+  set_reciprocals(p);
+  p->window = window > (1u << 30) ? 0u : window;
+  p->sinks = d_sinks;
+  p->scale_log2 = scale_log2;
+  return MER_OK;
+}
+
+// Plans a call whose arguments are in p, gets it its workspace and launches it.
+template <class Reserve, class Plan, class Launch>
+int run_attention(AttnParams &p, size_t cap, size_t max_q_len, size_t max_kv_len, void *stream, Reserve reserve_for,
+                  Plan plan_for, Launch launch) {
+  int rc;
+  const size_t n_seqs = p.n_seqs, n_tokens = p.n_tokens;
+  if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
+  if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
+  const int cus = g_dev[g_device].cus;
+  const size_t reserve = reserve_for(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
+  p.status = g_dev[g_device].status;
+  const hipStream_t st = (hipStream_t)stream;
+  std::shared_ptr<Workspace> w = workspace_for(st);
+  if (!w) return require_init();
+  std::lock_guard<std::mutex> wl(w->mu);
+  if (w->released) return released_error();
+  // Every call reserves what its sizes may need, one chunk or not, so that no
+  // smaller one moves the buffer.  Where the device refuses that, the call is
+  // planned within what there is, down to one chunk without partial sums.
+  if ((rc = grow_if_possible(*w, &w->attn_buf, &w->attn_floats, &w->attn_refused, reserve))) return rc;
+  const size_t floats = w->attn_refused == SIZE_MAX ? reserve : w->attn_floats;
+  const AttnPlan plan = plan_for(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
+                                 p.window, cus, floats);
+  if (plan.n_wgs >= (1u << 24))
+    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
+  p.min_granules = plan.min_granules;
+  p.n_units = plan.n_units;
+  p.chunk = plan.chunk;
+  p.n_chunks = plan.n_chunks;
+  const size_t need = plan.part_o_floats + plan.part_ml_floats;
+  // (there already, but for a captured call that no other went before)
+  if (need && (rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, need, 0, false, "attention workspace"))) return rc;
+  if (need || (!w->attn_counters && !capturing(st))) {
+    rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, attn_counters(cus), 0, true, "attention counters");
+    if (rc) return rc;
+  }
+  if (need) {
+    p.counters = w->attn_counters;
+    p.part_o = w->attn_buf;
+    p.part_ml = w->attn_buf + plan.part_o_floats;
+  }
+  const hipError_t e = launch(plan, st);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "attention launch");
   return MER_OK;
 }
 
@@ -1589,22 +1733,9 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
                       const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
                       const float *d_inv_freq, size_t rot_dim, int interleaved, const float *d_k_norm, float eps,
                       void *stream) {
-  int rc;
-  if ((rc = check_cache(cache)) || (rc = check_float_type(in_type, true)) || (rc = check_rope(d_inv_freq, rot_dim, cache->head_dim)))
-    return rc;
-  if ((rc = check_rows(n_tokens, 2 * (size_t)cache->n_kv_heads))) return rc;
-  if (n_tokens == 0) return MER_OK;
-  const size_t row = (size_t)cache->n_kv_heads * cache->head_dim;
-  if ((rc = check_tensor("k", d_k, in_type, k_stride, row, n_tokens)) ||
-      (rc = check_tensor("v", d_v, in_type, v_stride, row, n_tokens)))
-    return rc;
-  if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
-  if (rot_dim && !d_positions) return fail(MER_ERR_INVALID_LAYOUT, "a rotation needs positions");
-  if ((rc = check_eps(d_k_norm, eps)) || (rc = check_words("positions", d_positions, 4)) ||
-      (rc = check_words("slots", d_slots, 8)))
-    return rc;
-  if ((uintptr_t)d_k_norm & 15u) return fail(MER_ERR_MISALIGNED, "norm weights must be 16-byte aligned");
-  if ((rc = require_current_device())) return rc;
+  const int rc = check_append(cache, in_type, n_tokens, d_k, k_stride, d_v, v_stride, d_slots, d_positions, d_inv_freq,
+                              rot_dim, d_k_norm, eps);
+  if (rc || n_tokens == 0) return rc;
   NormRopeParams p{};
   p.t[0] = RopeTensor{d_k, cache->k, d_k_norm, k_stride, 0, cache->n_kv_heads};
   p.t[1] = RopeTensor{d_v, cache->v, nullptr, v_stride, 0, cache->n_kv_heads};
@@ -1618,94 +1749,91 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
   return MER_OK;
 }
 
+int mer_hip_kv_append_q4(const mer_kv_cache_q4 *cache, int in_type, size_t n_tokens, const void *d_k, size_t k_stride,
+                         const void *d_v, size_t v_stride, const int64_t *d_slots, const int32_t *d_positions,
+                         const float *d_inv_freq, size_t rot_dim, int interleaved, const float *d_k_norm, float eps,
+                         void *stream) {
+  const int rc = check_append(cache, in_type, n_tokens, d_k, k_stride, d_v, v_stride, d_slots, d_positions, d_inv_freq,
+                              rot_dim, d_k_norm, eps);
+  if (rc || n_tokens == 0) return rc;
+  AppendQ4Params p{};
+  p.cache = planes(*cache);
+  p.in[0] = d_k;
+  p.in[1] = d_v;
+  p.in_stride[0] = k_stride;
+  p.in_stride[1] = v_stride;
+  p.norm = d_k_norm;
+  p.positions = d_positions;
+  p.inv_freq = d_inv_freq;
+  p.slots = d_slots;
+  p.n_tokens = (uint32_t)n_tokens;
+  p.rot = (uint32_t)rot_dim;
+  p.interleaved = interleaved != 0;
+  p.eps = eps;
+  p.status = g_dev[g_device].status;
+  const hipError_t e = launch_append_q4(in_type, p, g_dev[g_device].cus, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "cache append launch");
+  return MER_OK;
+}
+
+int mer_hip_kv_read_q4(const mer_kv_cache_q4 *cache, int out_type, size_t n_rows, const int64_t *d_slots, void *d_k,
+                       size_t k_stride, void *d_v, size_t v_stride, void *stream) {
+  int rc;
+  if ((rc = check_cache(cache)) || (rc = check_float_type(out_type, true))) return rc;
+  if ((rc = check_rows(n_rows, 2 * (size_t)cache->n_kv_heads))) return rc;
+  if (n_rows == 0) return MER_OK;
+  const size_t row = (size_t)cache->n_kv_heads * cache->head_dim;
+  if ((rc = check_tensor("k", d_k, out_type, k_stride, row, n_rows)) ||
+      (rc = check_tensor("v", d_v, out_type, v_stride, row, n_rows)))
+    return rc;
+  if (!d_slots) return fail(MER_ERR_INVALID_LAYOUT, "null slot list");
+  if ((rc = check_words("slots", d_slots, 8)) || (rc = require_current_device())) return rc;
+  ReadQ4Params p{};
+  p.cache = planes(*cache);
+  p.slots = d_slots;
+  p.out[0] = d_k;
+  p.out[1] = d_v;
+  p.out_stride[0] = k_stride;
+  p.out_stride[1] = v_stride;
+  p.n_rows = (uint32_t)n_rows;
+  p.status = g_dev[g_device].status;
+  const hipError_t e = launch_read_q4(out_type, p, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "cache read launch");
+  return MER_OK;
+}
+
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
                             const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
                             const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
                             float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
                             void *stream) {
-  int rc;
-  if ((rc = check_cache(cache)) || (rc = check_rows(n_tokens, n_heads))) return rc;
-  if (n_heads == 0 || n_heads % cache->n_kv_heads != 0)
-    return fail(MER_ERR_INVALID_LAYOUT, "%zu heads are no multiple of %u kv heads", n_heads, cache->n_kv_heads);
-  if (n_seqs > (1u << 20)) return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "attention takes at most 1048576 sequences");
-  if (table_stride > (1u << 30) / cache->page_size)
-    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "a block table row of %zu pages of %u keys exceeds 2^30 keys",
-                table_stride, cache->page_size);
-  if (n_seqs == 0 || n_tokens == 0) return MER_OK;
-  const size_t row = n_heads * cache->head_dim;
-  if ((rc = check_tensor("q", d_q, cache->type, q_stride, row, n_tokens)) ||
-      (rc = check_tensor("output", d_out, cache->type, out_stride, row, n_tokens)))
-    return rc;
-  if (!d_q_start || !d_kv_len || (!d_block_table && table_stride))
-    return fail(MER_ERR_INVALID_LAYOUT, "null sequence description");
-  if ((rc = check_words("the block table", d_block_table, 4)) || (rc = check_words("q_start", d_q_start, 4)) ||
-      (rc = check_words("kv_len", d_kv_len, 4)) || (rc = check_words("sinks", d_sinks, 4)))
-    return rc;
-  if (scale == 0.0f) scale = (float)(1.0 / sqrt((double)cache->head_dim));
-  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
-  if (!(fabsf(scale_log2) < __builtin_inff())) return fail(MER_ERR_INVALID_LAYOUT, "the scale %g is not finite in base 2", (double)scale);
-  if ((rc = require_current_device())) return rc;
   AttnParams p{};
+  const int rc = attention_params(cache, cache ? cache->type : 0, n_seqs, n_tokens, n_heads, d_q, q_stride, d_block_table,
+                                  table_stride, d_q_start, d_kv_len, scale, window, d_sinks, d_out, out_stride, &p);
+  if (rc || p.n_tokens == 0) return rc;
   p.k = cache->k;
   p.v = cache->v;
-  p.q = d_q;
-  p.out = d_out;
-  p.table = d_block_table;
-  p.q_start = d_q_start;
-  p.kv_len = d_kv_len;
-  p.q_stride = q_stride;
-  p.out_stride = out_stride;
-  p.table_stride = (uint32_t)table_stride;
-  p.n_seqs = (uint32_t)n_seqs;
-  p.n_tokens = (uint32_t)n_tokens;
-  p.n_pages = (uint32_t)cache->n_pages;
-  p.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
-  p.n_kv_heads = cache->n_kv_heads;
-  p.head_dim = cache->head_dim;
-  p.group = (uint32_t)(n_heads / cache->n_kv_heads);
-  set_reciprocals(&p);
-  p.window = window > (1u << 30) ? 0u : window;
-  p.sinks = d_sinks;
-  p.scale_log2 = scale_log2;
-  const size_t cap = table_stride * cache->page_size;
-  if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
-  if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
-  const int cus = g_dev[g_device].cus;
-  const size_t reserve = attn_reserve(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
-  p.status = g_dev[g_device].status;
-  const hipStream_t st = (hipStream_t)stream;
-  std::shared_ptr<Workspace> w = workspace_for(st);
-  if (!w) return require_init();
-  std::lock_guard<std::mutex> wl(w->mu);
-  if (w->released) return released_error();
-  // Every call reserves what its sizes may need, one chunk or not, so that no
-  // smaller one moves the buffer.  Where the device refuses that, the call is
-  // planned within what there is, down to one chunk without partial sums.
-  if ((rc = grow_if_possible(*w, &w->attn_buf, &w->attn_floats, &w->attn_refused, reserve))) return rc;
-  const size_t floats = w->attn_refused == SIZE_MAX ? reserve : w->attn_floats;
-  const AttnPlan plan = attn_plan(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cap,
-                                  p.window, cus, floats);
-  if (plan.n_wgs >= (1u << 24))
-    return fail(MER_ERR_SHAPE_EXCEEDS_WORKSPACE, "too many rows in one attention call");
-  p.min_granules = plan.min_granules;
-  p.n_units = plan.n_units;
-  p.chunk = plan.chunk;
-  p.n_chunks = plan.n_chunks;
-  const size_t need = plan.part_o_floats + plan.part_ml_floats;
-  // (there already, but for a captured call that no other went before)
-  if (need && (rc = ensure_buf(*w, &w->attn_buf, &w->attn_floats, need, 0, false, "attention workspace"))) return rc;
-  if (need || (!w->attn_counters && !capturing(st))) {
-    rc = ensure_buf(*w, &w->attn_counters, &w->attn_counter_words, attn_counters(cus), 0, true, "attention counters");
-    if (rc) return rc;
-  }
-  if (need) {
-    p.counters = w->attn_counters;
-    p.part_o = w->attn_buf;
-    p.part_ml = w->attn_buf + plan.part_o_floats;
-  }
-  const hipError_t e = launch_attention(cache->type, plan, p, st);
-  if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "attention launch");
-  return MER_OK;
+  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_reserve, attn_plan,
+                       [&](const AttnPlan &plan, hipStream_t st) { return launch_attention(cache->type, plan, p, st); });
+}
+
+int mer_hip_paged_attention_q4(const mer_kv_cache_q4 *cache, int type, size_t n_seqs, size_t n_tokens, size_t n_heads,
+                               const void *d_q, size_t q_stride, const int32_t *d_block_table, size_t table_stride,
+                               const int32_t *d_q_start, const int32_t *d_kv_len, size_t max_q_len, size_t max_kv_len,
+                               float scale, uint32_t window, const float *d_sinks, void *d_out, size_t out_stride,
+                               void *stream) {
+  int rc = check_float_type(type, false);
+  if (rc) return rc;
+  AttnQ4Params p{};
+  rc = attention_params(cache, type, n_seqs, n_tokens, n_heads, d_q, q_stride, d_block_table, table_stride, d_q_start,
+                        d_kv_len, scale, window, d_sinks, d_out, out_stride, &p);
+  if (rc || p.n_tokens == 0) return rc;
+  p.k = cache->k_codes;
+  p.v = cache->v_codes;
+  p.k_scales = cache->k_scales;
+  p.v_scales = cache->v_scales;
+  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_q4_reserve, attn_q4_plan,
+                       [&](const AttnPlan &plan, hipStream_t st) { return launch_attention_q4(type, plan, p, st); });
 }
 
 int mer_hip_fill_synthetic(int dtype, uint64_t seed, uint64_t expert_index, uint64_t block_begin, uint64_t n_blocks,

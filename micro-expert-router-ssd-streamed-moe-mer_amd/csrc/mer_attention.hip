@@ -16,223 +16,15 @@
 // operand repeats, what O^T = V^T P^T reads as its second operand: P never
 // leaves the registers.  P is rounded to the cache's type for that product
 // (half a step of a weight <= 1; its sum is kept from the f32 values).
-#include "mer_attention.hpp"
+#include "mer_attention_device.hpp"
 
-#include <atomic>
 #include <math.h>
 
 namespace mer {
 namespace {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f8 __attribute__((ext_vector_type(8)));
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
-struct F16 {
-  typedef _Float16 T;
-  typedef h8 V8;
-  static constexpr uint32_t kExponent = 0x7c00u, kOne = 0x3c00u;
-  // Weights are taken 2^7 times larger, their sum and the sinks with them: up to
-  // 2^15 where the maximum lags by 8, and subnormal only below 2^-21 of the
-  // largest (2^-14 as they are, where a row's one large weight may meet a value
-  // smaller than what 32 others lose).
-  static constexpr float kUp = 7.0f;
-  static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-};
-struct BF16 {
-  typedef __bf16 T;
-  typedef b8 V8;
-  static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
-  static constexpr float kUp = 0.0f;
-  static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-};
-
-constexpr float kLog2E = 1.44269504088896341f;
-
 // What a lane reads for a key outside the tile's range: rows of zeros.
 __device__ u4 g_zero_row[kMaxHeadDim * 2 / 16];
-
-__device__ __forceinline__ uint32_t lane_id() { return __lane_id(); }
-__device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-
-// x / group and x / n_kv_heads for x below 2^26, by the reciprocals that the
-// host prepared: exact, since m = ceil(2^s / d) with s = 26 + ceil(log2 d)
-// makes x m / 2^s exceed x / d by less than 1 / d.
-__device__ __forceinline__ uint32_t by_group(const AttnParams &p, uint32_t x) {
-  return (uint32_t)(((uint64_t)x * p.group_mul) >> p.group_shift);
-}
-__device__ __forceinline__ uint32_t by_heads(const AttnParams &p, uint32_t x) {
-  return (uint32_t)(((uint64_t)x * p.heads_mul) >> p.heads_shift);
-}
-
-// A word of an argument array that the whole wave reads, by the scalar path.
-__device__ __forceinline__ int32_t sload(const int32_t *p, uint64_t i) {
-  return ((const __attribute__((address_space(4))) int32_t *)p)[i];
-}
-
-// Asynchronous copy of 16 bytes per lane to LDS at `lds` + 16 * lane.  The
-// compiler does not see it: wait_vm before the data is read.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void async_row16(const uint8_t *src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-}
-// The same from a base that the whole wave shares, with a byte offset per lane.
-__device__ __forceinline__ void async_row16(const uint8_t *base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
-}
-// The same by the lanes whose offset is not kNone; the others' places stay as
-// they are.  All lanes are on before and after (waves are full and branch as
-// one here).
-constexpr uint32_t kNone = 0xffffffffu;
-__device__ __forceinline__ void async_row16_some(const uint8_t *base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tv_cmpx_ne_u32_e32 vcc, -1, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" ::"v"(off),
-               "s"(base), "s"(lds)
-               : "memory", "m0", "vcc", "exec");
-}
-#pragma clang diagnostic pop
-// vmcnt(0) alone, in the form that the compiler's own wait counting sees.
-constexpr int kWaitVm0 = 0x0F70;
-
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// The same and this wave's LDS reads, then the workgroup's barrier.
-template <int N>
-__device__ __forceinline__ void wait_vm_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-// This wave's LDS reads are done: what they read may be overwritten.
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-// The value of lane ^ 32 (^ 16).
-__device__ __forceinline__ float other_half(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(lane_id() < 32 ? r[1] : r[0]);
-}
-__device__ __forceinline__ float other_row(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(lane_id() & 16 ? r[0] : r[1]);
-}
-// Maximum / sum over the four lanes that hold a 16-row tile's row.
-__device__ __forceinline__ float max_quad(float x) {
-  x = fmaxf(x, other_row(x));
-  return fmaxf(x, other_half(x));
-}
-__device__ __forceinline__ float sum_quad(float x) {
-  x += other_row(x);
-  return x + other_half(x);
-}
-// The same over 32 lanes.
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-__device__ __forceinline__ float max_32(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));   // lane ^ 1
-  x = fmaxf(x, dpp<0x4E>(x));   // lane ^ 2
-  x = fmaxf(x, dpp<0x141>(x));  // the other four of eight
-  x = fmaxf(x, dpp<0x140>(x));  // the other eight of sixteen
-  return fmaxf(x, other_row(x));
-}
-__device__ __forceinline__ float sum_32(float x) {
-  x += dpp<0xB1>(x);
-  x += dpp<0x4E>(x);
-  x += dpp<0x141>(x);
-  x += dpp<0x140>(x);
-  return x + other_row(x);
-}
-
-// Sequence and row tile of unit u.  Sequence s owns the units from
-// q_start[s] * group / rows + s on: at least as many as it has row tiles,
-// whatever the lengths, so no prefix sum over the sequences is needed.
-// 64 candidates a step.
-template <int ROWS>
-__device__ __forceinline__ void find_unit(const AttnParams &p, uint32_t u, uint32_t *seq, uint32_t *tile) {
-  uint32_t lo = 0, hi = p.n_seqs;
-  auto base = [&](uint32_t s) {
-    const int32_t q = p.q_start[s];
-    return (uint64_t)(q < 0 ? 0 : q) * p.group / ROWS + s;
-  };
-  while (hi - lo > 1) {
-    const uint32_t step = (hi - lo + 63) / 64, s = lo + lane_id() * step;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(s < hi && base(s) <= u);
-    const uint32_t n = m ? (uint32_t)__popcll(m) : 1u;
-    lo += (n - 1) * step;
-    if (lo >= hi) lo = hi - 1;
-    hi = hi < lo + step ? hi : lo + step;
-  }
-  *seq = uni(lo);
-  const uint64_t b = base(lo);
-  *tile = uni(u >= b ? (uint32_t)(u - b) : 0xffffffffu);
-}
-
-// A sequence's rows and keys, clear of what q and the table cannot hold.
-// (Rows are below 2^26 and keys up to 2^30.)
-struct Span {
-  int32_t tok0, n;   // first token in q / out, new tokens
-  int32_t len;       // keys
-};
-__device__ __forceinline__ Span make_span(const AttnParams &p, int32_t b, int32_t e, int32_t len) {
-  const int32_t n_tokens = (int32_t)p.n_tokens, cap = (int32_t)(p.table_stride << p.page_shift);
-  Span s;
-  s.tok0 = b < 0 ? 0 : (b > n_tokens ? n_tokens : b);
-  const int32_t tok1 = e < s.tok0 ? s.tok0 : (e > n_tokens ? n_tokens : e);
-  s.n = tok1 - s.tok0;
-  s.len = len < 0 ? 0 : (len > cap ? cap : len);
-  return s;
-}
-// Keys [lo, hi) that some of the rows [row0, row1) of a span see.
-__device__ __forceinline__ void see(const AttnParams &p, const Span &s, int32_t row0, int32_t row1, int32_t *lo, int32_t *hi) {
-  const int32_t pos0 = s.len - s.n;
-  const int32_t h = pos0 + (int32_t)by_group(p, (uint32_t)(row1 - 1)) + 1;
-  const int32_t l = p.window ? pos0 + (int32_t)by_group(p, (uint32_t)row0) - (int32_t)p.window + 1 : 0;
-  *hi = h < 0 ? 0 : h;
-  *lo = l < 0 ? 0 : (l > *hi ? *hi : l);
-}
-
-// What one row tile of one sequence covers; every field is the same in the
-// whole wave.
-struct Tile {
-  uint32_t row0;     // first (token, head) row of the tile in its sequence
-  uint32_t n_rows;   // rows of the sequence
-  uint32_t tok0;     // first token of the sequence in q / out
-  int32_t pos0;      // position of the sequence's first new token
-  int32_t lo, hi;    // keys that some row of the tile sees
-};
-template <int ROWS>
-__device__ __forceinline__ bool make_tile(const AttnParams &p, const Span &s, uint32_t tile, Tile *t) {
-  const int32_t rows = s.n * (int32_t)p.group;
-  if (tile >= (uint32_t)(rows + ROWS - 1) / ROWS) return false;
-  const int32_t row0 = (int32_t)tile * ROWS;
-  int32_t lo, hi;
-  see(p, s, row0, row0 + ROWS < rows ? row0 + ROWS : rows, &lo, &hi);
-  t->row0 = uni((uint32_t)row0);
-  t->n_rows = uni((uint32_t)rows);
-  t->tok0 = uni((uint32_t)s.tok0);
-  t->pos0 = (int32_t)uni((uint32_t)(s.len - s.n));
-  t->lo = (int32_t)uni((uint32_t)lo);
-  t->hi = (int32_t)uni((uint32_t)hi);
-  return true;
-}
 
 // Geometry of a head row in LDS: DP elements (head_dim rounded up), in 16-byte
 // pieces whose places are permuted by the row so that neither the row-wise
@@ -388,8 +180,6 @@ struct Share {
 // tiles that rows see in part, every time, cost prompts 1 - 2% and a window of
 // 1024 with heads of 64 5%.)
 // Marks are two bits an element: +inf, -inf, both for a NaN.
-template <bool CAREFUL> struct Pass { static constexpr bool careful = CAREFUL; };
-
 // Whether one of the values of [at, at + 64 * BYTES) of LDS is not finite.
 template <class E, int BYTES>
 __device__ __forceinline__ bool not_finite(uint32_t at) {
@@ -454,171 +244,6 @@ __device__ __forceinline__ float add_mark(float o, uint32_t bits) {
   return o + (bits & 2 ? -__builtin_inff() : 0.0f);
 }
 
-// x * w; with care an infinity (a mark's) stays one where the weight is zero.
-template <class V, class P>
-__device__ __forceinline__ V weigh(V x, float w, P) {
-  V y = x * w;
-  if constexpr (P::careful) {
-#pragma unroll
-    for (uint32_t i = 0; i < sizeof(V) / sizeof(float); ++i) y[i] = w == 0.0f && fabsf(x[i]) == __builtin_inff() ? x[i] : y[i];
-  }
-  return y;
-}
-// Zero, or a NaN if one of x's elements is not finite.
-template <class V>
-__device__ __forceinline__ float probe(V x) {
-  float z = 0.0f;
-#pragma unroll
-  for (uint32_t i = 0; i < sizeof(V) / sizeof(float); ++i) z = __builtin_fmaf(x[i], 0.0f, z);
-  return z;
-}
-// Whether some lane has a NaN.
-__device__ __forceinline__ bool not_a_number(float x) { return __builtin_amdgcn_ballot_w64(x != x) != 0; }
-
-// ---- joining the pieces of a unit ----
-// A workgroup that has done one of several pieces leaves its sums in memory
-// (device-scope stores) and counts itself in; the one that comes last adds
-// the pieces up, in their order.
-constexpr int kDeviceScope = 16;  // sc1: past the caches that other XCDs do not see
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float *p) {
-  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00020000);
-}
-__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t r, uint32_t index, f4 x) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), r, index * 4, 0, kDeviceScope);
-}
-__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, uint32_t index, f2 x) {
-  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, x), r, index * 4, 0, kDeviceScope);
-}
-
-// True in every thread of the workgroup that comes last.  `epoch`: the launch's,
-// in thread 0; `flag`: a word of LDS.
-__device__ __forceinline__ bool last_piece(uint64_t *counter, uint64_t epoch, uint32_t n_pieces, uint32_t *flag) {
-  wait_vm<0>();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    (void)__hip_atomic_fetch_max(counter, epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const uint64_t n = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = attn_is_last(n, n_pieces);
-  }
-  __syncthreads();
-  return *flag != 0;
-}
-
-// Adds up pieces c0, c0 + every, .. (n of them) of a unit: piece 0 is at
-// first_slot of the partial sums, piece c at 2 * (first_wg + c).  The result is
-// the unit's (`done`), or takes piece c0's place.  32 lanes hold a row's dims; the groups of 32 take
-// a row each, or share a row's pieces where there are fewer rows than groups.
-// A batch of pieces is in flight at once; what a lane reads beyond the pieces,
-// rows or dims that there are is left out.
-// `lds`: [THREADS / 32][DP] floats.
-template <class E, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, uint32_t head, uint32_t first_wg,
-                                            uint32_t first_slot, uint32_t c0, uint32_t every, uint32_t n, bool done,
-                                            float *lds) {
-  typedef typename E::T T;
-  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = DP == 256 ? 8 : 16;
-  typedef float fd __attribute__((ext_vector_type(kDims)));
-  typedef T td __attribute__((ext_vector_type(kDims)));
-  const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);
-  const uint32_t g = threadIdx.x / 32, ln = threadIdx.x % 32, dim = ln * kDims;
-  const uint32_t rows = t.n_rows - t.row0 < ROWS ? t.n_rows - t.row0 : ROWS;
-  const uint32_t share = rows < kGroups ? kGroups / rows : 1;  // groups of a row
-  const uint32_t step = kGroups / share, part = g % share;     // rows at a time
-  auto row_of = [&](uint32_t i, uint32_t r) {
-    const uint32_t c = c0 + i * every;
-    return (c ? 2 * (first_wg + c) : first_slot) * ROWS + r;
-  };
-  auto ml_of = [&](uint32_t i, uint32_t r) {  // nothing beyond the pieces
-    const f2 none = {-__builtin_inff(), 0.0f};
-    const f2 ml = __builtin_bit_cast(
-        f2, __builtin_amdgcn_raw_buffer_load_b64(rm, row_of(i < n ? i : 0, r) * 8, 0, kDeviceScope));
-    return i < n ? ml : none;
-  };
-  const uint32_t my_dim = dim < p.head_dim ? dim : 0;
-  auto o_of = [&](uint32_t i, uint32_t r) {
-    const uint32_t at = (row_of(i, r) * p.head_dim + my_dim) * 4;
-    if constexpr (kDims == 2) {
-      return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b64(ro, at, 0, kDeviceScope));
-    } else if constexpr (kDims == 4) {
-      return __builtin_bit_cast(fd, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
-    } else {
-      const f4 lo = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 0, kDeviceScope));
-      const f4 hi = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, at, 16, kDeviceScope));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  };
-  for (uint32_t r0 = 0; r0 < rows; r0 += step) {
-    const uint32_t mine = r0 + g / share, r = mine < rows ? mine : rows - 1;
-    // The first batch of sums is under way with the weights; `first`: of the
-    // pieces 0 .. 31, a lane each.
-    const f2 first = ml_of(ln, r);
-    fd acc, x[kBatch];
-    auto load = [&](uint32_t i0) {
-#pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint32_t i = i0 + b * share + part;
-        x[b] = o_of(i < n ? i : n - 1, r);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    load(0);
-    float m = first[0], l = first[1];
-    for (uint32_t i0 = 32; i0 < n; i0 += 32) {
-      const f2 ml = ml_of(i0 + ln, r);
-      const float mn = fmaxf(m, ml[0]), mu = mn == -__builtin_inff() ? 0.0f : mn;
-      l = l * __builtin_amdgcn_exp2f(m - mu) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
-      m = mn;
-    }
-    const float mm = max_32(m), mu = mm == -__builtin_inff() ? 0.0f : mm;
-    l = sum_32(l * __builtin_amdgcn_exp2f(m - mu));
-    auto add_up = [&](auto pass) {
-      acc = fd{};
-      for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-        const f2 ml = i0 ? ml_of(i0 + ln, r) : first;
-        const float w = __builtin_amdgcn_exp2f(ml[0] - mu);  // of piece i0 + lane
-        for (uint32_t k0 = 0; k0 < 32 && i0 + k0 < n; k0 += share * kBatch) {
-          if (i0 + k0 || decltype(pass)::careful) load(i0 + k0);
-#pragma unroll
-          for (uint32_t b = 0; b < kBatch; ++b) {
-            const uint32_t k = k0 + b * share + part;
-            const float wk = __shfl(w, (int)((threadIdx.x & 32) + (k & 31)));
-            if (k < 32 && i0 + k < n) acc += weigh(x[b], wk, pass);
-          }
-        }
-      }
-    };
-    add_up(Pass<false>());
-    if (not_a_number(probe(acc))) add_up(Pass<true>());
-    if (share > 1) {  // in the one pass that there is then
-      if (part) *(fd *)&lds[g * DP + dim] = acc;
-      __syncthreads();
-      if (part == 0)
-        for (uint32_t k = 1; k < share; ++k) acc += *(fd *)&lds[(g + k) * DP + dim];
-    }
-    if (mine < rows && part == 0 && dim < p.head_dim && !done) {
-      const uint32_t to = row_of(0, r);
-      typedef uint32_t ud __attribute__((ext_vector_type(kDims < 4 ? kDims : 4)));
-#pragma unroll
-      for (uint32_t k = 0; k < kDims; k += 4) {
-        ud u;
-#pragma unroll
-        for (uint32_t e = 0; e < (kDims < 4 ? kDims : 4); ++e) u[e] = __float_as_uint(acc[k + e]);
-        if constexpr (kDims == 2) __builtin_amdgcn_raw_buffer_store_b64(u, ro, (to * p.head_dim + dim) * 4, 0, kDeviceScope);
-        else __builtin_amdgcn_raw_buffer_store_b128(u, ro, (to * p.head_dim + dim + k) * 4, 0, kDeviceScope);
-      }
-      if (ln == 0) put2(rm, to * 2, f2{mm, l});
-    }
-    if (mine < rows && part == 0 && dim < p.head_dim && done) {
-      const uint32_t gr = t.row0 + r, tk = by_group(p, gr), hq = head * p.group + gr - tk * p.group;
-      if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - mu + E::kUp);
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      T *op = (T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + dim;
-      *(td *)op = __builtin_convertvector(weigh(acc, inv, Pass<true>()), td);
-    }
-  }
-}
-
 // Sixteen rows: decode and short chunks.
 //
 // The work is cut into pieces of equal length whatever the sequences are: a
@@ -648,89 +273,6 @@ struct Rows16 {
   static constexpr int kLds = kWaves * kStages * 2 * kTileBytes;
 };
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t scan_step(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-
-// Walks the sequences' granules; a wave looks at 256 sequences at a time, four
-// to a lane.  (attn_plan keeps the total below 2^31.)
-struct Granules {
-  uint32_t base, total;  // granules before the sequences in view, of those in view
-  uint32_t upto;         // of the lanes up to this one, within the view
-  uint32_t w[4];
-  int32_t q[5], len[4];  // their q_start and kv_len
-  uint32_t seq0;
-
-  template <int GRANULE, int ROWS>
-  __device__ __forceinline__ void view(const AttnParams &p, uint32_t first) {
-    seq0 = first;
-    const uint32_t s0 = first + lane_id() * 4;
-#pragma unroll
-    for (uint32_t i = 0; i < 5; ++i) {
-      q[i] = p.q_start[s0 + i < p.n_seqs ? s0 + i : p.n_seqs];
-      if (i < 4) len[i] = p.kv_len[s0 + i < p.n_seqs ? s0 + i : 0];
-    }
-    upto = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      const Span s = make_span(p, q[i], q[i + 1], len[i]);  // past the last sequence: no rows
-      const uint32_t rows = (uint32_t)s.n * p.group;
-      w[i] = (rows + ROWS - 1) / ROWS * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
-      upto += w[i];
-    }
-    upto += scan_step<0x111, 0xf>(upto);  // from 1, 2, 4 and 8 lanes before, in rows of 16
-    upto += scan_step<0x112, 0xf>(upto);
-    upto += scan_step<0x114, 0xf>(upto);
-    upto += scan_step<0x118, 0xf>(upto);
-    upto += scan_step<0x142, 0xa>(upto);  // the row before's last to rows 1 and 3
-    upto += scan_step<0x143, 0xc>(upto);  // lane 31's to rows 2 and 3
-    total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-  }
-
-  // The sequence at granule x of the view or a later one: its number, the
-  // granules before it and its span.  False if there is none (lengths that
-  // change under the kernel).
-  template <int GRANULE, int ROWS>
-  __device__ __forceinline__ bool find(const AttnParams &p, uint32_t x, uint32_t *seq, uint32_t *before, Span *span) {
-    while (x >= base + total && seq0 + 256 < p.n_seqs) {
-      base += total;
-      view<GRANULE, ROWS>(p, seq0 + 256);
-    }
-    const uint64_t beyond = __builtin_amdgcn_ballot_w64(base + upto > x);
-    if (!beyond) return false;
-    const int at = __builtin_ctzll(beyond);
-    auto get = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-    const uint32_t w0 = get(w[0]), w1 = get(w[1]), w2 = get(w[2]), w3 = get(w[3]);
-    const uint32_t b0 = base + get(upto) - w0 - w1 - w2 - w3, b1 = b0 + w0, b2 = b1 + w1, b3 = b2 + w2;
-    const int i = (x >= b1) + (x >= b2) + (x >= b3);
-    *seq = seq0 + (uint32_t)(at * 4 + i);
-    *before = i == 0 ? b0 : (i == 1 ? b1 : (i == 2 ? b2 : b3));
-    int32_t v[5], n[4];
-#pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      v[k] = (int32_t)get((uint32_t)q[k]);
-      if (k < 4) n[k] = (int32_t)get((uint32_t)len[k]);
-    }
-    const int32_t vb = i == 0 ? v[0] : (i == 1 ? v[1] : (i == 2 ? v[2] : v[3]));
-    const int32_t ve = i == 0 ? v[1] : (i == 1 ? v[2] : (i == 2 ? v[3] : v[4]));
-    *span = make_span(p, vb, ve, i == 0 ? n[0] : (i == 1 ? n[1] : (i == 2 ? n[2] : n[3])));
-    return true;
-  }
-
-  // Granules of each of a sequence's units, over the keys that its rows see.
-  template <int GRANULE>
-  static __device__ __forceinline__ uint32_t granules(const AttnParams &p, const Span &s, int32_t *start) {
-    if (s.n == 0) return 0;
-    int32_t lo, hi;
-    see(p, s, 0, s.n * (int32_t)p.group, &lo, &hi);
-    lo &= ~31;
-    if (start) *start = lo;
-    const uint32_t g = (uint32_t)(hi - lo + GRANULE - 1) / GRANULE;
-    return g ? g : 1;  // rows without keys are done, too
-  }
-};
-
 template <class E, int DP, int WAVES, int NR, bool PAD>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, DP == 64 ? 2 : 1))) void attn_rows16_kernel(AttnParams p) {
   typedef Rows16<DP, WAVES, NR> C;
@@ -757,7 +299,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     epoch = attn_epoch(__hip_atomic_fetch_add(p.counters + blockIdx.x % kAttnTickets * kAttnTicketWords,
                                               attn_ticket(blockIdx.x, gridDim.x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 
-  Granules gr;
+  typedef Granules<32> G;
+  G gr;
   gr.base = 0;
   gr.view<C::kGranule, C::kRows>(p, 0);
   uint32_t all = gr.total;
@@ -778,7 +321,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
     Span span;
     if (!gr.find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
     int32_t start = 0;
-    const uint32_t n_gran = uni(Granules::granules<C::kGranule>(p, span, &start));
+    const uint32_t n_gran = uni(G::granules<C::kGranule>(p, span, &start));
     const uint32_t unit = uni((x - before) / n_gran), tile = uni(by_heads(p, unit)), head = unit - tile * p.n_kv_heads;
     const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
     const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
@@ -984,62 +527,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[at * DP + d * 16 + quad * 4] = o[n][d];
     }
     __syncthreads();
-    const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);
-    for (uint32_t w = tid; w < C::kRows * (DP / 8); w += 64 * C::kWaves) {
-      const uint32_t r = w / (DP / 8), d = w % (DP / 8) * 8, rr = t.row0 + r;
-      if (rr >= t.n_rows || d >= p.head_dim) continue;
-      float mm = -__builtin_inff();
-#pragma unroll
-      for (int v = 0; v < C::kWaves; ++v) mm = fmaxf(mm, jm[(v * C::kRows + r) * 2]);
-      float ls;
-      f8 acc;
-      auto add_up = [&](auto pass) {
-        ls = 0.0f;
-        acc = f8{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int v = 0; v < C::kWaves; ++v) {
-          const float mv = jm[(v * C::kRows + r) * 2];
-          const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
-          ls += a * jm[(v * C::kRows + r) * 2 + 1];
-          acc += weigh(*(const f8 *)&jo[(v * C::kRows + r) * DP + d], a, pass);
-        }
-      };
-      add_up(Pass<false>());
-      if (not_a_number(probe(acc))) add_up(Pass<true>());
-      const uint32_t tk = by_group(p, rr), hq = head * p.group + rr - tk * p.group;
-      if (n_pieces == 1) {
-        if (p.sinks) ls += __builtin_amdgcn_exp2f(p.sinks[hq] * kLog2E - (mm == -__builtin_inff() ? 0.0f : mm) + E::kUp);
-        const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;
-        const V8 r8 = __builtin_convertvector(weigh(acc, inv, Pass<true>()), V8);
-        *(V8 *)((T *)p.out + (uint64_t)(t.tok0 + tk) * p.out_stride + (uint64_t)hq * p.head_dim + d) = r8;
-      } else {
-        const uint32_t to = my_slot * C::kRows + r;
-        put4(ro, to * p.head_dim + d, f4{acc[0], acc[1], acc[2], acc[3]});
-        put4(ro, to * p.head_dim + d + 4, f4{acc[4], acc[5], acc[6], acc[7]});
-        if (d == 0) put2(rm, to * 2, f2{mm, ls});
-      }
-    }
-    // Many pieces are joined in two steps, sixteen at a time (a unit's counters
-    // do not meet another one's: in each third of them a workgroup begins, or
-    // goes on with, one unit that is cut).  128 pieces (a token over 131,000 keys
-    // of 2 heads of 256): 81 us in one step, 59 us in two; 32 pieces (8000 keys of
-    // 8 heads of 128): 17 us in one, 21 us in two.
-    if (n_pieces > 1) {
-      uint32_t *flag = (uint32_t *)(jm + C::kWaves * C::kRows * 2);
-      auto join = [&](uint32_t c0, uint32_t every, uint32_t n, bool done) {
-        join_pieces<E, DP, C::kRows, 64 * C::kWaves>(p, t, head, first_wg, first_slot, c0, every, n, done, jo);
-      };
-      constexpr uint32_t kJoin = 16;
-      const uint32_t c0 = (blockIdx.x - first_wg) / kJoin * kJoin, n = n_pieces - c0 < kJoin ? n_pieces - c0 : kJoin;
-      uint64_t *const counters = p.counters + kAttnTickets * kAttnTicketWords + first_wg;
-      if (n_pieces <= 2 * kJoin) {
-        if (last_piece(counters, epoch, n_pieces, flag)) join(0, 1, n_pieces, true);
-      } else if (n == 1 || last_piece(counters + (c0 ? gridDim.x : 0) + c0, epoch, n, flag)) {
-        if (n > 1) join(c0, 1, n, false);
-        if (last_piece(counters + 2 * gridDim.x, epoch, (n_pieces + kJoin - 1) / kJoin, flag))
-          join(0, kJoin, (n_pieces + kJoin - 1) / kJoin, true);
-      }
-    }
+    join_waves<E, DP, C::kWaves, C::kRows>(p, t, head, Piece{first_wg, n_pieces, first_slot, my_slot, epoch}, jo, jm);
   }
 }
 
@@ -1067,16 +555,6 @@ struct Rows32 {
   static constexpr int kLoads = Share<DP, kShare, false>::kLoads;
   static constexpr int kLds = 2 * 2 * kTileBytes + 2 * WAVES * 4;  // and flags
 };
-
-// Keys of a chunk and chunks of a tile: the plan's, longer ones where the keys
-// are more than it was told.
-template <int KEYS>
-__device__ __forceinline__ void chunks_of(const AttnParams &p, const Tile &t, uint32_t *chunk, uint32_t *n_chunks) {
-  const uint32_t keys = (uint32_t)(t.hi - (t.lo & ~(KEYS - 1)));
-  const uint32_t c = ((keys + p.n_chunks - 1) / p.n_chunks + KEYS - 1) & ~(KEYS - 1);
-  *chunk = uni(c < p.chunk ? p.chunk : c);
-  *n_chunks = uni(keys ? (keys + *chunk - 1) / *chunk : 1);
-}
 
 template <class E, int DP, int WAVES, bool PAD>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) void attn_rows32_kernel(AttnParams p) {
@@ -1411,16 +889,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(weigh(acc[v], inv, Pass<true>()), T4);
   }
-}
-
-// More than 64 KiB of LDS has to be asked for, once per kernel and device.
-hipError_t allow_lds(const void *fn, int bytes, std::atomic<uint64_t> *devices) {
-  int d = 0;
-  hipError_t e = hipGetDevice(&d);
-  if (e != hipSuccess || (devices->load(std::memory_order_relaxed) >> d & 1)) return e;
-  e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) devices->fetch_or(1ull << d, std::memory_order_relaxed);
-  return e;
 }
 
 template <class E, int DP, int WAVES, int NR, bool PAD>

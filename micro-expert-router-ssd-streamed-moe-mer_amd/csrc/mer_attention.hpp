@@ -65,7 +65,47 @@ struct AttnParams {
   uint32_t *status;
 };
 
+// The cache held in 4 bits: k and v of AttnParams are codes
+// [n_pages][n_kv_heads][page_size][head_dim / 2], their blocks' scales f16
+// [n_pages][n_kv_heads][head_dim / 32][page_size].
+constexpr uint32_t kQ4Block = 32;
+struct AttnQ4Params : AttnParams {
+  const void *k_scales, *v_scales;
+};
+
+// A cache's two planes of keys and of values.
+struct CacheQ4 {
+  uint8_t *codes[2];
+  uint16_t *scales[2];
+  uint64_t n_slots;          // n_pages * page_size
+  uint32_t page_shift, heads, head_dim;
+};
+struct AppendQ4Params {
+  CacheQ4 cache;
+  const void *in[2];         // k and v: [n_tokens] rows of heads, in_stride elements apart
+  uint64_t in_stride[2];
+  const float *norm;         // [head_dim] of the keys, or null
+  const int32_t *positions;  // [n_tokens], or null without rotation
+  const float *inv_freq;     // [rot / 2]
+  const int64_t *slots;      // [n_tokens]; negative = no row
+  uint32_t n_tokens, rot, interleaved;
+  uint32_t heads_per_wave;   // consecutive heads that one wave walks
+  float eps;
+  uint32_t *status;
+};
+struct ReadQ4Params {
+  CacheQ4 cache;
+  const int64_t *slots;      // [n_rows]; negative = a row of zeros
+  void *out[2];              // k and v, out_stride elements apart
+  uint64_t out_stride[2];
+  uint32_t n_rows;
+  uint32_t *status;
+};
+hipError_t launch_append_q4(int in_type, const AppendQ4Params &p, int cus, hipStream_t st);
+hipError_t launch_read_q4(int out_type, const ReadQ4Params &p, hipStream_t st);
+
 void set_reciprocals(AttnParams *p);
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
+hipError_t launch_attention_q4(int type, const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st);
 
 }  // namespace mer

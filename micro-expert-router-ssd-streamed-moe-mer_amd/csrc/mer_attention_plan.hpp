@@ -160,4 +160,27 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
   return a;
 }
 
+// ---- the cache held in 4 bits (mer_attention_q4.hip) ----
+
+// Floats that a call reserves, as attn_reserve says.
+inline size_t attn_q4_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                              size_t max_q_len, size_t max_kv_len, int cus) {
+  (void)n_seqs, (void)n_tokens, (void)group, (void)n_kv_heads, (void)head_dim, (void)max_q_len, (void)max_kv_len;
+  return 2 * 2 * 32 * (128 + 2) * (size_t)cus;
+}
+
+inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                             size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
+                             size_t floats) {
+  (void)n_seqs, (void)n_tokens, (void)n_kv_heads, (void)max_kv_len, (void)table_keys, (void)window, (void)floats;
+  AttnPlan a{};
+  a.rows = max_q_len * group <= 16 || head_dim > 128 ? 16 : 32;
+  a.waves = 4;
+  a.n_wgs = (uint32_t)cus * (head_dim <= 128 ? 2 : 1);
+  a.min_granules = 1;
+  a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
+  a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
+  return a;
+}
+
 }  // namespace mer

@@ -1,0 +1,591 @@
+// mer_attention_q4.hip -- attention of a chunk of new tokens over a paged cache
+// held in 4 bits (the mathematics is that of mer_attention.hip, which has it
+// over 16-bit caches).
+//
+// Blocks of 32 elements with a scale d; a code n stands for d (n - 8), which
+// kv_append's five-bit scales make exact in f16.  So a tile's codes become f16
+// operands without a rounding and the products run on f16 MFMA whatever the
+// queries' type.  bf16 queries are brought to f16 by a power of two for each
+// row that puts its largest element below 2^15: exact for elements down to
+// 2^-29 of that, and off by 2^-39 of it at most below.  The weights are rounded
+// to f16, 2^7 times larger as in mer_attention.hip.
+#include "mer_attention_device.hpp"
+
+#include <math.h>
+
+namespace mer {
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+
+// What the answers are rounded to.
+struct ToF16 {
+  typedef _Float16 T;
+  typedef h8 V8;
+  static constexpr float kUp = 7.0f;
+};
+struct ToBF16 {
+  typedef __bf16 T;
+  typedef b8 V8;
+  static constexpr float kUp = 7.0f;
+};
+
+// Eight codes of a word, less 8 each, as f16: (0, 4), (1, 5), (2, 6), (3, 7).
+// An f16 of 1024 + n has n in its last four bits, one of 64 + n in the four
+// above them.
+__device__ __forceinline__ void unpack(uint32_t w, h2 x[4]) {
+  const h2 far = {(_Float16)1032.0f, (_Float16)1032.0f}, near = {(_Float16)72.0f, (_Float16)72.0f};
+  x[0] = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - far;
+  x[1] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - near;
+  w >>= 8;
+  x[2] = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - far;
+  x[3] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - near;
+}
+__device__ __forceinline__ h8 eight(const h2 x[4]) {
+  h8 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = x[i][0], v[2 * i + 1] = x[i][1];
+  return v;
+}
+
+// Geometry of a tile of 64 keys: codes of K, codes of V, scales of K and of V
+// ([block][key]).  A row's pieces of 16 bytes, a block each, lie permuted by
+// the row, against bank conflicts.
+template <int DP>
+struct TileQ4 {
+  static constexpr int kKeys = 64;
+  static constexpr int kRowBytes = DP / 2;
+  static constexpr int kPieces = DP / 32;              // of a row: blocks
+  static constexpr int kCodeBytes = kKeys * kRowBytes; // K or V
+  static constexpr int kScaleBytes = kPieces * kKeys * 2;
+  static constexpr int kBytes = 2 * kCodeBytes + 2 * kScaleBytes;
+  static constexpr int kRows = 64 / kPieces;           // of an asynchronous copy
+  static constexpr int kCopies = kKeys / kRows;        // of K's codes, and of V's
+  static constexpr int kScaleCopies = 2 * kScaleBytes > 1024 ? 2 : 1;  // of both
+  static constexpr int kLoads = 2 * kCopies + kScaleCopies;
+  // K: 16 lanes read a piece of the rows 16 q + 4 t + r, q and r from 0 to 3.
+  static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
+    return DP == 64 ? row >> 4 & 1 : (DP == 128 ? row >> 4 & 3 : (row >> 1 & 1) | (row >> 4 & 3) << 1);
+  }
+  // V: 16 lanes read a piece of 16 rows.
+  static __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
+    return DP == 64 ? row >> 3 & 1 : (DP == 128 ? row >> 2 & 3 : row >> 1 & 7);
+  }
+};
+
+// Asynchronous copies of a tile by one wave.  Pages are looked up by groups of
+// eight keys, a tile ahead.
+template <int DP>
+struct ShareQ4 {
+  typedef TileQ4<DP> G;
+  static constexpr int kGroups = G::kKeys / 8;
+  static constexpr int kPerCopy = G::kRows / 8;  // groups of a copy of codes
+
+  const uint8_t *k, *v, *ks, *vs;  // of this head in page 0
+  uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages, n_blocks;
+  const int32_t *table;
+  int32_t lo, hi;
+  int32_t key0, next_key;
+  uint32_t id[kGroups];
+  int32_t next_id[kGroups];
+  uint32_t known;                   // groups of pages that the cache has, a bit each
+  uint32_t koff[G::kCopies], voff[G::kCopies];  // a lane's piece, from its copy's first row
+  uint32_t soff[G::kScaleCopies];   // a lane's scales, from its group's (kNone: beyond the head)
+
+  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, const Tile &t) {
+    row_bytes = p.head_dim / 2;
+    n_blocks = p.head_dim / kQ4Block;
+    page_shift = p.page_shift;
+    code_bytes = (p.n_kv_heads << page_shift) * row_bytes;
+    scale_bytes = ((p.n_kv_heads * n_blocks) << page_shift) * 2;
+    n_pages = p.n_pages;
+    k = (const uint8_t *)p.k + (uint64_t)(head << page_shift) * row_bytes;
+    v = (const uint8_t *)p.v + (uint64_t)(head << page_shift) * row_bytes;
+    ks = (const uint8_t *)p.k_scales + (uint64_t)((head * n_blocks) << page_shift) * 2;
+    vs = (const uint8_t *)p.v_scales + (uint64_t)((head * n_blocks) << page_shift) * 2;
+    table = seq_table;
+    lo = t.lo;
+    hi = t.hi;
+    const uint32_t lane = lane_id(), sub = lane / G::kPieces, piece = lane % G::kPieces;
+    // Codes beyond the head are the first block's: any code will do beside a
+    // scale of zero, which clear_pads leaves there.
+    auto at = [&](uint32_t row, uint32_t block) { return row % G::kRows * row_bytes + (block < n_blocks ? block * 16 : 0); };
+#pragma unroll
+    for (uint32_t j = 0; j < G::kCopies; ++j) {
+      const uint32_t row = j * G::kRows + sub;
+      koff[j] = at(row, piece ^ G::k_swizzle(row));
+      voff[j] = at(row, piece ^ G::v_swizzle(row));
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < G::kScaleCopies; ++j) {
+      const uint32_t block = (j * 64 + lane) / 8 % G::kPieces;
+      soff[j] = j * 64 + lane < 2 * G::kPieces * 8 && block < n_blocks ? (block << page_shift) * 2 : kNone;
+    }
+  }
+
+  // Any key will do: page places are cut to those of [lo, hi), which is not
+  // empty; keys outside have no weight.
+  __device__ __forceinline__ void lookup(int32_t key) {
+    next_key = key;
+    const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      int32_t pg = (key + g * 8) >> page_shift;
+      pg = pg > last ? last : (pg < first ? first : pg);
+      next_id[g] = sload(table, (uint32_t)pg);
+    }
+  }
+
+  // On to the tile last looked up, before its copies.
+  __device__ __forceinline__ void advance(uint32_t *status) {
+    key0 = next_key;
+    known = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const bool is = (uint32_t)next_id[g] < n_pages;
+      id[g] = is ? (uint32_t)next_id[g] : 0;
+      known |= is ? 1u << g : 0u;
+    }
+    if (known != (1u << kGroups) - 1 && lane_id() < kGroups) {
+      const int32_t k0 = key0 + (int32_t)lane_id() * 8;
+      if (!(known >> lane_id() & 1) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
+    }
+  }
+
+  // Zero scales for the blocks that a padded head has not, in a tile's place.
+  __device__ __forceinline__ void clear_pads(uint32_t lds) const {
+    if (n_blocks == G::kPieces) return;
+    for (uint32_t i = lane_id(); i < 2 * G::kPieces * 8; i += 64)
+      if (i / 8 % G::kPieces >= n_blocks)
+        *(__attribute__((address_space(3))) u4 *)(uintptr_t)(lds + 2 * G::kCodeBytes + i * 16) = u4{0, 0, 0, 0};
+  }
+  // Zero scales for the keys of unknown pages, once the tile is there.
+  __device__ __forceinline__ void clear_unknown(uint32_t lds, uint32_t tile_known) const {
+    if (tile_known == (1u << kGroups) - 1) return;
+    for (uint32_t i = lane_id(); i < 2 * G::kPieces * 8; i += 64)
+      if (!(tile_known >> i % 8 & 1))
+        *(__attribute__((address_space(3))) u4 *)(uintptr_t)(lds + 2 * G::kCodeBytes + i * 16) = u4{0, 0, 0, 0};
+  }
+
+  // Lane x's of n words that the whole wave has.
+  template <int N>
+  static __device__ __forceinline__ uint32_t pick(const uint32_t *w, uint32_t x) {
+    uint32_t r = w[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) r = x == (uint32_t)i ? w[i] : r;
+    return r;
+  }
+
+  template <bool V>
+  __device__ __forceinline__ void copy_codes(uint32_t lds) const {
+    const uint8_t *base = V ? v : k;
+    const uint32_t mask = (1u << page_shift) - 1;
+    if (kPerCopy == 1 || (8u * kPerCopy) >> page_shift <= 1) {
+      // a copy's keys lie in one page
+#pragma unroll
+      for (int j = 0; j < G::kCopies; ++j) {
+        const uint32_t place = (uint32_t)(key0 + j * G::kRows) & mask;
+        async_row16(base + (uint64_t)id[j * kPerCopy] * code_bytes + place * row_bytes, V ? voff[j] : koff[j], lds + j * 1024u);
+      }
+    } else {
+      const uint32_t g = lane_id() / G::kPieces / 8;  // of a copy's groups
+#pragma unroll
+      for (int j = 0; j < G::kCopies; ++j) {
+        const uint32_t page = pick<kPerCopy>(id + j * kPerCopy, g), place = (uint32_t)(key0 + j * G::kRows + (int32_t)g * 8) & mask;
+        const uint32_t in_group = (V ? voff[j] : koff[j]) - g * 8 * row_bytes;
+        async_row16(base + (uint64_t)page * code_bytes + place * row_bytes + in_group, lds + j * 1024u);
+      }
+    }
+  }
+  __device__ __forceinline__ void copy_scales(uint32_t lds) const {
+    const uint32_t mask = (1u << page_shift) - 1, g = lane_id() % 8;
+    const uint32_t page = pick<kGroups>(id, g), place = (uint32_t)(key0 + (int32_t)g * 8) & mask;
+    const uint64_t at = (uint64_t)page * scale_bytes + place * 2;
+#pragma unroll
+    for (int j = 0; j < G::kScaleCopies; ++j) {
+      const bool is_v = j * 64 + lane_id() >= G::kPieces * 8;
+      if (soff[j] != kNone) async_row16((is_v ? vs : ks) + at + soff[j], lds + j * 1024u);
+    }
+  }
+  __device__ __forceinline__ void copy(uint32_t lds) const {
+    copy_codes<false>(lds);
+    copy_codes<true>(lds + G::kCodeBytes);
+    copy_scales(lds + 2 * G::kCodeBytes);
+  }
+};
+
+// Scales that no value may have: 8192 and more, infinities and NaN.
+__device__ __forceinline__ bool wild(u4 x) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) found |= (x[i] & 0x70007000u) + 0x10001000u;  // three ones carry into the sign's place
+  return (found & 0x80008000u) != 0;
+}
+__device__ __forceinline__ u4 tame(u4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((x[i] & 0x7000u) == 0x7000u) x[i] &= 0xffff0000u;
+    if ((x[i] & 0x70000000u) == 0x70000000u) x[i] &= 0x0000ffffu;
+  }
+  return x;
+}
+
+// A row of queries as operands of products over 32 dims each, in the order in
+// which unpack leaves a word of codes; returns what its scores are to be
+// multiplied with.
+template <class E, int DP>
+__device__ __forceinline__ float load_q(const typename E::T *row, bool there, uint32_t head_dim, uint32_t quad,
+                                        float scale, h8 q[DP / 32]) {
+  typedef typename E::T T;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 x[DP / 32][2];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) {
+    const uint32_t d = DP == 64 ? quad / 2 * 32 + (quad % 2 * 2 + i) * 4 : (i / 4 * 4 + quad) * 32 + i % 4 * 4;
+    x[i][0] = x[i][1] = T4{};
+    if (there && d < head_dim) {
+      x[i][0] = *(const T4 *)(row + d);
+      x[i][1] = *(const T4 *)(row + d + 16);
+    }
+  }
+  int down = 0;
+  if constexpr (__is_same(T, __bf16)) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[i][e / 4][e % 4]));
+    most = max_quad(most);
+    down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
+    scale = ldexpf(scale, down);
+  }
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // pairs (0, 2), (16, 18), (1, 3), (17, 19) of the word's elements
+      const T y = x[i][e / 2 % 2][e / 4 + e % 2 * 2];
+      if constexpr (__is_same(T, __bf16)) q[i][e] = (_Float16)ldexpf((float)y, -down);
+      else q[i][e] = y;
+    }
+  return scale;
+}
+
+// Up to 16 or 32 rows of a group a sequence; the work is cut as in
+// mer_attention.hip's kernel of this shape: equal stretches of all sequences'
+// granules to every workgroup, pieces of a unit joined by who comes last.
+//
+// A wave takes tiles of 64 keys.  Lane (r, q) = (lane % 16, lane / 16) of K^T's
+// product t reads key 16 q' + 4 t + r % 4, q' = r / 4, so that its four scores
+// of product t are those of the keys 16 q + 4 t + 0 .. 3, and its 16 scores the
+// keys that V's transposed read of 4-bit codes (16 rows x 16 codes) gives lane
+// q's group: P stays where it is.  Rows go to that read so that the two codes
+// which unpack makes a pair are neighbouring keys, whose scales are a pair too.
+template <int DP, int WAVES, int NR>
+struct Rows16Q4 {
+  typedef TileQ4<DP> G;
+  static constexpr int kWaves = WAVES, kRows = 16 * NR, kKeys = 64, kGranule = 128, kStages = 2;
+  static constexpr int kRing = WAVES * kStages * G::kBytes, kJoin = WAVES * kRows * (DP + 2) * 4 + 16;
+  static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+};
+
+template <class E, int DP, int WAVES, int NR>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, 2))) void attn_q4_rows16_kernel(AttnQ4Params p) {
+  typedef Rows16Q4<DP, WAVES, NR> C;
+  typedef TileQ4<DP> G;
+  typedef typename E::T T;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
+  const uint32_t col = lane % 16, quad = lane / 16;
+
+  // where a lane reads its operands, from a tile's start
+  uint32_t k_lane[4][DP / 128 ? DP / 128 : 1], v_lane[G::kPieces];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t row = col / 4 * 16 + t * 4 + col % 4;
+    if constexpr (DP == 64) {
+      k_lane[t][0] = row * G::kRowBytes + ((quad / 2) ^ G::k_swizzle(row)) * 16 + quad % 2 * 8;
+    } else {
+#pragma unroll
+      for (int c = 0; c < DP / 128; ++c) k_lane[t][c] = row * G::kRowBytes + ((c * 4 + quad) ^ G::k_swizzle(row)) * 16;
+    }
+  }
+  const uint32_t v_row = quad * 16 + (col & 8) + (col & 3) * 2 + (col >> 2 & 1);
+#pragma unroll
+  for (int b = 0; b < G::kPieces; ++b) v_lane[b] = G::kCodeBytes + v_row * G::kRowBytes + (b ^ G::v_swizzle(v_row)) * 16;
+  const uint32_t ks_lane = 2 * G::kCodeBytes + (DP == 64 ? quad / 2 : quad) * (G::kKeys * 2) + (col / 4 * 16 + col % 4) * 2;
+  const uint32_t vs_lane = 2 * G::kCodeBytes + G::kScaleBytes + quad * 32;
+
+  uint64_t epoch = 0;  // in thread 0
+  if (tid == 0)
+    epoch = attn_epoch(__hip_atomic_fetch_add(p.counters + blockIdx.x % kAttnTickets * kAttnTicketWords,
+                                              attn_ticket(blockIdx.x, gridDim.x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+
+  typedef Granules<C::kKeys> Gr;
+  Gr gr;
+  gr.base = 0;
+  gr.template view<C::kGranule, C::kRows>(p, 0);
+  uint32_t all = gr.total;
+  if (p.n_seqs > 256) {
+    for (uint32_t s = 256; s < p.n_seqs; s += 256) {
+      gr.template view<C::kGranule, C::kRows>(p, s);
+      all += gr.total;
+    }
+    gr.template view<C::kGranule, C::kRows>(p, 0);
+  }
+  uint32_t per = uni((all + gridDim.x - 1) / gridDim.x);
+  per = per < p.min_granules ? p.min_granules : per;
+  uint32_t x = blockIdx.x * per;
+  const uint32_t x1 = all - (all < x ? all : x) < per ? all : x + per;
+  bool first_piece = true;
+  while (x < x1) {
+    uint32_t seq, before;
+    Span span;
+    if (!gr.template find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
+    int32_t start = 0;
+    const uint32_t n_gran = uni(Gr::template granules<C::kGranule>(p, span, &start));
+    const uint32_t unit = uni((x - before) / n_gran), tile = uni(by_heads(p, unit)), head = unit - tile * p.n_kv_heads;
+    const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
+    const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
+    // the unit's pieces: workgroups first_wg .. first_wg + n_pieces - 1
+    const uint32_t first_wg = g0 == 0 ? blockIdx.x : (per == 1 ? unit0 : uni(unit0 / per));
+    const uint32_t last_wg = g0 + count == n_gran ? blockIdx.x : (per == 1 ? unit0 + n_gran - 1 : uni((unit0 + n_gran - 1) / per));
+    const uint32_t n_pieces = last_wg - first_wg + 1;
+    const uint32_t first_slot = 2 * first_wg + (first_wg * per == unit0 ? 0 : 1);
+    const uint32_t my_slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+    first_piece = false;
+    x += count;
+    Tile t;
+    // (spans that overlap, past 2^32, or lengths that change under the kernel)
+    if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads || last_wg >= gridDim.x) return;
+    start = (int32_t)uni((uint32_t)start);
+    int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
+    if (p.window && begin < (t.lo & ~(C::kKeys - 1))) begin = t.lo & ~(C::kKeys - 1);
+    end = end < t.hi ? end : t.hi;
+
+    const int32_t window = p.window ? (int32_t)p.window : 0x40000000;
+    h8 q[NR][DP / 32];
+    int32_t pos[NR];
+    float scale[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const uint32_t row = t.row0 + n * 16 + col, tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
+      pos[n] = t.pos0 + (int32_t)tok;
+      scale[n] = load_q<E, DP>((const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim,
+                               row < t.n_rows, p.head_dim, quad, p.scale_log2, q[n]);
+    }
+    const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
+    const int32_t pos_first = t.pos0 + (int32_t)by_group(p, t.row0), pos_last = t.pos0 + (int32_t)by_group(p, last);
+
+    const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
+    const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
+    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + wave * (C::kStages * G::kBytes);
+    auto key_of = [&](int32_t i) { return begin + (i * C::kWaves + (int32_t)wave) * C::kKeys; };
+    auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * G::kBytes; };
+    __syncthreads();  // the last piece is done with the LDS
+    ShareQ4<DP> sh;
+    sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t);
+    if (mine > 0) sh.lookup(key_of(0));
+    for (int32_t i = 0; i < C::kStages; ++i) sh.clear_pads(slot_of(i));
+    wait_lds();
+    // q has to be there before the first copy goes out: a later wait for it,
+    // which the compiler would put into the loop, would drain the copies.
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    float m[NR], l[NR];
+    f4 o[NR][DP / 16];
+    uint32_t known[C::kStages] = {};
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i)
+      if (i < mine) {
+        sh.advance(p.status);
+        known[i] = sh.known;
+        sh.lookup(key_of(i + 1));
+        sh.copy(slot_of(i));
+      }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      m[n] = -__builtin_inff();
+      l[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[n][d] = f4{0, 0, 0, 0};
+    }
+    for (int32_t i = 0; i < mine; ++i) {
+      const int32_t left = mine - i, key0 = key_of(i);
+      const uint32_t at = slot_of(i);
+      if (left == 1) wait_vm<0>();
+      else wait_vm<G::kLoads>();
+      sh.clear_unknown(at, known[0]);
+      // scores: lane's key of product tt is 16 quad + 4 tt + e
+      f4 s[NR][4];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][tt] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < (DP > 64 ? DP / 128 : 1); ++c) {
+          uint32_t w[4];
+          if constexpr (DP == 64) {
+            const u2 y = *(const __attribute__((address_space(3))) u2 *)(uintptr_t)(at + k_lane[tt][0]);
+            w[0] = y[0], w[1] = y[1];
+          } else {
+            const u4 y = *(const __attribute__((address_space(3))) u4 *)(uintptr_t)(at + k_lane[tt][c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = y[j];
+          }
+          const _Float16 d = *(const __attribute__((address_space(3))) _Float16 *)(uintptr_t)(
+              at + ks_lane + tt * 8 + c * (4 * G::kKeys * 2));
+          const h2 dd = {d, d};
+#pragma unroll
+          for (int j = 0; j < (DP == 64 ? 2 : 4); ++j) {
+            h2 y[4];
+            unpack(w[j], y);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] *= dd;
+            const h8 k8 = eight(y);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              s[n][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[n][c * 4 + j], s[n][tt], 0, 0, 0);
+          }
+        }
+      }
+      // V's scales, looked over
+#pragma unroll
+      for (int j = 0; j < (G::kScaleBytes + 1023) / 1024; ++j) {
+        __attribute__((address_space(3))) u4 *const place = (__attribute__((address_space(3))) u4 *)(uintptr_t)(
+            at + 2 * G::kCodeBytes + G::kScaleBytes + j * 1024 + lane % (G::kScaleBytes / 16) * 16);
+        const u4 y = *place;
+        if (__builtin_amdgcn_ballot_w64(wild(y))) {
+          *place = tame(y);
+          wait_lds();
+        }
+      }
+      const int32_t key_end = key0 + C::kKeys;
+      const bool partial = key_end > pos_first + 1 || key_end > t.hi || key0 <= pos_last - window;
+      h8 pr[NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float z[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = s[n][e / 4][e % 4] * scale[n];
+        if (partial) {
+          const int32_t last_key = pos[n] - key0 - (int32_t)quad * 16, before_key = last_key - window;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[e] = e > last_key || e <= before_key ? -__builtin_inff() : z[e];
+        }
+        float mx = z[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
+        mx = max_quad(mx);
+        // The maximum in use may lag by up to 8 (weights up to 2^8).
+        if (__builtin_amdgcn_ballot_w64(mx > m[n] + 8.0f)) {
+          const float mn = fmaxf(m[n], mx);
+          const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+          m[n] = mn;
+          l[n] *= a;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) o[n][d] *= a;
+        }
+        const float mu = (m[n] == -__builtin_inff() ? 0.0f : m[n]) - E::kUp;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          z[e] = __builtin_amdgcn_exp2f(z[e] - mu);
+          sum += z[e];
+        }
+        l[n] += sum;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          f8 y;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = z[b * 8 + e];
+          pr[n][b] = __builtin_convertvector(y, h8);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < G::kPieces; ++b) {
+        u4 sc[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          sc[j] = *(const __attribute__((address_space(3))) u4 *)(uintptr_t)(at + vs_lane + b * (G::kKeys * 2) + j * 16);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              (__attribute__((address_space(3))) v2i *)(uintptr_t)(at + v_lane[b] + hh * 8));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            h2 y[4];
+            unpack((uint32_t)w[j], y);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] *= __builtin_bit_cast(h2, (uint32_t)sc[j][k]);
+            const h8 v8 = eight(y);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              o[n][2 * b + hh] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pr[n][j], o[n][2 * b + hh], 0, 0, 0);
+          }
+        }
+      }
+      wait_lds();
+#pragma unroll
+      for (int j = 0; j + 1 < C::kStages; ++j) known[j] = known[j + 1];
+      if (left > C::kStages) {
+        sh.advance(p.status);
+        known[C::kStages - 1] = sh.known;
+        sh.lookup(key_of(i + C::kStages + 1));
+        sh.copy(at);
+      }
+    }
+    // join the waves: m, l and O of each in LDS
+    __syncthreads();
+    float *jo = (float *)smem;                      // [wave][row][DP]
+    float *jm = jo + C::kWaves * C::kRows * DP;     // [wave][row][2]
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const uint32_t r = wave * C::kRows + n * 16 + col;
+      l[n] = sum_quad(l[n]);
+      if (quad == 0) *(f2 *)&jm[r * 2] = f2{m[n], l[n]};
+      // an accumulator's elements e are the dims 2 quad + e / 2 (+ 16 if e is odd)
+      // of half a block
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        float *to = &jo[r * DP + d / 2 * 32 + d % 2 * 8 + quad * 2];
+        *(f2 *)to = f2{o[n][d][0], o[n][d][2]};
+        *(f2 *)(to + 16) = f2{o[n][d][1], o[n][d][3]};
+      }
+    }
+    __syncthreads();
+    join_waves<E, DP, C::kWaves, C::kRows>(p, t, head, Piece{first_wg, n_pieces, first_slot, my_slot, epoch}, jo, jm);
+  }
+}
+
+template <class E, int DP, int WAVES, int NR>
+hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  typedef Rows16Q4<DP, WAVES, NR> C;
+  static std::atomic<uint64_t> devices{0};
+  const hipError_t e = allow_lds((const void *)attn_q4_rows16_kernel<E, DP, WAVES, NR>, C::kLds, &devices);
+  if (e != hipSuccess) return e;
+  attn_q4_rows16_kernel<E, DP, WAVES, NR><<<plan.n_wgs, 64 * WAVES, C::kLds, st>>>(p);
+  return hipGetLastError();
+}
+
+template <class E, int DP>
+hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
+  if constexpr (DP < 256) return launch16<E, DP, 4, 2>(plan, p, st);
+  return hipErrorInvalidValue;
+}
+
+template <class E>
+hipError_t launch_typed(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  if (p.head_dim <= 64) return launch_dim<E, 64>(plan, p, st);
+  if (p.head_dim <= 128) return launch_dim<E, 128>(plan, p, st);
+  return launch_dim<E, 256>(plan, p, st);
+}
+
+}  // namespace
+
+hipError_t launch_attention_q4(int type, const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  return type == kF16 ? launch_typed<ToF16>(plan, p, st) : launch_typed<ToBF16>(plan, p, st);
+}
+
+}  // namespace mer

@@ -1,0 +1,312 @@
+// mer_cache_q4.hip -- keys and values into a paged cache held in 4 bits, with
+// the key's norm and rotation on the way, and rows of it back.
+//
+// A block is 32 neighbouring elements x of a head, as GGUF's Q4_0 has them:
+//   a = the x of largest magnitude (the positive one of two equal ones)
+//   d = |a| / 8 rounded to five bits, as f16, at most 7936; sign opposite to a's
+//   n = round(x / d) + 8, within 0 .. 15;   value = d (n - 8)
+// Five bits of scale cost nothing that shows beside codes of four (|a| comes
+// out within a quarter of a step) and make every value exact in f16 and in
+// bf16: 5 + 3 bits.  So attention and kv_read have no rounding of their own.
+// 7936 = 31 * 2^8 is the largest such scale whose eightfold is an f16.
+//
+// Keys are normed and rotated in 64 bits and rounded to f32 once: which code
+// an element next to a border gets then does not hang on the order of a sum or
+// on a sine's last bit (f32 arithmetic gives another code once in some 10^6
+// elements, this one less than once in 10^9).  f64 runs at the rate of plain
+// f32 here, and both kernels are bound by the memory.
+//
+// A head's row (key and value of a token) that holds something not finite, or
+// larger than the largest f16, is held as NaN: all its scales are.
+#include "../../include/mer_hip.h"
+#include "mer_attention.hpp"
+
+namespace mer {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef double d2 __attribute__((ext_vector_type(2)));
+typedef double d4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+template <int TYPE> struct Elem;
+template <> struct Elem<kF32> { typedef float T; typedef f4 V4; typedef f8 V8; };
+template <> struct Elem<kF16> { typedef _Float16 T; typedef h4 V4; typedef h8 V8; };
+template <> struct Elem<kBF16> { typedef __bf16 T; typedef b4 V4; typedef b8 V8; };
+
+constexpr float kMostScale = 7936.0f, kMostValue = 65504.0f;
+constexpr uint16_t kNanScale = 0x7e00;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+
+// This wave's LDS writes come before its reads.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Codes and scale of a block that four lanes hold, each elements 4t .. 4t + 3
+// (a) and 16 + 4t .. (b): the lane's four bytes of codes.
+__device__ __forceinline__ uint32_t quantise(f4 a, f4 b, _Float16 *scale) {
+  float hi = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+  float lo = fminf(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])), fminf(fminf(b[0], b[1]), fminf(b[2], b[3])));
+  hi = fmaxf(hi, dpp<0xB1>(hi));  // lane ^ 1
+  lo = fminf(lo, dpp<0xB1>(lo));
+  hi = fmaxf(hi, dpp<0x4E>(hi));  // lane ^ 2
+  lo = fminf(lo, dpp<0x4E>(lo));
+  const bool positive = hi >= -lo && hi > 0.0f;
+  uint32_t u = __float_as_uint(fmaxf(hi, -lo) * 0.125f);
+  u = (u + 0x3ffffu + (u >> 19 & 1)) & ~0x7ffffu;  // four bits behind the first, half to even
+  float d = (float)(_Float16)fminf(__uint_as_float(u), kMostScale);
+  d = positive ? -d : d;
+  *scale = (_Float16)d;
+  // Next to a border the quotient's rounding does not matter: d (n + 1/2) has
+  // ten bits, so an f32 x beside it is off by more than half a step of the
+  // quotient.
+  const float zero = d == 0.0f ? 1.0f : d;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p = __builtin_amdgcn_fmed3f(rintf(a[i] / zero), -8.0f, 7.0f) + 8.0f;
+    const float q = __builtin_amdgcn_fmed3f(rintf(b[i] / zero), -8.0f, 7.0f) + 8.0f;
+    codes |= ((uint32_t)p | (uint32_t)q << 4) << 8 * i;
+  }
+  return codes;
+}
+
+__device__ __forceinline__ bool does_not_fit(f4 a) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= !(fabsf(a[i]) <= kMostValue);
+  return bad;
+}
+
+// Passes of a wave: loads of all of them are in flight before the first is used.
+constexpr uint32_t kPasses = 2;
+
+// A wave has one token; LANES lanes have a head's key and value, eight elements
+// each (head_dim / 8 rounded up to a power of two).  Keys are loaded and turned
+// as two groups of four that hold both halves of their pairs, and go through
+// LDS to the lanes that have them as elements of a block; values are loaded as
+// those.
+template <int IN, int LANES>
+__global__ __launch_bounds__(256) void append_q4_kernel(AppendQ4Params p) {
+  typedef typename Elem<IN>::V4 V4;
+  typedef typename Elem<IN>::T T;
+  constexpr uint32_t kHeads = 64 / LANES;  // of a pass
+  constexpr int kAngles = LANES > 16 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float rows[4][64 * 8];
+  __shared__ __attribute__((aligned(16))) d2 turns[4][LANES * 4];  // cosine and sine
+  const uint32_t head_dim = p.cache.head_dim, heads = p.cache.heads, n_blocks = head_dim / kQ4Block;
+  const uint32_t per_token = (heads + p.heads_per_wave - 1) / p.heads_per_wave;
+  const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave = blockIdx.x * 4 + w;
+  const uint32_t token = (uint32_t)__builtin_amdgcn_readfirstlane(wave / per_token);
+  if (token >= p.n_tokens) return;
+  const uint32_t head0 = (wave - token * per_token) * p.heads_per_wave;
+  const uint32_t head1 = head0 + p.heads_per_wave < heads ? head0 + p.heads_per_wave : heads;
+  const uint32_t lane = __lane_id(), j = lane % LANES, sub = lane / LANES;
+  const bool in_row = j * 8 < head_dim;
+  const bool split = !p.interleaved && j * 8 < p.rot;
+  const uint32_t o0 = split ? 4 * j : 8 * j, o1 = split ? p.rot / 2 + 4 * j : 8 * j + 4;
+  const uint32_t block = j / 4, e0 = block * kQ4Block + j % 4 * 4, e1 = e0 + 16;
+
+  const int64_t slot = p.slots[token];
+  if (slot < 0) return;
+  if ((uint64_t)slot >= p.cache.n_slots) {
+    if (lane == 0) atomicCAS(p.status, 0u, (uint32_t)MER_ERR_RESIDENCY_MISS);
+    return;
+  }
+
+  f4 w0 = {1, 1, 1, 1}, w1 = {1, 1, 1, 1};
+  if (in_row && p.norm) w0 = *(const f4 *)(p.norm + o0), w1 = *(const f4 *)(p.norm + o1);
+  V4 k0[kPasses], k1[kPasses], v0[kPasses], v1[kPasses];
+  const T *kp = (const T *)p.in[0] + (uint64_t)token * p.in_stride[0], *vp = (const T *)p.in[1] + (uint64_t)token * p.in_stride[1];
+#pragma unroll
+  for (uint32_t i = 0; i < kPasses; ++i) {
+    const uint32_t h = head0 + i * kHeads + sub;
+    k0[i] = k1[i] = v0[i] = v1[i] = V4{};
+    if (h < head1 && in_row) {
+      k0[i] = *(const V4 *)(kp + h * head_dim + o0);
+      k1[i] = *(const V4 *)(kp + h * head_dim + o1);
+      v0[i] = *(const V4 *)(vp + h * head_dim + e0);
+      v1[i] = *(const V4 *)(vp + h * head_dim + e1);
+    }
+  }
+  const bool turned = in_row && j * 8 < p.rot;
+  double cs[4] = {1, 1, 1, 1}, sn[4] = {0, 0, 0, 0};
+  if (p.rot) {
+    // The wave's lanes make an angle each (two where there are more than 64):
+    // turns = position * inv_freq / 2 pi less its nearest whole number, the
+    // product with 1 / 2 pi in two words.
+    const double pos = (double)p.positions[token];
+#pragma unroll
+    for (int a = 0; a < kAngles; ++a) {
+      const uint32_t f = a * 64 + lane;
+      if (f < p.rot / 2) {
+        const double x = pos * (double)p.inv_freq[f], t = x * 0.15915494309189535;
+        const double rest = __builtin_fma(x, 0.15915494309189535, -t) + x * -9.839338337591243e-18;
+        double s, c;
+        sincospi(2.0 * ((t - rint(t)) + rest), &s, &c);
+        turns[w][f] = d2{c, s};
+      }
+    }
+    wave_sync();
+    if (turned)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const d2 x = turns[w][4 * j + i];
+        cs[i] = x[0];
+        sn[i] = x[1];
+      }
+  }
+  const uint64_t page = (uint64_t)slot >> p.cache.page_shift, off = (uint64_t)slot & ((1u << p.cache.page_shift) - 1);
+  float *const row = rows[w] + sub * (LANES * 8);
+#pragma unroll
+  for (uint32_t i = 0; i < kPasses; ++i) {
+    const uint32_t h = head0 + i * kHeads + sub;
+    if (head0 + i * kHeads >= head1) break;  // the whole wave
+    f4 a = __builtin_convertvector(k0[i], f4), b = __builtin_convertvector(k1[i], f4);
+    if (p.norm || p.rot) {
+      d4 x = __builtin_convertvector(a, d4), y = __builtin_convertvector(b, d4);
+      if (p.norm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+        for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
+        const double r = 1.0 / sqrt(ss / (double)head_dim + (double)p.eps);
+        x = x * r * __builtin_convertvector(w0, d4);
+        y = y * r * __builtin_convertvector(w1, d4);
+      }
+      if (turned) {
+        const d4 u = x, v = y;
+        if (split) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = u[e] * cs[e] - v[e] * sn[e];
+            y[e] = v[e] * cs[e] + u[e] * sn[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            x[e] = u[e] * cs[e / 2] - u[e + 1] * sn[e / 2];
+            x[e + 1] = u[e + 1] * cs[e / 2] + u[e] * sn[e / 2];
+            y[e] = v[e] * cs[2 + e / 2] - v[e + 1] * sn[2 + e / 2];
+            y[e + 1] = v[e + 1] * cs[2 + e / 2] + v[e] * sn[2 + e / 2];
+          }
+        }
+      }
+      a = __builtin_convertvector(x, f4);
+      b = __builtin_convertvector(y, f4);
+    }
+    const f4 va = __builtin_convertvector(v0[i], f4), vb = __builtin_convertvector(v1[i], f4);
+    const uint64_t wrong = __builtin_amdgcn_ballot_w64(does_not_fit(a) || does_not_fit(b) || does_not_fit(va) || does_not_fit(vb));
+    const bool bad = (wrong >> sub * LANES & (LANES == 64 ? ~0ull : (1ull << LANES) - 1)) != 0;
+    wave_sync();
+    if (in_row) {
+      *(f4 *)(row + o0) = a;
+      *(f4 *)(row + o1) = b;
+    }
+    wave_sync();
+    if (in_row) {
+      a = *(const f4 *)(row + e0);
+      b = *(const f4 *)(row + e1);
+    }
+    _Float16 kd, vd;
+    const uint32_t kc = quantise(a, b, &kd), vc = quantise(va, vb, &vd);
+    if (h < head1 && in_row) {
+      const uint64_t unit = page * heads + h;
+      const uint64_t code = ((unit << p.cache.page_shift) + off) * (head_dim / 2) + 4 * j;
+      *(uint32_t *)(p.cache.codes[0] + code) = bad ? 0x88888888u : kc;
+      *(uint32_t *)(p.cache.codes[1] + code) = bad ? 0x88888888u : vc;
+      if (j % 4 == 0) {
+        const uint64_t at = ((unit * n_blocks + block) << p.cache.page_shift) + off;
+        p.cache.scales[0][at] = bad ? kNanScale : __builtin_bit_cast(uint16_t, kd);
+        p.cache.scales[1][at] = bad ? kNanScale : __builtin_bit_cast(uint16_t, vd);
+      }
+    }
+  }
+}
+
+template <int IN>
+hipError_t launch_append(AppendQ4Params p, int cus, hipStream_t st) {
+  const uint32_t heads = p.cache.heads, lanes = p.cache.head_dim <= 64 ? 8 : (p.cache.head_dim <= 128 ? 16 : 32);
+  const uint32_t per_pass = 64 / lanes, all = (heads + per_pass - 1) / per_pass;
+  // Heads of a wave: as many as its passes hold, fewer while that leaves the
+  // chip with less than eight waves a CU.
+  uint32_t passes = all < kPasses ? all : kPasses;
+  while (passes > 1 && (uint64_t)p.n_tokens * ((all + passes - 1) / passes) < 8ull * cus) --passes;
+  p.heads_per_wave = passes * per_pass;
+  const uint64_t waves = (uint64_t)p.n_tokens * ((heads + p.heads_per_wave - 1) / p.heads_per_wave);
+  const uint32_t grid = (uint32_t)((waves + 3) / 4);
+  if (lanes == 8) append_q4_kernel<IN, 8><<<grid, 256, 0, st>>>(p);
+  else if (lanes == 16) append_q4_kernel<IN, 16><<<grid, 256, 0, st>>>(p);
+  else append_q4_kernel<IN, 32><<<grid, 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+// A thread has eight bytes of codes, half a block: elements 8h .. 8h + 7 in
+// their low halves and 16 + 8h .. in their high ones.
+template <int OUT>
+__global__ __launch_bounds__(256) void read_q4_kernel(ReadQ4Params p) {
+  typedef typename Elem<OUT>::V8 V8;
+  typedef typename Elem<OUT>::T T;
+  const uint32_t head_dim = p.cache.head_dim, heads = p.cache.heads, halves = head_dim / 16, per_row = heads * halves;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / per_row;
+  if (row >= p.n_rows) return;
+  const uint32_t at = i - row * per_row, head = at / halves, half = at - head * halves;
+  const int64_t slot = p.slots[row];
+  const bool there = (uint64_t)slot < p.cache.n_slots;
+  if (!there && slot >= 0 && at == 0 && blockIdx.y == 0) atomicCAS(p.status, 0u, (uint32_t)MER_ERR_RESIDENCY_MISS);
+  f8 a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a;
+  if (there) {
+    const uint64_t page = (uint64_t)slot >> p.cache.page_shift, off = (uint64_t)slot & ((1u << p.cache.page_shift) - 1);
+    const uint64_t unit = page * heads + head;
+    const u2 c = *(const u2 *)(p.cache.codes[blockIdx.y] + ((unit << p.cache.page_shift) + off) * (head_dim / 2) + half * 8);
+    const float d = (float)__builtin_bit_cast(
+        _Float16, p.cache.scales[blockIdx.y][((unit * (halves / 2) + half / 2) << p.cache.page_shift) + off]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t byte = c[e / 4] >> e % 4 * 8;
+      a[e] = (float)((int32_t)(byte & 15) - 8) * d;
+      b[e] = (float)((int32_t)(byte >> 4 & 15) - 8) * d;
+    }
+  }
+  T *out = (T *)p.out[blockIdx.y] + (uint64_t)row * p.out_stride[blockIdx.y] + head * head_dim + half / 2 * kQ4Block + half % 2 * 8;
+  *(V8 *)out = __builtin_convertvector(a, V8);
+  *(V8 *)(out + 16) = __builtin_convertvector(b, V8);
+}
+
+template <int OUT>
+hipError_t launch_read(const ReadQ4Params &p, hipStream_t st) {
+  const uint64_t threads = (uint64_t)p.n_rows * p.cache.heads * (p.cache.head_dim / 16);
+  read_q4_kernel<OUT><<<dim3((uint32_t)((threads + 255) / 256), 2), 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_append_q4(int in_type, const AppendQ4Params &p, int cus, hipStream_t st) {
+  switch (in_type) {
+    case kF32: return launch_append<kF32>(p, cus, st);
+    case kF16: return launch_append<kF16>(p, cus, st);
+    default: return launch_append<kBF16>(p, cus, st);
+  }
+}
+hipError_t launch_read_q4(int out_type, const ReadQ4Params &p, hipStream_t st) {
+  switch (out_type) {
+    case kF32: return launch_read<kF32>(p, st);
+    case kF16: return launch_read<kF16>(p, st);
+    default: return launch_read<kBF16>(p, st);
+  }
+}
+
+}  // namespace mer
