@@ -548,6 +548,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
 // 4096 tokens of 80 140 us, of 96 142, of 112 145.
 template <int DP, int WAVES>
 struct Rows32 {
+  static constexpr int kWaves = WAVES;
   static constexpr int kRows = 32 * WAVES;
   static constexpr int kKeys = 64;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
@@ -835,62 +836,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) voi
   }
 }
 
-// Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
-// its accumulators spread over four waves.  Bound by the memory: four chunks
-// of 1040 tokens x 32 heads of 128 in 16 us.
-template <class E, int DP, int WAVES>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
-  typedef Rows32<DP, WAVES> C;
-  typedef typename E::T T;
-  constexpr int kVecs = DP / 32;  // 1 KiB vectors of accumulators of each of the four waves
-  const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64), col = lane % 32, half = lane / 32;
-  const uint32_t w = blockIdx.x % WAVES, uh = blockIdx.x / WAVES, head = uh % p.n_kv_heads, unit = uh / p.n_kv_heads;
-  uint32_t seq, tile, chunk, n_chunks;
-  find_unit<C::kRows>(p, unit, &seq, &tile);
-  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
-  Tile t;
-  if (!make_tile<C::kRows>(p, span, tile, &t)) return;
-  chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
-  const uint32_t row = t.row0 + w * 32 + col;
-  if (n_chunks == 1 || row - col >= t.n_rows) return;
-  const uint64_t slot0 = (uint64_t)uh * p.n_chunks;
-  const float *ml = p.part_ml + ((slot0 * WAVES + w) * 32 + col) * 2;
-  const float *po = p.part_o + (slot0 * WAVES + w) * (32 * DP) + wave * 256 + lane * 4;
-  float m = -__builtin_inff(), l;
-  for (uint32_t c = 0; c < n_chunks; ++c) m = fmaxf(m, ml[c * (WAVES * 64)]);
-  const float mu = m == -__builtin_inff() ? 0.0f : m;
-  f4 acc[kVecs];
-  auto add_up = [&](auto pass) {
-    l = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) acc[v] = f4{0, 0, 0, 0};
-#pragma unroll 4
-    for (uint32_t c = 0; c < n_chunks; ++c) {
-      const f2 x = *(const f2 *)(ml + c * (WAVES * 64));
-      const float a = __builtin_amdgcn_exp2f(x[0] - mu);
-      l += a * x[1];
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) acc[v] += weigh(*(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024), a, pass);
-    }
-  };
-  add_up(Pass<false>());
-  float z = 0.0f;
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) z += probe(acc[v]);
-  if (not_a_number(z)) add_up(Pass<true>());
-  if (row >= t.n_rows) return;
-  const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
-  if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu + E::kUp);
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const uint32_t at = v * 32 + wave * 8 + half * 4;  // vector v * 4 + wave
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(weigh(acc[v], inv, Pass<true>()), T4);
-  }
-}
-
 template <class E, int DP, int WAVES, int NR, bool PAD>
 hipError_t launch16p(const AttnPlan &plan, const AttnParams &p, hipStream_t st) {
   typedef Rows16<DP, WAVES, NR> C;
@@ -923,7 +868,7 @@ hipError_t launch32p(const AttnPlan &plan, const AttnParams &p, hipStream_t st) 
   const hipError_t e = allow_lds((const void *)attn_rows32_kernel<E, DP, 4, PAD>, C::kLds, &devices);
   if (e != hipSuccess) return e;
   attn_rows32_kernel<E, DP, 4, PAD><<<plan.n_wgs, 256, C::kLds, st>>>(p);
-  if (plan.n_chunks > 1) attn_join_kernel<E, DP, 4><<<plan.n_units * p.n_kv_heads * 4, 256, 0, st>>>(p);
+  if (plan.n_chunks > 1) attn_join_kernel<Rows32<DP, 4>, E, DP><<<plan.n_units * p.n_kv_heads * 4, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 

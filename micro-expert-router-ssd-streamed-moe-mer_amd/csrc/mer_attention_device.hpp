@@ -29,6 +29,7 @@ struct F16 {
   // largest (2^-14 as they are, where a row's one large weight may meet a value
   // smaller than what 32 others lose).
   static constexpr float kUp = 7.0f;
+  static constexpr bool kCodes = false;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -41,6 +42,7 @@ struct BF16 {
   typedef b8 V8;
   static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
   static constexpr float kUp = 0.0f;
+  static constexpr bool kCodes = false;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -551,6 +553,83 @@ __device__ __forceinline__ void chunks_of(const AttnParams &p, const Tile &t, ui
   const uint32_t c = ((keys + p.n_chunks - 1) / p.n_chunks + KEYS - 1) & ~(KEYS - 1);
   *chunk = uni(c < p.chunk ? p.chunk : c);
   *n_chunks = uni(keys ? (keys + *chunk - 1) / *chunk : 1);
+}
+
+// Four neighbouring dims of a row from an accumulator's elements 4 g .. 4 g + 3
+// over the dims 32 d ..: lanes below 32 hold the first four of eight dims, the
+// others the last.  Where the eight are a word of 4-bit codes as unpacked (E:
+// kCodes), they are 4 g + 0, 2, 16, 18 in the lower lanes and 1, 3, 17, 19 in
+// the upper ones, which exchange halves (all lanes are on).
+template <class E>
+__device__ __forceinline__ f4 four_of(f4 x, uint32_t d, uint32_t g, uint32_t half, uint32_t *at) {
+  if constexpr (E::kCodes) {
+    *at = d * 32 + half * 16 + g * 4;
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[0]), __float_as_uint(x[2]), false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[1]), __float_as_uint(x[3]), false, false);
+    return f4{__uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(b[0]), __uint_as_float(b[1])};
+  } else {
+    *at = d * 32 + g * 8 + half * 4;
+    return x;
+  }
+}
+
+// Joins the chunks of 32 rows: one workgroup for a wave of the kernel above,
+// its accumulators spread over four waves.  Bound by the memory: four chunks
+// of 1040 tokens x 32 heads of 128 in 16 us.
+// C: the kernel's rows, waves and keys of a tile.  E: the answers' type, and
+// whether the accumulators of 32 dims lie as unpacked codes (four_of).
+template <class C, class E, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+  typedef typename E::T T;
+  constexpr int WAVES = C::kWaves;
+  constexpr int kVecs = DP / 32;  // 1 KiB vectors of accumulators of each of the four waves
+  const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64), col = lane % 32, half = lane / 32;
+  const uint32_t w = blockIdx.x % WAVES, uh = blockIdx.x / WAVES, head = uh % p.n_kv_heads, unit = uh / p.n_kv_heads;
+  uint32_t seq, tile, chunk, n_chunks;
+  find_unit<C::kRows>(p, unit, &seq, &tile);
+  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
+  Tile t;
+  if (!make_tile<C::kRows>(p, span, tile, &t)) return;
+  chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
+  const uint32_t row = t.row0 + w * 32 + col;
+  if (n_chunks == 1 || row - col >= t.n_rows) return;
+  const uint64_t slot0 = (uint64_t)uh * p.n_chunks;
+  const float *ml = p.part_ml + ((slot0 * WAVES + w) * 32 + col) * 2;
+  const float *po = p.part_o + (slot0 * WAVES + w) * (32 * DP) + wave * 256 + lane * 4;
+  float m = -__builtin_inff(), l;
+  for (uint32_t c = 0; c < n_chunks; ++c) m = fmaxf(m, ml[c * (WAVES * 64)]);
+  const float mu = m == -__builtin_inff() ? 0.0f : m;
+  f4 acc[kVecs];
+  auto add_up = [&](auto pass) {
+    l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) acc[v] = f4{0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t c = 0; c < n_chunks; ++c) {
+      const f2 x = *(const f2 *)(ml + c * (WAVES * 64));
+      const float a = __builtin_amdgcn_exp2f(x[0] - mu);
+      l += a * x[1];
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) acc[v] += weigh(*(const f4 *)(po + c * (uint64_t)(WAVES * 32 * DP) + v * 1024), a, pass);
+    }
+  };
+  add_up(Pass<false>());
+  float z = 0.0f;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) z += probe(acc[v]);
+  if (not_a_number(z)) add_up(Pass<true>());
+  const bool row_ok = row < t.n_rows;
+  const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
+  if (row_ok && p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - mu + E::kUp);
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    uint32_t at;  // of vector v * 4 + wave
+    const f4 x = four_of<E>(weigh(acc[v], inv, Pass<true>()), v, wave, half, &at);
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (row_ok && at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x, T4);
+  }
 }
 
 // More than 64 KiB of LDS has to be asked for, once per kernel and device.

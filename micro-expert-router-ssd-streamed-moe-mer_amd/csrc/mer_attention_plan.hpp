@@ -68,45 +68,11 @@ inline size_t attn_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint3
   return cap < small ? small : cap;
 }
 
-// The plan of a call whose partial sums may take `floats`.  With none it is
-// 128-row tiles in one chunk, which every call can be.
-inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                          size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
-                          size_t floats) {
+// 128-row tiles: how many chunks a row tile's keys are cut into.
+inline AttnPlan attn_plan_128(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                              size_t max_q_len, size_t max_kv_len, uint32_t window, int cus, size_t floats) {
   AttnPlan a{};
-  // Up to 16 rows a sequence: tiles of 16.  17 to 32 (a few tokens, or groups of
-  // more than 16 heads): 128-row tiles where there are units enough to give the
-  // CUs two workgroups (64 sequences of 8 x 4 rows, 500 - 2000 keys, 8 kv heads of
-  // 128: 68 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 60 us); two tiles of
-  // 16 where there is little to read (1 of 4000: 17 us, 32 23 us; 8 of 4000 - 8000:
-  // 66 and 52 us) and for heads of 256, whose 32 rows would not fit the registers
-  // (8 of 4000 - 8000: 75 and 86 us).  Above, tiles of 128 (8 x 48 rows: 46 us, 32
-  // 75 us).
-  const uint64_t pairs = (uint64_t)n_seqs * n_kv_heads;
   a.rows = 128;
-  if (max_q_len * group <= 16) a.rows = 16;
-  else if (max_q_len * group <= 32 && pairs < (uint64_t)cus)
-    a.rows = head_dim > 128 || pairs * max_kv_len < 1024ull * cus ? 16 : 32;
-  // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
-  const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
-  if (small_tiles * (table_keys / 128 + 2) >= (1ull << 31)) a.rows = 128;
-  if (a.rows <= 32) {
-    // Long stretches of few units: the widest workgroups, as many as the CUs
-    // hold at once.  Many short units: as many waves, each a workgroup of its
-    // own, so that one's piece ends while the others' keys stream (512
-    // sequences of 60 - 300 keys: 135 us wide, 98 us narrow; 8 of 1000: 11 us
-    // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
-    const bool narrow = head_dim <= 128 && pairs >= 4ull * cus;
-    a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);
-    a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 64 ? 2 : 1);
-    a.min_granules = 1;
-    a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
-    a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
-    // (a launch takes every ticket and counts up to kAttnEpoch at most)
-    if (a.part_o_floats + a.part_ml_floats <= floats && a.n_wgs >= kAttnTickets && a.n_wgs < kAttnEpoch / 2) return a;
-    a = AttnPlan{};
-    a.rows = 128;
-  }
   a.n_units = (uint32_t)((n_tokens * group + a.rows - 1) / a.rows + n_seqs);
   // keys of a row tile, from a whole key tile's start on
   size_t max_keys = max_kv_len;
@@ -160,27 +126,67 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
   return a;
 }
 
-// ---- the cache held in 4 bits (mer_attention_q4.hip) ----
-
-// Floats that a call reserves, as attn_reserve says.
-inline size_t attn_q4_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                              size_t max_q_len, size_t max_kv_len, int cus) {
-  (void)n_seqs, (void)n_tokens, (void)group, (void)n_kv_heads, (void)head_dim, (void)max_q_len, (void)max_kv_len;
-  return 2 * 2 * 32 * (128 + 2) * (size_t)cus;
+// The plan of a call whose partial sums may take `floats`.  With none it is
+// 128-row tiles in one chunk, which every call can be.
+inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                          size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
+                          size_t floats) {
+  AttnPlan a{};
+  // Up to 16 rows a sequence: tiles of 16.  17 to 32 (a few tokens, or groups of
+  // more than 16 heads): 128-row tiles where there are units enough to give the
+  // CUs two workgroups (64 sequences of 8 x 4 rows, 500 - 2000 keys, 8 kv heads of
+  // 128: 68 us, tiles of 32 95 us; 16 of 2000 - 6000: 73 and 60 us); two tiles of
+  // 16 where there is little to read (1 of 4000: 17 us, 32 23 us; 8 of 4000 - 8000:
+  // 66 and 52 us) and for heads of 256, whose 32 rows would not fit the registers
+  // (8 of 4000 - 8000: 75 and 86 us).  Above, tiles of 128 (8 x 48 rows: 46 us, 32
+  // 75 us).
+  const uint64_t pairs = (uint64_t)n_seqs * n_kv_heads;
+  a.rows = 128;
+  if (max_q_len * group <= 16) a.rows = 16;
+  else if (max_q_len * group <= 32 && pairs < (uint64_t)cus)
+    a.rows = head_dim > 128 || pairs * max_kv_len < 1024ull * cus ? 16 : 32;
+  // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
+  const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
+  if (small_tiles * (table_keys / 128 + 2) >= (1ull << 31)) a.rows = 128;
+  if (a.rows <= 32) {
+    // Long stretches of few units: the widest workgroups, as many as the CUs
+    // hold at once.  Many short units: as many waves, each a workgroup of its
+    // own, so that one's piece ends while the others' keys stream (512
+    // sequences of 60 - 300 keys: 135 us wide, 98 us narrow; 8 of 1000: 11 us
+    // wide, 16 us narrow).  Heads of 256 fill the LDS with two waves.
+    const bool narrow = head_dim <= 128 && pairs >= 4ull * cus;
+    a.waves = narrow ? 1 : (head_dim <= 128 ? 4 : 2);
+    a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 64 ? 2 : 1);
+    a.min_granules = 1;
+    a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
+    a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
+    // (a launch takes every ticket and counts up to kAttnEpoch at most)
+    if (a.part_o_floats + a.part_ml_floats <= floats && a.n_wgs >= kAttnTickets && a.n_wgs < kAttnEpoch / 2) return a;
+  }
+  return attn_plan_128(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, window, cus, floats);
 }
+
+// ---- the cache held in 4 bits (mer_attention_q4.hip) ----
+// It reserves what attn_reserve says, whose least holds the sums of its 16- and
+// 32-row tiles too.
 
 inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                              size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
                              size_t floats) {
-  (void)n_seqs, (void)n_tokens, (void)n_kv_heads, (void)max_kv_len, (void)table_keys, (void)window, (void)floats;
   AttnPlan a{};
-  a.rows = max_q_len * group <= 16 || head_dim > 128 ? 16 : 32;
-  a.waves = 4;
-  a.n_wgs = (uint32_t)cus * (head_dim <= 128 ? 2 : 1);
-  a.min_granules = 1;
-  a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
-  a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
-  return a;
+  const size_t rows = max_q_len * group;
+  a.rows = rows <= 16 ? 16 : (rows <= 32 ? (head_dim > 128 ? 16 : 32) : 128);
+  // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
+  const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
+  if (a.rows <= 32 && small_tiles * (table_keys / 128 + 2) < (1ull << 31)) {
+    a.waves = 4;
+    a.n_wgs = (uint32_t)cus * (head_dim <= 128 ? 2 : 1);
+    a.min_granules = 1;
+    a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
+    a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
+    if (a.part_o_floats + a.part_ml_floats <= floats && a.n_wgs >= kAttnTickets && a.n_wgs < kAttnEpoch / 2) return a;
+  }
+  return attn_plan_128(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, window, cus, floats);
 }
 
 }  // namespace mer

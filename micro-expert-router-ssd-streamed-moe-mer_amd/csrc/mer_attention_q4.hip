@@ -24,11 +24,13 @@ struct ToF16 {
   typedef _Float16 T;
   typedef h8 V8;
   static constexpr float kUp = 7.0f;
+  static constexpr bool kCodes = true;
 };
 struct ToBF16 {
   typedef __bf16 T;
   typedef b8 V8;
   static constexpr float kUp = 7.0f;
+  static constexpr bool kCodes = true;
 };
 
 // Eight codes of a word, less 8 each, as f16: (0, 4), (1, 5), (2, 6), (3, 7).
@@ -231,18 +233,19 @@ __device__ __forceinline__ u4 tame(u4 x) {
   return x;
 }
 
-// A row of queries as operands of products over 32 dims each, in the order in
-// which unpack leaves a word of codes; returns what its scores are to be
-// multiplied with.
-template <class E, int DP>
-__device__ __forceinline__ float load_q(const typename E::T *row, bool there, uint32_t head_dim, uint32_t quad,
-                                        float scale, h8 q[DP / 32]) {
+// A row's queries as N operands of eight dims each, in the order in which
+// unpack leaves a word of codes: operand i is word `word_of(i)` of a row's codes,
+// four to a block.  `most_of`: the maximum over the lanes that have the row.
+// Returns what its scores are to be multiplied with.
+template <class E, int N, class Word, class Most>
+__device__ __forceinline__ float load_q(const typename E::T *row, bool there, uint32_t head_dim, float scale, h8 q[N],
+                                        Word word_of, Most most_of) {
   typedef typename E::T T;
   typedef T T4 __attribute__((ext_vector_type(4)));
-  T4 x[DP / 32][2];
+  T4 x[N][2];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) {
-    const uint32_t d = DP == 64 ? quad / 2 * 32 + (quad % 2 * 2 + i) * 4 : (i / 4 * 4 + quad) * 32 + i % 4 * 4;
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w = word_of(i), d = w / 4 * 32 + w % 4 * 4;
     x[i][0] = x[i][1] = T4{};
     if (there && d < head_dim) {
       x[i][0] = *(const T4 *)(row + d);
@@ -253,15 +256,15 @@ __device__ __forceinline__ float load_q(const typename E::T *row, bool there, ui
   if constexpr (__is_same(T, __bf16)) {
     float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[i][e / 4][e % 4]));
-    most = max_quad(most);
+    most = most_of(most);
     down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
     scale = ldexpf(scale, down);
   }
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // pairs (0, 2), (16, 18), (1, 3), (17, 19) of the word's elements
@@ -372,8 +375,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, 2
     for (int n = 0; n < NR; ++n) {
       const uint32_t row = t.row0 + n * 16 + col, tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
       pos[n] = t.pos0 + (int32_t)tok;
-      scale[n] = load_q<E, DP>((const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim,
-                               row < t.n_rows, p.head_dim, quad, p.scale_log2, q[n]);
+      scale[n] = load_q<E, DP / 32>(
+          (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row < t.n_rows, p.head_dim,
+          p.scale_log2, q[n], [&](uint32_t i) { return DP == 64 ? quad * 2 + i : (i / 4 * 4 + quad) * 4 + i % 4; }, max_quad);
     }
     const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
     const int32_t pos_first = t.pos0 + (int32_t)by_group(p, t.row0), pos_last = t.pos0 + (int32_t)by_group(p, last);
@@ -558,6 +562,344 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, 2
   }
 }
 
+// 32 rows a wave: prompts and larger chunks.  The waves of a workgroup share
+// tiles of 64 keys, which lie in LDS as f16, two stages of K and V.  Each wave
+// brings its share of the next tile there: codes and scales go to registers a
+// tile ahead, and become f16 a word of eight codes at a time between the
+// products of the present tile's scores, whose matrix instructions leave the
+// vector unit free.
+//
+// In LDS a row is pieces of eight elements in unpack's order, places permuted
+// by the row; queries have that order too, and the answers' is turned back at
+// the end (four_of).
+template <int DP>
+struct Rows32Q4 {
+  static constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;
+  static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
+  static constexpr int kShare = kKeys / kWaves;      // keys that a wave brings
+  static constexpr int kBlocks = DP / 32;            // of a row
+  static constexpr int kMine = 2 * kShare * kBlocks / 64;  // blocks of a lane, K's and V's
+  static constexpr int kLds = 2 * 2 * kTileBytes;
+  static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
+    return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+  }
+};
+
+// A wave's share of the tiles, from memory to f16 in LDS.
+template <int DP>
+struct Bring {
+  typedef Rows32Q4<DP> C;
+  const int32_t *table;
+  const uint8_t *codes[C::kMine], *scales[C::kMine];  // a lane's block of its row in page 0 at place 0
+  uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages;
+  int32_t lo, hi, key0, next_key, next_id[2];
+  uint32_t key[C::kMine];     // a lane's key within the share
+  uint32_t to[C::kMine][4];   // where its words go, from a stage's start
+  bool there[C::kMine];       // the head has that block
+  u4 w[C::kMine];
+  uint16_t d[C::kMine];
+
+  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, uint32_t wave, const Tile &t) {
+    row_bytes = p.head_dim / 2;
+    page_shift = p.page_shift;
+    const uint32_t n_blocks = p.head_dim / kQ4Block;
+    code_bytes = (p.n_kv_heads << page_shift) * row_bytes;
+    scale_bytes = ((p.n_kv_heads * n_blocks) << page_shift) * 2;
+    n_pages = p.n_pages;
+    table = seq_table;
+    lo = t.lo;
+    hi = t.hi;
+#pragma unroll
+    for (int j = 0; j < C::kMine; ++j) {
+      const uint32_t u = j * 64 + lane_id(), block = u % C::kBlocks;
+      const bool is_v = u >= C::kShare * C::kBlocks;
+      key[j] = u / C::kBlocks % C::kShare;
+      there[j] = block < n_blocks;
+      const uint32_t b = there[j] ? block : 0, row = wave * C::kShare + key[j];
+      codes[j] = (const uint8_t *)(is_v ? p.v : p.k) + (uint64_t)(head << page_shift) * row_bytes + b * 16;
+      scales[j] = (const uint8_t *)(is_v ? p.v_scales : p.k_scales) + ((uint64_t)(head * n_blocks + b) << page_shift) * 2;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        to[j][i] = (is_v ? C::kTileBytes : 0) + row * (DP * 2) +
+                   ((block * 4 + i) ^ (is_v ? C::v_swizzle(row) : C::k_swizzle(row))) * 16;
+    }
+  }
+  // Any key will do: page places are cut to those of [lo, hi), which is not
+  // empty; keys outside have no weight.
+  __device__ __forceinline__ void lookup(int32_t first_key) {
+    next_key = first_key;
+    const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      int32_t pg = (first_key + g * 8) >> page_shift;
+      pg = pg > last ? last : (pg < first ? first : pg);
+      next_id[g] = sload(table, (uint32_t)pg);
+    }
+  }
+  // The share last looked up is on its way.
+  __device__ __forceinline__ void load(uint32_t *status) {
+    key0 = next_key;
+    const uint32_t mask = (1u << page_shift) - 1;
+    const bool known0 = (uint32_t)next_id[0] < n_pages, known1 = (uint32_t)next_id[1] < n_pages;
+    if (!(known0 && known1) && lane_id() < 2) {
+      const int32_t k0 = key0 + (int32_t)lane_id() * 8;
+      if (!(lane_id() ? known1 : known0) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
+    }
+    const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[1] : 0;
+#pragma unroll
+    for (int j = 0; j < C::kMine; ++j) {
+      const uint32_t page = key[j] < 8 ? id0 : id1, place = ((uint32_t)key0 + key[j]) & mask;
+      w[j] = *(const u4 *)(codes[j] + (uint64_t)page * code_bytes + place * row_bytes);
+      const uint16_t s = *(const uint16_t *)(scales[j] + (uint64_t)page * scale_bytes + place * 2);
+      // zero where there is no such block or page, and for values that are not finite
+      const bool is_v = j * 64 + lane_id() >= C::kShare * C::kBlocks;
+      const bool gone = !there[j] || !(key[j] < 8 ? known0 : known1) || (is_v && (s & 0x7000u) == 0x7000u);
+      d[j] = gone ? 0 : s;
+    }
+  }
+  // Word i of 4 kMine to the stage at `lds`.
+  __device__ __forceinline__ void word(uint32_t lds, int i) const {
+    const int j = i / 4;
+    const h2 dd = {__builtin_bit_cast(_Float16, d[j]), __builtin_bit_cast(_Float16, d[j])};
+    h2 y[4];
+    unpack(w[j][i % 4], y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] *= dd;
+    *(__attribute__((address_space(3))) h8 *)(uintptr_t)(lds + to[j][i % 4]) = eight(y);
+  }
+};
+
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(AttnQ4Params p) {
+  typedef Rows32Q4<DP> C;
+  typedef typename E::T T;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
+  const uint32_t head = blockIdx.x % p.n_kv_heads;
+  const uint32_t rest = blockIdx.x / p.n_kv_heads;
+  // Chunk by chunk, so that neighbours are alike; late rows, with more keys, first.
+  const uint32_t c = rest / p.n_units, unit = p.n_units - 1 - rest % p.n_units;
+  uint32_t seq, tile;
+  find_unit<C::kRows>(p, unit, &seq, &tile);
+  Tile t;
+  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
+  if (!make_tile<C::kRows>(p, span, tile, &t)) return;
+  uint32_t chunk, n_chunks;
+  chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
+  const int32_t start = t.lo & ~(C::kKeys - 1);
+  if (c >= n_chunks) return;
+  const uint32_t col = lane % 32, half = lane / 32;
+  const uint32_t row = t.row0 + wave * 32 + col;
+  const bool row_ok = row < t.n_rows;
+  const uint32_t tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
+  const int32_t pos = t.pos0 + (int32_t)tok, window = p.window ? (int32_t)p.window : 0x40000000;
+  // the wave's positions; a wave without rows has none (first > last)
+  const uint32_t wrow = t.row0 + wave * 32, wlast = wrow + 31 < t.n_rows ? wrow + 31 : t.n_rows - 1;
+  const bool any = wrow < t.n_rows;
+  const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
+
+  h8 q[DP / 16];
+  float scale = load_q<E, DP / 16>(
+      (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row_ok, p.head_dim,
+      fabsf(p.scale_log2), q, [&](uint32_t i) { return i * 2 + half; }, [](float x) { return fmaxf(x, other_half(x)); });
+  // (not zero, which a masked score must not meet; the scores are zero either way)
+  scale = fmaxf(scale, 0x1p-126f);
+  if (p.scale_log2 < 0) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) q[s] = -q[s];
+  }
+
+  const int32_t begin = start + (int32_t)(c * chunk);
+  int32_t end = begin + (int32_t)chunk;
+  end = end < t.hi ? end : t.hi;
+  const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
+  const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+  Bring<DP> br;
+  br.init(p, p.table + (uint64_t)seq * p.table_stride, head, wave, t);
+  const int32_t my_key = begin + (int32_t)wave * C::kShare;
+  auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
+  constexpr int kWords = 4 * C::kMine;
+
+  // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
+  // dims a product.  V: 16 keys x 32 dims, 4 + 4 keys of a lane in the order
+  // in which the scores lie in their lanes.
+  uint32_t k_lane[DP / 16], v_lane[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) k_lane[d] = col * (DP * 2) + ((d * 2 + half) ^ C::k_swizzle(col)) * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) {
+    const uint32_t r = half * 4 + lane % 16 / 4;
+    v_lane[d] = r * (DP * 2) + ((d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ C::v_swizzle(r)) * 16 + lane % 2 * 8;
+  }
+
+  float m = -__builtin_inff(), l = 0.0f;
+  f16v o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  if (n_tiles > 0) {
+    br.lookup(my_key);
+    br.load(p.status);
+    br.lookup(my_key + C::kKeys);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) br.word(stage(0), i);
+    if (n_tiles > 1) {
+      br.load(p.status);
+      br.lookup(my_key + 2 * C::kKeys);
+    }
+  }
+  for (int32_t i = 0; i < n_tiles; ++i) {
+    const int32_t key0 = begin + i * C::kKeys;
+    const uint32_t kb = stage(i), vb = kb + C::kTileBytes, next = stage(i + 1);
+    const bool more = i + 1 < n_tiles;
+    // the tile is whole, and everyone is done with the other stage
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    auto v_of = [&](int ks, uint32_t at) {
+      s4 x[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
+      return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
+    if (!live) {
+      if (more) {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) br.word(next, w);
+      }
+    } else {
+      f16v s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+      // operands are read a batch ahead of the products
+      constexpr int kBatch = DP == 128 ? 8 : 4, kSteps = DP / 16;
+#pragma unroll
+      for (int d0 = 0; d0 < kSteps; d0 += kBatch) {
+        h8 k[2][kBatch];
+#pragma unroll
+        for (int d = 0; d < kBatch; ++d)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            k[b][d] = *(const __attribute__((address_space(3))) h8 *)(uintptr_t)(kb + k_lane[d0 + d] + b * 32 * (DP * 2));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < kBatch; ++d) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][d], q[d0 + d], s[b], 0, 0, 0);
+          if (more) {
+#pragma unroll
+            for (int w = (d0 + d) * kWords / kSteps; w < (d0 + d + 1) * kWords / kSteps; ++w) br.word(next, w);
+          }
+        }
+      }
+      constexpr int kAhead = DP == 256 ? 1 : 2;
+      h8 v[kAhead][DP / 32];
+#pragma unroll
+      for (int ks = 0; ks < kAhead; ++ks)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
+      __builtin_amdgcn_sched_barrier(0);
+      // From here to the tile's end a wave goes before one that is at its scores.
+      __builtin_amdgcn_s_setprio(1);
+      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
+        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
+            s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
+          }
+      }
+      float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+      mx = fmaxf(mx, other_half(mx)) * scale;
+      // The maximum in use may lag by up to 8 (weights up to 2^8).
+      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx);
+        const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[d] *= a;
+      }
+      const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
+      h8 pr[4];
+      float sums[2] = {0.0f, 0.0f};
+      auto weights = [&](int ks) {
+        f8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
+          sums[e % 2] += x[e];
+        }
+        pr[ks] = __builtin_convertvector(x, h8);
+      };
+      weights(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks + 1 < 4) weights(ks + 1);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[ks % kAhead][d], pr[ks], o[d], 0, 0, 0);
+          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      l += sums[0] + sums[1];
+    }
+    if (i + 2 < n_tiles) {
+      br.load(p.status);
+      br.lookup(my_key + (i + 3) * C::kKeys);
+    }
+  }
+  l += other_half(l);
+  if (n_chunks == 1) {
+    if (row_ok && p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m) + E::kUp);
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    T *op = (T *)p.out + (uint64_t)(t.tok0 + tok) * p.out_stride + (uint64_t)hd * p.head_dim;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        uint32_t at;
+        const f4 x = four_of<E>(f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]} * inv, d, g, half, &at);
+        if (row_ok && at < p.head_dim) *(T4 *)(op + at) = __builtin_convertvector(x, T4);
+      }
+  } else {
+    // A partial sum lies as the accumulators do, so every store is a whole
+    // kilobyte.
+    const uint64_t slot = (uint64_t)(unit * p.n_kv_heads + head) * p.n_chunks + c;
+    float *po = p.part_o + (slot * C::kWaves + wave) * (32 * DP) + lane * 4;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(f4 *)(po + (d * 4 + g) * 256) = f4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+    if (half == 0) *(f2 *)(p.part_ml + ((slot * C::kWaves + wave) * 32 + col) * 2) = f2{m, l};
+  }
+}
+
+template <class E, int DP>
+hipError_t launch32(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  typedef Rows32Q4<DP> C;
+  static std::atomic<uint64_t> devices{0};
+  const hipError_t e = allow_lds((const void *)attn_q4_rows32_kernel<E, DP>, C::kLds, &devices);
+  if (e != hipSuccess) return e;
+  attn_q4_rows32_kernel<E, DP><<<plan.n_wgs, 256, C::kLds, st>>>(p);
+  if (plan.n_chunks > 1) attn_join_kernel<C, E, DP><<<plan.n_units * p.n_kv_heads * C::kWaves, 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+
 template <class E, int DP, int WAVES, int NR>
 hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
   typedef Rows16Q4<DP, WAVES, NR> C;
@@ -570,6 +912,7 @@ hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st)
 
 template <class E, int DP>
 hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
+  if (plan.rows == 128) return launch32<E, DP>(plan, p, st);
   if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
   if constexpr (DP < 256) return launch16<E, DP, 4, 2>(plan, p, st);
   return hipErrorInvalidValue;
