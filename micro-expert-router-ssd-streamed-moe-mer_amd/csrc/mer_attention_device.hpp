@@ -30,6 +30,7 @@ struct F16 {
   // smaller than what 32 others lose).
   static constexpr float kUp = 7.0f;
   static constexpr bool kCodes = false;
+  static constexpr uint32_t kJoinBatch = 16;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -43,6 +44,7 @@ struct BF16 {
   static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
   static constexpr float kUp = 0.0f;
   static constexpr bool kCodes = false;
+  static constexpr uint32_t kJoinBatch = 16;
   static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -285,7 +287,7 @@ __device__ __forceinline__ void join_pieces(const AttnParams &p, const Tile &t, 
                                             uint32_t first_slot, uint32_t c0, uint32_t every, uint32_t n, bool done,
                                             float *lds) {
   typedef typename E::T T;
-  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = DP == 256 ? 8 : 16;
+  constexpr uint32_t kGroups = THREADS / 32, kDims = DP / 32, kBatch = DP == 256 ? E::kJoinBatch / 2 : E::kJoinBatch;
   typedef float fd __attribute__((ext_vector_type(kDims)));
   typedef T td __attribute__((ext_vector_type(kDims)));
   const __amdgpu_buffer_rsrc_t ro = part_rsrc(p.part_o), rm = part_rsrc(p.part_ml);

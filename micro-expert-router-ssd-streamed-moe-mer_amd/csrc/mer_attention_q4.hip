@@ -25,25 +25,34 @@ struct ToF16 {
   typedef h8 V8;
   static constexpr float kUp = 7.0f;
   static constexpr bool kCodes = true;
+  static constexpr uint32_t kJoinBatch = 8;
 };
 struct ToBF16 {
   typedef __bf16 T;
   typedef b8 V8;
   static constexpr float kUp = 7.0f;
   static constexpr bool kCodes = true;
+  static constexpr uint32_t kJoinBatch = 8;
 };
 
 // Eight codes of a word, less 8 each, as f16: (0, 4), (1, 5), (2, 6), (3, 7).
 // An f16 of 1024 + n has n in its last four bits, one of 64 + n in the four
-// above them.
-__device__ __forceinline__ void unpack(uint32_t w, h2 x[4]) {
-  const h2 far = {(_Float16)1032.0f, (_Float16)1032.0f}, near = {(_Float16)72.0f, (_Float16)72.0f};
-  x[0] = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - far;
-  x[1] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - near;
-  w >>= 8;
-  x[2] = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - far;
-  x[3] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - near;
-}
+// above them.  The two exponents are kept in registers: one instruction masks
+// and ors, but it takes no two literals.
+struct Unpack {
+  uint32_t far, near;
+  __device__ __forceinline__ Unpack() : far(0x64006400u), near(0x54005400u) {
+    asm("" : "+v"(far), "+v"(near));
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, h2 x[4]) const {
+    const h2 f = {(_Float16)1032.0f, (_Float16)1032.0f}, n = {(_Float16)72.0f, (_Float16)72.0f};
+    x[0] = __builtin_bit_cast(h2, (w & 0x000f000fu) | far) - f;
+    x[1] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | near) - n;
+    w >>= 8;
+    x[2] = __builtin_bit_cast(h2, (w & 0x000f000fu) | far) - f;
+    x[3] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | near) - n;
+  }
+};
 __device__ __forceinline__ h8 eight(const h2 x[4]) {
   h8 v;
 #pragma unroll
@@ -170,39 +179,37 @@ struct ShareQ4 {
         *(__attribute__((address_space(3))) u4 *)(uintptr_t)(lds + 2 * G::kCodeBytes + i * 16) = u4{0, 0, 0, 0};
   }
 
-  // Lane x's of n words that the whole wave has.
-  template <int N>
-  static __device__ __forceinline__ uint32_t pick(const uint32_t *w, uint32_t x) {
-    uint32_t r = w[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) r = x == (uint32_t)i ? w[i] : r;
-    return r;
+  // The page of group FIRST + x, x < N, where lanes differ in x.
+  template <int FIRST, int N>
+  __device__ __forceinline__ uint32_t page_of(uint32_t x) const {
+    if constexpr (N == 1) {
+      return id[FIRST];
+    } else {
+      const uint32_t lo_half = page_of<FIRST, N / 2>(x), hi_half = page_of<FIRST + N / 2, N / 2>(x);
+      return x & (N / 2) ? hi_half : lo_half;
+    }
   }
 
-  template <bool V>
+  template <bool V, int J>
   __device__ __forceinline__ void copy_codes(uint32_t lds) const {
-    const uint8_t *base = V ? v : k;
-    const uint32_t mask = (1u << page_shift) - 1;
-    if (kPerCopy == 1 || (8u * kPerCopy) >> page_shift <= 1) {
-      // a copy's keys lie in one page
-#pragma unroll
-      for (int j = 0; j < G::kCopies; ++j) {
-        const uint32_t place = (uint32_t)(key0 + j * G::kRows) & mask;
-        async_row16(base + (uint64_t)id[j * kPerCopy] * code_bytes + place * row_bytes, V ? voff[j] : koff[j], lds + j * 1024u);
+    if constexpr (J < G::kCopies) {
+      const uint8_t *base = V ? v : k;
+      const uint32_t mask = (1u << page_shift) - 1, off = V ? voff[J] : koff[J];
+      if (kPerCopy == 1 || (8u * kPerCopy) >> page_shift <= 1) {
+        // a copy's keys lie in one page
+        const uint32_t place = (uint32_t)(key0 + J * G::kRows) & mask;
+        async_row16(base + (uint64_t)id[J * kPerCopy] * code_bytes + place * row_bytes, off, lds + J * 1024u);
+      } else {
+        const uint32_t g = lane_id() / G::kPieces / 8;  // of a copy's groups
+        const uint32_t page = page_of<J * kPerCopy, kPerCopy>(g), place = (uint32_t)(key0 + J * G::kRows + (int32_t)g * 8) & mask;
+        async_row16(base + (uint64_t)page * code_bytes + (place * row_bytes + off - g * 8 * row_bytes), lds + J * 1024u);
       }
-    } else {
-      const uint32_t g = lane_id() / G::kPieces / 8;  // of a copy's groups
-#pragma unroll
-      for (int j = 0; j < G::kCopies; ++j) {
-        const uint32_t page = pick<kPerCopy>(id + j * kPerCopy, g), place = (uint32_t)(key0 + j * G::kRows + (int32_t)g * 8) & mask;
-        const uint32_t in_group = (V ? voff[j] : koff[j]) - g * 8 * row_bytes;
-        async_row16(base + (uint64_t)page * code_bytes + place * row_bytes + in_group, lds + j * 1024u);
-      }
+      copy_codes<V, J + 1>(lds);
     }
   }
   __device__ __forceinline__ void copy_scales(uint32_t lds) const {
     const uint32_t mask = (1u << page_shift) - 1, g = lane_id() % 8;
-    const uint32_t page = pick<kGroups>(id, g), place = (uint32_t)(key0 + (int32_t)g * 8) & mask;
+    const uint32_t page = page_of<0, kGroups>(g), place = (uint32_t)(key0 + (int32_t)g * 8) & mask;
     const uint64_t at = (uint64_t)page * scale_bytes + place * 2;
 #pragma unroll
     for (int j = 0; j < G::kScaleCopies; ++j) {
@@ -211,8 +218,8 @@ struct ShareQ4 {
     }
   }
   __device__ __forceinline__ void copy(uint32_t lds) const {
-    copy_codes<false>(lds);
-    copy_codes<true>(lds + G::kCodeBytes);
+    copy_codes<false, 0>(lds);
+    copy_codes<true, 0>(lds + G::kCodeBytes);
     copy_scales(lds + 2 * G::kCodeBytes);
   }
 };
@@ -294,11 +301,12 @@ struct Rows16Q4 {
 };
 
 template <class E, int DP, int WAVES, int NR>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, 2))) void attn_q4_rows16_kernel(AttnQ4Params p) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_q4_rows16_kernel(AttnQ4Params p) {
   typedef Rows16Q4<DP, WAVES, NR> C;
   typedef TileQ4<DP> G;
   typedef typename E::T T;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const Unpack unpack;
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
   const uint32_t col = lane % 16, quad = lane / 16;
 
@@ -586,43 +594,51 @@ struct Rows32Q4 {
   }
 };
 
-// A wave's share of the tiles, from memory to f16 in LDS.
+// A wave's share of the tiles, from memory to f16 in LDS: 16 keys of K and V.
+// Lanes take a block each, K's and V's of the same keys where a row has four
+// blocks or more; with two, K's are the lower lanes' and V's the upper ones'.
 template <int DP>
 struct Bring {
   typedef Rows32Q4<DP> C;
+  static constexpr bool kSplit = DP == 64;
+  static constexpr int kPlaces = kSplit ? 1 : C::kMine / 2;   // blocks of a lane, of K or of V
+  static constexpr uint32_t kKeysAtOnce = kSplit ? 16 : 64 / C::kBlocks;
   const int32_t *table;
-  const uint8_t *codes[C::kMine], *scales[C::kMine];  // a lane's block of its row in page 0 at place 0
+  const uint8_t *k, *v, *ks, *vs;  // of this head in page 0
   uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages;
   int32_t lo, hi, key0, next_key, next_id[2];
-  uint32_t key[C::kMine];     // a lane's key within the share
-  uint32_t to[C::kMine][4];   // where its words go, from a stage's start
-  bool there[C::kMine];       // the head has that block
+  uint32_t block;                  // a lane's; that of the first where the head has no such block
+  bool there, is_v;                // it has; the lane's are V's (kSplit)
+  uint32_t key;                    // a lane's first
+  uint32_t to[C::kMine];           // where a block's first word goes, from a stage's start
   u4 w[C::kMine];
   uint16_t d[C::kMine];
+  Unpack unpack;
 
   __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, uint32_t wave, const Tile &t) {
     row_bytes = p.head_dim / 2;
     page_shift = p.page_shift;
-    const uint32_t n_blocks = p.head_dim / kQ4Block;
+    const uint32_t n_blocks = p.head_dim / kQ4Block, u = lane_id() % (kSplit ? 32 : 64);
     code_bytes = (p.n_kv_heads << page_shift) * row_bytes;
     scale_bytes = ((p.n_kv_heads * n_blocks) << page_shift) * 2;
     n_pages = p.n_pages;
     table = seq_table;
     lo = t.lo;
     hi = t.hi;
+    k = (const uint8_t *)p.k + (uint64_t)(head << page_shift) * row_bytes;
+    v = (const uint8_t *)p.v + (uint64_t)(head << page_shift) * row_bytes;
+    ks = (const uint8_t *)p.k_scales + ((uint64_t)(head * n_blocks) << page_shift) * 2;
+    vs = (const uint8_t *)p.v_scales + ((uint64_t)(head * n_blocks) << page_shift) * 2;
+    is_v = kSplit && lane_id() >= 32;
+    key = u / C::kBlocks;
+    const uint32_t b = u % C::kBlocks;
+    there = b < n_blocks;
+    block = there ? b : 0;
 #pragma unroll
     for (int j = 0; j < C::kMine; ++j) {
-      const uint32_t u = j * 64 + lane_id(), block = u % C::kBlocks;
-      const bool is_v = u >= C::kShare * C::kBlocks;
-      key[j] = u / C::kBlocks % C::kShare;
-      there[j] = block < n_blocks;
-      const uint32_t b = there[j] ? block : 0, row = wave * C::kShare + key[j];
-      codes[j] = (const uint8_t *)(is_v ? p.v : p.k) + (uint64_t)(head << page_shift) * row_bytes + b * 16;
-      scales[j] = (const uint8_t *)(is_v ? p.v_scales : p.k_scales) + ((uint64_t)(head * n_blocks + b) << page_shift) * 2;
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        to[j][i] = (is_v ? C::kTileBytes : 0) + row * (DP * 2) +
-                   ((block * 4 + i) ^ (is_v ? C::v_swizzle(row) : C::k_swizzle(row))) * 16;
+      const uint32_t row = wave * C::kShare + j % kPlaces * kKeysAtOnce + key;
+      const bool of_v = kSplit ? is_v : j >= kPlaces;
+      to[j] = (of_v ? C::kTileBytes : 0) + row * (DP * 2) + ((b * 4) ^ (of_v ? C::v_swizzle(row) : C::k_swizzle(row))) * 16;
     }
   }
   // Any key will do: page places are cut to those of [lo, hi), which is not
@@ -648,14 +664,23 @@ struct Bring {
     }
     const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[1] : 0;
 #pragma unroll
-    for (int j = 0; j < C::kMine; ++j) {
-      const uint32_t page = key[j] < 8 ? id0 : id1, place = ((uint32_t)key0 + key[j]) & mask;
-      w[j] = *(const u4 *)(codes[j] + (uint64_t)page * code_bytes + place * row_bytes);
-      const uint16_t s = *(const uint16_t *)(scales[j] + (uint64_t)page * scale_bytes + place * 2);
+    for (int i = 0; i < kPlaces; ++i) {
+      const uint32_t at = i * kKeysAtOnce + key, page = at < 8 ? id0 : id1, place = ((uint32_t)key0 + at) & mask;
+      const uint64_t c = (uint64_t)page * code_bytes + (place * row_bytes + block * 16);
+      const uint64_t s = (uint64_t)page * scale_bytes + ((block << page_shift) + place) * 2;
       // zero where there is no such block or page, and for values that are not finite
-      const bool is_v = j * 64 + lane_id() >= C::kShare * C::kBlocks;
-      const bool gone = !there[j] || !(key[j] < 8 ? known0 : known1) || (is_v && (s & 0x7000u) == 0x7000u);
-      d[j] = gone ? 0 : s;
+      const bool gone = !there || !(at < 8 ? known0 : known1);
+      if constexpr (kSplit) {
+        w[i] = *(const u4 *)((is_v ? v : k) + c);
+        const uint16_t x = *(const uint16_t *)((is_v ? vs : ks) + s);
+        d[i] = gone || (is_v && (x & 0x7000u) == 0x7000u) ? 0 : x;
+      } else {
+        w[i] = *(const u4 *)(k + c);
+        w[i + kPlaces] = *(const u4 *)(v + c);
+        const uint16_t x = *(const uint16_t *)(ks + s), y = *(const uint16_t *)(vs + s);
+        d[i] = gone ? 0 : x;
+        d[i + kPlaces] = gone || (y & 0x7000u) == 0x7000u ? 0 : y;
+      }
     }
   }
   // Word i of 4 kMine to the stage at `lds`.
@@ -665,8 +690,8 @@ struct Bring {
     h2 y[4];
     unpack(w[j][i % 4], y);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] *= dd;
-    *(__attribute__((address_space(3))) h8 *)(uintptr_t)(lds + to[j][i % 4]) = eight(y);
+    for (int e = 0; e < 4; ++e) y[e] *= dd;
+    *(__attribute__((address_space(3))) h8 *)(uintptr_t)((lds + to[j]) ^ (uint32_t)(i % 4) * 16) = eight(y);
   }
 };
 
@@ -721,17 +746,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
   constexpr int kWords = 4 * C::kMine;
 
-  // Where a lane reads its operands, from a tile's start.  K: 32 keys x 16
-  // dims a product.  V: 16 keys x 32 dims, 4 + 4 keys of a lane in the order
-  // in which the scores lie in their lanes.
-  uint32_t k_lane[DP / 16], v_lane[DP / 32];
-#pragma unroll
-  for (int d = 0; d < DP / 16; ++d) k_lane[d] = col * (DP * 2) + ((d * 2 + half) ^ C::k_swizzle(col)) * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d) {
-    const uint32_t r = half * 4 + lane % 16 / 4;
-    v_lane[d] = r * (DP * 2) + ((d * 4 + lane / 16 % 2 * 2 + lane % 4 / 2) ^ C::v_swizzle(r)) * 16 + lane % 2 * 8;
-  }
+  // Where a lane reads its first operands, from a tile's start; the others' places
+  // differ in bits of the piece.  K: 32 keys x 16 dims a product.  V: 16 keys x 32
+  // dims, 4 + 4 keys of a lane in the order in which the scores lie in their lanes.
+  const uint32_t k_lane = col * (DP * 2) + (half ^ C::k_swizzle(col)) * 16, v_row = half * 4 + lane % 16 / 4;
+  const uint32_t v_lane = v_row * (DP * 2) + ((lane / 16 % 2 * 2 + lane % 4 / 2) ^ C::v_swizzle(v_row)) * 16 + lane % 2 * 8;
 
   float m = -__builtin_inff(), l = 0.0f;
   f16v o[DP / 32];
@@ -750,117 +769,126 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
       br.lookup(my_key + 2 * C::kKeys);
     }
   }
-  for (int32_t i = 0; i < n_tiles; ++i) {
+  // A tile is whole, and everyone is done with the other stage.
+  auto arrive = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  auto fetch = [&](int32_t i) {
+    if (i < n_tiles) {
+      br.load(p.status);
+      br.lookup(my_key + (i + 1) * C::kKeys);
+    }
+  };
+  // Tiles that no row of this wave sees, before and after the others: it brings
+  // its share of the next one.  (After the last tile words are written once
+  // more, and nobody reads them.)
+  auto pass_by = [&](int32_t i) {
+    arrive();
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) br.word(stage(i + 1), w);
+    fetch(i + 2);
+  };
+  int32_t first_live = pos_first - window + 1, live_end = any && pos_last >= begin ? (pos_last - begin) / C::kKeys + 1 : 0;
+  live_end = (int32_t)uni((uint32_t)(live_end < n_tiles ? live_end : n_tiles));
+  first_live = first_live > begin ? (first_live - begin) / C::kKeys : 0;
+  first_live = (int32_t)uni((uint32_t)(first_live < live_end ? first_live : live_end));
+  int32_t i = 0;
+  for (; i < first_live; ++i) pass_by(i);
+  for (; i < live_end; ++i) {
     const int32_t key0 = begin + i * C::kKeys;
     const uint32_t kb = stage(i), vb = kb + C::kTileBytes, next = stage(i + 1);
-    const bool more = i + 1 < n_tiles;
-    // the tile is whole, and everyone is done with the other stage
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    auto v_of = [&](int ks, uint32_t at) {
+    arrive();
+    auto v_of = [&](int ks, uint32_t d) {
       s4 x[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
         x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4 *)(uintptr_t)(vb + at + (ks * 16 + b * 8) * (DP * 2)));
+            (__attribute__((address_space(3))) s4 *)(uintptr_t)(((vb + v_lane) ^ d * 64) + (ks * 16 + b * 8) * (DP * 2)));
       return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    const bool live = any && key0 <= pos_last && key0 + C::kKeys > pos_first - window + 1;
-    if (!live) {
-      if (more) {
+    f16v s[2];
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) br.word(next, w);
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+    // operands are read a batch ahead of the products
+    constexpr int kBatch = 4, kSteps = DP / 16;
+#pragma unroll
+    for (int d0 = 0; d0 < kSteps; d0 += kBatch) {
+      h8 k[2][kBatch];
+#pragma unroll
+      for (int d = 0; d < kBatch; ++d)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          k[b][d] = *(const __attribute__((address_space(3))) h8 *)(uintptr_t)(((kb + k_lane) ^ (uint32_t)(d0 + d) * 32) + b * 32 * (DP * 2));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < kBatch; ++d) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][d], q[d0 + d], s[b], 0, 0, 0);
+#pragma unroll
+        for (int w = (d0 + d) * kWords / kSteps; w < (d0 + d + 1) * kWords / kSteps; ++w) br.word(next, w);
       }
-    } else {
-      f16v s[2];
+    }
+    constexpr int kAhead = DP == 256 ? 1 : 2;
+    h8 v[kAhead][DP / 32];
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, d);
+    __builtin_amdgcn_sched_barrier(0);
+    // From here to the tile's end a wave goes before one that is at its scores.
+    __builtin_amdgcn_s_setprio(1);
+    if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
+      const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-      // operands are read a batch ahead of the products
-      constexpr int kBatch = DP == 128 ? 8 : 4, kSteps = DP / 16;
-#pragma unroll
-      for (int d0 = 0; d0 < kSteps; d0 += kBatch) {
-        h8 k[2][kBatch];
-#pragma unroll
-        for (int d = 0; d < kBatch; ++d)
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            k[b][d] = *(const __attribute__((address_space(3))) h8 *)(uintptr_t)(kb + k_lane[d0 + d] + b * 32 * (DP * 2));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int d = 0; d < kBatch; ++d) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][d], q[d0 + d], s[b], 0, 0, 0);
-          if (more) {
-#pragma unroll
-            for (int w = (d0 + d) * kWords / kSteps; w < (d0 + d + 1) * kWords / kSteps; ++w) br.word(next, w);
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
+          s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
         }
-      }
-      constexpr int kAhead = DP == 256 ? 1 : 2;
-      h8 v[kAhead][DP / 32];
-#pragma unroll
-      for (int ks = 0; ks < kAhead; ++ks)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) v[ks][d] = v_of(ks, v_lane[d]);
-      __builtin_amdgcn_sched_barrier(0);
-      // From here to the tile's end a wave goes before one that is at its scores.
-      __builtin_amdgcn_s_setprio(1);
-      if (key0 + C::kKeys > pos_first + 1 || key0 + C::kKeys > t.hi || key0 <= pos_last - window) {
-        const int32_t last = pos - key0 - (int32_t)half * 4, before = last - window;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int32_t at = b * 32 + (e / 4) * 8 + e % 4;
-            s[b][e] = at > last || at <= before ? -__builtin_inff() : s[b][e];
-          }
-      }
-      float mx = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
-      mx = fmaxf(mx, other_half(mx)) * scale;
-      // The maximum in use may lag by up to 8 (weights up to 2^8).
-      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
-        const float mn = fmaxf(m, mx);
-        const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= a;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] *= a;
-      }
-      const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
-      h8 pr[4];
-      float sums[2] = {0.0f, 0.0f};
-      auto weights = [&](int ks) {
-        f8 x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
-          sums[e % 2] += x[e];
-        }
-        pr[ks] = __builtin_convertvector(x, h8);
-      };
-      weights(0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks + 1 < 4) weights(ks + 1);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[ks % kAhead][d], pr[ks], o[d], 0, 0, 0);
-          if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, v_lane[d]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      l += sums[0] + sums[1];
     }
-    if (i + 2 < n_tiles) {
-      br.load(p.status);
-      br.lookup(my_key + (i + 3) * C::kKeys);
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+    mx = fmaxf(mx, other_half(mx)) * scale;
+    // The maximum in use may lag by up to 8 (weights up to 2^8).
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
+      const float mn = fmaxf(m, mx);
+      const float a = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] *= a;
     }
+    const float mu = (m == -__builtin_inff() ? 0.0f : m) - E::kUp;
+    h8 pr[4];
+    float sums[2] = {0.0f, 0.0f};
+    auto weights = [&](int ks) {
+      f8 x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
+        sums[e % 2] += x[e];
+      }
+      pr[ks] = __builtin_convertvector(x, h8);
+    };
+    weights(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks + 1 < 4) weights(ks + 1);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[ks % kAhead][d], pr[ks], o[d], 0, 0, 0);
+        if (ks + kAhead < 4) v[ks % kAhead][d] = v_of(ks + kAhead, d);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    l += sums[0] + sums[1];
+    fetch(i + 2);
   }
+  for (; i < n_tiles; ++i) pass_by(i);
   l += other_half(l);
   if (n_chunks == 1) {
     if (row_ok && p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[hd] * kLog2E - (m == -__builtin_inff() ? 0.0f : m) + E::kUp);
