@@ -527,7 +527,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(1, D
       for (int d = 0; d < DP / 16; ++d) *(f4 *)&jo[at * DP + d * 16 + quad * 4] = o[n][d];
     }
     __syncthreads();
-    join_waves<E, DP, C::kWaves, C::kRows>(p, t, head, Piece{first_wg, n_pieces, first_slot, my_slot, epoch}, jo, jm);
+    const Piece piece = {first_wg, n_pieces, first_slot, my_slot, epoch};
+    join_waves<E, DP, C::kWaves, C::kRows>(p, t, head, piece, jo, jm);
+    if (n_pieces > 1) finish_piece<E, DP, C::kWaves, C::kRows>(p, t, head, piece, jo, (uint32_t *)(jm + C::kWaves * C::kRows * 2));
   }
 }
 

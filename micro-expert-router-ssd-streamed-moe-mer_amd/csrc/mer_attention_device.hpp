@@ -84,6 +84,10 @@ __device__ __forceinline__ void async_row16(const uint8_t *src, uint32_t lds) {
 __device__ __forceinline__ void async_row16(const uint8_t *base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
+// The same of four bytes a lane.
+__device__ __forceinline__ void async_word(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
 // The same by the lanes whose offset is not kNone; the others' places stay as
 // they are.  All lanes are on before and after (waves are full and branch as
 // one here).
@@ -261,16 +265,17 @@ __device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, uint32_t index, f
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, x), r, index * 4, 0, kDeviceScope);
 }
 
+// Counts a workgroup in (one thread of it); what the counter stood at.
+__device__ __forceinline__ uint64_t count_in(uint64_t *counter, uint64_t epoch) {
+  (void)__hip_atomic_fetch_max(counter, epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 // True in every thread of the workgroup that comes last.  `epoch`: the launch's,
 // in thread 0; `flag`: a word of LDS.
 __device__ __forceinline__ bool last_piece(uint64_t *counter, uint64_t epoch, uint32_t n_pieces, uint32_t *flag) {
   wait_vm<0>();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    (void)__hip_atomic_fetch_max(counter, epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const uint64_t n = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = attn_is_last(n, n_pieces);
-  }
+  if (threadIdx.x == 0) *flag = attn_is_last(count_in(counter, epoch), n_pieces);
   __syncthreads();
   return *flag != 0;
 }
@@ -396,10 +401,10 @@ struct Piece {
   uint64_t epoch;
 };
 
-// Joins what a workgroup's waves have of a piece, O [wave][row][DP] at jo and
+// Joins what a workgroup's waves have of a piece, O [wave][row][STRIDE] at jo and
 // maxima and sums [wave][row][2] at jm: the answer of a whole unit, or a
-// piece's sums, which the workgroup that comes last joins.
-template <class E, int DP, int WAVES, int ROWS>
+// piece's sums (finish_piece).
+template <class E, int DP, int WAVES, int ROWS, int STRIDE = DP>
 __device__ __forceinline__ void join_waves(const AttnParams &p, const Tile &t, uint32_t head, const Piece &x, float *jo,
                                            float *jm) {
   typedef typename E::V8 V8;
@@ -421,7 +426,7 @@ __device__ __forceinline__ void join_waves(const AttnParams &p, const Tile &t, u
         const float mv = jm[(v * ROWS + r) * 2];
         const float a = mv == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mv - mm);
         ls += a * jm[(v * ROWS + r) * 2 + 1];
-        acc += weigh(*(const f8 *)&jo[(v * ROWS + r) * DP + d], a, pass);
+        acc += weigh(*(const f8 *)&jo[(v * ROWS + r) * STRIDE + d], a, pass);
       }
     };
     add_up(Pass<false>());
@@ -439,27 +444,49 @@ __device__ __forceinline__ void join_waves(const AttnParams &p, const Tile &t, u
       if (d == 0) put2(rm, to * 2, f2{mm, ls});
     }
   }
-  // Many pieces are joined in two steps, sixteen at a time (a unit's counters
-  // do not meet another one's: in each third of them a workgroup begins, or
-  // goes on with, one unit that is cut).  128 pieces (a token over 131,000 keys
-  // of 2 heads of 256): 81 us in one step, 59 us in two; 32 pieces (8000 keys of
-  // 8 heads of 128): 17 us in one, 21 us in two.
-  if (x.n_pieces > 1) {
-    uint32_t *flag = (uint32_t *)(jm + WAVES * ROWS * 2);
-    auto join = [&](uint32_t c0, uint32_t every, uint32_t n, bool done) {
-      join_pieces<E, DP, ROWS, 64 * WAVES>(p, t, head, x.first_wg, x.first_slot, c0, every, n, done, jo);
-    };
-    constexpr uint32_t kJoin = 16;
-    const uint32_t c0 = (blockIdx.x - x.first_wg) / kJoin * kJoin, n = x.n_pieces - c0 < kJoin ? x.n_pieces - c0 : kJoin;
-    uint64_t *const counters = p.counters + kAttnTickets * kAttnTicketWords + x.first_wg;
-    if (x.n_pieces <= 2 * kJoin) {
-      if (last_piece(counters, x.epoch, x.n_pieces, flag)) join(0, 1, x.n_pieces, true);
-    } else if (n == 1 || last_piece(counters + (c0 ? gridDim.x : 0) + c0, x.epoch, n, flag)) {
-      if (n > 1) join(c0, 1, n, false);
-      if (last_piece(counters + 2 * gridDim.x, x.epoch, (x.n_pieces + kJoin - 1) / kJoin, flag))
-        join(0, kJoin, (x.n_pieces + kJoin - 1) / kJoin, true);
-    }
+}
+
+// Many pieces are joined in two steps, sixteen at a time (a unit's counters do
+// not meet another one's: in each third of them a workgroup begins, or goes on
+// with, one unit that is cut).  128 pieces (a token over 131,000 keys of 2 heads
+// of 256): 81 us in one step, 59 us in two; 32 pieces (8000 keys of 8 heads of
+// 128): 17 us in one, 21 us in two.
+constexpr uint32_t kJoin = 16;
+// The pieces that are joined with a workgroup's in the first step: c0 .. c0 + n.
+__device__ __forceinline__ void first_step(const Piece &x, uint32_t *c0, uint32_t *n) {
+  *c0 = 0;
+  *n = x.n_pieces;
+  if (x.n_pieces > 2 * kJoin) {
+    *c0 = (blockIdx.x - x.first_wg) / kJoin * kJoin;
+    *n = x.n_pieces - *c0 < kJoin ? x.n_pieces - *c0 : kJoin;
   }
+}
+__device__ __forceinline__ uint64_t *first_counter(const AttnParams &p, const Piece &x, uint32_t c0) {
+  return p.counters + kAttnTickets * kAttnTicketWords + x.first_wg + (c0 ? gridDim.x : 0) + c0;
+}
+// What the workgroup that comes last of a first step does.  `lds`: [2 WAVES][DP]
+// floats, and a word at `flag`.
+template <class E, int DP, int WAVES, int ROWS>
+__device__ __forceinline__ void join_steps(const AttnParams &p, const Tile &t, uint32_t head, const Piece &x, uint32_t c0,
+                                           uint32_t n, float *lds, uint32_t *flag) {
+  auto join = [&](uint32_t first, uint32_t every, uint32_t count, bool done) {
+    join_pieces<E, DP, ROWS, 64 * WAVES>(p, t, head, x.first_wg, x.first_slot, first, every, count, done, lds);
+  };
+  if (x.n_pieces <= 2 * kJoin) {
+    join(0, 1, x.n_pieces, true);
+  } else {
+    if (n > 1) join(c0, 1, n, false);
+    const uint32_t all = (x.n_pieces + kJoin - 1) / kJoin;
+    if (last_piece(first_counter(p, x, 0) + 2 * gridDim.x, x.epoch, all, flag)) join(0, kJoin, all, true);
+  }
+}
+// Counts a piece of several in, and joins them if it is the last.
+template <class E, int DP, int WAVES, int ROWS>
+__device__ __forceinline__ void finish_piece(const AttnParams &p, const Tile &t, uint32_t head, const Piece &x, float *lds,
+                                             uint32_t *flag) {
+  uint32_t c0, n;
+  first_step(x, &c0, &n);
+  if (n == 1 || last_piece(first_counter(p, x, c0), x.epoch, n, flag)) join_steps<E, DP, WAVES, ROWS>(p, t, head, x, c0, n, lds, flag);
 }
 
 template <int CTRL, int ROWS>

@@ -167,8 +167,15 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
 }
 
 // ---- the cache held in 4 bits (mer_attention_q4.hip) ----
-// It reserves what attn_reserve says, whose least holds the sums of its 16- and
-// 32-row tiles too.
+
+// Floats that a call reserves, as attn_reserve says; up to 16 rows a sequence 34 MB
+// on 256 CUs.
+inline size_t attn_q4_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
+                              size_t max_q_len, size_t max_kv_len, int cus) {
+  const size_t small = 2 * 8 * 16 * (128 + 2) * (size_t)cus;  // of all shapes of the 16- and 32-row tiles
+  const size_t more = attn_reserve(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, cus);
+  return more < small ? small : more;
+}
 
 inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                              size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
@@ -179,8 +186,10 @@ inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uin
   // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
   const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
   if (a.rows <= 32 && small_tiles * (table_keys / 128 + 2) < (1ull << 31)) {
-    a.waves = 4;
-    a.n_wgs = (uint32_t)cus * (head_dim <= 128 ? 2 : 1);
+    // Many units: every wave is a workgroup of its own.
+    const bool narrow = a.rows == 16 && head_dim <= 128 && (uint64_t)n_seqs * n_kv_heads >= 2ull * cus;
+    a.waves = narrow ? 1 : 4;
+    a.n_wgs = (uint32_t)cus * (narrow ? 8 : (head_dim <= 128 ? 2 : 1));
     a.min_granules = 1;
     a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;

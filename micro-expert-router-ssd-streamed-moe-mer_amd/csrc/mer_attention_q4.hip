@@ -75,7 +75,8 @@ struct TileQ4 {
   static constexpr int kCopies = kKeys / kRows;        // of K's codes, and of V's
   static constexpr int kScaleCopies = 2 * kScaleBytes > 1024 ? 2 : 1;  // of both
   static constexpr int kLoads = 2 * kCopies + kScaleCopies;
-  // K: 16 lanes read a piece of the rows 16 q + 4 t + r, q and r from 0 to 3.
+  // K: 16 lanes read a piece of the rows 16 q + 4 t + r, q and r from 0 to 3 (t
+  // does not matter).
   static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) {
     return DP == 64 ? row >> 4 & 1 : (DP == 128 ? row >> 4 & 3 : (row >> 1 & 1) | (row >> 4 & 3) << 1);
   }
@@ -85,26 +86,31 @@ struct TileQ4 {
   }
 };
 
-// Asynchronous copies of a tile by one wave.  Pages are looked up by groups of
-// eight keys, a tile ahead.
-template <int DP>
+// Asynchronous copies of a tile by one wave.  Page ids, one for eight keys, are
+// brought to LDS for eight tiles of the wave at once.
+template <int DP, int WAVES>
 struct ShareQ4 {
   typedef TileQ4<DP> G;
-  static constexpr int kGroups = G::kKeys / 8;
+  static constexpr int kGroups = G::kKeys / 8, kBatch = 64 / kGroups;  // tiles of a batch of ids
   static constexpr int kPerCopy = G::kRows / 8;  // groups of a copy of codes
+  static constexpr uint32_t kAll = (1u << kGroups) - 1;
 
   const uint8_t *k, *v, *ks, *vs;  // of this head in page 0
   uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages, n_blocks;
   const int32_t *table;
-  int32_t lo, hi;
-  int32_t key0, next_key;
+  int32_t lo, hi, first_key;        // keys that count; the wave's first tile
+  uint32_t ids;                     // LDS: two batches of 64 ids
+  int32_t key0;
+  uint32_t mine;                    // the page of a lane's group, lane % 8
   uint32_t id[kGroups];
-  int32_t next_id[kGroups];
   uint32_t known;                   // groups of pages that the cache has, a bit each
   uint32_t koff[G::kCopies], voff[G::kCopies];  // a lane's piece, from its copy's first row
   uint32_t soff[G::kScaleCopies];   // a lane's scales, from its group's (kNone: beyond the head)
 
-  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, const Tile &t) {
+  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, const Tile &t,
+                                       int32_t first_tile, uint32_t ids_lds) {
+    first_key = first_tile;
+    ids = ids_lds;
     row_bytes = p.head_dim / 2;
     n_blocks = p.head_dim / kQ4Block;
     page_shift = p.page_shift;
@@ -135,33 +141,31 @@ struct ShareQ4 {
     }
   }
 
-  // Any key will do: page places are cut to those of [lo, hi), which is not
-  // empty; keys outside have no weight.
-  __device__ __forceinline__ void lookup(int32_t key) {
-    next_key = key;
+  __device__ __forceinline__ int32_t key_of(int32_t tile) const { return first_key + tile * (WAVES * G::kKeys); }
+  // The ids of tiles kBatch * batch .. on their way.  Page places are cut to
+  // those of [lo, hi), which is not empty; keys outside have no weight.
+  __device__ __forceinline__ void lookup(int32_t batch) const {
+    const int32_t key = key_of(batch * kBatch + (int32_t)(lane_id() / kGroups)) + (int32_t)(lane_id() % kGroups) * 8;
     const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      int32_t pg = (key + g * 8) >> page_shift;
-      pg = pg > last ? last : (pg < first ? first : pg);
-      next_id[g] = sload(table, (uint32_t)pg);
-    }
+    int32_t pg = key >> page_shift;
+    pg = pg > last ? last : (pg < first ? first : pg);
+    async_word(table + pg, ids + (uint32_t)(batch & 1) * 256);
   }
-
-  // On to the tile last looked up, before its copies.
-  __device__ __forceinline__ void advance(uint32_t *status) {
-    key0 = next_key;
-    known = 0;
+  // On to a tile whose ids are there, before its copies; a batch ahead of need
+  // the next ids are sent for.
+  __device__ __forceinline__ void advance(int32_t tile, uint32_t *status) {
+    key0 = key_of(tile);
+    const uint32_t at = ids + (uint32_t)(tile & (2 * kBatch - 1)) * (kGroups * 4) + lane_id() % kGroups * 4;
+    const uint32_t page = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)at;
+    mine = page < n_pages ? page : 0;
+    known = (uint32_t)__builtin_amdgcn_ballot_w64(page < n_pages) & kAll;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const bool is = (uint32_t)next_id[g] < n_pages;
-      id[g] = is ? (uint32_t)next_id[g] : 0;
-      known |= is ? 1u << g : 0u;
-    }
-    if (known != (1u << kGroups) - 1 && lane_id() < kGroups) {
+    for (int g = 0; g < kGroups; ++g) id[g] = (uint32_t)__builtin_amdgcn_readlane((int)mine, g);
+    if (known != kAll && lane_id() < kGroups) {
       const int32_t k0 = key0 + (int32_t)lane_id() * 8;
       if (!(known >> lane_id() & 1) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
     }
+    if ((tile & (kBatch - 1)) == kBatch / 2) lookup(tile / kBatch + 1);
   }
 
   // Zero scales for the blocks that a padded head has not, in a tile's place.
@@ -173,21 +177,10 @@ struct ShareQ4 {
   }
   // Zero scales for the keys of unknown pages, once the tile is there.
   __device__ __forceinline__ void clear_unknown(uint32_t lds, uint32_t tile_known) const {
-    if (tile_known == (1u << kGroups) - 1) return;
+    if (tile_known == kAll) return;
     for (uint32_t i = lane_id(); i < 2 * G::kPieces * 8; i += 64)
       if (!(tile_known >> i % 8 & 1))
         *(__attribute__((address_space(3))) u4 *)(uintptr_t)(lds + 2 * G::kCodeBytes + i * 16) = u4{0, 0, 0, 0};
-  }
-
-  // The page of group FIRST + x, x < N, where lanes differ in x.
-  template <int FIRST, int N>
-  __device__ __forceinline__ uint32_t page_of(uint32_t x) const {
-    if constexpr (N == 1) {
-      return id[FIRST];
-    } else {
-      const uint32_t lo_half = page_of<FIRST, N / 2>(x), hi_half = page_of<FIRST + N / 2, N / 2>(x);
-      return x & (N / 2) ? hi_half : lo_half;
-    }
   }
 
   template <bool V, int J>
@@ -201,7 +194,10 @@ struct ShareQ4 {
         async_row16(base + (uint64_t)id[J * kPerCopy] * code_bytes + place * row_bytes, off, lds + J * 1024u);
       } else {
         const uint32_t g = lane_id() / G::kPieces / 8;  // of a copy's groups
-        const uint32_t page = page_of<J * kPerCopy, kPerCopy>(g), place = (uint32_t)(key0 + J * G::kRows + (int32_t)g * 8) & mask;
+        uint32_t page = id[J * kPerCopy];
+        if constexpr (kPerCopy > 1) page = g & 1 ? id[J * kPerCopy + 1] : page;
+        if constexpr (kPerCopy > 2) page = g & 2 ? (g & 1 ? id[J * kPerCopy + 3] : id[J * kPerCopy + 2]) : page;
+        const uint32_t place = (uint32_t)(key0 + J * G::kRows + (int32_t)g * 8) & mask;
         async_row16(base + (uint64_t)page * code_bytes + (place * row_bytes + off - g * 8 * row_bytes), lds + J * 1024u);
       }
       copy_codes<V, J + 1>(lds);
@@ -209,8 +205,7 @@ struct ShareQ4 {
   }
   __device__ __forceinline__ void copy_scales(uint32_t lds) const {
     const uint32_t mask = (1u << page_shift) - 1, g = lane_id() % 8;
-    const uint32_t page = page_of<0, kGroups>(g), place = (uint32_t)(key0 + (int32_t)g * 8) & mask;
-    const uint64_t at = (uint64_t)page * scale_bytes + place * 2;
+    const uint64_t at = (uint64_t)mine * scale_bytes + ((uint32_t)(key0 + (int32_t)g * 8) & mask) * 2;
 #pragma unroll
     for (int j = 0; j < G::kScaleCopies; ++j) {
       const bool is_v = j * 64 + lane_id() >= G::kPieces * 8;
@@ -243,7 +238,9 @@ __device__ __forceinline__ u4 tame(u4 x) {
 // A row's queries as N operands of eight dims each, in the order in which
 // unpack leaves a word of codes: operand i is word `word_of(i)` of a row's codes,
 // four to a block.  `most_of`: the maximum over the lanes that have the row.
-// Returns what its scores are to be multiplied with.
+// Returns what its scores are to be multiplied with, which is positive: q takes
+// the scale's sign, and 2^-126 stands for less (a masked score must not meet a
+// zero; the others are zero either way).
 template <class E, int N, class Word, class Most>
 __device__ __forceinline__ float load_q(const typename E::T *row, bool there, uint32_t head_dim, float scale, h8 q[N],
                                         Word word_of, Most most_of) {
@@ -268,7 +265,6 @@ __device__ __forceinline__ float load_q(const typename E::T *row, bool there, ui
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[i][e / 4][e % 4]));
     most = most_of(most);
     down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
-    scale = ldexpf(scale, down);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -279,7 +275,11 @@ __device__ __forceinline__ float load_q(const typename E::T *row, bool there, ui
       if constexpr (__is_same(T, __bf16)) q[i][e] = (_Float16)ldexpf((float)y, -down);
       else q[i][e] = y;
     }
-  return scale;
+  if (scale < 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = -q[i];
+  }
+  return fmaxf(ldexpf(fabsf(scale), down), 0x1p-126f);
 }
 
 // Up to 16 or 32 rows of a group a sequence; the work is cut as in
@@ -296,8 +296,12 @@ template <int DP, int WAVES, int NR>
 struct Rows16Q4 {
   typedef TileQ4<DP> G;
   static constexpr int kWaves = WAVES, kRows = 16 * NR, kKeys = 64, kGranule = 128, kStages = 2;
-  static constexpr int kRing = WAVES * kStages * G::kBytes, kJoin = WAVES * kRows * (DP + 2) * 4 + 16;
-  static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kStride = DP + 4;  // of a row of the waves' sums
+  static constexpr int kRing = WAVES * kStages * G::kBytes, kWaveSums = WAVES * kRows * (kStride + 2) * 4;
+  static constexpr int kIds = kRing > kWaveSums ? kRing : kWaveSums;  // beside the ring: [WAVES][2][64]
+  static constexpr int kPieceSums = kIds + WAVES * 512;               // [2 WAVES][DP]
+  static constexpr int kFlag = kPieceSums + 2 * WAVES * DP * 4;
+  static constexpr int kLds = kFlag + 16;
 };
 
 template <class E, int DP, int WAVES, int NR>
@@ -310,21 +314,19 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = uni(tid / 64);
   const uint32_t col = lane % 16, quad = lane / 16;
 
-  // where a lane reads its operands, from a tile's start
-  uint32_t k_lane[4][DP / 128 ? DP / 128 : 1], v_lane[G::kPieces];
+  // Where a lane reads its operands, from a tile's start.  K: product t's are 4 t
+  // rows on, in the same place of their rows.  V: those of block b differ in bits
+  // of the piece.
+  const uint32_t k_row = col / 4 * 16 + col % 4;
+  uint32_t k_lane[DP / 128 ? DP / 128 : 1];
+  if constexpr (DP == 64) {
+    k_lane[0] = k_row * G::kRowBytes + ((quad / 2) ^ G::k_swizzle(k_row)) * 16 + quad % 2 * 8;
+  } else {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t row = col / 4 * 16 + t * 4 + col % 4;
-    if constexpr (DP == 64) {
-      k_lane[t][0] = row * G::kRowBytes + ((quad / 2) ^ G::k_swizzle(row)) * 16 + quad % 2 * 8;
-    } else {
-#pragma unroll
-      for (int c = 0; c < DP / 128; ++c) k_lane[t][c] = row * G::kRowBytes + ((c * 4 + quad) ^ G::k_swizzle(row)) * 16;
-    }
+    for (int c = 0; c < DP / 128; ++c) k_lane[c] = k_row * G::kRowBytes + ((c * 4 + quad) ^ G::k_swizzle(k_row)) * 16;
   }
   const uint32_t v_row = quad * 16 + (col & 8) + (col & 3) * 2 + (col >> 2 & 1);
-#pragma unroll
-  for (int b = 0; b < G::kPieces; ++b) v_lane[b] = G::kCodeBytes + v_row * G::kRowBytes + (b ^ G::v_swizzle(v_row)) * 16;
+  const uint32_t v_lane = G::kCodeBytes + v_row * G::kRowBytes + G::v_swizzle(v_row) * 16;
   const uint32_t ks_lane = 2 * G::kCodeBytes + (DP == 64 ? quad / 2 : quad) * (G::kKeys * 2) + (col / 4 * 16 + col % 4) * 2;
   const uint32_t vs_lane = 2 * G::kCodeBytes + G::kScaleBytes + quad * 32;
 
@@ -350,30 +352,79 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   uint32_t x = blockIdx.x * per;
   const uint32_t x1 = all - (all < x ? all : x) < per ? all : x + per;
   bool first_piece = true;
-  while (x < x1) {
-    uint32_t seq, before;
-    Span span;
-    if (!gr.template find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
-    int32_t start = 0;
-    const uint32_t n_gran = uni(Gr::template granules<C::kGranule>(p, span, &start));
-    const uint32_t unit = uni((x - before) / n_gran), tile = uni(by_heads(p, unit)), head = unit - tile * p.n_kv_heads;
-    const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
-    const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
-    // the unit's pieces: workgroups first_wg .. first_wg + n_pieces - 1
-    const uint32_t first_wg = g0 == 0 ? blockIdx.x : (per == 1 ? unit0 : uni(unit0 / per));
-    const uint32_t last_wg = g0 + count == n_gran ? blockIdx.x : (per == 1 ? unit0 + n_gran - 1 : uni((unit0 + n_gran - 1) / per));
-    const uint32_t n_pieces = last_wg - first_wg + 1;
-    const uint32_t first_slot = 2 * first_wg + (first_wg * per == unit0 ? 0 : 1);
-    const uint32_t my_slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
-    first_piece = false;
-    x += count;
-    Tile t;
-    // (spans that overlap, past 2^32, or lengths that change under the kernel)
-    if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads || last_wg >= gridDim.x) return;
-    start = (int32_t)uni((uint32_t)start);
-    int32_t begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
-    if (p.window && begin < (t.lo & ~(C::kKeys - 1))) begin = t.lo & ~(C::kKeys - 1);
-    end = end < t.hi ? end : t.hi;
+  // A unit that is cut is joined by who comes last, while the first tiles of its
+  // next piece are on their way.
+  Tile old_t{};
+  uint32_t old_head = 0;
+  Piece old{0, 0, 0, 0, epoch};
+  uint64_t counted = 0;  // in thread 0: what the old piece's counter stood at
+  for (;;) {
+    const bool more = x < x1;
+    Tile t{};
+    uint32_t head = 0, seq = 0;
+    Piece piece{0, 0, 0, 0, epoch};
+    int32_t begin = 0, end = 0;
+    if (more) {
+      uint32_t before;
+      Span span;
+      if (!gr.template find<C::kGranule, C::kRows>(p, x, &seq, &before, &span)) return;
+      int32_t start = 0;
+      const uint32_t n_gran = uni(Gr::template granules<C::kGranule>(p, span, &start));
+      const uint32_t unit = uni((x - before) / n_gran), tile = uni(by_heads(p, unit));
+      head = unit - tile * p.n_kv_heads;
+      const uint32_t unit0 = before + unit * n_gran, g0 = x - unit0;
+      const uint32_t count = n_gran - g0 < x1 - x ? n_gran - g0 : x1 - x;
+      // the unit's pieces: workgroups first_wg .. first_wg + n_pieces - 1
+      const uint32_t first_wg = g0 == 0 ? blockIdx.x : (per == 1 ? unit0 : uni(unit0 / per));
+      const uint32_t last_wg = g0 + count == n_gran ? blockIdx.x : (per == 1 ? unit0 + n_gran - 1 : uni((unit0 + n_gran - 1) / per));
+      piece.first_wg = first_wg;
+      piece.n_pieces = last_wg - first_wg + 1;
+      piece.first_slot = 2 * first_wg + (first_wg * per == unit0 ? 0 : 1);
+      piece.my_slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+      first_piece = false;
+      x += count;
+      // (spans that overlap, past 2^32, or lengths that change under the kernel)
+      if (!make_tile<C::kRows>(p, span, tile, &t) || head >= p.n_kv_heads || last_wg >= gridDim.x) return;
+      start = (int32_t)uni((uint32_t)start);
+      begin = start + (int32_t)(g0 * C::kGranule), end = begin + (int32_t)(count * C::kGranule);
+      if (p.window && begin < (t.lo & ~(C::kKeys - 1))) begin = t.lo & ~(C::kKeys - 1);
+      end = end < t.hi ? end : t.hi;
+    }
+    const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
+    const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+    const uint32_t ring = lds + wave * (C::kStages * G::kBytes);
+    auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * G::kBytes; };
+    ShareQ4<DP, WAVES> sh;
+    if (more) {
+      sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t, begin + (int32_t)wave * C::kKeys, lds + C::kIds + wave * 512);
+      if (mine > 0) sh.lookup(0);
+    }
+    const bool cut = old.n_pieces > 1;
+    uint32_t c0, n_joined;
+    first_step(old, &c0, &n_joined);
+    uint32_t *const flag = (uint32_t *)(smem + C::kFlag);
+    if (cut && tid == 0) *flag = n_joined == 1 || attn_is_last(counted, n_joined);
+    wait_vm<0>();     // the ids
+    __syncthreads();  // the flag
+    uint32_t known[C::kStages] = {};
+    if (more) {
+      for (int32_t i = 0; i < C::kStages; ++i) sh.clear_pads(slot_of(i));
+      wait_lds();
+#pragma unroll
+      for (int i = 0; i < C::kStages; ++i)
+        if (i < mine) {
+          sh.advance(i, p.status);
+          known[i] = sh.known;
+          sh.copy(slot_of(i));
+        }
+    }
+    if (cut && *flag)
+      join_steps<E, DP, C::kWaves, C::kRows>(p, old_t, old_head, old, c0, n_joined, (float *)(smem + C::kPieceSums), flag);
+    if (!more) break;
+    old_t = t;
+    old_head = head;
+    old = piece;
 
     const int32_t window = p.window ? (int32_t)p.window : 0x40000000;
     h8 q[NR][DP / 32];
@@ -389,32 +440,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
     const int32_t pos_first = t.pos0 + (int32_t)by_group(p, t.row0), pos_last = t.pos0 + (int32_t)by_group(p, last);
-
-    const int32_t n_tiles = end > begin ? (end - begin + C::kKeys - 1) / C::kKeys : 0;
-    const int32_t mine = n_tiles > (int32_t)wave ? (n_tiles - (int32_t)wave + C::kWaves - 1) / C::kWaves : 0;
-    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + wave * (C::kStages * G::kBytes);
-    auto key_of = [&](int32_t i) { return begin + (i * C::kWaves + (int32_t)wave) * C::kKeys; };
-    auto slot_of = [&](int32_t i) { return ring + (uint32_t)(i & 1) * G::kBytes; };
-    __syncthreads();  // the last piece is done with the LDS
-    ShareQ4<DP> sh;
-    sh.init(p, p.table + (uint64_t)seq * p.table_stride, head, t);
-    if (mine > 0) sh.lookup(key_of(0));
-    for (int32_t i = 0; i < C::kStages; ++i) sh.clear_pads(slot_of(i));
-    wait_lds();
-    // q has to be there before the first copy goes out: a later wait for it,
-    // which the compiler would put into the loop, would drain the copies.
+    // A wait for q that the compiler would put into the loop would drain the
+    // copies there; here the first ones are due anyway.
     __builtin_amdgcn_s_waitcnt(kWaitVm0);
     float m[NR], l[NR];
     f4 o[NR][DP / 16];
-    uint32_t known[C::kStages] = {};
-#pragma unroll
-    for (int i = 0; i < C::kStages; ++i)
-      if (i < mine) {
-        sh.advance(p.status);
-        known[i] = sh.known;
-        sh.lookup(key_of(i + 1));
-        sh.copy(slot_of(i));
-      }
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       m[n] = -__builtin_inff();
@@ -423,7 +453,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       for (int d = 0; d < DP / 16; ++d) o[n][d] = f4{0, 0, 0, 0};
     }
     for (int32_t i = 0; i < mine; ++i) {
-      const int32_t left = mine - i, key0 = key_of(i);
+      const int32_t left = mine - i, key0 = sh.key_of(i);
       const uint32_t at = slot_of(i);
       if (left == 1) wait_vm<0>();
       else wait_vm<G::kLoads>();
@@ -438,10 +468,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         for (int c = 0; c < (DP > 64 ? DP / 128 : 1); ++c) {
           uint32_t w[4];
           if constexpr (DP == 64) {
-            const u2 y = *(const __attribute__((address_space(3))) u2 *)(uintptr_t)(at + k_lane[tt][0]);
+            const u2 y = *(const __attribute__((address_space(3))) u2 *)(uintptr_t)(at + k_lane[0] + tt * 4 * G::kRowBytes);
             w[0] = y[0], w[1] = y[1];
           } else {
-            const u4 y = *(const __attribute__((address_space(3))) u4 *)(uintptr_t)(at + k_lane[tt][c]);
+            const u4 y = *(const __attribute__((address_space(3))) u4 *)(uintptr_t)(at + k_lane[c] + tt * 4 * G::kRowBytes);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = y[j];
           }
@@ -479,7 +509,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       for (int n = 0; n < NR; ++n) {
         float z[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = s[n][e / 4][e % 4] * scale[n];
+        for (int e = 0; e < 16; ++e) z[e] = s[n][e / 4][e % 4];
         if (partial) {
           const int32_t last_key = pos[n] - key0 - (int32_t)quad * 16, before_key = last_key - window;
 #pragma unroll
@@ -488,7 +518,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         float mx = z[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
-        mx = max_quad(mx);
+        mx = max_quad(mx) * scale[n];
         // The maximum in use may lag by up to 8 (weights up to 2^8).
         if (__builtin_amdgcn_ballot_w64(mx > m[n] + 8.0f)) {
           const float mn = fmaxf(m[n], mx);
@@ -502,7 +532,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          z[e] = __builtin_amdgcn_exp2f(z[e] - mu);
+          z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], scale[n], -mu));
           sum += z[e];
         }
         l[n] += sum;
@@ -523,7 +553,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              (__attribute__((address_space(3))) v2i *)(uintptr_t)(at + v_lane[b] + hh * 8));
+              (__attribute__((address_space(3))) v2i *)(uintptr_t)(((at + v_lane) ^ (uint32_t)b * 16) + hh * 8));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             h2 y[4];
@@ -541,16 +571,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int j = 0; j + 1 < C::kStages; ++j) known[j] = known[j + 1];
       if (left > C::kStages) {
-        sh.advance(p.status);
+        sh.advance(i + C::kStages, p.status);
         known[C::kStages - 1] = sh.known;
-        sh.lookup(key_of(i + C::kStages + 1));
         sh.copy(at);
       }
     }
     // join the waves: m, l and O of each in LDS
     __syncthreads();
-    float *jo = (float *)smem;                      // [wave][row][DP]
-    float *jm = jo + C::kWaves * C::kRows * DP;     // [wave][row][2]
+    float *jo = (float *)smem;                         // [wave][row][kStride]
+    float *jm = jo + C::kWaves * C::kRows * C::kStride;  // [wave][row][2]
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const uint32_t r = wave * C::kRows + n * 16 + col;
@@ -560,13 +589,20 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       // of half a block
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
-        float *to = &jo[r * DP + d / 2 * 32 + d % 2 * 8 + quad * 2];
+        float *to = &jo[r * C::kStride + d / 2 * 32 + d % 2 * 8 + quad * 2];
         *(f2 *)to = f2{o[n][d][0], o[n][d][2]};
         *(f2 *)(to + 16) = f2{o[n][d][1], o[n][d][3]};
       }
     }
     __syncthreads();
-    join_waves<E, DP, C::kWaves, C::kRows>(p, t, head, Piece{first_wg, n_pieces, first_slot, my_slot, epoch}, jo, jm);
+    join_waves<E, DP, C::kWaves, C::kRows, C::kStride>(p, t, head, piece, jo, jm);
+    if (piece.n_pieces > 1) wait_vm<0>();  // this wave's sums are out
+    __syncthreads();                       // everyone's, and the ring is free
+    if (piece.n_pieces > 1 && tid == 0) {
+      uint32_t c, n;
+      first_step(piece, &c, &n);
+      if (n > 1) counted = count_in(first_counter(p, piece, c), epoch);
+    }
   }
 }
 
@@ -725,15 +761,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
   const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
 
   h8 q[DP / 16];
-  float scale = load_q<E, DP / 16>(
+  const float scale = load_q<E, DP / 16>(
       (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row_ok, p.head_dim,
-      fabsf(p.scale_log2), q, [&](uint32_t i) { return i * 2 + half; }, [](float x) { return fmaxf(x, other_half(x)); });
-  // (not zero, which a masked score must not meet; the scores are zero either way)
-  scale = fmaxf(scale, 0x1p-126f);
-  if (p.scale_log2 < 0) {
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) q[s] = -q[s];
-  }
+      p.scale_log2, q, [&](uint32_t i) { return i * 2 + half; }, [](float x) { return fmaxf(x, other_half(x)); });
 
   const int32_t begin = start + (int32_t)(c * chunk);
   int32_t end = begin + (int32_t)chunk;
@@ -941,6 +971,8 @@ hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st)
 template <class E, int DP>
 hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
   if (plan.rows == 128) return launch32<E, DP>(plan, p, st);
+  if constexpr (DP < 256)
+    if (plan.rows == 16 && plan.waves == 1) return launch16<E, DP, 1, 1>(plan, p, st);
   if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
   if constexpr (DP < 256) return launch16<E, DP, 4, 2>(plan, p, st);
   return hipErrorInvalidValue;

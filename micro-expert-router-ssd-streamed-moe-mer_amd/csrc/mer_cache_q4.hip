@@ -253,41 +253,38 @@ hipError_t launch_append(AppendQ4Params p, int cus, hipStream_t st) {
   return hipGetLastError();
 }
 
-// A thread has eight bytes of codes, half a block: elements 8h .. 8h + 7 in
-// their low halves and 16 + 8h .. in their high ones.
+// A thread makes eight elements: a block's quarter q has the low (q < 2) or high
+// halves of eight bytes of its codes, which two threads load, so that a wave's
+// stores lie side by side.
 template <int OUT>
 __global__ __launch_bounds__(256) void read_q4_kernel(ReadQ4Params p) {
   typedef typename Elem<OUT>::V8 V8;
   typedef typename Elem<OUT>::T T;
-  const uint32_t head_dim = p.cache.head_dim, heads = p.cache.heads, halves = head_dim / 16, per_row = heads * halves;
+  const uint32_t head_dim = p.cache.head_dim, heads = p.cache.heads, quarters = head_dim / 8, per_row = heads * quarters;
   const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / per_row;
   if (row >= p.n_rows) return;
-  const uint32_t at = i - row * per_row, head = at / halves, half = at - head * halves;
+  const uint32_t at = i - row * per_row, head = at / quarters, quarter = at - head * quarters, q = quarter % 4;
   const int64_t slot = p.slots[row];
   const bool there = (uint64_t)slot < p.cache.n_slots;
   if (!there && slot >= 0 && at == 0 && blockIdx.y == 0) atomicCAS(p.status, 0u, (uint32_t)MER_ERR_RESIDENCY_MISS);
-  f8 a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a;
+  f8 a = {0, 0, 0, 0, 0, 0, 0, 0};
   if (there) {
     const uint64_t page = (uint64_t)slot >> p.cache.page_shift, off = (uint64_t)slot & ((1u << p.cache.page_shift) - 1);
     const uint64_t unit = page * heads + head;
-    const u2 c = *(const u2 *)(p.cache.codes[blockIdx.y] + ((unit << p.cache.page_shift) + off) * (head_dim / 2) + half * 8);
+    const u2 c = *(const u2 *)(p.cache.codes[blockIdx.y] + ((unit << p.cache.page_shift) + off) * (head_dim / 2) +
+                               quarter / 4 * 16 + q % 2 * 8);
     const float d = (float)__builtin_bit_cast(
-        _Float16, p.cache.scales[blockIdx.y][((unit * (halves / 2) + half / 2) << p.cache.page_shift) + off]);
+        _Float16, p.cache.scales[blockIdx.y][((unit * (quarters / 4) + quarter / 4) << p.cache.page_shift) + off]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t byte = c[e / 4] >> e % 4 * 8;
-      a[e] = (float)((int32_t)(byte & 15) - 8) * d;
-      b[e] = (float)((int32_t)(byte >> 4 & 15) - 8) * d;
-    }
+    for (int e = 0; e < 8; ++e) a[e] = (float)((int32_t)(c[e / 4] >> (e % 4 * 8 + q / 2 * 4) & 15) - 8) * d;
   }
-  T *out = (T *)p.out[blockIdx.y] + (uint64_t)row * p.out_stride[blockIdx.y] + head * head_dim + half / 2 * kQ4Block + half % 2 * 8;
-  *(V8 *)out = __builtin_convertvector(a, V8);
-  *(V8 *)(out + 16) = __builtin_convertvector(b, V8);
+  *(V8 *)((T *)p.out[blockIdx.y] + (uint64_t)row * p.out_stride[blockIdx.y] + head * head_dim + quarter * 8) =
+      __builtin_convertvector(a, V8);
 }
 
 template <int OUT>
 hipError_t launch_read(const ReadQ4Params &p, hipStream_t st) {
-  const uint64_t threads = (uint64_t)p.n_rows * p.cache.heads * (p.cache.head_dim / 16);
+  const uint64_t threads = (uint64_t)p.n_rows * p.cache.heads * (p.cache.head_dim / 8);
   read_q4_kernel<OUT><<<dim3((uint32_t)((threads + 255) / 256), 2), 256, 0, st>>>(p);
   return hipGetLastError();
 }
