@@ -1797,7 +1797,7 @@ int mer_hip_kv_read_q4(const mer_kv_cache_q4 *cache, int out_type, size_t n_rows
   p.out_stride[1] = v_stride;
   p.n_rows = (uint32_t)n_rows;
   p.status = g_dev[g_device].status;
-  const hipError_t e = launch_read_q4(out_type, p, (hipStream_t)stream);
+  const hipError_t e = launch_read_q4(out_type, p, g_dev[g_device].cus, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, MER_ERR_SUBMISSION, "cache read launch");
   return MER_OK;
 }

@@ -102,7 +102,7 @@ struct ReadQ4Params {
   uint32_t *status;
 };
 hipError_t launch_append_q4(int in_type, const AppendQ4Params &p, int cus, hipStream_t st);
-hipError_t launch_read_q4(int out_type, const ReadQ4Params &p, hipStream_t st);
+hipError_t launch_read_q4(int out_type, const ReadQ4Params &p, int cus, hipStream_t st);
 
 void set_reciprocals(AttnParams *p);
 hipError_t launch_attention(int type, const AttnPlan &plan, const AttnParams &p, hipStream_t st);
