@@ -237,50 +237,57 @@ __device__ __forceinline__ u4 tame(u4 x) {
 
 // A row's queries as N operands of eight dims each, in the order in which
 // unpack leaves a word of codes: operand i is word `word_of(i)` of a row's codes,
-// four to a block.  `most_of`: the maximum over the lanes that have the row.
-// Returns what its scores are to be multiplied with, which is positive: q takes
-// the scale's sign, and 2^-126 stands for less (a masked score must not meet a
-// zero; the others are zero either way).
-template <class E, int N, class Word, class Most>
-__device__ __forceinline__ float load_q(const typename E::T *row, bool there, uint32_t head_dim, float scale, h8 q[N],
-                                        Word word_of, Most most_of) {
+// four to a block.  They are sent for (load) before they are needed (operands).
+template <class E, int N>
+struct Queries {
   typedef typename E::T T;
   typedef T T4 __attribute__((ext_vector_type(4)));
   T4 x[N][2];
+
+  template <class Word>
+  __device__ __forceinline__ void load(const T *row, bool there, uint32_t head_dim, Word word_of) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t w = word_of(i), d = w / 4 * 32 + w % 4 * 4;
-    x[i][0] = x[i][1] = T4{};
-    if (there && d < head_dim) {
-      x[i][0] = *(const T4 *)(row + d);
-      x[i][1] = *(const T4 *)(row + d + 16);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t w = word_of(i), d = w / 4 * 32 + w % 4 * 4;
+      x[i][0] = x[i][1] = T4{};
+      if (there && d < head_dim) {
+        x[i][0] = *(const T4 *)(row + d);
+        x[i][1] = *(const T4 *)(row + d + 16);
+      }
     }
   }
-  int down = 0;
-  if constexpr (__is_same(T, __bf16)) {
-    float most = 0.0f;
+  // Returns what the scores are to be multiplied with, which is positive: q takes
+  // the scale's sign, and 2^-126 stands for less (a masked score must not meet a
+  // zero; the others are zero either way).  `most_of`: the maximum over the lanes
+  // that have the row.
+  template <class Most>
+  __device__ __forceinline__ float operands(float scale, h8 q[N], Most most_of) const {
+    int down = 0;
+    if constexpr (__is_same(T, __bf16)) {
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[i][e / 4][e % 4]));
+      most = most_of(most);
+      down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)x[i][e / 4][e % 4]));
-    most = most_of(most);
-    down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
-  }
+      for (int e = 0; e < 8; ++e) {
+        // pairs (0, 2), (16, 18), (1, 3), (17, 19) of the word's elements
+        const T y = x[i][e / 2 % 2][e / 4 + e % 2 * 2];
+        if constexpr (__is_same(T, __bf16)) q[i][e] = (_Float16)ldexpf((float)y, -down);
+        else q[i][e] = y;
+      }
+    if (scale < 0.0f) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // pairs (0, 2), (16, 18), (1, 3), (17, 19) of the word's elements
-      const T y = x[i][e / 2 % 2][e / 4 + e % 2 * 2];
-      if constexpr (__is_same(T, __bf16)) q[i][e] = (_Float16)ldexpf((float)y, -down);
-      else q[i][e] = y;
+      for (int i = 0; i < N; ++i) q[i] = -q[i];
     }
-  if (scale < 0.0f) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = -q[i];
+    return fmaxf(ldexpf(fabsf(scale), down), 0x1p-126f);
   }
-  return fmaxf(ldexpf(fabsf(scale), down), 0x1p-126f);
-}
+};
 
 // Up to 16 or 32 rows of a group a sequence; the work is cut as in
 // mer_attention.hip's kernel of this shape: equal stretches of all sequences'
@@ -434,9 +441,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int n = 0; n < NR; ++n) {
       const uint32_t row = t.row0 + n * 16 + col, tok = by_group(p, row), hd = head * p.group + row - tok * p.group;
       pos[n] = t.pos0 + (int32_t)tok;
-      scale[n] = load_q<E, DP / 32>(
-          (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row < t.n_rows, p.head_dim,
-          p.scale_log2, q[n], [&](uint32_t i) { return DP == 64 ? quad * 2 + i : (i / 4 * 4 + quad) * 4 + i % 4; }, max_quad);
+      Queries<E, DP / 32> raw;
+      raw.load((const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row < t.n_rows, p.head_dim,
+               [&](uint32_t i) { return DP == 64 ? quad * 2 + i : (i / 4 * 4 + quad) * 4 + i % 4; });
+      scale[n] = raw.operands(p.scale_log2, q[n], max_quad);
     }
     const uint32_t last = t.row0 + C::kRows - 1 < t.n_rows ? t.row0 + C::kRows - 1 : t.n_rows - 1;
     const int32_t pos_first = t.pos0 + (int32_t)by_group(p, t.row0), pos_last = t.pos0 + (int32_t)by_group(p, last);
@@ -606,6 +614,25 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   }
 }
 
+// find_unit with the sequence's span.  Up to 63 sequences: one round trip to
+// memory, in which every lane asks for a sequence's start and length.
+template <int ROWS>
+__device__ __forceinline__ Span find_span(const AttnParams &p, uint32_t unit, uint32_t *seq, uint32_t *tile) {
+  if (p.n_seqs < 64) {
+    const uint32_t s = lane_id() < p.n_seqs ? lane_id() : p.n_seqs;
+    const int32_t q = p.q_start[s], len = p.kv_len[s < p.n_seqs ? s : 0];
+    const uint64_t base = (uint64_t)(q < 0 ? 0 : q) * p.group / ROWS + lane_id();
+    const uint64_t m = __builtin_amdgcn_ballot_w64(lane_id() < p.n_seqs && base <= unit);
+    const int at = m ? (int)__popcll(m) - 1 : 0;
+    const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)base, at);
+    *seq = (uint32_t)at;
+    *tile = unit >= b ? unit - b : 0xffffffffu;
+    return make_span(p, __builtin_amdgcn_readlane(q, at), __builtin_amdgcn_readlane(q, at + 1), __builtin_amdgcn_readlane(len, at));
+  }
+  find_unit<ROWS>(p, unit, seq, tile);
+  return make_span(p, sload(p.q_start, *seq), sload(p.q_start, *seq + 1), sload(p.kv_len, *seq));
+}
+
 // 32 rows a wave: prompts and larger chunks.  The waves of a workgroup share
 // tiles of 64 keys, which lie in LDS as f16, two stages of K and V.  Each wave
 // brings its share of the next tile there: codes and scales go to registers a
@@ -616,33 +643,36 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 // In LDS a row is pieces of eight elements in unpack's order, places permuted
 // by the row; queries have that order too, and the answers' is turned back at
 // the end (four_of).
-template <int DP>
+template <int DP, int WAVES>
 struct Rows32Q4 {
-  static constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;
+  static constexpr int kWaves = WAVES, kRows = 32 * kWaves, kKeys = 64;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kShare = kKeys / kWaves;      // keys that a wave brings
   static constexpr int kBlocks = DP / 32;            // of a row
   static constexpr int kMine = 2 * kShare * kBlocks / 64;  // blocks of a lane, K's and V's
   static constexpr int kLds = 2 * 2 * kTileBytes;
   static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
+  // V: a transposed read takes 64 bytes of each of four rows, a write of a word
+  // one piece in four of each of four rows.
   static __device__ __forceinline__ uint32_t v_swizzle(uint32_t row) {
-    return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+    return DP == 64 ? (row >> 1 & 1) << 2 | (row >> 1 & 3) : (row & 3) * 5;
   }
 };
 
-// A wave's share of the tiles, from memory to f16 in LDS: 16 keys of K and V.
-// Lanes take a block each, K's and V's of the same keys where a row has four
-// blocks or more; with two, K's are the lower lanes' and V's the upper ones'.
-template <int DP>
+// A wave's share of the tiles, from memory to f16 in LDS.  Lanes take a block
+// each, K's and V's of the same keys where the share has 64 blocks of each or
+// more; with 32, K's are the lower lanes' and V's the upper ones'.
+template <class C, int DP>
 struct Bring {
-  typedef Rows32Q4<DP> C;
-  static constexpr bool kSplit = DP == 64;
+  static constexpr bool kSplit = C::kShare * C::kBlocks == 32;
   static constexpr int kPlaces = kSplit ? 1 : C::kMine / 2;   // blocks of a lane, of K or of V
-  static constexpr uint32_t kKeysAtOnce = kSplit ? 16 : 64 / C::kBlocks;
+  static constexpr uint32_t kKeysAtOnce = kSplit ? C::kShare : 64 / C::kBlocks;
+  static constexpr int kPages = C::kShare / 8;
+  static_assert(C::kMine >= 1 && (kPages == 1 || kPages == 2), "");
   const int32_t *table;
   const uint8_t *k, *v, *ks, *vs;  // of this head in page 0
   uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages;
-  int32_t lo, hi, key0, next_key, next_id[2];
+  int32_t lo, hi, key0, next_key, next_id[kPages];
   uint32_t block;                  // a lane's; that of the first where the head has no such block
   bool there, is_v;                // it has; the lane's are V's (kSplit)
   uint32_t key;                    // a lane's first
@@ -683,7 +713,7 @@ struct Bring {
     next_key = first_key;
     const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < kPages; ++g) {
       int32_t pg = (first_key + g * 8) >> page_shift;
       pg = pg > last ? last : (pg < first ? first : pg);
       next_id[g] = sload(table, (uint32_t)pg);
@@ -693,12 +723,12 @@ struct Bring {
   __device__ __forceinline__ void load(uint32_t *status) {
     key0 = next_key;
     const uint32_t mask = (1u << page_shift) - 1;
-    const bool known0 = (uint32_t)next_id[0] < n_pages, known1 = (uint32_t)next_id[1] < n_pages;
-    if (!(known0 && known1) && lane_id() < 2) {
+    const bool known0 = (uint32_t)next_id[0] < n_pages, known1 = (uint32_t)next_id[kPages - 1] < n_pages;
+    if (!(known0 && known1) && lane_id() < kPages) {
       const int32_t k0 = key0 + (int32_t)lane_id() * 8;
       if (!(lane_id() ? known1 : known0) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
     }
-    const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[1] : 0;
+    const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[kPages - 1] : 0;
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
       const uint32_t at = i * kKeysAtOnce + key, page = at < 8 ? id0 : id1, place = ((uint32_t)key0 + at) & mask;
@@ -731,9 +761,9 @@ struct Bring {
   }
 };
 
-template <class E, int DP>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(AttnQ4Params p) {
-  typedef Rows32Q4<DP> C;
+template <class E, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64 ? 3 : 2)) void attn_q4_rows32_kernel(AttnQ4Params p) {
+  typedef Rows32Q4<DP, WAVES> C;
   typedef typename E::T T;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
@@ -742,9 +772,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
   // Chunk by chunk, so that neighbours are alike; late rows, with more keys, first.
   const uint32_t c = rest / p.n_units, unit = p.n_units - 1 - rest % p.n_units;
   uint32_t seq, tile;
-  find_unit<C::kRows>(p, unit, &seq, &tile);
   Tile t;
-  const Span span = make_span(p, sload(p.q_start, seq), sload(p.q_start, seq + 1), sload(p.kv_len, seq));
+  const Span span = find_span<C::kRows>(p, unit, &seq, &tile);
   if (!make_tile<C::kRows>(p, span, tile, &t)) return;
   uint32_t chunk, n_chunks;
   chunks_of<C::kKeys>(p, t, &chunk, &n_chunks);
@@ -760,19 +789,25 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
   const bool any = wrow < t.n_rows;
   const int32_t pos_first = t.pos0 + (int32_t)by_group(p, wrow), pos_last = t.pos0 + (int32_t)by_group(p, wlast);
 
-  h8 q[DP / 16];
-  const float scale = load_q<E, DP / 16>(
-      (const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row_ok, p.head_dim,
-      p.scale_log2, q, [&](uint32_t i) { return i * 2 + half; }, [](float x) { return fmaxf(x, other_half(x)); });
-
   const int32_t begin = start + (int32_t)(c * chunk);
   int32_t end = begin + (int32_t)chunk;
   end = end < t.hi ? end : t.hi;
   const int32_t n_tiles = (end - begin + C::kKeys - 1) / C::kKeys;
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
-  Bring<DP> br;
+  // Page ids, queries and the first tile are on their way together.
+  Bring<C, DP> br;
   br.init(p, p.table + (uint64_t)seq * p.table_stride, head, wave, t);
   const int32_t my_key = begin + (int32_t)wave * C::kShare;
+  if (n_tiles > 0) br.lookup(my_key);
+  Queries<E, DP / 16> raw;
+  raw.load((const T *)p.q + (uint64_t)(t.tok0 + tok) * p.q_stride + (uint64_t)hd * p.head_dim, row_ok, p.head_dim,
+           [&](uint32_t i) { return i * 2 + half; });
+  if (n_tiles > 0) {
+    br.load(p.status);
+    br.lookup(my_key + C::kKeys);
+  }
+  h8 q[DP / 16];
+  const float scale = raw.operands(p.scale_log2, q, [](float x) { return fmaxf(x, other_half(x)); });
   auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
   constexpr int kWords = 4 * C::kMine;
 
@@ -789,9 +824,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   if (n_tiles > 0) {
-    br.lookup(my_key);
-    br.load(p.status);
-    br.lookup(my_key + C::kKeys);
 #pragma unroll
     for (int i = 0; i < kWords; ++i) br.word(stage(0), i);
     if (n_tiles > 1) {
@@ -947,13 +979,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_q4_rows32_kernel(
   }
 }
 
-template <class E, int DP>
+template <class E, int DP, int WAVES>
 hipError_t launch32(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
-  typedef Rows32Q4<DP> C;
+  typedef Rows32Q4<DP, WAVES> C;
   static std::atomic<uint64_t> devices{0};
-  const hipError_t e = allow_lds((const void *)attn_q4_rows32_kernel<E, DP>, C::kLds, &devices);
+  const hipError_t e = allow_lds((const void *)attn_q4_rows32_kernel<E, DP, WAVES>, C::kLds, &devices);
   if (e != hipSuccess) return e;
-  attn_q4_rows32_kernel<E, DP><<<plan.n_wgs, 256, C::kLds, st>>>(p);
+  attn_q4_rows32_kernel<E, DP, WAVES><<<plan.n_wgs, 64 * WAVES, C::kLds, st>>>(p);
   if (plan.n_chunks > 1) attn_join_kernel<C, E, DP><<<plan.n_units * p.n_kv_heads * C::kWaves, 256, 0, st>>>(p);
   return hipGetLastError();
 }
@@ -970,7 +1002,9 @@ hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st)
 
 template <class E, int DP>
 hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
-  if (plan.rows == 128) return launch32<E, DP>(plan, p, st);
+  if constexpr (DP == 128)
+    if (plan.rows == 256) return launch32<E, DP, 8>(plan, p, st);
+  if (plan.rows == 128) return launch32<E, DP, 4>(plan, p, st);
   if constexpr (DP < 256)
     if (plan.rows == 16 && plan.waves == 1) return launch16<E, DP, 1, 1>(plan, p, st);
   if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
