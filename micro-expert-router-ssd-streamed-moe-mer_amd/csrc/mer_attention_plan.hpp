@@ -187,10 +187,15 @@ inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uin
   // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
   const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
   if (a.rows <= 32 && small_tiles * (table_keys / 128 + 2) < (1ull << 31)) {
-    // Many units: every wave is a workgroup of its own.
-    const bool narrow = a.rows == 16 && head_dim <= 128 && (uint64_t)n_seqs * n_kv_heads >= 2ull * cus;
+    // Long stretches of few units: workgroups of four waves.  Many units: every
+    // wave a workgroup of its own, so that one's piece ends while the others' keys
+    // stream.  Sequences of 200 - 8000 keys, 8 kv heads of 128: 16 of them 36 us wide
+    // and 37 us narrow, 24 47 and 43, 64 106 and 85; 16 of 4096 28 and 32 us, 64
+    // 69 and 73; 512 of 300 - 700 135 and 94.  Either way as many waves as the LDS
+    // holds.
+    const bool narrow = a.rows == 16 && (uint64_t)n_seqs * n_kv_heads * 4 >= 3ull * cus;
     a.waves = narrow ? 1 : 4;
-    a.n_wgs = (uint32_t)cus * (narrow ? 8 : (head_dim <= 128 ? 2 : 1));
+    a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 128 ? 2 : 1);
     a.min_granules = 1;
     a.part_o_floats = 2 * (size_t)a.n_wgs * a.rows * head_dim;
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;

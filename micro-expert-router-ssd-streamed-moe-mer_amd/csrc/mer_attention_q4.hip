@@ -1005,8 +1005,7 @@ hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t s
   if constexpr (DP == 128)
     if (plan.rows == 256) return launch32<E, DP, 8>(plan, p, st);
   if (plan.rows == 128) return launch32<E, DP, 4>(plan, p, st);
-  if constexpr (DP < 256)
-    if (plan.rows == 16 && plan.waves == 1) return launch16<E, DP, 1, 1>(plan, p, st);
+  if (plan.rows == 16 && plan.waves == 1) return launch16<E, DP, 1, 1>(plan, p, st);
   if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
   if constexpr (DP < 256) return launch16<E, DP, 4, 2>(plan, p, st);
   return hipErrorInvalidValue;
