@@ -91,6 +91,7 @@ struct AppendQ4Params {
   uint32_t n_tokens, rot, interleaved;
   uint32_t heads_per_wave;   // consecutive heads that one wave walks
   float eps;
+  double inv_dim;
   uint32_t *status;
 };
 struct ReadQ4Params {

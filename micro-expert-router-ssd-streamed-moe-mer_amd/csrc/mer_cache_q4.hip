@@ -41,11 +41,6 @@ template <> struct Elem<kBF16> { typedef __bf16 T; typedef b4 V4; typedef b8 V16
 constexpr float kMostScale = 7936.0f, kMostValue = 65504.0f;
 constexpr uint16_t kNanScale = 0x7e00;
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-
 // Workgroups go round the eight XCDs; those of one XCD take neighbouring tokens,
 // whose codes and scales share cache lines.
 constexpr uint32_t kXcds = 8;
@@ -58,40 +53,54 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int larger(int a, int b) { return a > b ? a : b; }
+
 // Codes and scale of a block that four lanes hold, each elements 4t .. 4t + 3
-// (a) and 16 + 4t .. (b): the lane's four bytes of codes.
-__device__ __forceinline__ uint32_t quantise(f4 a, f4 b, _Float16 *scale) {
-  float hi = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
-  float lo = fminf(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])), fminf(fminf(b[0], b[1]), fminf(b[2], b[3])));
-  hi = fmaxf(hi, dpp<0xB1>(hi));  // lane ^ 1
-  lo = fminf(lo, dpp<0xB1>(lo));
-  hi = fmaxf(hi, dpp<0x4E>(hi));  // lane ^ 2
-  lo = fminf(lo, dpp<0x4E>(lo));
-  const bool positive = hi >= -lo && hi > 0.0f;
-  uint32_t u = __float_as_uint(fmaxf(hi, -lo) * 0.125f);
+// (a) and 16 + 4t .. (b): the lane's four bytes of codes.  `bits`: of the largest
+// magnitude, from which on an element is no finite number that fits.
+__device__ __forceinline__ uint32_t quantise(f4 a, f4 b, _Float16 *scale, int *bits) {
+  // As whole numbers floats of one sign are in order, and negative ones below
+  // the others: the largest is the positive one of largest magnitude, if there is
+  // any.  NaN and infinities are above all that fits.
+  int most = 0, top = (int)0x80000000;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = __float_as_int(a[i]), y = __float_as_int(b[i]);
+    most = larger(larger(most, x & 0x7fffffff), y & 0x7fffffff);
+    top = larger(larger(top, x), y);
+  }
+  most = larger(most, dpp<0xB1>(most));  // lane ^ 1
+  top = larger(top, dpp<0xB1>(top));
+  most = larger(most, dpp<0x4E>(most));  // lane ^ 2
+  top = larger(top, dpp<0x4E>(top));
+  *bits = most;
+  uint32_t u = __float_as_uint(__int_as_float(most) * 0.125f);
   u = (u + 0x3ffffu + (u >> 19 & 1)) & ~0x7ffffu;  // four bits behind the first, half to even
   float d = (float)(_Float16)fminf(__uint_as_float(u), kMostScale);
-  d = positive ? -d : d;
+  d = top == most ? -d : d;
   *scale = (_Float16)d;
   // x / d by d's reciprocal in f64, which gives the code of the quotient: x is an
   // f32 and a border d (n + 1/2) has ten bits, so an x beside it is off by 2^-24 of
-  // it, and on it the product is n + 1/2 itself (for all sixteen d and all n).
+  // it, and on it the product, rounded, is n + 1/2 itself (for all sixteen d and all
+  // n).  Adding 3 * 2^51 leaves the whole quotient in the low word; not as one fma,
+  // which would not round the product first.
   const double r = 1.0 / (double)(d == 0.0f ? 1.0f : d);
   uint32_t codes = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int p = (int)rint((double)a[i] * r), q = (int)rint((double)b[i] * r);
-    codes |= (uint32_t)((p > 7 ? 7 : (p < -8 ? -8 : p)) & 15) << 8 * i;
-    codes |= (uint32_t)((q > 7 ? 7 : (q < -8 ? -8 : q)) & 15) << (8 * i + 4);
+    auto code = [&](float x) {
+#pragma clang fp contract(off)
+      const double y = (double)x * r;
+      const int n = (int)(uint32_t)__double_as_longlong(y + 0x1.8p52);
+      return (uint32_t)((n > 7 ? 7 : (n < -8 ? -8 : n)) & 15);
+    };
+    codes |= code(a[i]) << 8 * i | code(b[i]) << (8 * i + 4);
   }
   return codes ^ 0x88888888u;  // n + 8 for n
-}
-
-__device__ __forceinline__ bool does_not_fit(f4 a) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= !(fabsf(a[i]) <= kMostValue);
-  return bad;
 }
 
 // Passes of a wave: loads of all of them are in flight before the first is used.
@@ -187,7 +196,7 @@ __global__ __launch_bounds__(256) void append_q4_kernel(AppendQ4Params p) {
         for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
 #pragma unroll
         for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
-        const double r = 1.0 / sqrt(ss / (double)head_dim + (double)p.eps);
+        const double r = rsqrt(__builtin_fma(ss, p.inv_dim, (double)p.eps));
         x = x * r * __builtin_convertvector(w0, d4);
         y = y * r * __builtin_convertvector(w1, d4);
       }
@@ -213,8 +222,6 @@ __global__ __launch_bounds__(256) void append_q4_kernel(AppendQ4Params p) {
       b = __builtin_convertvector(y, f4);
     }
     const f4 va = __builtin_convertvector(v0[i], f4), vb = __builtin_convertvector(v1[i], f4);
-    const uint64_t wrong = __builtin_amdgcn_ballot_w64(does_not_fit(a) || does_not_fit(b) || does_not_fit(va) || does_not_fit(vb));
-    const bool bad = (wrong >> sub * LANES & (LANES == 64 ? ~0ull : (1ull << LANES) - 1)) != 0;
     wave_sync();
     if (in_row) {
       *(f4 *)(row + o0) = a;
@@ -226,7 +233,10 @@ __global__ __launch_bounds__(256) void append_q4_kernel(AppendQ4Params p) {
       b = *(const f4 *)(row + e1);
     }
     _Float16 kd, vd;
-    const uint32_t kc = quantise(a, b, &kd), vc = quantise(va, vb, &vd);
+    int km, vm;
+    const uint32_t kc = quantise(a, b, &kd, &km), vc = quantise(va, vb, &vd, &vm);
+    const uint64_t wrong = __builtin_amdgcn_ballot_w64(larger(km, vm) > __float_as_int(kMostValue));
+    const bool bad = (wrong >> sub * LANES & ((1ull << LANES) - 1)) != 0;
     if (h < head1 && in_row) {
       const uint64_t unit = page * heads + h;
       const uint64_t code = ((unit << p.cache.page_shift) + off) * (head_dim / 2) + 4 * j;
@@ -250,6 +260,7 @@ hipError_t launch_append(AppendQ4Params p, int cus, hipStream_t st) {
   uint32_t passes = all < kPasses ? all : kPasses;
   while (passes > 1 && (uint64_t)p.n_tokens * ((all + passes - 1) / passes) < 8ull * cus) --passes;
   p.heads_per_wave = passes * per_pass;
+  p.inv_dim = 1.0 / p.cache.head_dim;
   const uint64_t waves = (uint64_t)p.n_tokens * ((heads + p.heads_per_wave - 1) / p.heads_per_wave);
   const uint32_t grid = xcd_grid((waves + 3) / 4);
   if (lanes == 8) append_q4_kernel<IN, 8><<<grid, 256, 0, st>>>(p);
