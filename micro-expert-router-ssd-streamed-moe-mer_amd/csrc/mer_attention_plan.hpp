@@ -3,7 +3,6 @@
 // sizes only, without HIP, so that it can be compiled and checked anywhere.
 #pragma once
 #include <math.h>
-#include <stdlib.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -71,9 +70,9 @@ inline size_t attn_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint3
 
 // 128-row tiles: how many chunks a row tile's keys are cut into.
 inline AttnPlan attn_plan_128(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                              size_t max_q_len, size_t max_kv_len, uint32_t window, int cus, size_t floats, uint32_t rows_ = 128) {
+                              size_t max_q_len, size_t max_kv_len, uint32_t window, int cus, size_t floats) {
   AttnPlan a{};
-  a.rows = rows_;
+  a.rows = 128;
   a.n_units = (uint32_t)((n_tokens * group + a.rows - 1) / a.rows + n_seqs);
   // keys of a row tile, from a whole key tile's start on
   size_t max_keys = max_kv_len;
@@ -201,7 +200,7 @@ inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uin
     a.part_ml_floats = 2 * (size_t)a.n_wgs * a.rows * 2;
     if (a.part_o_floats + a.part_ml_floats <= floats && a.n_wgs >= kAttnTickets && a.n_wgs < kAttnEpoch / 2) return a;
   }
-  return attn_plan_128(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, window, cus, floats, head_dim > 64 && head_dim <= 128 && getenv("R256") ? 256 : 128);
+  return attn_plan_128(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, window, cus, floats);
 }
 
 }  // namespace mer

@@ -53,6 +53,14 @@ struct Unpack {
     x[3] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | near) - n;
   }
 };
+// The sum of eight weights, as they enter the product, added to `sum` in 32 bits:
+// half the additions that the weights before rounding would take.
+__device__ __forceinline__ float add_eight(h8 x, float sum) {
+  const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2(h2{x[2 * i], x[2 * i + 1]}, one, sum, false);
+  return sum;
+}
 __device__ __forceinline__ h8 eight(const h2 x[4]) {
   h8 v;
 #pragma unroll
@@ -539,18 +547,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         const float mu = (m[n] == -__builtin_inff() ? 0.0f : m[n]) - E::kUp;
         float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], scale[n], -mu));
-          sum += z[e];
-        }
-        l[n] += sum;
-#pragma unroll
         for (int b = 0; b < 2; ++b) {
           f8 y;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = z[b * 8 + e];
+          for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[b * 8 + e], scale[n], -mu));
           pr[n][b] = __builtin_convertvector(y, h8);
+          sum = add_eight(pr[n][b], sum);
         }
+        l[n] += sum;
       }
 #pragma unroll
       for (int b = 0; b < G::kPieces; ++b) {
@@ -643,14 +647,14 @@ __device__ __forceinline__ Span find_span(const AttnParams &p, uint32_t unit, ui
 // In LDS a row is pieces of eight elements in unpack's order, places permuted
 // by the row; queries have that order too, and the answers' is turned back at
 // the end (four_of).
-template <int DP, int WAVES>
+template <int DP>
 struct Rows32Q4 {
-  static constexpr int kWaves = WAVES, kRows = 32 * kWaves, kKeys = 64;
+  static constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;
   static constexpr int kTileBytes = kKeys * DP * 2;  // K or V of a tile
   static constexpr int kShare = kKeys / kWaves;      // keys that a wave brings
   static constexpr int kBlocks = DP / 32;            // of a row
   static constexpr int kMine = 2 * kShare * kBlocks / 64;  // blocks of a lane, K's and V's
-  static constexpr int kLds = 2 * 2 * kTileBytes;
+  static constexpr int kStageBytes = 2 * kTileBytes, kLds = 2 * kStageBytes;
   static __device__ __forceinline__ uint32_t k_swizzle(uint32_t row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
   // V: a transposed read takes 64 bytes of each of four rows, a write of a word
   // one piece in four of each of four rows.
@@ -667,21 +671,20 @@ struct Bring {
   static constexpr bool kSplit = C::kShare * C::kBlocks == 32;
   static constexpr int kPlaces = kSplit ? 1 : C::kMine / 2;   // blocks of a lane, of K or of V
   static constexpr uint32_t kKeysAtOnce = kSplit ? C::kShare : 64 / C::kBlocks;
-  static constexpr int kPages = C::kShare / 8;
-  static_assert(C::kMine >= 1 && (kPages == 1 || kPages == 2), "");
+  static_assert(C::kMine >= 1 && C::kShare == 16, "two pages of 8 keys at most");
   const int32_t *table;
   const uint8_t *k, *v, *ks, *vs;  // of this head in page 0
   uint32_t code_bytes, scale_bytes, row_bytes, page_shift, n_pages;
-  int32_t lo, hi, key0, next_key, next_id[kPages];
-  uint32_t block;                  // a lane's; that of the first where the head has no such block
-  bool there, is_v;                // it has; the lane's are V's (kSplit)
+  int32_t lo, hi, key0, next_key, next_id[2];
+  bool there, is_v;                // the head has a lane's block; it is V's (kSplit)
   uint32_t key;                    // a lane's first
-  uint32_t to[C::kMine];           // where a block's first word goes, from a stage's start
+  uint32_t code_at, scale_at;      // a lane's part of the addresses (the first block's where there is none)
+  uint32_t to[C::kMine];           // where a block's first word goes in the first stage
   u4 w[C::kMine];
   uint16_t d[C::kMine];
   Unpack unpack;
 
-  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, uint32_t wave, const Tile &t) {
+  __device__ __forceinline__ void init(const AttnQ4Params &p, const int32_t *seq_table, uint32_t head, uint32_t wave, const Tile &t, uint32_t ring) {
     row_bytes = p.head_dim / 2;
     page_shift = p.page_shift;
     const uint32_t n_blocks = p.head_dim / kQ4Block, u = lane_id() % (kSplit ? 32 : 64);
@@ -699,12 +702,13 @@ struct Bring {
     key = u / C::kBlocks;
     const uint32_t b = u % C::kBlocks;
     there = b < n_blocks;
-    block = there ? b : 0;
+    code_at = key * row_bytes + (there ? b : 0) * 16;
+    scale_at = (((there ? b : 0) << page_shift) + key) * 2;
 #pragma unroll
     for (int j = 0; j < C::kMine; ++j) {
       const uint32_t row = wave * C::kShare + j % kPlaces * kKeysAtOnce + key;
       const bool of_v = kSplit ? is_v : j >= kPlaces;
-      to[j] = (of_v ? C::kTileBytes : 0) + row * (DP * 2) + ((b * 4) ^ (of_v ? C::v_swizzle(row) : C::k_swizzle(row))) * 16;
+      to[j] = ring + (of_v ? C::kTileBytes : 0) + row * (DP * 2) + ((b * 4) ^ (of_v ? C::v_swizzle(row) : C::k_swizzle(row))) * 16;
     }
   }
   // Any key will do: page places are cut to those of [lo, hi), which is not
@@ -713,57 +717,73 @@ struct Bring {
     next_key = first_key;
     const int32_t first = lo >> page_shift, last = (hi - 1) >> page_shift;
 #pragma unroll
-    for (int g = 0; g < kPages; ++g) {
+    for (int g = 0; g < 2; ++g) {
       int32_t pg = (first_key + g * 8) >> page_shift;
       pg = pg > last ? last : (pg < first ? first : pg);
       next_id[g] = sload(table, (uint32_t)pg);
     }
   }
-  // The share last looked up is on its way.
+  // The share last looked up is on its way.  Pages of 16 keys and more hold a
+  // whole share, whose addresses are a scalar's and a lane's own part; the
+  // general case costs 45 vector instructions a tile more.
   __device__ __forceinline__ void load(uint32_t *status) {
     key0 = next_key;
     const uint32_t mask = (1u << page_shift) - 1;
-    const bool known0 = (uint32_t)next_id[0] < n_pages, known1 = (uint32_t)next_id[kPages - 1] < n_pages;
-    if (!(known0 && known1) && lane_id() < kPages) {
-      const int32_t k0 = key0 + (int32_t)lane_id() * 8;
-      if (!(lane_id() ? known1 : known0) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
-    }
-    const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[kPages - 1] : 0;
+    if (page_shift >= 4) {
+      const bool known = (uint32_t)next_id[0] < n_pages;
+      if (!known && lane_id() == 0 && key0 < hi && key0 + C::kShare > lo)
+        atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
+      const uint32_t id = known ? (uint32_t)next_id[0] : 0, place = (uint32_t)key0 & mask;
+      const uint64_t c = (uint64_t)id * code_bytes + place * row_bytes, s = (uint64_t)id * scale_bytes + place * 2;
 #pragma unroll
-    for (int i = 0; i < kPlaces; ++i) {
-      const uint32_t at = i * kKeysAtOnce + key, page = at < 8 ? id0 : id1, place = ((uint32_t)key0 + at) & mask;
-      const uint64_t c = (uint64_t)page * code_bytes + (place * row_bytes + block * 16);
-      const uint64_t s = (uint64_t)page * scale_bytes + ((block << page_shift) + place) * 2;
-      // zero where there is no such block or page, and for values that are not finite
-      const bool gone = !there || !(at < 8 ? known0 : known1);
-      if constexpr (kSplit) {
-        w[i] = *(const u4 *)((is_v ? v : k) + c);
-        const uint16_t x = *(const uint16_t *)((is_v ? vs : ks) + s);
-        d[i] = gone || (is_v && (x & 0x7000u) == 0x7000u) ? 0 : x;
-      } else {
-        w[i] = *(const u4 *)(k + c);
-        w[i + kPlaces] = *(const u4 *)(v + c);
-        const uint16_t x = *(const uint16_t *)(ks + s), y = *(const uint16_t *)(vs + s);
-        d[i] = gone ? 0 : x;
-        d[i + kPlaces] = gone || (y & 0x7000u) == 0x7000u ? 0 : y;
+      for (int i = 0; i < kPlaces; ++i)
+        take(i, c + i * kKeysAtOnce * row_bytes, code_at, s + i * kKeysAtOnce * 2, scale_at, !there || !known);
+    } else {
+      const bool known0 = (uint32_t)next_id[0] < n_pages, known1 = (uint32_t)next_id[1] < n_pages;
+      if (!(known0 && known1) && lane_id() < 2) {
+        const int32_t k0 = key0 + (int32_t)lane_id() * 8;
+        if (!(lane_id() ? known1 : known0) && k0 < hi && k0 + 8 > lo) atomicCAS(status, 0u, 16u /* MER_ERR_RESIDENCY_MISS */);
+      }
+      const uint32_t id0 = known0 ? (uint32_t)next_id[0] : 0, id1 = known1 ? (uint32_t)next_id[1] : 0;
+#pragma unroll
+      for (int i = 0; i < kPlaces; ++i) {
+        const uint32_t at = i * kKeysAtOnce + key, page = at < 8 ? id0 : id1, place = ((uint32_t)key0 + at) & mask;
+        take(i, (uint64_t)page * code_bytes + place * row_bytes, code_at - key * row_bytes,
+             (uint64_t)page * scale_bytes + place * 2, scale_at - key * 2, !there || !(at < 8 ? known0 : known1));
       }
     }
   }
-  // Word i of 4 kMine to the stage at `lds`.
-  __device__ __forceinline__ void word(uint32_t lds, int i) const {
+  // Block i of K and of V at byte `c` + `cl` of the codes and `s` + `sl` of the
+  // scales; zero scales where there is no such block or page, and for values that
+  // are not finite.
+  __device__ __forceinline__ void take(int i, uint64_t c, uint32_t cl, uint64_t s, uint32_t sl, bool gone) {
+    if constexpr (kSplit) {
+      w[i] = *(const u4 *)((is_v ? v : k) + c + cl);
+      const uint16_t x = *(const uint16_t *)((is_v ? vs : ks) + s + sl);
+      d[i] = gone || (is_v && (x & 0x7000u) == 0x7000u) ? 0 : x;
+    } else {
+      w[i] = *(const u4 *)(k + c + cl);
+      w[i + kPlaces] = *(const u4 *)(v + c + cl);
+      const uint16_t x = *(const uint16_t *)(ks + s + sl), y = *(const uint16_t *)(vs + s + sl);
+      d[i] = gone ? 0 : x;
+      d[i + kPlaces] = gone || (y & 0x7000u) == 0x7000u ? 0 : y;
+    }
+  }
+  // Word i of 4 kMine to a stage.
+  __device__ __forceinline__ void word(uint32_t stage, int i) const {
     const int j = i / 4;
     const h2 dd = {__builtin_bit_cast(_Float16, d[j]), __builtin_bit_cast(_Float16, d[j])};
     h2 y[4];
     unpack(w[j][i % 4], y);
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] *= dd;
-    *(__attribute__((address_space(3))) h8 *)(uintptr_t)((lds + to[j]) ^ (uint32_t)(i % 4) * 16) = eight(y);
+    *(__attribute__((address_space(3))) h8 *)(uintptr_t)((stage + to[j]) ^ (uint32_t)(i % 4) * 16) = eight(y);
   }
 };
 
-template <class E, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64 ? 3 : 2)) void attn_q4_rows32_kernel(AttnQ4Params p) {
-  typedef Rows32Q4<DP, WAVES> C;
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : (DP == 64 ? 3 : 2)) void attn_q4_rows32_kernel(AttnQ4Params p) {
+  typedef Rows32Q4<DP> C;
   typedef typename E::T T;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lane = lane_id(), wave = uni(threadIdx.x / 64);
@@ -796,7 +816,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
   // Page ids, queries and the first tile are on their way together.
   Bring<C, DP> br;
-  br.init(p, p.table + (uint64_t)seq * p.table_stride, head, wave, t);
+  br.init(p, p.table + (uint64_t)seq * p.table_stride, head, wave, t, ring);
   const int32_t my_key = begin + (int32_t)wave * C::kShare;
   if (n_tiles > 0) br.lookup(my_key);
   Queries<E, DP / 16> raw;
@@ -808,14 +828,14 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
   }
   h8 q[DP / 16];
   const float scale = raw.operands(p.scale_log2, q, [](float x) { return fmaxf(x, other_half(x)); });
-  auto stage = [&](int32_t i) { return ring + (uint32_t)(i & 1) * (2 * C::kTileBytes); };
+  auto stage = [](int32_t i) { return (uint32_t)(i & 1) * C::kStageBytes; };
   constexpr int kWords = 4 * C::kMine;
 
-  // Where a lane reads its first operands, from a tile's start; the others' places
+  // Where a lane reads its first operands in the first stage; the others' places
   // differ in bits of the piece.  K: 32 keys x 16 dims a product.  V: 16 keys x 32
   // dims, 4 + 4 keys of a lane in the order in which the scores lie in their lanes.
-  const uint32_t k_lane = col * (DP * 2) + (half ^ C::k_swizzle(col)) * 16, v_row = half * 4 + lane % 16 / 4;
-  const uint32_t v_lane = v_row * (DP * 2) + ((lane / 16 % 2 * 2 + lane % 4 / 2) ^ C::v_swizzle(v_row)) * 16 + lane % 2 * 8;
+  const uint32_t k_lane = ring + col * (DP * 2) + (half ^ C::k_swizzle(col)) * 16, v_row = half * 4 + lane % 16 / 4;
+  const uint32_t v_lane = ring + C::kTileBytes + v_row * (DP * 2) + ((lane / 16 % 2 * 2 + lane % 4 / 2) ^ C::v_swizzle(v_row)) * 16 + lane % 2 * 8;
 
   float m = -__builtin_inff(), l = 0.0f;
   f16v o[DP / 32];
@@ -854,16 +874,15 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
   first_live = (int32_t)uni((uint32_t)(first_live < live_end ? first_live : live_end));
   int32_t i = 0;
   for (; i < first_live; ++i) pass_by(i);
-  for (; i < live_end; ++i) {
+  auto live = [&](uint32_t here, uint32_t next) {
     const int32_t key0 = begin + i * C::kKeys;
-    const uint32_t kb = stage(i), vb = kb + C::kTileBytes, next = stage(i + 1);
     arrive();
     auto v_of = [&](int ks, uint32_t d) {
       s4 x[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
         x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4 *)(uintptr_t)(((vb + v_lane) ^ d * 64) + (ks * 16 + b * 8) * (DP * 2)));
+            (__attribute__((address_space(3))) s4 *)(uintptr_t)(((here + v_lane) ^ d * 64) + (ks * 16 + b * 8) * (DP * 2)));
       return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
     };
     f16v s[2];
@@ -880,7 +899,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
       for (int d = 0; d < kBatch; ++d)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          k[b][d] = *(const __attribute__((address_space(3))) h8 *)(uintptr_t)(((kb + k_lane) ^ (uint32_t)(d0 + d) * 32) + b * 32 * (DP * 2));
+          k[b][d] = *(const __attribute__((address_space(3))) h8 *)(uintptr_t)(((here + k_lane) ^ (uint32_t)(d0 + d) * 32) + b * 32 * (DP * 2));
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int d = 0; d < kBatch; ++d) {
@@ -890,6 +909,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
         for (int w = (d0 + d) * kWords / kSteps; w < (d0 + d + 1) * kWords / kSteps; ++w) br.word(next, w);
       }
     }
+    fetch(i + 2);
     constexpr int kAhead = DP == 256 ? 1 : 2;
     h8 v[kAhead][DP / 32];
 #pragma unroll
@@ -928,11 +948,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
     auto weights = [&](int ks) {
       f8 x;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
-        sums[e % 2] += x[e];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][ks % 2 * 8 + e], scale, -mu));
       pr[ks] = __builtin_convertvector(x, h8);
+      sums[ks % 2] = add_eight(pr[ks], sums[ks % 2]);
     };
     weights(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -948,8 +966,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
     }
     __builtin_amdgcn_s_setprio(0);
     l += sums[0] + sums[1];
-    fetch(i + 2);
-  }
+  };
+  for (; i < live_end; ++i) live(stage(i), stage(i + 1));
   for (; i < n_tiles; ++i) pass_by(i);
   l += other_half(l);
   if (n_chunks == 1) {
@@ -979,13 +997,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 || WAVES == 8 ? 1 : (DP == 64
   }
 }
 
-template <class E, int DP, int WAVES>
+template <class E, int DP>
 hipError_t launch32(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
-  typedef Rows32Q4<DP, WAVES> C;
+  typedef Rows32Q4<DP> C;
   static std::atomic<uint64_t> devices{0};
-  const hipError_t e = allow_lds((const void *)attn_q4_rows32_kernel<E, DP, WAVES>, C::kLds, &devices);
+  const hipError_t e = allow_lds((const void *)attn_q4_rows32_kernel<E, DP>, C::kLds, &devices);
   if (e != hipSuccess) return e;
-  attn_q4_rows32_kernel<E, DP, WAVES><<<plan.n_wgs, 64 * WAVES, C::kLds, st>>>(p);
+  attn_q4_rows32_kernel<E, DP><<<plan.n_wgs, 256, C::kLds, st>>>(p);
   if (plan.n_chunks > 1) attn_join_kernel<C, E, DP><<<plan.n_units * p.n_kv_heads * C::kWaves, 256, 0, st>>>(p);
   return hipGetLastError();
 }
@@ -1002,9 +1020,7 @@ hipError_t launch16(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st)
 
 template <class E, int DP>
 hipError_t launch_dim(const AttnPlan &plan, const AttnQ4Params &p, hipStream_t st) {
-  if constexpr (DP == 128)
-    if (plan.rows == 256) return launch32<E, DP, 8>(plan, p, st);
-  if (plan.rows == 128) return launch32<E, DP, 4>(plan, p, st);
+  if (plan.rows == 128) return launch32<E, DP>(plan, p, st);
   if (plan.rows == 16 && plan.waves == 1) return launch16<E, DP, 1, 1>(plan, p, st);
   if (plan.rows == 16) return launch16<E, DP, 4, 1>(plan, p, st);
   if constexpr (DP < 256) return launch16<E, DP, 4, 2>(plan, p, st);
