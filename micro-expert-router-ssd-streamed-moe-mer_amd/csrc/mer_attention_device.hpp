@@ -502,6 +502,7 @@ struct Granules {
   uint32_t base, total;  // granules before the sequences in view, of those in view
   uint32_t upto;         // of the lanes up to this one, within the view
   uint32_t w[4];
+  uint32_t units[4], of_unit[4];  // w's factors
   int32_t q[5], len[4];  // their q_start and kv_len
   uint32_t seq0;
 
@@ -514,14 +515,25 @@ struct Granules {
       q[i] = p.q_start[s0 + i < p.n_seqs ? s0 + i : p.n_seqs];
       if (i < 4) len[i] = p.kv_len[s0 + i < p.n_seqs ? s0 + i : 0];
     }
-    upto = 0;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       const Span s = make_span(p, q[i], q[i + 1], len[i]);  // past the last sequence: no rows
       const uint32_t rows = (uint32_t)s.n * p.group;
-      w[i] = (rows + ROWS - 1) / ROWS * p.n_kv_heads * granules<GRANULE>(p, s, nullptr);
-      upto += w[i];
+      units[i] = (rows + ROWS - 1) / ROWS * p.n_kv_heads;
+      of_unit[i] = granules<GRANULE>(p, s, nullptr);
+      w[i] = units[i] * of_unit[i];
     }
+    sum();
+  }
+  // As if each unit had a multiple of `piece` granules; the total.
+  __device__ __forceinline__ uint32_t fill(uint32_t piece) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) w[i] = units[i] * ((of_unit[i] + piece - 1) / piece * piece);
+    sum();
+    return total;
+  }
+  __device__ __forceinline__ void sum() {
+    upto = w[0] + w[1] + w[2] + w[3];
     upto += scan_step<0x111, 0xf>(upto);  // from 1, 2, 4 and 8 lanes before, in rows of 16
     upto += scan_step<0x112, 0xf>(upto);
     upto += scan_step<0x114, 0xf>(upto);
