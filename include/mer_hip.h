@@ -480,9 +480,10 @@ int mer_hip_kv_append(const mer_kv_cache *cache, int in_type, size_t n_tokens, c
  * and replays of the graphs captured on it, must not overlap each other (on
  * one stream they do not).  What a call reserves there grows with its sizes
  * (sequences, tokens, kv heads, query heads of each, head_dim, max_q_len and
- * max_kv_len, unknown ones as n_tokens and the table): 17 MB for up to 16 rows
+ * max_kv_len, unknown ones as n_tokens and the table): 34 MB for up to 16 rows
  * (max_q_len x query heads of a kv head), up to 256 MiB above.  A call that is
- * no larger than an earlier one in any of them leaves it where it is.  What
+ * no larger than an earlier one in any of them leaves it where it is, and
+ * mer_hip_paged_attention_q4 reserves the same in the same place.  What
  * the device refuses is not asked for again, nor is the buffer then moved for
  * less: the keys are cut into as many chunks as it holds sums of, down to one. */
 int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_tokens, size_t n_heads,
@@ -501,8 +502,10 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
  *   scales [n_pages][n_kv_heads][head_dim / 32][page_size] f16
  * head_dim is a multiple of 32 up to MER_MAX_HEAD_DIM, page_size a power of
  * two from 8 to 4096; the memory is the caller's and 16-byte aligned.
- * Attention takes what is there: any codes, any finite scale (products of code
- * and scale are rounded to f16 where a scale has more than eight bits). */
+ * Attention takes what is there: any codes, any scale below 8192 (products of
+ * code and scale are rounded to f16 where a scale has more than eight bits);
+ * scales of 8192 and more, which kv_append_q4 never writes, are taken for ones
+ * that are not finite. */
 typedef struct mer_kv_cache_q4 {
   void *k_codes, *v_codes, *k_scales, *v_scales;
   uint32_t page_size, n_kv_heads, head_dim;

@@ -1832,7 +1832,7 @@ int mer_hip_paged_attention_q4(const mer_kv_cache_q4 *cache, int type, size_t n_
   p.v = cache->v_codes;
   p.k_scales = cache->k_scales;
   p.v_scales = cache->v_scales;
-  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_q4_reserve, attn_q4_plan,
+  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_reserve, attn_q4_plan,
                        [&](const AttnPlan &plan, hipStream_t st) { return launch_attention_q4(type, plan, p, st); });
 }
 

@@ -53,12 +53,13 @@ inline size_t attn_most_chunks(size_t keys) {
 // holds its address), while the number of chunks goes up and down with the
 // sizes: so what is reserved grows with every size, and attn_plan keeps within
 // it.  Sizes are the sequences, tokens, kv heads, query heads of each, head_dim
-// and both lengths.  Up to 16 rows a sequence (decode): what the 16- and 32-row
-// kernels' workgroups leave, at most two pieces each (attn_plan's n_wgs; 17 MB
-// on 256 CUs).  Above: as many chunks as the keys allow, up to the region.
+// and both lengths.  Caches of 16 and of 4 bits share a stream's workspace and
+// reserve alike.  Up to 16 rows a sequence (decode): what the 16- and 32-row
+// kernels' workgroups leave, at most two pieces each (the plans' n_wgs; 34 MB
+// on 256 CUs, half of which the 16-bit kernels use).  Above: as many chunks as the keys allow, up to the region.
 inline size_t attn_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                            size_t max_q_len, size_t max_kv_len, int cus) {
-  const size_t small = 2 * 8 * 16 * (64 + 2) * (size_t)cus;  // of all their shapes
+  const size_t small = 2 * 8 * 16 * (128 + 2) * (size_t)cus;  // of all their shapes
   if (max_q_len * group <= 16) return small;
   const size_t n = attn_most_chunks(max_kv_len);
   if (n == 1) return small;
@@ -168,15 +169,9 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
 
 // ---- the cache held in 4 bits (mer_attention_q4.hip) ----
 
-// Floats that a call reserves, as attn_reserve says; up to 16 rows a sequence 34 MB
-// on 256 CUs.
-inline size_t attn_q4_reserve(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
-                              size_t max_q_len, size_t max_kv_len, int cus) {
-  const size_t small = 2 * 8 * 16 * (128 + 2) * (size_t)cus;  // of all shapes of the 16- and 32-row tiles
-  const size_t more = attn_reserve(n_seqs, n_tokens, group, n_kv_heads, head_dim, max_q_len, max_kv_len, cus);
-  return more < small ? small : more;
-}
-
+// As attn_plan: with no floats it is 128-row tiles in one chunk.  Up to 16 rows a
+// sequence tiles of 16, up to 32 tiles of 32, for heads of 256 two of 16, since 32
+// rows would not fit the registers.
 inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                              size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
                              size_t floats) {
