@@ -525,10 +525,24 @@ struct Granules {
     }
     sum();
   }
+  // Units of the view; leaves the granules to be filled in again.
+  __device__ __forceinline__ uint32_t n_units() {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) w[i] = units[i];
+    sum();
+    return total;
+  }
   // As if each unit had a multiple of `piece` granules; the total.
   __device__ __forceinline__ uint32_t fill(uint32_t piece) {
+    const float inv = 1.0f / (float)piece;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) w[i] = units[i] * ((of_unit[i] + piece - 1) / piece * piece);
+    for (uint32_t i = 0; i < 4; ++i) {
+      // the quotient in f32 is off by one at most (granules are below 2^24)
+      const uint32_t x = of_unit[i] + piece - 1;
+      uint32_t y = (uint32_t)((float)x * inv) * piece;
+      y = (int32_t)(x - y) < 0 ? y - piece : (x - y >= piece ? y + piece : y);
+      w[i] = units[i] * y;
+    }
     sum();
     return total;
   }

@@ -170,24 +170,30 @@ inline AttnPlan attn_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32
 // ---- the cache held in 4 bits (mer_attention_q4.hip) ----
 
 // As attn_plan: with no floats it is 128-row tiles in one chunk.  Up to 16 rows a
-// sequence tiles of 16, up to 32 tiles of 32, for heads of 256 two of 16, since 32
-// rows would not fit the registers.
+// sequence: tiles of 16.  17 to 32: tiles of 32; two of 16 where there is little to
+// read, so that starts and joins are what counts (8 x 4 rows, 8 kv heads of 128: 1
+// sequence of 4000 keys 29 us in tiles of 32 and 23 in tiles of 16, of 30000 44 and
+// 34; 8 of 2000 - 6000 34 and 29; but 16 of 2000 - 6000 43 and 51, 4 of 20000 -
+// 40000 56 and 61), and for heads of 256, whose 32 rows would not fit the registers.
 inline AttnPlan attn_q4_plan(size_t n_seqs, size_t n_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t head_dim,
                              size_t max_q_len, size_t max_kv_len, size_t table_keys, uint32_t window, int cus,
                              size_t floats) {
   AttnPlan a{};
   const size_t rows = max_q_len * group;
-  a.rows = rows <= 16 ? 16 : (rows <= 32 ? (head_dim > 128 ? 16 : 32) : 128);
+  const uint64_t pairs = (uint64_t)n_seqs * n_kv_heads;
+  const bool few = 2 * pairs <= (uint64_t)cus && pairs * max_kv_len < 2048ull * cus;
+  a.rows = rows <= 16 ? 16 : (rows <= 32 ? (head_dim > 128 || few ? 16 : 32) : 128);
   // 16- and 32-row tiles count their granules of 128 keys in 32 bits.
   const uint64_t small_tiles = (n_tokens * group / 16 + n_seqs) * (uint64_t)n_kv_heads;
   if (a.rows <= 32 && small_tiles * (table_keys / 128 + 2) < (1ull << 31)) {
-    // Long stretches of few units: workgroups of four waves.  Many units: every
-    // wave a workgroup of its own, so that one's piece ends while the others' keys
-    // stream.  Sequences of 200 - 8000 keys, 8 kv heads of 128: 16 of them 36 us wide
-    // and 37 us narrow, 24 47 and 43, 64 106 and 85; 16 of 4096 28 and 32 us, 64
-    // 69 and 73; 512 of 300 - 700 135 and 94.  Either way as many waves as the LDS
-    // holds.
-    const bool narrow = a.rows == 16 && (uint64_t)n_seqs * n_kv_heads * 4 >= 3ull * cus;
+    // Few units: workgroups of four waves, most of which begin with a unit.  From a
+    // unit a CU on: every wave a workgroup of its own, so that one's piece ends while
+    // the others' keys stream.  Sequences of 200 - 8000 keys, 8 kv heads of 128: 16 of
+    // them 30.6 us wide and 35.6 us narrow, 24 37.2 and 40.0, 32 51.0 and 51.7, 48 86.5
+    // and 66.6, 64 108 and 77.8; of 4096 keys, 32 42.8 and 45.1, 64 70.2 and 74.4; of
+    // 300 - 700, 128 45.1 and 35.6, 512 135 and 94.5; heads of 256, 4 of them, 32
+    // 56.8 and 62.6, 64 118 and 89.3.  Either way as many waves as the LDS holds.
+    const bool narrow = a.rows == 16 && pairs >= (uint64_t)cus;
     a.waves = narrow ? 1 : 4;
     a.n_wgs = (uint32_t)cus * (narrow ? 4 : 1) * (head_dim <= 128 ? 2 : 1);
     a.min_granules = 1;

@@ -364,19 +364,27 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   }
   uint32_t per = uni((all + gridDim.x - 1) / gridDim.x);
   // A workgroup that crosses into another unit pays for a second start (page ids,
-  // queries, first tiles) and a second join.  Where a stretch up to a quarter longer
-  // lets every unit begin with a workgroup, units are taken for multiples of that
-  // stretch: sequences of 200 - 8000 keys, 8 kv heads of 128, 4 of them 22.7 us
-  // crossing and 15.5 not, 16 36.5 and 30.8, 64 81.5 and 78.8.
+  // queries, first tiles) and a second join.  Where a stretch up to twice as long
+  // lets every unit begin with a workgroup, units are taken for multiples of the
+  // shortest such one: sequences of 200 - 8000 keys, 8 kv heads of 128, 4 of them
+  // 22.7 us crossing and 15.5 not, 16 36.5 and 30.8; drafts of 8 x 4 rows, 64
+  // sequences of 500 - 2000 keys 66 and 46 us, of 2000 - 6000 113 and 105.  (The
+  // bound on `all` keeps the filled total in 32 bits.)
   uint32_t whole = 1;
-  if (p.n_seqs <= 256 && per > 1) {
-    for (uint32_t s = per; s <= per + per / 4 + 1; ++s)
-      if (gr.fill(s) <= gridDim.x * s) {
-        whole = s;
-        break;
-      }
-    all = whole > 1 ? gr.total : gr.fill(1);
-    per = whole > 1 ? whole : per;
+  if (p.n_seqs <= 256 && per > 1 && all < (1u << 29)) {
+    // A stretch of all / (workgroups - units) will do whatever the lengths; from there
+    // (or from twice as long) towards the least, to a sixteenth.
+    const uint32_t n_units = gr.n_units(), n = gridDim.x, near = per / 16;
+    uint32_t least = per, most = 2 * per, tried = 0;
+    if (2 * n_units <= n) most = (all + n - n_units - 1) / (n - n_units);
+    else if (n_units > n || gr.fill(tried = most) > n * most) most = 0;
+    while (least + near < most) {
+      tried = (least + most) / 2;
+      if (gr.fill(tried) <= n * tried) most = tried;
+      else least = tried + 1;
+    }
+    if (most) whole = per = most;
+    all = uni(tried == whole ? gr.total : gr.fill(whole));
   }
   uint32_t x = blockIdx.x * per;
   const uint32_t x1 = all - (all < x ? all : x) < per ? all : x + per;

@@ -40,7 +40,7 @@ int main() {
         (p.rows == 32 ? rows32 : p.waves == 1 ? narrow : wide) += 1;
         CHECK(p.waves == 4 || (p.waves == 1 && p.rows == 16));  // what there are kernels for
         CHECK(p.rows == 16 || (dim <= 128 && rows > 16));
-        CHECK(rows <= (dim <= 128 ? p.rows : 32));
+        CHECK(rows <= 32 && (p.rows == 32 || rows <= 16 || dim > 128 || (2 * seqs * heads <= (size_t)cus && seqs * heads * keys < 2048ull * cus)));
         CHECK((tokens * group / 16 + seqs) * heads * (keys / 128 + 2) < (1ull << 31));
         CHECK(p.n_wgs >= kAttnTickets && p.n_wgs < kAttnEpoch && 3 * (size_t)p.n_wgs + kAttnTickets * kAttnTicketWords <= attn_counters(cus));
         CHECK(need == 2 * (size_t)p.n_wgs * p.rows * (dim + 2) && p.min_granules == 1);

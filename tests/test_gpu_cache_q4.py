@@ -469,6 +469,15 @@ def test_many_units(mer, gpu, d, page, window, sink):
     b.check(b.run(mer, gpu, window=window, sinks=sinks), window, sinks)
 
 
+@pytest.mark.parametrize("n,heads,kv", [(1, 16, 16), (5, 64, 16), (1, 5, 5)])
+@pytest.mark.parametrize("seqs", [70, 250])
+def test_more_units_than_workgroups(mer, gpu, n, heads, kv, seqs):
+    g = torch.Generator().manual_seed(39)
+    lens = torch.randint(n, 400, (seqs,), generator=g).tolist()
+    b = Batch([(n, l) for l in lens], heads, kv, 32, 16, BF16, seed=40)
+    b.check(b.run(mer, gpu))
+
+
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("d", [32, 64, 128, 224])
 @pytest.mark.parametrize("window", [0, 70])
