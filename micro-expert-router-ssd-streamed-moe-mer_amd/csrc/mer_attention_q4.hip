@@ -372,14 +372,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   // bound on `all` keeps the filled total in 32 bits.)
   uint32_t whole = 1;
   if (p.n_seqs <= 256 && per > 1 && all < (1u << 29)) {
-    // A stretch of all / (workgroups - units) will do whatever the lengths; from there
-    // (or from twice as long) towards the least, to a sixteenth.
+    // A stretch of all / (workgroups - units) will do whatever the lengths.  The equal
+    // share itself is tried (lengths alike), then between it and that (or twice the
+    // share), to a sixteenth.
     const uint32_t n_units = gr.n_units(), n = gridDim.x, near = per / 16;
     uint32_t least = per, most = 2 * per, tried = 0;
     if (2 * n_units <= n) most = (all + n - n_units - 1) / (n - n_units);
     else if (n_units > n || gr.fill(tried = most) > n * most) most = 0;
-    while (least + near < most) {
-      tried = (least + most) / 2;
+    while (least + near < most || (least == per && least < most)) {
+      tried = least == per ? per : (least + most) / 2;
       if (gr.fill(tried) <= n * tried) most = tried;
       else least = tried + 1;
     }
