@@ -382,6 +382,23 @@ def test_scales_of_values_that_are_not_finite_count_as_zero(mer, gpu, n, d):
     b.check(b.run(mer, gpu))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("seqs", [[(1, 300), (2, 80)], [(5, 300)], [(100, 400), (1, 90)]])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_queries_that_are_not_finite(mer, gpu, dt, seqs, d):
+    """Their own rows have no answer, the others the one that they have without them."""
+    b = Batch(seqs, 8, 2, d, 16, dt, seed=41)
+    want = b.run(mer, gpu)
+    bad = {(0, 3): math.nan, (b.n - 1, 0): math.inf, (b.n // 2, 7): -math.inf}
+    for (row, head), x in bad.items():
+        b.q[row, head, d - 1] = x
+    got = b.run(mer, gpu)
+    for row, head in bad:
+        assert got[row, head].isnan().all()
+        got[row, head] = want[row, head]
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
 @pytest.mark.parametrize("page", [8, 16, 64])
 @pytest.mark.parametrize("n", [1, 50])
 def test_page_outside_the_cache(mer, gpu, page, n):
