@@ -304,7 +304,7 @@ def paged_attention(cache: PagedKvCache | PagedKvCacheQ4, q: torch.Tensor, block
     dev, stream = _enter(q)
     n, h, d = _shape(q, "q")
     q4 = isinstance(cache, PagedKvCacheQ4)
-    fits = q.dtype != torch.float32 if q4 else q.dtype == cache.k.dtype
+    fits = q.dtype in (torch.float16, torch.bfloat16) if q4 else q.dtype == cache.k.dtype
     if d != cache.head_dim or not fits or cache.device != dev:
         held = "held in 4 bits" if q4 else str(cache.k.dtype)
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} on cuda:{dev} does not go with a cache of head_dim "

@@ -1083,15 +1083,15 @@ int attention_params(const Cache *cache, int type, size_t n_seqs, size_t n_token
 }
 
 // Plans a call whose arguments are in p, gets it its workspace and launches it.
-template <class Reserve, class Plan, class Launch>
-int run_attention(AttnParams &p, size_t cap, size_t max_q_len, size_t max_kv_len, void *stream, Reserve reserve_for,
-                  Plan plan_for, Launch launch) {
+template <class Plan, class Launch>
+int run_attention(AttnParams &p, size_t cap, size_t max_q_len, size_t max_kv_len, void *stream, Plan plan_for,
+                  Launch launch) {
   int rc;
   const size_t n_seqs = p.n_seqs, n_tokens = p.n_tokens;
   if (max_q_len == 0 || max_q_len > n_tokens) max_q_len = n_tokens;
   if (max_kv_len == 0 || max_kv_len > cap) max_kv_len = cap;
   const int cus = g_dev[g_device].cus;
-  const size_t reserve = reserve_for(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
+  const size_t reserve = attn_reserve(n_seqs, n_tokens, p.group, p.n_kv_heads, p.head_dim, max_q_len, max_kv_len, cus);
   p.status = g_dev[g_device].status;
   const hipStream_t st = (hipStream_t)stream;
   std::shared_ptr<Workspace> w = workspace_for(st);
@@ -1813,7 +1813,7 @@ int mer_hip_paged_attention(const mer_kv_cache *cache, size_t n_seqs, size_t n_t
   if (rc || p.n_tokens == 0) return rc;
   p.k = cache->k;
   p.v = cache->v;
-  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_reserve, attn_plan,
+  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_plan,
                        [&](const AttnPlan &plan, hipStream_t st) { return launch_attention(cache->type, plan, p, st); });
 }
 
@@ -1832,7 +1832,7 @@ int mer_hip_paged_attention_q4(const mer_kv_cache_q4 *cache, int type, size_t n_
   p.v = cache->v_codes;
   p.k_scales = cache->k_scales;
   p.v_scales = cache->v_scales;
-  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_reserve, attn_q4_plan,
+  return run_attention(p, table_stride * cache->page_size, max_q_len, max_kv_len, stream, attn_q4_plan,
                        [&](const AttnPlan &plan, hipStream_t st) { return launch_attention_q4(type, plan, p, st); });
 }
 

@@ -830,7 +830,8 @@ def test_python_refusals(mer, gpu):
     for t in (cache.k_scales, cache.v_scales):
         t.zero_()
     att(), app(), read()
-    for call, bad in [(att, dict(q=z(2, 4, 64, dtype=F32))), (att, dict(q=z(2, 4, 128))), (att, dict(scale=0.0)),
+    for call, bad in [(att, dict(q=z(2, 4, 64, dtype=F32))), (att, dict(q=z(2, 4, 64, dtype=torch.float64))),
+                      (att, dict(q=z(2, 4, 64, dtype=torch.int16))), (att, dict(q=z(2, 4, 128))), (att, dict(scale=0.0)),
                       (att, dict(window=-1)), (att, dict(kv_len=i32(20, 1))), (att, dict(out=z(2, 4, 64, dtype=BF16))),
                       (att, dict(q=z(2, 3, 64))), (app, dict(k=z(2, 2, 128))), (app, dict(v=z(2, 2, 64, dtype=BF16))),
                       (app, dict(slots=i32(0, 1))), (app, dict(slots=torch.arange(2))), (read, dict(slots=i32(0, 1))),
